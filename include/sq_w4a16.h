@@ -465,6 +465,69 @@ int sq_f16_gemv(const void* x, const void* w, void* y, void* part_val, void* par
 int sq_greedy_feedback(const void* part_val, const void* part_idx, int parts, int M, void* tok, void* pos, void* history,
                        void* step, long long history_rows, void* stream);
 
+/* A key/value cache held in 4 bits, in pages: what decoding reads beside the weights, at a quarter of fp16's bytes.
+ *
+ * pool       uint8 [num_pages][H][record], a record of sq_kv4_record_bytes(D, group_size) bytes per page of 64 rows and
+ *            key/value head.  A row's group of group_size elements reads as s * code + m: m = min(x), s = fp16((max(x) -
+ *            m) / 15), code = round((x - m) / s) in 0..15 (0 where s is 0), each step rounded once in fp32; a group that
+ *            holds an infinity or a NaN reads as NaN.  Behind codes, scales and minima a record holds the page's largest
+ *            and smallest key, element by element.  The pool needs no initial value.
+ * pages      int32 [B][page_stride], `width` entries used: entry j of sequence b is the page of its rows 64 j .. 64 j + 63.
+ *            Pages may be shared between sequences that do not append to them.
+ * lengths    int32 [B]: rows of each sequence, the rows of this call among them.
+ * starts     int32 [B + 1]: sequence b has the tokens starts[b] .. starts[b + 1] - 1 of the call; NULL: T / B each.  The
+ *            tokens are the last rows of their sequence: token i of n is row lengths[b] - n + i.
+ * All four lie on the device and are read by the kernels: a captured HIP graph follows them.  Whatever they hold, nothing
+ * outside the pool, the T tokens and the outputs is touched: a page outside [0, num_pages) does not exist (nothing is
+ * stored there, nobody sees its rows), lengths are clamped to [0, 64 width], starts to [0, T].
+ * D in {64, 128}, group_size in {32, 64, 128} and at most D; strides in elements and multiples of 8; k, v, q, outputs and
+ * pool 16-byte aligned.  T == 0 is no work. */
+int sq_kv4_record_bytes(int D, int group_size);
+
+/* Rows k, v fp16 (element (t, h, d) at k[t * strides[0] + h * strides[1] + d], v with strides[2], strides[3]) are
+ * quantised into their pages and take part in their pages' bounds; a page that gets its row 0 starts its bounds anew.
+ * A page that two sequences of the call name must not get rows from both.  k_hat, v_hat: both NULL, or fp16 [T][H][D]
+ * that receive what the rows read as from now on (rounded once): what a prompt's own attention is given so that it
+ * sees what decoding will see.  Tokens without a page (a negative row, one beyond the table, a page outside the pool)
+ * are left out, their k_hat and v_hat as they were. */
+int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* pool, const void* pages, const void* lengths,
+                  const void* starts, int T, int B, int H, int D, int group_size, int num_pages, int width, int page_stride,
+                  const long* strides, void* stream);
+
+/* out[t, h, :] = sum_j P[j] v_hat[j, :], P = softmax_j(sm_scale * q[t, h, :] . k_hat[j, :]) over the cached rows of t's
+ * sequence up to its own; query head h reads key/value head h / (Hq / H).  q fp16, element (t, h, d) at q[t * q_tstride +
+ * h * q_hstride + d], out fp16 [T][Hq][D] contiguous.  Softmax and sums in fp32; a token without a visible row gives 0;
+ * tokens that belong to no sequence (behind the last) are left as they were.
+ * selected   NULL, or int32 [B][H][count] with T == B and no starts: the token sees only the rows of these pages (their
+ *            places in the sequence).  The first min(count, pages of the sequence) entries are read; one outside the
+ *            sequence is no page; one that stands there twice counts twice.
+ * workspace  NULL, or sq_kv4_attention_workspace_bytes(D) bytes, 16-byte aligned, of any content: a sequence's pages are
+ *            then dealt to several workgroups where there are few, and a second launch joins their shares.  Not shared by
+ *            calls that may run at the same time. */
+size_t sq_kv4_attention_workspace_bytes(int D);
+int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
+                     const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
+                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The pages that matter to a sequence's next token: selected int32 [B][H][count] receives the places of the `count` pages
+ * of the highest score in ascending order, -1 behind the last where a sequence has fewer.  score = max over the query
+ * heads of h of sum_d max(q_d hi_d, q_d lo_d) with the page's bounds: no key of the page scores higher; sums in 64 bits,
+ * equals go to the lowest place, a score that is no number is the lowest.  The first keep_first and the last keep_last
+ * pages are always among them (keep_first + keep_last <= count).  q as above, one token per sequence.  width at most
+ * 16384, B * H at most 65535.  workspace: sq_kv4_select_workspace_bytes(B, H, width) bytes, 16-byte aligned, of any
+ * content; may be NULL where width <= count.  Not shared by calls that may run at the same time. */
+size_t sq_kv4_select_workspace_bytes(int B, int H, int width);
+int sq_kv4_select(const void* q, void* selected, const void* pool, const void* pages, const void* lengths, int B, int Hq, int H,
+                  int D, int group_size, int num_pages, int width, int page_stride, int count, int keep_first, int keep_last,
+                  long q_tstride, long q_hstride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Page src[i] to page dst[i] in every layer, i < n (int32 on the device): layer l's pages lie at pool + l * layer_bytes,
+ * page_bytes each.  What a fork, a copy before a write and a pool made compact need.  No page may be a destination twice,
+ * or a destination and another pair's source; a pair with an index outside [0, num_pages) is left out. */
+int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int num_pages, int layers, size_t page_bytes,
+                      size_t layer_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "sq_kernels.h"
+#include "sq_kv4.h"
 
 // Workspace of sq_w4a16_gemm_static_ws: device memory that belongs to the library, so that the
 // call allocates nothing.  Every GPU the library runs on holds its own copy of the array until the
@@ -357,6 +358,44 @@ int gemm_dispatch(const void* x, const void* w, const void* zs, void* y, int M, 
         default:
             return SQ_ERR_BAD_ALGO;
     }
+}
+
+}  // namespace
+
+namespace {
+
+bool kv4_groups_ok(int D, int g) { return (D == 64 || D == 128) && (g == 32 || g == 64 || g == 128) && g <= D; }
+
+int check_kv4(const void* pool, const void* pages, const void* lengths, const void* starts, int T, int B, int H, int D, int g,
+              int num_pages, int width, int page_stride) {
+    if (T < 0 || B < 0 || H <= 0 || (D != 64 && D != 128) || num_pages <= 0 || width < 0 || page_stride < width)
+        return SQ_ERR_BAD_SHAPE;
+    if (!kv4_groups_ok(D, g)) return SQ_ERR_BAD_GROUP;
+    if (width > (1 << 24) || (long)(T + 2l * B) * H > (1L << 30)) return SQ_ERR_BAD_SHAPE;
+    if (!starts && B > 0 && T % B != 0) return SQ_ERR_BAD_SHAPE;
+    if (T == 0 || B == 0) return SQ_OK;
+    if (!pool || (!pages && width > 0) || !lengths) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(pool) ||
+        ((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(starts)) & 3u))
+        return SQ_ERR_MISALIGNED;
+    return SQ_OK;
+}
+
+sq::Kv4Cache kv4_cache(const void* pool, const void* pages, const void* lengths, const void* starts, int T, int B, int H,
+                       int num_pages, int width, int page_stride) {
+    sq::Kv4Cache c;
+    c.pool = static_cast<uint8_t*>(const_cast<void*>(pool));
+    c.table = static_cast<const int*>(pages);
+    c.lengths = static_cast<const int*>(lengths);
+    c.starts = static_cast<const int*>(starts);
+    c.B = B;
+    c.T = T;
+    c.H = H;
+    c.num_pages = num_pages;
+    c.width = width;
+    c.table_stride = page_stride;
+    c.each = T / B;
+    return c;
 }
 
 }  // namespace
@@ -1096,6 +1135,80 @@ int sq_greedy_feedback(const void* part_val, const void* part_idx, int parts, in
     return launch_code(sq::launch_greedy_feedback(static_cast<const float*>(part_val), static_cast<const int*>(part_idx),
                                                   parts, M, tok, pos, history, step, history_rows,
                                                   static_cast<hipStream_t>(stream)));
+}
+
+int sq_kv4_record_bytes(int D, int group_size) { return kv4_groups_ok(D, group_size) ? sq::kv4_record_bytes(D, group_size) : 0; }
+
+int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* pool, const void* pages, const void* lengths,
+                  const void* starts, int T, int B, int H, int D, int group_size, int num_pages, int width, int page_stride,
+                  const long* strides, void* stream) {
+    const int rc = check_kv4(pool, pages, lengths, starts, T, B, H, D, group_size, num_pages, width, page_stride);
+    if (rc != SQ_OK) return rc;
+    if (T == 0 || B == 0 || width == 0) return SQ_OK;
+    if (!k || !v || !strides || (k_hat == nullptr) != (v_hat == nullptr)) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_hat) || !aligned16(v_hat)) return SQ_ERR_MISALIGNED;
+    for (int i = 0; i < 4; i++) {
+        if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
+        if (strides[i] % 8 != 0) return SQ_ERR_MISALIGNED;
+    }
+    return launch_code(sq::launch_kv4_append(kv4_cache(pool, pages, lengths, starts, T, B, H, num_pages, width, page_stride), k,
+                                             v, k_hat, v_hat, D, group_size, strides, static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_kv4_attention_workspace_bytes(int D) { return D == 64 || D == 128 ? sq::kv4_attention_workspace_bytes(D) : 0; }
+
+int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
+                     const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
+                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    const int rc = check_kv4(pool, pages, lengths, starts, T, B, H, D, group_size, num_pages, width, page_stride);
+    if (rc != SQ_OK) return rc;
+    if (Hq <= 0 || Hq % H != 0 || (long)T * Hq > (1L << 30) || q_tstride < 0 || q_hstride < 0) return SQ_ERR_BAD_SHAPE;
+    if (selected && (count <= 0 || starts || T != B)) return SQ_ERR_BAD_SHAPE;
+    if (T == 0 || B == 0) return SQ_OK;
+    if (!q || !out) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(out) || (q_tstride | q_hstride) % 8 != 0 || (reinterpret_cast<uintptr_t>(selected) & 3u))
+        return SQ_ERR_MISALIGNED;
+    if (workspace && (!aligned16(workspace) || workspace_bytes < sq::kv4_attention_workspace_bytes(D))) return SQ_ERR_WORKSPACE;
+    return launch_code(sq::launch_kv4_attention(kv4_cache(pool, pages, lengths, starts, T, B, H, num_pages, width, page_stride),
+                                                q, out, static_cast<const int*>(selected), workspace, D, group_size, Hq / H,
+                                                selected ? count : 0, q_tstride, q_hstride, sm_scale,
+                                                static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_kv4_select_workspace_bytes(int B, int H, int width) {
+    return B > 0 && H > 0 && width > 0 ? (size_t)B * H * width * sizeof(double) : 0;
+}
+
+int sq_kv4_select(const void* q, void* selected, const void* pool, const void* pages, const void* lengths, int B, int Hq, int H,
+                  int D, int group_size, int num_pages, int width, int page_stride, int count, int keep_first, int keep_last,
+                  long q_tstride, long q_hstride, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_kv4(pool, pages, lengths, nullptr, B, B, H, D, group_size, num_pages, width, page_stride);
+    if (rc != SQ_OK) return rc;
+    if (Hq <= 0 || Hq % H != 0 || q_tstride < 0 || q_hstride < 0) return SQ_ERR_BAD_SHAPE;
+    if (count <= 0 || keep_first < 0 || keep_last < 0 || (long)keep_first + keep_last > count) return SQ_ERR_BAD_SHAPE;
+    if ((long)B * H > 65535 || (long)B * H * count > (1L << 30) || width > sq::KV4_SELECT_MAX_PAGES) return SQ_ERR_BAD_SHAPE;
+    if (B == 0) return SQ_OK;
+    if (!q || !selected) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(q) || (q_tstride | q_hstride) % 8 != 0 || (reinterpret_cast<uintptr_t>(selected) & 3u)) return SQ_ERR_MISALIGNED;
+    if (width > count && (!workspace || !aligned16(workspace) || workspace_bytes < sq_kv4_select_workspace_bytes(B, H, width)))
+        return SQ_ERR_WORKSPACE;
+    return launch_code(sq::launch_kv4_select(kv4_cache(pool, pages, lengths, nullptr, B, B, H, num_pages, width, page_stride), q,
+                                             selected, workspace, D, group_size, Hq / H, q_tstride, q_hstride, count, keep_first,
+                                             keep_last, static_cast<hipStream_t>(stream)));
+}
+
+int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int num_pages, int layers, size_t page_bytes,
+                      size_t layer_bytes, void* stream) {
+    if (n < 0 || num_pages <= 0 || layers <= 0 || layers > 65535 || page_bytes == 0 || page_bytes % 16 != 0 ||
+        page_bytes > (1u << 30) || layer_bytes % 16 != 0 || (layers > 1 && layer_bytes < page_bytes * num_pages))
+        return SQ_ERR_BAD_SHAPE;
+    if ((long)n * (long)((page_bytes + 16383) / 16384) > (1L << 30)) return SQ_ERR_BAD_SHAPE;
+    if (n == 0) return SQ_OK;
+    if (!pool || !src || !dst) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(pool) || ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3u)) return SQ_ERR_MISALIGNED;
+    return launch_code(sq::launch_kv4_copy_pages(pool, static_cast<const int*>(src), static_cast<const int*>(dst), n, num_pages,
+                                                 layers, (long)page_bytes, (long)layer_bytes, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

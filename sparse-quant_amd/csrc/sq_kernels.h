@@ -130,6 +130,20 @@ hipError_t launch_decode_attention(const void* q, const void* k_new, const void*
 constexpr int DECODE_ATTN_MAX_SPLIT = 16;
 size_t decode_attention_workspace_bytes(int B, int H, int D);
 
+// sq_kv4.hip, sq_kv4_attn.hip: a key/value cache held in 4 bits (layout: sq_kv4.h).  strides: of k over token and head,
+// then of v.
+struct Kv4Cache;
+hipError_t launch_kv4_append(const Kv4Cache& c, const void* k, const void* v, void* k_hat, void* v_hat, int D, int g,
+                             const long* strides, hipStream_t st);
+hipError_t launch_kv4_copy_pages(void* pool, const int* src, const int* dst, int n, int num_pages, int layers,
+                                 long page_bytes, long layer_bytes, hipStream_t st);
+constexpr int KV4_SELECT_MAX_PAGES = 16384;  // their keys lie in LDS
+hipError_t launch_kv4_select(const Kv4Cache& c, const void* q, void* selected, void* workspace, int D, int g, int share,
+                             long q_ts, long q_hs, int count, int keep_first, int keep_last, hipStream_t st);
+size_t kv4_attention_workspace_bytes(int D);
+hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, const int* selected, void* workspace, int D, int g,
+                                int share, int count, long q_ts, long q_hs, float sm_scale, hipStream_t st);
+
 // sq_lm_head.hip: the ends of a greedy decode step around the W4A16 layers (the end-to-end harness).
 // out[r, :] = embed[tok[r], :] + pos_table[*pos + pos_offset, :] (fp16; indices clamped to their tables).
 hipError_t launch_embed_rows(const void* embed, const void* pos_table, const void* tok, const void* pos, long long pos_offset,

@@ -1,0 +1,482 @@
+// A key/value cache held in 4 bits: quantising new rows into it, choosing pages by a bound of their scores, copying
+// pages (layout: sq_kv4.h; attention: sq_kv4_attn.hip).
+#include "sq_kernels.h"
+#include "sq_kv4.h"
+
+#include <type_traits>
+
+namespace sq {
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------- append
+//
+// Per row and group of g elements: m = min x, s = fp16((max x - m) / 15), code = round((x - m) / s) in 0..15, the
+// element then reads as s * code + m.  All steps in fp32 with one rounding each (the division included), so that the
+// codes are those of any IEEE implementation.  An infinity or a NaN in a group makes its scale one: the group reads
+// as NaN.  A workgroup owns one page of one head and with it the page's bounds, so nothing is shared between
+// workgroups and nothing is atomic.
+struct Kv4AppendArgs {
+    Kv4Cache c;
+    const half_t* k;
+    const half_t* v;
+    half_t* k_hat;  // what the rows read as, contiguous [T][H][D], or null
+    half_t* v_hat;
+    long k_ts, k_hs, v_ts, v_hs;  // element strides over token and head
+};
+
+struct Group {
+    float s, m;
+    half_t sh, mh;
+};
+
+// A group's scale and minimum from its extremes; bad: 0, or NaN where an element is no finite number.
+__device__ __forceinline__ Group group_of(float lo, float hi, float bad) {
+    Group r;
+    r.sh = (half_t)((hi - lo) / 15.f + bad);
+    r.mh = (half_t)lo;
+    r.s = (float)r.sh;
+    r.m = lo;
+    return r;
+}
+__device__ __forceinline__ int code_of(float x, const Group& g) {
+    const float c = rintf((x - g.m) / g.s);
+    return g.s > 0.f ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
+}
+
+template <int D, int G, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void kv4_append_kernel(Kv4AppendArgs a) {
+    constexpr int g = D / G;
+    constexpr int LPR = D / 8;     // lanes of a row
+    constexpr int RPW = 64 / LPR;  // rows of a wave
+    constexpr int REC = kv4_record_bytes(D, g);
+    __shared__ float ext[WAVES][2][D];
+    const Kv4Cache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int head = blockIdx.x % c.H;
+    int unit = blockIdx.x / c.H;
+
+    // The sequence and its unit-th page that gets rows.
+    int b = 0, first = 0, count = 0, len = 0;
+    if (!c.starts) {
+        const int per = (c.each + KV4_PAGE - 2) / KV4_PAGE + 1;
+        b = unit / per;
+        unit -= b * per;
+        if (b >= c.B) return;
+        kv4_tokens(c, b, first, count);
+        len = c.lengths[b];
+    } else {
+        bool found = false;
+        for (int b0 = 0; b0 < c.B && !found; b0 += 64) {
+            int f = 0, n = 0, l = 0, touched = 0;
+            if (b0 + lane < c.B) {
+                kv4_tokens(c, b0 + lane, f, n);
+                l = c.lengths[b0 + lane];
+                touched = n > 0 ? (n + KV4_PAGE - 2) / KV4_PAGE + 1 : 0;
+            }
+            const int upto = wave_scan(touched);
+            const unsigned long long past = __ballot(upto > unit);
+            if (past) {
+                const int at = __ffsll(past) - 1;
+                b = b0 + at;
+                unit -= __shfl(upto - touched, at, 64);
+                first = __shfl(f, at, 64);
+                count = __shfl(n, at, 64);
+                len = __shfl(l, at, 64);
+                found = true;
+            } else {
+                unit -= __shfl(upto, 63, 64);
+            }
+        }
+        if (!found) return;
+    }
+    if (len <= 0 || count <= 0) return;
+    // Rows [len - count, len), those inside the table; rows of this page [r0, r1).
+    const long begin = (long)len - count;
+    const long row_lo = begin < 0 ? 0 : begin;
+    const long row_hi = len < (long)c.width * KV4_PAGE ? len : (long)c.width * KV4_PAGE;
+    const long page = row_lo / KV4_PAGE + unit;
+    const long pr = page * KV4_PAGE;
+    const int r0 = (int)((row_lo > pr ? row_lo : pr) - pr);
+    const int r1 = (int)((row_hi < pr + KV4_PAGE ? row_hi : pr + KV4_PAGE) - pr);
+    if (r0 >= r1) return;
+    const int id = c.table[(long)b * c.table_stride + page];
+    if ((unsigned)id >= (unsigned)c.num_pages) return;
+    uint8_t* const rec = c.pool + ((long)id * c.H + head) * REC;
+    const long token0 = first + (pr - begin);  // token of row 0 of the page (it may lie before the first)
+
+    const int sub = lane % LPR, slot = lane / LPR;
+    float kmax[8], kmin[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) kmax[e] = -INFINITY, kmin[e] = INFINITY;
+
+    for (int rb = r0 + wave * RPW; rb < r1; rb += WAVES * RPW) {
+        const int row = rb + slot;
+        const bool live = row < r1;
+        const long t = token0 + (live ? row : rb);
+        const int quad = row >> 2, in_quad = row & 3;
+        // Keys: lane `sub` holds elements 8 sub .. 8 sub + 7.
+        {
+            const half8_t x8 = *(const half8_t*)(a.k + t * a.k_ts + head * a.k_hs + 8 * sub);
+            float x[8], lo, hi, bad = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = (float)x8[e];
+                lo = e ? fminf(lo, x[e]) : x[e];
+                hi = e ? fmaxf(hi, x[e]) : x[e];
+                bad += 0.f * x[e];
+                if (live) {
+                    kmax[e] = fmaxf(kmax[e], x[e]);
+                    kmin[e] = fminf(kmin[e], x[e]);
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < g / 8; d <<= 1) {
+                lo = fminf(lo, __shfl_xor(lo, d, 64));
+                hi = fmaxf(hi, __shfl_xor(hi, d, 64));
+                bad += __shfl_xor(bad, d, 64);
+            }
+            const Group gr = group_of(lo, hi, bad);
+            const int cl = sub & 3, h = (sub >> 2) & 1, p = sub >> 3;
+            uint32_t w0 = 0, w1 = 0;
+            half8_t y8;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int code = code_of(x[e], gr);
+                const uint32_t bits = (uint32_t)code << (4 * (4 * (e & 1) + 2 * (e >> 2)));
+                if (e & 2)
+                    w1 |= bits;
+                else
+                    w0 |= bits;
+                y8[e] = (half_t)(gr.s * (float)code + gr.m);
+            }
+            w0 <<= 4 * h;
+            w1 <<= 4 * h;
+            const uint32_t o0 = __shfl_xor((int)w0, 4, 64), o1 = __shfl_xor((int)w1, 4, 64);
+            const uint32_t word = h ? (w1 | o1) : (w0 | o0);
+            if (live) {
+                *(uint32_t*)(rec + row * (D / 2) + (cl * (D / 32) + 2 * p + h) * 4) = word;
+                if (sub % (g / 8) == 0) {
+                    half_t* sm = (half_t*)(rec + 64 * D) + ((sub / (g / 8)) * 16 + quad) * 8 + in_quad;
+                    sm[0] = gr.sh;
+                    sm[4] = gr.mh;
+                }
+                if (a.k_hat) *(half8_t*)(a.k_hat + (t * c.H + head) * D + 8 * sub) = y8;
+            }
+        }
+        // Values: lane `sub` holds the elements of word `sub`.
+        {
+            const half_t* src = a.v + t * a.v_ts + head * a.v_hs + sub;
+            float x[8];
+#pragma unroll
+            for (int n = 0; n < 8; n++) x[n] = (float)src[D == 128 ? 16 * n : 16 * (n & 3) + 8 * (n >> 2)];
+            uint32_t word = 0;
+#pragma unroll
+            for (int gi = 0; gi < G; gi++) {
+                float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+                    if ((D == 128 ? 16 * n : 16 * (n & 3)) / g == gi) {
+                        lo = fminf(lo, x[n]);
+                        hi = fmaxf(hi, x[n]);
+                        bad += 0.f * x[n];
+                    }
+#pragma unroll
+                for (int d = 1; d < LPR; d <<= 1) {
+                    lo = fminf(lo, __shfl_xor(lo, d, 64));
+                    hi = fmaxf(hi, __shfl_xor(hi, d, 64));
+                    bad += __shfl_xor(bad, d, 64);
+                }
+                const Group gr = group_of(lo, hi, bad);
+#pragma unroll
+                for (int n = 0; n < 8; n++) {
+                    const int off = D == 128 ? 16 * n : 16 * (n & 3) + 8 * (n >> 2);
+                    if ((D == 128 ? 16 * n : 16 * (n & 3)) / g == gi) {
+                        const int code = code_of(x[n], gr);
+                        word |= (uint32_t)code << (4 * n);
+                        if (live && a.v_hat) a.v_hat[(t * c.H + head) * D + off + sub] = (half_t)(gr.s * (float)code + gr.m);
+                    }
+                }
+                if (live && sub == gi) {
+                    half_t* sm = (half_t*)(rec + 64 * D + 256 * G) + (gi * 16 + quad) * 8 + in_quad;
+                    sm[0] = gr.sh;
+                    sm[4] = gr.mh;
+                }
+            }
+            if (live) *(uint32_t*)(rec + 32 * D + (quad * (D / 8) + sub) * 16 + in_quad * 4) = word;
+        }
+    }
+    // Bounds: over the rows of this call, then with those that the page had unless its row 0 is among them.
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+#pragma unroll
+        for (int d = LPR; d < 64; d <<= 1) {
+            kmax[e] = fmaxf(kmax[e], __shfl_xor(kmax[e], d, 64));
+            kmin[e] = fminf(kmin[e], __shfl_xor(kmin[e], d, 64));
+        }
+        if (slot == 0) {
+            ext[wave][0][8 * sub + e] = kmax[e];
+            ext[wave][1][8 * sub + e] = kmin[e];
+        }
+    }
+    __syncthreads();
+    half_t* const bounds = (half_t*)(rec + 64 * D + 512 * G);
+    for (int d = threadIdx.x; d < D; d += 64 * WAVES) {
+        float hi = ext[0][0][d], lo = ext[0][1][d];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            hi = fmaxf(hi, ext[w][0][d]);
+            lo = fminf(lo, ext[w][1][d]);
+        }
+        if (r0 > 0) {
+            hi = fmaxf(hi, (float)bounds[d]);
+            lo = fminf(lo, (float)bounds[D + d]);
+        }
+        bounds[d] = (half_t)hi;
+        bounds[D + d] = (half_t)lo;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- copy
+
+// Pages of all layers, src[i] to dst[i]; a pair with an index outside the pool is left out.
+__global__ __launch_bounds__(256) void kv4_copy_kernel(uint8_t* pool, const int* src, const int* dst, int num_pages,
+                                                       int parts, long page_bytes, long layer_bytes) {
+    const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int from = src[pair], to = dst[pair];
+    if ((unsigned)from >= (unsigned)num_pages || (unsigned)to >= (unsigned)num_pages || from == to) return;
+    uint8_t* const base = pool + (long)blockIdx.y * layer_bytes;
+    const u32x4_t* s = (const u32x4_t*)(base + from * page_bytes);
+    u32x4_t* d = (u32x4_t*)(base + to * page_bytes);
+    const int n = (int)(page_bytes / 16);
+    const int i0 = part * 1024 + threadIdx.x;
+    u32x4_t t[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (i0 + 256 * j < n) t[j] = s[i0 + 256 * j];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (i0 + 256 * j < n) d[i0 + 256 * j] = t[j];
+}
+
+// ------------------------------------------------------------------------------------------------------- select
+//
+// score(page) = max over the head's queries of sum_d max(q_d hi_d, q_d lo_d), hi and lo the page's largest and
+// smallest keys: no key of the page can score higher.  Sums in 64 bits: which of two pages is the better one must not
+// hang on the order of a sum.  A lane owns a page and walks over its bounds; the queries come from LDS, split into
+// their positive and negative parts, so that the choice between hi and lo is two products and no comparison.
+constexpr int SELECT_QUERIES = 8;  // of a round
+
+struct Kv4SelectArgs {
+    Kv4Cache c;
+    const half_t* q;
+    int* selected;   // [B][H][count]
+    double* scores;  // [B][H][width]
+    long q_ts, q_hs;
+    int share, count, keep_first, keep_last;
+};
+
+template <int D>
+__global__ __launch_bounds__(64) void kv4_score_kernel(Kv4SelectArgs a, int rec_bytes) {
+    __shared__ double qs[SELECT_QUERIES][D][2];
+    const Kv4Cache& c = a.c;
+    const int lane = threadIdx.x;
+    const int head = blockIdx.y % c.H, b = blockIdx.y / c.H;
+    const int pages = (kv4_length(c, b) + KV4_PAGE - 1) / KV4_PAGE;
+    const int page = blockIdx.x * 64 + lane;
+    if (pages <= a.count || (int)(blockIdx.x * 64) >= pages) return;
+    int id = page < pages ? c.table[(long)b * c.table_stride + page] : -1;
+    const bool real = (unsigned)id < (unsigned)c.num_pages;
+    if (!real) id = 0;
+    const half8_t* const hi = (const half8_t*)(c.pool + ((long)id * c.H + head) * rec_bytes + rec_bytes - 4 * D);
+    const half8_t* const lo = hi + D / 8;
+    double best = -INFINITY;
+    for (int g0 = 0; g0 < a.share; g0 += SELECT_QUERIES) {
+        const int ng = imin(SELECT_QUERIES, a.share - g0);
+        __syncthreads();
+        for (int i = lane; i < SELECT_QUERIES * D; i += 64) {
+            const int g = i / D, d = i % D;
+            const float x = g < ng ? (float)a.q[(long)b * a.q_ts + (long)(head * a.share + g0 + g) * a.q_hs + d] : 0.f;
+            qs[g][d][0] = fmaxf(x, 0.f);
+            qs[g][d][1] = fminf(x, 0.f);
+        }
+        __syncthreads();
+        double s[SELECT_QUERIES];
+#pragma unroll
+        for (int g = 0; g < SELECT_QUERIES; g++) s[g] = 0.0;
+        for (int d8 = 0; d8 < D / 8; d8++) {
+            const half8_t h8 = hi[d8], l8 = lo[d8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const double h = (double)(float)h8[e], l = (double)(float)l8[e];
+#pragma unroll
+                for (int g = 0; g < SELECT_QUERIES; g++)
+                    s[g] += qs[g][8 * d8 + e][0] * h + qs[g][8 * d8 + e][1] * l;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < SELECT_QUERIES; g++)
+            if (g < ng && s[g] > best) best = s[g];
+    }
+    if (page < pages) a.scores[((long)b * c.H + head) * c.width + page] = real ? best : -INFINITY;
+}
+
+// A double as an unsigned number of the same order; one that is no number is the lowest.
+__device__ __forceinline__ unsigned long long ordered(double x) {
+    if (!(x == x)) return 0;
+    const unsigned long long u = bit_cast<unsigned long long>(x + 0.0);
+    return u & 0x8000000000000000ull ? ~u : u | 0x8000000000000000ull;
+}
+
+constexpr int SELECT_THREADS = 1024;
+
+// The `count` best pages of a head in ascending order, ties to the lowest; -1 behind the last where there are fewer.
+// The count-th largest key is found digit by digit, from the top, until no other key shares its digits.
+__global__ __launch_bounds__(SELECT_THREADS) void kv4_select_kernel(Kv4SelectArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned long long keys[];
+    __shared__ unsigned hist[256];
+    __shared__ unsigned waves[SELECT_THREADS / 64][2];
+    __shared__ unsigned digit_at, left_at, shared_by;
+    const Kv4Cache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = blockIdx.x / c.H;
+    const int pages = (kv4_length(c, b) + KV4_PAGE - 1) / KV4_PAGE;
+    int* const out = a.selected + (long)blockIdx.x * a.count;
+    if (pages <= a.count) {
+        for (int i = tid; i < a.count; i += SELECT_THREADS) out[i] = i < pages ? i : -1;
+        return;
+    }
+    const double* const scores = a.scores + (long)blockIdx.x * c.width;
+    for (int i = tid; i < pages; i += SELECT_THREADS)
+        keys[i] = i < a.keep_first || i >= pages - a.keep_last ? ~0ull : ordered(scores[i]);
+    unsigned long long prefix = 0, mask = 0;
+    unsigned left = a.count;  // of the keys that share the prefix, how many are taken
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < pages; i += SELECT_THREADS)
+            if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1u);
+        __syncthreads();
+        if (tid < 64) {
+            // keys of digits above: lane l has digits 255 - 4 l downwards
+            unsigned n[4], sum = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum += n[j] = hist[255 - 4 * lane - j];
+            unsigned before = (unsigned)wave_scan((int)sum) - sum;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (before < left && before + n[j] >= left) {
+                    digit_at = 255 - 4 * lane - j;
+                    left_at = left - before;
+                    shared_by = n[j];
+                }
+                before += n[j];
+            }
+        }
+        __syncthreads();
+        prefix |= (unsigned long long)digit_at << shift;
+        mask |= 255ull << shift;
+        left = left_at;
+        if (shared_by == left) break;  // every key that shares the prefix is taken
+        // (the next pass writes these three behind its second barrier)
+    }
+    // Keys above the prefix are taken, of those that share it the first `left`.
+    unsigned taken = 0, ties = 0;
+    for (int i0 = 0; i0 < pages; i0 += SELECT_THREADS) {
+        const int i = i0 + tid;
+        const unsigned long long key = i < pages ? keys[i] & mask : 0;
+        const bool above = i < pages && key > prefix, tie = i < pages && key == prefix;
+        const unsigned long long am = __ballot(above), tm = __ballot(tie);
+        __syncthreads();
+        if (lane == 0) {
+            waves[wave][0] = __popcll(am);
+            waves[wave][1] = __popcll(tm);
+        }
+        __syncthreads();
+        unsigned a_before = 0, t_before = 0, a_all = 0, t_all = 0;
+#pragma unroll
+        for (int w = 0; w < SELECT_THREADS / 64; w++) {
+            if (w == wave) a_before = a_all, t_before = t_all;
+            a_all += waves[w][0];
+            t_all += waves[w][1];
+        }
+        const unsigned long long below = (1ull << lane) - 1;
+        a_before += __popcll(am & below);
+        t_before += __popcll(tm & below) + ties;
+        const unsigned at = taken + a_before + (t_before < left ? t_before : left) - (ties < left ? ties : left);
+        if (above || (tie && t_before < left)) out[at] = i;
+        const unsigned t_new = ties + t_all;
+        taken += a_all + (t_new < left ? t_new : left) - (ties < left ? ties : left);
+        ties = t_new;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_kv4_append(const Kv4Cache& c, const void* k, const void* v, void* k_hat, void* v_hat, int D, int g,
+                             const long* strides, hipStream_t st) {
+    Kv4AppendArgs a;
+    a.c = c;
+    a.k = (const half_t*)k;
+    a.v = (const half_t*)v;
+    a.k_hat = (half_t*)k_hat;
+    a.v_hat = (half_t*)v_hat;
+    a.k_ts = strides[0];
+    a.k_hs = strides[1];
+    a.v_ts = strides[2];
+    a.v_hs = strides[3];
+    // Pages that get rows: n tokens touch at most (n + 62) / 64 + 1 of them.
+    const long units = c.starts ? c.T / KV4_PAGE + 2l * (c.B < c.T ? c.B : c.T)
+                                : (long)c.B * ((c.each + KV4_PAGE - 2) / KV4_PAGE + 1);
+    const dim3 grid((unsigned)(units * c.H));
+    auto go = [&](auto d, auto groups) {
+        // one row per sequence: one wave; otherwise four share a page
+        if (!c.starts && c.each == 1)
+            hipLaunchKernelGGL((kv4_append_kernel<d.value, groups.value, 1>), grid, dim3(64), 0, st, a);
+        else
+            hipLaunchKernelGGL((kv4_append_kernel<d.value, groups.value, 4>), grid, dim3(256), 0, st, a);
+    };
+    if (D == 128 && g == 128) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
+    if (D == 128 && g == 64) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
+    if (D == 128 && g == 32) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+    if (D == 64 && g == 64) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    if (D == 64 && g == 32) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_copy_pages(void* pool, const int* src, const int* dst, int n, int num_pages, int layers,
+                                 long page_bytes, long layer_bytes, hipStream_t st) {
+    const int parts = (int)((page_bytes / 16 + 1023) / 1024);
+    hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n * parts, layers), dim3(256), 0, st, (uint8_t*)pool, src, dst, num_pages,
+                       parts, page_bytes, layer_bytes);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_select(const Kv4Cache& c, const void* q, void* selected, void* workspace, int D, int g, int share,
+                             long q_ts, long q_hs, int count, int keep_first, int keep_last, hipStream_t st) {
+    Kv4SelectArgs a;
+    a.c = c;
+    a.q = (const half_t*)q;
+    a.selected = (int*)selected;
+    a.scores = (double*)workspace;
+    a.q_ts = q_ts;
+    a.q_hs = q_hs;
+    a.share = share;
+    a.count = count;
+    a.keep_first = keep_first;
+    a.keep_last = keep_last;
+    const int heads = c.B * c.H;
+    if (c.width > count) {
+        const dim3 grid((c.width + 63) / 64, heads);
+        if (D == 128)
+            hipLaunchKernelGGL(kv4_score_kernel<128>, grid, dim3(64), 0, st, a, kv4_record_bytes(D, g));
+        else
+            hipLaunchKernelGGL(kv4_score_kernel<64>, grid, dim3(64), 0, st, a, kv4_record_bytes(D, g));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kv4_select_kernel, dim3(heads), dim3(SELECT_THREADS), (size_t)c.width * 8, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace sq

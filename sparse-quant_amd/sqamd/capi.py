@@ -57,6 +57,14 @@ SIGNATURES = {
                                     _vp, ctypes.c_size_t, _vp]),
     "sq_lut_attention_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, ctypes.c_float, _i, _vp]),
     "sq_lut_attention_strided": (_i, [_vp] * 7 + [_i] * 6 + [_vp, ctypes.c_float, _i, _vp]),
+    "sq_kv4_record_bytes": (_i, [_i, _i]),
+    "sq_kv4_append": (_i, [_vp] * 8 + [_i] * 8 + [_vp, _vp]),
+    "sq_kv4_attention_workspace_bytes": (ctypes.c_size_t, [_i]),
+    "sq_kv4_attention": (_i, [_vp] * 7 + [_i] * 10 + [ctypes.c_long, ctypes.c_long, ctypes.c_float, _vp, ctypes.c_size_t,
+                                                      _vp]),
+    "sq_kv4_select_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
+    "sq_kv4_select": (_i, [_vp] * 5 + [_i] * 11 + [ctypes.c_long, ctypes.c_long, _vp, ctypes.c_size_t, _vp]),
+    "sq_kv4_copy_pages": (_i, [_vp] * 3 + [_i] * 3 + [ctypes.c_size_t, ctypes.c_size_t, _vp]),
     "sq_embed_rows": (_i, [_vp, _vp, _vp, _vp, ctypes.c_longlong, _vp, _i, _i, ctypes.c_longlong, ctypes.c_longlong, _vp]),
     "sq_f16_gemv_parts": (_i, [_i]),
     "sq_f16_gemv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),

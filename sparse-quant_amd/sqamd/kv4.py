@@ -1,0 +1,386 @@
+"""A key/value cache held in 4 bits, in pages: the operators on it and its bookkeeping.
+
+The cache is a pool of pages of 64 rows, uint8 [pages, kv_heads, record] (`new_pool`); the record's layout is written down
+with sq_kv4_append in include/sq_w4a16.h.  A sequence's pages stand in a row of `pages` int32 [sequences, width], its rows
+are counted by `lengths` int32 [sequences], the rows of the present call among them; tokens of several sequences lie one
+behind the other, `starts` int32 [sequences + 1] says where each begins (None: equally many each).  All are device tensors,
+read by the kernels, so that a captured HIP graph follows them.
+
+    append        quantise the key and value rows of new tokens into their pages
+    attention     causal attention of the tokens over their sequence's rows, or over the rows of selected pages
+    select_pages  for one token of each sequence, the pages whose keys can score highest
+    copy_pages    copy pages in every layer
+
+`KV4Cache` keeps pools of all layers, tables and free pages: sequences that grow, fork (pages are shared until one of them
+is written to), shrink and end, and a pool made compact.
+
+The reference keeps its cache in fp16 tensors that grow by torch.cat (sparse-attention/nvidia/playground/kernels/
+block_sparse_attention_lut.py:272-300 reads them); nothing here has a counterpart there.
+"""
+import ctypes
+import heapq
+
+import torch
+
+from . import capi
+from .capi import _check, _ptr, _stream
+
+PAGE = 64
+GROUPS = (32, 64, 128)
+
+
+def record_bytes(head_dim, group_size):
+    """Bytes of one page of one key/value head."""
+    if head_dim not in (64, 128) or group_size not in GROUPS or group_size > head_dim:
+        raise ValueError("a 4-bit cache has heads of 64 or 128 and groups of 32, 64 or 128 within a head, not %d and %d"
+                         % (head_dim, group_size))
+    return 68 * head_dim + 512 * (head_dim // group_size)
+
+
+def new_pool(num_pages, kv_heads, head_dim, group_size=64, layers=None, device="cuda"):
+    """uint8 [num_pages, kv_heads, record], or [layers, ...]; of any content: what no row was stored to is never seen."""
+    shape = (num_pages, kv_heads, record_bytes(head_dim, group_size))
+    return torch.empty(shape if layers is None else (layers,) + shape, dtype=torch.uint8, device=device)
+
+
+def _group_size(pool, head_dim):
+    for g in GROUPS:
+        if head_dim in (64, 128) and g <= head_dim and record_bytes(head_dim, g) == pool.shape[-1]:
+            return g
+    raise ValueError("a pool with records of %d bytes holds no heads of %d" % (pool.shape[-1], head_dim))
+
+
+def _check_cache(x, pool, pages, lengths, starts):
+    """The cache's tensors against rows or queries x [T, heads, D]; returns (T, B, group size)."""
+    if x.dim() != 3 or x.dtype != torch.float16 or not x.is_cuda:
+        raise ValueError("expected fp16 [tokens, heads, dim] on the device, got %s %s" % (x.dtype, tuple(x.shape)))
+    if pool.dim() != 3 or pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.shape[0] < 1:
+        raise ValueError("the pool must be a contiguous uint8 [pages, kv_heads, record] of at least one page")
+    for name, t, dims in (("pages", pages, 2), ("lengths", lengths, 1), ("starts", starts, 1)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+            raise ValueError("%s must be int32 with %d dimensions and adjacent elements" % (name, dims))
+    for t in (pool, pages, lengths, starts):
+        if t is not None and t.device != x.device:
+            raise ValueError("all tensors must be on %s" % x.device)
+    b = lengths.shape[0]
+    if pages.shape[0] != b or (starts is not None and starts.shape[0] != b + 1):
+        raise ValueError("%d lengths, but pages %s%s" % (b, tuple(pages.shape), "" if starts is None else
+                                                         " and starts %s" % (tuple(starts.shape),)))
+    t = x.shape[0]
+    if starts is None and (t % b if b else t):
+        raise ValueError("%d tokens cannot be dealt equally to %d sequences; pass starts" % (t, b))
+    return t, b, _group_size(pool, x.shape[-1])
+
+
+def _readable(x):
+    """x [T, heads, D] as the kernels can address it: rows of 16-byte chunks (a copy where it is not)."""
+    ok = x.stride(2) == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in x.stride()[:2])
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def _table_stride(pages):
+    return max(pages.stride(0), pages.shape[1]) if pages.shape[0] > 1 else pages.shape[1]
+
+
+def append(k, v, pool, pages, lengths, starts=None, values=False, stream=None):
+    """Quantise the rows k, v fp16 [T, kv_heads, D] (any token and head strides) of new tokens into their pages; they are
+    the last rows of their sequences.  With `values` returns (k_hat, v_hat) fp16 [T, kv_heads, D], what the cache holds
+    of them (of no defined content where a token has no page); otherwise None."""
+    t, b, g = _check_cache(k, pool, pages, lengths, starts)
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError("k and v must be alike, got %s %s and %s %s" % (k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
+    h, d = k.shape[1:]
+    if pool.shape[1] != h:
+        raise ValueError("rows of %d heads for a pool of %d" % (h, pool.shape[1]))
+    k, v = _readable(k), _readable(v)
+    hats = torch.empty((2, t, h, d), dtype=k.dtype, device=k.device).unbind(0) if values else (None, None)
+    strides = (ctypes.c_long * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with torch.cuda.device(k.device):
+        _check(capi.lib().sq_kv4_append(_ptr(k), _ptr(v), _ptr(hats[0]), _ptr(hats[1]), _ptr(pool), _ptr(pages), _ptr(lengths),
+                                        _ptr(starts), t, b, h, d, g, pool.shape[0], pages.shape[1], _table_stride(pages),
+                                        strides, _stream(stream)), "sq_kv4_append")
+    return hats if values else None
+
+
+def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out=None, stream=None):
+    """Causal attention of q fp16 [T, heads, D], the last tokens of their sequences (their own rows are in the cache), over
+    the cached rows; query head h reads key/value head h // (heads // kv_heads).  selected int32 [sequences, kv_heads,
+    count] (one token per sequence): over the rows of these pages only, as select_pages gives them.  Returns fp16
+    [T, heads, D]; a token that sees no row gets 0, tokens behind the last sequence's are left as `out` had them."""
+    t, b, g = _check_cache(q, pool, pages, lengths, starts)
+    hq, d = q.shape[1:]
+    h = pool.shape[1]
+    if hq % h:
+        raise ValueError("%d query heads over %d key/value heads" % (hq, h))
+    count = 0
+    if selected is not None:
+        if starts is not None or t != b:
+            raise ValueError("selected pages are for one token per sequence")
+        if selected.dtype != torch.int32 or not selected.is_contiguous() or selected.device != q.device \
+                or selected.dim() != 3 or tuple(selected.shape[:2]) != (b, h) or selected.shape[2] < 1:
+            raise ValueError("selected must be a contiguous int32 [sequences, kv_heads, count] on the device of q")
+        count = selected.shape[2]
+    q = _readable(q)
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous fp16 %s on the device of q" % (tuple(q.shape),))
+    # The workspace holds nothing between calls: one of its own for each, from the stream's (or a captured graph's) memory.
+    ws = torch.empty(capi.lib().sq_kv4_attention_workspace_bytes(d), dtype=torch.uint8, device=q.device) if t else None
+    with torch.cuda.device(q.device):
+        _check(capi.lib().sq_kv4_attention(_ptr(q), _ptr(out), _ptr(pool), _ptr(pages), _ptr(lengths), _ptr(starts),
+                                           _ptr(selected), t, b, hq, h, d, g, pool.shape[0], pages.shape[1],
+                                           _table_stride(pages), count, q.stride(0), q.stride(1), float(sm_scale), _ptr(ws),
+                                           0 if ws is None else ws.numel(), _stream(stream)), "sq_kv4_attention")
+    return out
+
+
+def select_pages(q, pool, pages, lengths, count, keep_first=1, keep_last=1, stream=None):
+    """int32 [sequences, kv_heads, count]: for the next token of each sequence, q fp16 [sequences, heads, D], the places of
+    the `count` pages that can hold the highest scores, ascending, -1 behind the last where there are fewer; the first
+    keep_first and the last keep_last are always among them."""
+    t, b, g = _check_cache(q, pool, pages, lengths, None)
+    hq, d = q.shape[1:]
+    h = pool.shape[1]
+    if t != b:
+        raise ValueError("pages are selected for one token per sequence, got %d tokens for %d" % (t, b))
+    if hq % h:
+        raise ValueError("%d query heads over %d key/value heads" % (hq, h))
+    if count < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > count:
+        raise ValueError("cannot keep the first %d and the last %d among %d pages" % (keep_first, keep_last, count))
+    q = _readable(q)
+    selected = torch.empty((b, h, count), dtype=torch.int32, device=q.device)
+    width = pages.shape[1]
+    need = capi.lib().sq_kv4_select_workspace_bytes(b, h, width) if width > count else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    with torch.cuda.device(q.device):
+        _check(capi.lib().sq_kv4_select(_ptr(q), _ptr(selected), _ptr(pool), _ptr(pages), _ptr(lengths), b, hq, h, d, g,
+                                        pool.shape[0], width, _table_stride(pages), int(count), int(keep_first),
+                                        int(keep_last), q.stride(0), q.stride(1), _ptr(ws), need, _stream(stream)),
+               "sq_kv4_select")
+    return selected
+
+
+def copy_pages(pool, src, dst, stream=None):
+    """Copy page src[i] to page dst[i], int32 on the device, in a pool [pages, ...] or in every layer of [layers, pages,
+    kv_heads, record].  No page may be a destination twice, or a destination and another pair's source."""
+    if pool.dim() not in (3, 4) or pool.dtype != torch.uint8 or not pool.is_contiguous() or not pool.is_cuda:
+        raise ValueError("the pool must be a contiguous uint8 [pages, kv_heads, record] or [layers, ...] on the device")
+    if src.shape != dst.shape or src.dim() != 1 or any(i.dtype != torch.int32 or i.device != pool.device
+                                                       or not i.is_contiguous() for i in (src, dst)):
+        raise ValueError("src and dst must be int32 vectors of one length on the device of the pool")
+    layers, (n, h, rec) = (1, pool.shape) if pool.dim() == 3 else (pool.shape[0], pool.shape[1:])
+    with torch.cuda.device(pool.device):
+        _check(capi.lib().sq_kv4_copy_pages(_ptr(pool), _ptr(src), _ptr(dst), src.numel(), n, layers, h * rec, n * h * rec,
+                                            _stream(stream)), "sq_kv4_copy_pages")
+
+
+class KV4Cache:
+    """The 4-bit cache of a model: pools of all layers, and which pages belong to which sequence.
+
+    Sequences are numbered 0 .. max_seqs - 1 (`add`, `fork`, `free`).  Rows are given room with `extend` (which also counts
+    them) or ahead of time with `reserve`; `append`, `attention` and `select_pages` then work on one layer for a list of
+    sequences, or for all of the first n (`seqs` an int).  Pages may be shared between sequences (`fork`): a page is copied
+    before a sequence that shares it gets rows in it.  `lengths` and `table` are the device's view of it and change in place; with
+    rows reserved a captured graph may count `lengths` up itself (`set_lengths` then brings the host's view after it)."""
+
+    def __init__(self, layers, num_pages, kv_heads, head_dim, group_size=64, max_seqs=8, max_rows=2048, device="cuda"):
+        self.pool = new_pool(num_pages, kv_heads, head_dim, group_size, layers, device)
+        self.layers, self.num_pages, self.max_seqs, self.max_rows = layers, num_pages, max_seqs, max_rows
+        self.kv_heads, self.head_dim, self.group_size = kv_heads, head_dim, group_size
+        self.width = (max_rows + PAGE - 1) // PAGE
+        self.table = torch.zeros((max_seqs, self.width), dtype=torch.int32, device=self.pool.device)
+        self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=self.pool.device)
+        self._pages = [None] * max_seqs  # of a sequence, in their order; None: no such sequence
+        self._rows = [0] * max_seqs
+        self._uses = [0] * num_pages
+        self._free = list(range(num_pages))  # a heap: the lowest page first
+
+    # ------------------------------------------------------------------------------------------------ bookkeeping
+
+    def _known(self, seq):
+        if not 0 <= seq < self.max_seqs or self._pages[seq] is None:
+            raise ValueError("no sequence %r" % (seq,))
+        return self._pages[seq]
+
+    def free_pages(self):
+        return len(self._free)
+
+    def rows(self, seq):
+        self._known(seq)
+        return self._rows[seq]
+
+    def pages(self, seq):
+        """The pages of a sequence, in their order."""
+        return list(self._known(seq))
+
+    def add(self):
+        """A new, empty sequence; returns its number (the lowest that is free)."""
+        for seq, pages in enumerate(self._pages):
+            if pages is None:
+                self._pages[seq] = []
+                self._rows[seq] = 0
+                self.lengths[seq:seq + 1].zero_()
+                return seq
+        raise RuntimeError("all %d sequences are in use" % self.max_seqs)
+
+    def _release(self, page):
+        self._uses[page] -= 1
+        if self._uses[page] == 0:
+            heapq.heappush(self._free, page)
+
+    def free(self, seq):
+        """End a sequence; pages that no other shares become free."""
+        for page in self._known(seq):
+            self._release(page)
+        self._pages[seq] = None
+        self._rows[seq] = 0
+        self.lengths[seq:seq + 1].zero_()
+
+    def fork(self, seq):
+        """A new sequence with the rows of `seq`, on the same pages; returns its number."""
+        pages = self._known(seq)
+        rows = self._rows[seq]
+        new = self.add()
+        used = pages[:(rows + PAGE - 1) // PAGE]
+        for page in used:
+            self._uses[page] += 1
+        self._pages[new] = list(used)
+        self._write([new])
+        self.set_lengths([new], [rows])
+        return new
+
+    def truncate(self, seq, rows):
+        """Keep the first `rows` rows of a sequence and release the pages behind them.  (The bounds of the page that becomes
+        its last still cover the rows that went, until its row 0 is stored again.)"""
+        pages = self._known(seq)
+        if not 0 <= rows <= self._rows[seq]:
+            raise ValueError("cannot keep %d of %d rows" % (rows, self._rows[seq]))
+        keep = (rows + PAGE - 1) // PAGE
+        for page in pages[keep:]:
+            self._release(page)
+        del pages[keep:]
+        self.set_lengths([seq], [rows])
+
+    def reserve(self, seqs, rows):
+        """Pages for the first rows[i] rows of seqs[i], of their own from the row behind the last one on."""
+        rows = self._per_sequence(seqs, rows)
+        fresh = {}   # sequence -> places that get a new page
+        for seq, n in zip(seqs, rows):
+            pages = self._known(seq)
+            if n > self.max_rows:
+                raise ValueError("%d rows in a cache of %d" % (n, self.max_rows))
+            if n > self._rows[seq]:
+                first = self._rows[seq] // PAGE
+                fresh[seq] = [j for j in range(first, (n + PAGE - 1) // PAGE) if j >= len(pages) or self._uses[pages[j]] > 1]
+        # a page shared by sequences of this very call is copied for all but the last of them
+        want = []
+        shared = dict()
+        for seq, places in fresh.items():
+            pages = self._pages[seq]
+            for j in places:
+                if j < len(pages):
+                    left = shared.get(pages[j], self._uses[pages[j]])
+                    if left == 1:
+                        continue
+                    shared[pages[j]] = left - 1
+                want.append((seq, j))
+        if len(want) > len(self._free):
+            raise RuntimeError("%d pages wanted, %d free of %d" % (len(want), len(self._free), self.num_pages))
+        src, dst = [], []
+        for seq, j in want:
+            pages = self._pages[seq]
+            page = heapq.heappop(self._free)
+            self._uses[page] = 1
+            if j < len(pages):
+                if j * PAGE < self._rows[seq]:  # it holds rows
+                    src.append(pages[j])
+                    dst.append(page)
+                self._release(pages[j])
+                pages[j] = page
+            else:
+                pages.append(page)
+        if src:
+            copy_pages(self.pool, *self._vectors(src, dst))
+        if want:
+            self._write(sorted({seq for seq, _ in want}))
+
+    def extend(self, seqs, rows):
+        """Room for rows[i] (or `rows`) more rows of seqs[i], and count them."""
+        more = self._per_sequence(seqs, rows)
+        total = [self.rows(seq) + n for seq, n in zip(seqs, more)]
+        if any(n < 0 for n in more):
+            raise ValueError("a sequence shrinks by truncate")
+        self.reserve(seqs, total)
+        self.set_lengths(seqs, total)
+
+    def set_lengths(self, seqs, rows):
+        """Count rows that have pages already."""
+        rows = self._per_sequence(seqs, rows)
+        for seq, n in zip(seqs, rows):
+            if not 0 <= n <= len(self._known(seq)) * PAGE:
+                raise ValueError("%d rows on %d pages" % (n, len(self._pages[seq])))
+        for seq, n in zip(seqs, rows):
+            self._rows[seq] = n
+        at, n = self._vectors(seqs, rows)
+        self.lengths[at.long()] = n
+
+    def compact(self):
+        """Move the pages in use to the front of the pool; returns how many they are.  Behind it the pool's tail is free."""
+        used = sum(1 for n in self._uses if n)
+        holes = [p for p in range(used) if not self._uses[p]]
+        tail = [p for p in range(used, self.num_pages) if self._uses[p]]
+        if not tail:
+            return used
+        to = dict(zip(tail, holes))
+        copy_pages(self.pool, *self._vectors(list(to), list(to.values())))
+        for a, b in to.items():
+            self._uses[b], self._uses[a] = self._uses[a], 0
+        touched = []
+        for seq, pages in enumerate(self._pages):
+            if pages and any(p in to for p in pages):
+                self._pages[seq] = [to.get(p, p) for p in pages]
+                touched.append(seq)
+        self._free = list(range(used, self.num_pages))
+        self._write(touched)
+        return used
+
+    @staticmethod
+    def _per_sequence(seqs, rows):
+        rows = [rows] * len(seqs) if isinstance(rows, int) else list(rows)
+        if len(rows) != len(seqs) or len(set(seqs)) != len(seqs):
+            raise ValueError("%d row counts for the sequences %s" % (len(rows), list(seqs)))
+        return rows
+
+    def _vectors(self, *lists):
+        return torch.tensor(lists, dtype=torch.int32).to(self.pool.device).unbind(0)
+
+    def _write(self, seqs):
+        """The device's table of these sequences."""
+        rows = torch.zeros((len(seqs), self.width), dtype=torch.int32)
+        for i, seq in enumerate(seqs):
+            rows[i, :len(self._pages[seq])] = torch.tensor(self._pages[seq], dtype=torch.int32)
+        self.table[torch.tensor(seqs, device=self.table.device)] = rows.to(self.table.device)
+
+    # -------------------------------------------------------------------------------------------------- operators
+
+    def batch(self, seqs):
+        """(pages, lengths) of these sequences; views of the cache's own where seqs is an int n (sequences 0 .. n - 1)."""
+        if isinstance(seqs, int):
+            return self.table[:seqs], self.lengths[:seqs]
+        at = torch.tensor(list(seqs), device=self.table.device)
+        return self.table[at], self.lengths[at]
+
+    def append(self, layer, k, v, seqs, starts=None, values=False):
+        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
+        return append(k, v, self.pool[layer], pages, lengths, starts, values)
+
+    def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None):
+        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
+        return attention(q, self.pool[layer], pages, lengths, sm_scale, starts, selected, out)
+
+    def select_pages(self, layer, q, count, seqs, keep_first=1, keep_last=1):
+        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
+        return select_pages(q, self.pool[layer], pages, lengths, count, keep_first, keep_last)

@@ -1,0 +1,192 @@
+"""The 4-bit cache without a GPU: refusals of the C ABI before any launch, sizes, and the oracle against itself."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_oracle as ko
+
+SIZES = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)]
+
+
+@pytest.mark.parametrize("d,g", SIZES)
+def test_every_code_and_scale_has_its_own_place(d, g):
+    p = ko.places(d, g)
+    nibbles = np.concatenate([(2 * p["kb"] + p["ks"] // 4).ravel(), (2 * p["vb"] + p["vs"] // 4).ravel()])
+    assert np.array_equal(np.sort(nibbles), np.arange(2 * 64 * d))  # all nibbles of the first 64 D bytes, each once
+    halves = np.unique(np.concatenate([(p[n] + o).ravel() for n in ("ksm", "vsm") for o in (0, 8)]))
+    assert np.array_equal(halves, 64 * d + 2 * np.arange(256 * (d // g)))
+    for n in ("ksm", "vsm"):
+        assert np.array_equal(p[n][:, ::g].repeat(g, 1), p[n])
+    assert ko.record_bytes(d, g) == 64 * d + 512 * (d // g) + 4 * d
+
+
+def test_quantisation_of_the_oracle():
+    x = np.array([[0.0, 1.5, 15.0, 7.5] * 8, [2.0] * 32, [-3.0, 12.0] * 16, [0.0, np.nan] + [1.0] * 30,
+                  [np.inf] + [0.0] * 31], dtype=np.float16)
+    c, s, m = ko.quantise(x, 32)
+    assert c[0, :4].tolist() == [0, 2, 15, 8]  # 1.5 and 7.5 are halves: to the even code
+    assert np.all(c[1] == 0) and np.all(s[1] == 0) and np.all(m[1] == 2.0)
+    assert np.all(s[2] == 1.0) and np.all(m[2] == -3.0) and c[2, :2].tolist() == [0, 15]
+    with np.errstate(invalid="ignore"):
+        assert np.all(np.isnan(ko.values(c, s, m)[3:]))
+
+
+@pytest.fixture(scope="module")
+def L(built_lib):
+    from sqamd import capi
+    return capi.lib()
+
+
+@pytest.fixture(scope="module")
+def p():
+    buf = np.zeros(64, dtype=np.uint8)
+    test_p = ctypes.c_void_p(buf.ctypes.data - buf.ctypes.data % 16 + 16)
+    test_p.keep = buf
+    return test_p
+
+
+def test_record_bytes(L):
+    from sqamd import kv4
+    for d, g in SIZES:
+        assert L.sq_kv4_record_bytes(d, g) == kv4.record_bytes(d, g) == ko.record_bytes(d, g)
+    for d, g in ((96, 32), (64, 128), (128, 16), (0, 0), (128, 48)):
+        assert L.sq_kv4_record_bytes(d, g) == 0
+        with pytest.raises(ValueError):
+            kv4.record_bytes(d, g)
+
+
+def test_append_refuses(L, p):
+    from sqamd import capi
+    strides = (ctypes.c_long * 4)(1024, 128, 1024, 128)
+
+    def call(k=p, v=p, kh=None, vh=None, pool=p, pages=p, lengths=p, starts=None, T=4, B=4, H=8, D=128, g=64, n=10, width=5,
+             stride=5, st=strides):
+        return L.sq_kv4_append(k, v, kh, vh, pool, pages, lengths, starts, T, B, H, D, g, n, width, stride, st, None)
+
+    odd = ctypes.c_void_p(p.value + 2)
+    null, shape, group, misaligned = (capi.SQ_ERR_NULL_POINTER, capi.SQ_ERR_BAD_SHAPE, capi.SQ_ERR_BAD_GROUP,
+                                      capi.SQ_ERR_MISALIGNED)
+    assert call(T=0) == capi.SQ_OK and call(T=0, B=0) == capi.SQ_OK and call(width=0, stride=0) == capi.SQ_OK
+    for bad in (dict(k=None), dict(v=None), dict(pool=None), dict(pages=None), dict(lengths=None), dict(kh=p), dict(vh=p),
+                dict(st=None)):
+        assert call(**bad) == null, bad
+    for bad in (dict(T=-1), dict(B=-1), dict(H=0), dict(D=96), dict(n=0), dict(width=-1), dict(width=6), dict(T=5),
+                dict(st=(ctypes.c_long * 4)(-8, 128, 1024, 128)), dict(T=1 << 28, B=1 << 28)):
+        assert call(**bad) == shape, bad
+    for bad in (dict(g=16), dict(g=128, D=64), dict(g=0)):
+        assert call(**bad) == group, bad
+    for bad in (dict(k=odd), dict(v=odd), dict(kh=odd, vh=odd), dict(pool=odd), dict(lengths=odd), dict(starts=odd),
+                dict(st=(ctypes.c_long * 4)(1024, 128, 1020, 128))):
+        assert call(**bad) == misaligned, bad
+
+
+def test_attention_refuses(L, p):
+    from sqamd import capi
+
+    def call(q=p, out=p, pool=p, pages=p, lengths=p, starts=None, sel=None, T=4, B=4, Hq=16, H=8, D=128, g=64, n=10, width=5,
+             stride=5, count=0, qt=2048, qh=128, ws=None, size=0):
+        return L.sq_kv4_attention(q, out, pool, pages, lengths, starts, sel, T, B, Hq, H, D, g, n, width, stride, count, qt, qh,
+                                  0.1, ws, size, None)
+
+    odd = ctypes.c_void_p(p.value + 2)
+    assert call(T=0) == capi.SQ_OK and call(T=0, B=0) == capi.SQ_OK
+    for bad in (dict(q=None), dict(out=None), dict(pool=None), dict(lengths=None), dict(pages=None)):
+        assert call(**bad) == capi.SQ_ERR_NULL_POINTER, bad
+    for bad in (dict(Hq=12), dict(Hq=0), dict(T=6), dict(D=80), dict(n=0), dict(stride=4), dict(qt=-8), dict(sel=p, count=0),
+                dict(sel=p, count=2, starts=p), dict(sel=p, count=2, T=8), dict(T=1 << 27, B=1, Hq=64, H=1)):
+        assert call(**bad) == capi.SQ_ERR_BAD_SHAPE, bad
+    for bad in (dict(q=odd), dict(out=odd), dict(qh=100), dict(sel=odd, count=2)):
+        assert call(**bad) == capi.SQ_ERR_MISALIGNED, bad
+    assert call(g=256) == capi.SQ_ERR_BAD_GROUP
+    assert call(ws=p, size=16) == capi.SQ_ERR_WORKSPACE
+    assert call(ws=odd, size=1 << 30) == capi.SQ_ERR_WORKSPACE
+    assert L.sq_kv4_attention_workspace_bytes(96) == 0 < L.sq_kv4_attention_workspace_bytes(64) \
+        < L.sq_kv4_attention_workspace_bytes(128)
+
+
+def test_select_refuses(L, p):
+    from sqamd import capi
+
+    def call(q=p, sel=p, B=4, Hq=16, H=8, D=128, g=64, n=10, width=50, stride=50, count=4, first=1, last=1, qt=2048, qh=128,
+             ws=p, size=1 << 20):
+        return L.sq_kv4_select(q, sel, p, p, p, B, Hq, H, D, g, n, width, stride, count, first, last, qt, qh, ws, size, None)
+
+    assert call(B=0) == capi.SQ_OK
+    for bad in (dict(count=0), dict(count=1), dict(first=-1), dict(last=-1), dict(first=4), dict(width=16385, stride=16385),
+                dict(B=1 << 14), dict(Hq=20), dict(first=2 ** 31 - 1, last=2 ** 31 - 1)):
+        assert call(**bad) == capi.SQ_ERR_BAD_SHAPE, bad
+    for bad in (dict(q=None), dict(sel=None)):
+        assert call(**bad) == capi.SQ_ERR_NULL_POINTER, bad
+    need = L.sq_kv4_select_workspace_bytes(4, 8, 50)
+    assert need > 0 and call(ws=None) == capi.SQ_ERR_WORKSPACE and call(size=need - 1) == capi.SQ_ERR_WORKSPACE
+    assert L.sq_kv4_select_workspace_bytes(0, 8, 50) == 0
+
+
+def test_copy_refuses(L, p):
+    from sqamd import capi
+
+    def call(pool=p, src=p, dst=p, n=3, pages=8, layers=2, page=4864, layer=8 * 4864):
+        return L.sq_kv4_copy_pages(pool, src, dst, n, pages, layers, page, layer, None)
+
+    assert call(n=0) == capi.SQ_OK
+    for bad in (dict(n=-1), dict(pages=0), dict(layers=0), dict(page=0), dict(page=4860), dict(layer=8 * 4864 - 16),
+                dict(layer=8 * 4864 + 8), dict(layers=1 << 16)):
+        assert call(**bad) == capi.SQ_ERR_BAD_SHAPE, bad
+    for bad in (dict(pool=None), dict(src=None), dict(dst=None)):
+        assert call(**bad) == capi.SQ_ERR_NULL_POINTER, bad
+    assert call(src=ctypes.c_void_p(p.value + 2)) == capi.SQ_ERR_MISALIGNED
+
+
+def test_python_refuses_host_tensors():
+    from sqamd import kv4
+    pool = kv4.new_pool(4, 2, 64, 32, device="cpu")
+    pages, lengths = torch.zeros((1, 4), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x = torch.zeros((1, 2, 64), dtype=torch.float16)
+    for call in (lambda: kv4.append(x, x, pool, pages, lengths), lambda: kv4.attention(x, pool, pages, lengths, 1.0),
+                 lambda: kv4.select_pages(x, pool, pages, lengths, 2), lambda: kv4.copy_pages(pool, lengths, lengths)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_bookkeeping_without_copies():
+    # sequences that share nothing need no device work but the tables': the host's side runs anywhere
+    from sqamd import kv4
+    c = kv4.KV4Cache(2, 10, 1, 64, 64, max_seqs=3, max_rows=300, device="cpu")
+    a, b = c.add(), c.add()
+    c.extend([a, b], [130, 1])
+    assert c.pages(a) == [0, 1, 2] and c.pages(b) == [3] and c.free_pages() == 6
+    assert c.lengths.tolist() == [130, 1, 0] and c.table[a, :3].tolist() == [0, 1, 2]
+    c.extend([b], 63)
+    assert c.pages(b) == [3]
+    c.extend([b], 1)
+    assert c.pages(b) == [3, 4]
+    c.truncate(a, 64)
+    assert c.pages(a) == [0] and c.rows(a) == 64 and c.free_pages() == 7
+    with pytest.raises(ValueError):
+        c.truncate(a, 65)
+    with pytest.raises(ValueError):
+        c.extend([a], 300)
+    with pytest.raises(ValueError):
+        c.extend([a, a], 1)
+    with pytest.raises(ValueError):
+        c.rows(2)
+    f = c.fork(a)  # a full page: shared, no copy
+    assert c.pages(f) == [0] and c.free_pages() == 7
+    c.extend([f, a], 1)
+    assert c.pages(f) == [0, 1] and c.pages(a) == [0, 2] and c.free_pages() == 5
+    c.free(a)
+    assert c.free_pages() == 6
+    c.free(f)
+    assert c.free_pages() == 8 and c.pages(b) == [3, 4]
+    with pytest.raises(ValueError):
+        c.free(f)
+    big, more = c.add(), c.add()
+    c.reserve([big], 300)
+    assert c.free_pages() == 3 and c.rows(big) == 0
+    with pytest.raises(RuntimeError):
+        c.reserve([more, b], [130, 130])
+    assert c.free_pages() == 3 and c.pages(more) == [] and c.pages(b) == [3, 4]
+    with pytest.raises(RuntimeError):
+        c.add()
