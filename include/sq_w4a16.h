@@ -501,10 +501,10 @@ int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* 
  * selected   NULL, or int32 [B][H][count] with T == B and no starts: the token sees only the rows of these pages (their
  *            places in the sequence).  The first min(count, pages of the sequence) entries are read; one outside the
  *            sequence is no page; one that stands there twice counts twice.
- * workspace  NULL, or sq_kv4_attention_workspace_bytes(D) bytes, 16-byte aligned, of any content: a sequence's pages are
+ * workspace  NULL, or sq_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, of any content: a sequence's pages are
  *            then dealt to several workgroups where there are few, and a second launch joins their shares.  Not shared by
- *            calls that may run at the same time. */
-size_t sq_kv4_attention_workspace_bytes(int D);
+ *            calls that may run at the same time.  The size is 0 where no sequence can be long enough. */
+size_t sq_kv4_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int width, int count);
 int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
                      const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
                      int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, void* workspace,

@@ -495,6 +495,117 @@ c10::optional<at::Tensor> decode_attention(const at::Tensor& q, const at::Tensor
     return out;
 }
 
+// The 4-bit key/value cache (sqamd/kv4.py, which does what these leave to it: copies of rows that cannot be read as they
+// lie, and the complaints).  Workspaces hold nothing between calls, so each call takes its own from the caching allocator:
+// stream-ordered there, a captured graph's own where one is being captured.
+bool kv4_rows(const at::Tensor& x) {
+    return x.dim() == 3 && x.is_cuda() && x.scalar_type() == at::kHalf && x.stride(2) == 1 && x.stride(0) % 8 == 0 &&
+           x.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+}
+bool kv4_ints(const at::Tensor& t, const at::Tensor& like, int64_t dims) {
+    return t.scalar_type() == at::kInt && t.device() == like.device() && t.dim() == dims && t.numel() > 0 && t.stride(-1) == 1;
+}
+// Whether the cache's tensors fit rows x; the group size, tokens, sequences and the table's pitch.
+bool kv4_fits(const at::Tensor& x, const at::Tensor& pool, const at::Tensor& pages, const at::Tensor& lengths,
+              const c10::optional<at::Tensor>& starts, int& g, int64_t& pitch) {
+    if (!kv4_rows(x) || x.numel() == 0 || pool.dim() != 3 || pool.scalar_type() != at::kByte || pool.device() != x.device() ||
+        !pool.is_contiguous() || pool.size(0) < 1 || pool.size(0) >= (1LL << 31) || !kv4_ints(pages, x, 2) ||
+        !kv4_ints(lengths, x, 1))
+        return false;
+    const int64_t B = lengths.size(0), T = x.size(0);
+    if (pages.size(0) != B || T >= (1LL << 31) || pages.size(1) >= (1LL << 24)) return false;
+    if (starts.has_value() ? !kv4_ints(*starts, x, 1) || starts->size(0) != B + 1 : T % B != 0) return false;
+    pitch = B > 1 ? pages.stride(0) : pages.size(1);
+    if (pitch < pages.size(1) || pitch >= (1LL << 31)) return false;
+    for (g = 32; g <= 128; g *= 2)
+        if (sq_kv4_record_bytes((int)x.size(2), g) == pool.size(2)) return true;
+    return false;
+}
+
+c10::optional<std::vector<at::Tensor>> kv4_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& pool,
+                                                  const at::Tensor& pages, const at::Tensor& lengths,
+                                                  const c10::optional<at::Tensor>& starts, bool values) {
+    int g;
+    int64_t pitch;
+    if (!kv4_fits(k, pool, pages, lengths, starts, g, pitch) || !kv4_rows(v) || v.sizes() != k.sizes() ||
+        v.device() != k.device() || pool.size(1) != k.size(1))
+        return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(k.device());
+    std::vector<at::Tensor> hats;
+    if (values) hats = {at::empty(k.sizes(), k.options()), at::empty(k.sizes(), k.options())};
+    const long strides[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+    const int rc = sq_kv4_append(k.data_ptr(), v.data_ptr(), values ? hats[0].data_ptr() : nullptr,
+                                 values ? hats[1].data_ptr() : nullptr, pool.data_ptr(), pages.data_ptr(), lengths.data_ptr(),
+                                 starts.has_value() ? starts->data_ptr() : nullptr, (int)k.size(0), (int)lengths.size(0),
+                                 (int)k.size(1), (int)k.size(2), g, (int)pool.size(0), (int)pages.size(1), (int)pitch, strides,
+                                 current_stream(k));
+    if (rc != SQ_OK) return c10::nullopt;
+    return hats;
+}
+
+c10::optional<at::Tensor> kv4_attention(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& pages,
+                                        const at::Tensor& lengths, double sm_scale, const c10::optional<at::Tensor>& starts,
+                                        const c10::optional<at::Tensor>& selected, const c10::optional<at::Tensor>& into) {
+    int g;
+    int64_t pitch;
+    if (!kv4_fits(q, pool, pages, lengths, starts, g, pitch)) return c10::nullopt;
+    const int64_t T = q.size(0), B = lengths.size(0), Hq = q.size(1), H = pool.size(1), D = q.size(2);
+    if (selected.has_value() && (starts.has_value() || T != B || !kv4_ints(*selected, q, 3) || !selected->is_contiguous() ||
+                                 selected->size(0) != B || selected->size(1) != H || selected->size(2) >= (1LL << 24)))
+        return c10::nullopt;
+    if (into.has_value() && (into->sizes() != q.sizes() || into->scalar_type() != at::kHalf || into->device() != q.device() ||
+                             !into->is_contiguous()))
+        return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = into.has_value() ? *into : at::empty({T, Hq, D}, q.options());
+    const int count = selected.has_value() ? (int)selected->size(2) : 0;
+    const size_t need = sq_kv4_attention_workspace_bytes((int)T, (int)B, (int)Hq, (int)H, (int)D, (int)pages.size(1), count);
+    at::Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+    const int rc = sq_kv4_attention(q.data_ptr(), out.data_ptr(), pool.data_ptr(), pages.data_ptr(), lengths.data_ptr(),
+                                    starts.has_value() ? starts->data_ptr() : nullptr,
+                                    selected.has_value() ? selected->data_ptr() : nullptr, (int)T, (int)B, (int)Hq, (int)H, (int)D,
+                                    g, (int)pool.size(0), (int)pages.size(1), (int)pitch, count, q.stride(0), q.stride(1),
+                                    (float)sm_scale, need ? ws.data_ptr() : nullptr, need, current_stream(q));
+    if (rc != SQ_OK) return c10::nullopt;
+    return out;
+}
+
+c10::optional<at::Tensor> kv4_select(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& pages,
+                                     const at::Tensor& lengths, int64_t count, int64_t keep_first, int64_t keep_last) {
+    int g;
+    int64_t pitch;
+    if (!kv4_fits(q, pool, pages, lengths, c10::nullopt, g, pitch)) return c10::nullopt;
+    const int64_t B = lengths.size(0), H = pool.size(1), width = pages.size(1);
+    if (q.size(0) != B || count < 1 || count >= (1LL << 24) || keep_first < 0 || keep_last < 0 || keep_first + keep_last > count)
+        return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(q.device());
+    at::Tensor selected = at::empty({B, H, count}, pages.options());
+    const size_t need = width > count ? sq_kv4_select_workspace_bytes((int)B, (int)H, (int)width) : 0;
+    at::Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+    const int rc = sq_kv4_select(q.data_ptr(), selected.data_ptr(), pool.data_ptr(), pages.data_ptr(), lengths.data_ptr(), (int)B,
+                                 (int)q.size(1), (int)H, (int)q.size(2), g, (int)pool.size(0), (int)width, (int)pitch, (int)count,
+                                 (int)keep_first, (int)keep_last, q.stride(0), q.stride(1), need ? ws.data_ptr() : nullptr, need,
+                                 current_stream(q));
+    if (rc != SQ_OK) return c10::nullopt;
+    return selected;
+}
+
+bool kv4_copy_pages(const at::Tensor& pool, const at::Tensor& src, const at::Tensor& dst) {
+    if ((pool.dim() != 3 && pool.dim() != 4) || !pool.is_cuda() || pool.scalar_type() != at::kByte || !pool.is_contiguous() ||
+        pool.numel() == 0 || !kv4_ints(src, pool, 1) || !kv4_ints(dst, pool, 1) || src.size(0) != dst.size(0))
+        return false;
+    const int64_t n = pool.size(-3), layers = pool.dim() == 4 ? pool.size(0) : 1, page = pool.size(-2) * pool.size(-1);
+    if (n >= (1LL << 31) || layers >= (1LL << 31) || src.size(0) >= (1LL << 31)) return false;
+    c10::DeviceGuard guard(pool.device());
+    return sq_kv4_copy_pages(pool.data_ptr(), src.data_ptr(), dst.data_ptr(), (int)src.size(0), (int)n, (int)layers, (size_t)page,
+                             (size_t)(page * n), current_stream(pool)) == SQ_OK;
+}
+
 // Same with an explicit kernel id (SQ_ALGO_* | tuning word << 8); for tests and benchmarks.
 at::Tensor gemm_awq_algo(at::Tensor I, at::Tensor W, at::Tensor W_zeros_scales, const int N, const int group_size,
                          const int algo) {
@@ -652,6 +763,10 @@ PYBIND11_MODULE(quant, m) {
     m.def("walinear_forward", &walinear_forward);
     m.def("lut_attention", &lut_attention);
     m.def("decode_attention", &decode_attention);
+    m.def("kv4_append", &kv4_append);
+    m.def("kv4_attention", &kv4_attention);
+    m.def("kv4_select", &kv4_select);
+    m.def("kv4_copy_pages", &kv4_copy_pages);
     m.def("gemm_awq_silu_dot_ut", &gemm_awq_silu_dot_ut, py::arg("I"), py::arg("W1") = py::none(),
           py::arg("W2") = py::none(), py::arg("ZS1") = py::none(), py::arg("ZS2") = py::none(),
           py::arg("W13") = py::none(), py::arg("ZS13") = py::none(), py::arg("M"), py::arg("N"), py::arg("K"),

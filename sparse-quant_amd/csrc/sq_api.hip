@@ -1155,7 +1155,10 @@ int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* 
                                              v, k_hat, v_hat, D, group_size, strides, static_cast<hipStream_t>(stream)));
 }
 
-size_t sq_kv4_attention_workspace_bytes(int D) { return D == 64 || D == 128 ? sq::kv4_attention_workspace_bytes(D) : 0; }
+size_t sq_kv4_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int width, int count) {
+    if (T <= 0 || B <= 0 || H <= 0 || Hq <= 0 || Hq % H != 0 || (D != 64 && D != 128) || width < 0 || count < 0) return 0;
+    return sq::kv4_attention_workspace_bytes(T, B, Hq / H, D, count > 0 && count < width ? count : width);
+}
 
 int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
                      const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
@@ -1169,7 +1172,9 @@ int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pag
     if (!q || !out) return SQ_ERR_NULL_POINTER;
     if (!aligned16(q) || !aligned16(out) || (q_tstride | q_hstride) % 8 != 0 || (reinterpret_cast<uintptr_t>(selected) & 3u))
         return SQ_ERR_MISALIGNED;
-    if (workspace && (!aligned16(workspace) || workspace_bytes < sq::kv4_attention_workspace_bytes(D))) return SQ_ERR_WORKSPACE;
+    if (workspace && (!aligned16(workspace) ||
+                      workspace_bytes < sq_kv4_attention_workspace_bytes(T, B, Hq, H, D, width, selected ? count : 0)))
+        return SQ_ERR_WORKSPACE;
     return launch_code(sq::launch_kv4_attention(kv4_cache(pool, pages, lengths, starts, T, B, H, num_pages, width, page_stride),
                                                 q, out, static_cast<const int*>(selected), workspace, D, group_size, Hq / H,
                                                 selected ? count : 0, q_tstride, q_hstride, sm_scale,

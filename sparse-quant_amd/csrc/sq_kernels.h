@@ -140,7 +140,7 @@ hipError_t launch_kv4_copy_pages(void* pool, const int* src, const int* dst, int
 constexpr int KV4_SELECT_MAX_PAGES = 16384;  // their keys lie in LDS
 hipError_t launch_kv4_select(const Kv4Cache& c, const void* q, void* selected, void* workspace, int D, int g, int share,
                              long q_ts, long q_hs, int count, int keep_first, int keep_last, hipStream_t st);
-size_t kv4_attention_workspace_bytes(int D);
+size_t kv4_attention_workspace_bytes(int T, int B, int share, int D, int pages);  // pages: the most of a sequence
 hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, const int* selected, void* workspace, int D, int g,
                                 int share, int count, long q_ts, long q_hs, float sm_scale, hipStream_t st);
 

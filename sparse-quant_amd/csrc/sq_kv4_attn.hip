@@ -27,6 +27,9 @@ namespace sq {
 
 namespace {
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 struct Kv4AttnArgs {
     Kv4Cache c;
     const half_t* q;
@@ -41,9 +44,10 @@ struct Kv4AttnArgs {
 
 // How a launch's work is dealt.  A tile is R of the rows (token, query head) of a sequence and key/value head; a
 // workgroup takes one tile over a share of its pages.  The share's length follows from the lengths on the device: the pages
-// of all tiles over 2^log_wgs workgroups, `least` at the fewest.
+// of all tiles over 256 per_cu workgroups, `least` at the fewest.
 struct Deal {
-    int log_wgs, least;
+    int per_cu, least;
+    __host__ __device__ int wgs() const { return 256 * per_cu; }
 };
 struct Piece {
     int b, tile, head, share, shares;  // share of how many
@@ -53,159 +57,227 @@ struct Piece {
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// A sequence's tokens, rows, pages and tiles.
+struct Sizes {
+    int first, count, len, pages, tiles;
+};
 template <int R>
-__device__ __forceinline__ int deal_sizes(const Kv4AttnArgs& a, int b, int& first, int& count, int& len, int& pages) {
-    kv4_tokens(a.c, b, first, count);
-    len = kv4_length(a.c, b);
-    pages = ceil_div(len, KV4_PAGE);
-    if (a.selected && pages > a.count) pages = a.count;
-    return ceil_div(count * a.share, R) * a.c.H;  // tiles
+__device__ __forceinline__ Sizes sizes_of(const Kv4AttnArgs& a, int b) {
+    Sizes s = {0, 0, 0, 0, 0};
+    if (b < a.c.B) {
+        kv4_tokens(a.c, b, s.first, s.count);
+        s.len = kv4_length(a.c, b);
+        s.pages = ceil_div(s.len, KV4_PAGE);
+        if (a.selected) s.pages = imin(s.pages, a.count);
+        s.tiles = ceil_div(s.count * a.share, R) * a.c.H;
+    }
+    return s;
 }
 
-// The piece of workgroup `index` (SPLIT: of the index-th tile among those that are shared), by every wave alone.
+// The piece of workgroup `index` (SPLIT: of the index-th tile among those that are shared), by every wave alone: lane i
+// looks at sequence 64 k + i.
 template <int R, bool SPLIT>
 __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int index, Piece& out) {
     const int lane = threadIdx.x & 63;
     const int B = a.c.B;
-    int least = d.least;
+    Sizes s = sizes_of<R>(a, lane);
+    int least = 1 << 30;
     if (a.ws) {
         unsigned long long units = 0;
-        for (int b = lane; b < B; b += 64) {
-            int f, n, l, p;
-            const int tiles = deal_sizes<R>(a, b, f, n, l, p);
-            units += (unsigned long long)tiles * p;
+        for (int b0 = 0; b0 < B; b0 += 64) {
+            const Sizes t = b0 ? sizes_of<R>(a, b0 + lane) : s;
+            const unsigned long long mine = (unsigned long long)t.tiles * t.pages;
+            units += (unsigned)wave_sum((int)(mine & 0xffff)) + ((unsigned long long)(unsigned)wave_sum((int)(mine >> 16)) << 16);
         }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) units += __shfl_xor(units, x, 64);
-        const int even = (int)((units + (1ull << d.log_wgs) - 1) >> d.log_wgs);
-        least = even > least ? even : least;
-    } else {
-        least = 1 << 30;
+        const unsigned even = (unsigned)ceil_div((int)((units + 255) >> 8), d.per_cu);  // (T * Hq <= 2^30: at most 2^48 pages)
+        least = even > (unsigned)d.least ? (int)even : d.least;
     }
     int slots = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
-        const int b = b0 + lane;
-        int f = 0, n = 0, l = 0, p = 0, tiles = 0;
-        if (b < B) tiles = deal_sizes<R>(a, b, f, n, l, p);
-        const int shares = p > least ? ceil_div(p, least) : 1;
-        const int mine = SPLIT ? (shares > 1 ? tiles : 0) : tiles * shares;
+        if (b0) s = sizes_of<R>(a, b0 + lane);
+        const int shares = s.pages > least ? ceil_div(s.pages, least) : 1;
+        const int mine = SPLIT ? (shares > 1 ? s.tiles : 0) : s.tiles * shares;
         const int upto = wave_scan(mine);
-        const int taken = shares > 1 ? tiles * shares : 0;
+        const int taken = shares > 1 ? s.tiles * shares : 0;
         const int slots_upto = wave_scan(taken);
         const unsigned long long past = __ballot(upto > index);
         if (past) {
             const int at = __ffsll(past) - 1;
-            const int rest = index - __shfl(upto - mine, at, 64);
-            out.shares = __shfl(shares, at, 64);
-            const int tile = SPLIT ? rest : rest / out.shares;
+            const int rest = index - __builtin_amdgcn_readlane(upto - mine, at);
+            out.shares = __builtin_amdgcn_readlane(shares, at);
+            const int tile = SPLIT || out.shares == 1 ? rest : rest / out.shares;
             out.b = b0 + at;
             out.share = SPLIT ? 0 : rest - tile * out.shares;
             out.head = tile % a.c.H;
             out.tile = tile / a.c.H;
-            out.slot = slots + __shfl(slots_upto - taken, at, 64) + tile * out.shares + out.share;
-            out.first = __shfl(f, at, 64);
-            out.count = __shfl(n, at, 64);
-            out.len = __shfl(l, at, 64);
+            out.slot = slots + __builtin_amdgcn_readlane(slots_upto - taken, at) + tile * out.shares + out.share;
+            out.first = __builtin_amdgcn_readlane(s.first, at);
+            out.count = __builtin_amdgcn_readlane(s.count, at);
+            out.len = __builtin_amdgcn_readlane(s.len, at);
             return true;
         }
-        index -= __shfl(upto, 63, 64);
-        slots += __shfl(slots_upto, 63, 64);
+        index -= __builtin_amdgcn_readlane(upto, 63);
+        slots += __builtin_amdgcn_readlane(slots_upto, 63);
     }
     return false;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) v = fmaxf(v, __shfl_xor(v, x, 64));
-    return v;
+template <int CTRL>
+__device__ __forceinline__ float row_move(float v) {
+    return bit_cast<float>(__builtin_amdgcn_update_dpp(0, bit_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
-__device__ __forceinline__ float rows_sum(float v) {  // over the four lanes of a query
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+// A value and that of the lane 16 (32) away, on every lane.
+__device__ __forceinline__ void pair16(float v, float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+    a = bit_cast<float>((uint32_t)r[0]);
+    b = bit_cast<float>((uint32_t)r[1]);
+}
+__device__ __forceinline__ void pair32(float v, float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+    a = bit_cast<float>((uint32_t)r[0]);
+    b = bit_cast<float>((uint32_t)r[1]);
+}
+__device__ __forceinline__ float rows_sum(float v) {  // over the four lanes of a column
+    float a, b;
+    pair16(v, a, b);
+    pair32(a + b, a, b);
+    return a + b;
 }
 __device__ __forceinline__ float rows_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    float a, b;
+    pair16(v, a, b);
+    pair32(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, row_move<0x121>(v));  // row_ror:1
+    v = fmaxf(v, row_move<0x122>(v));
+    v = fmaxf(v, row_move<0x124>(v));
+    v = fmaxf(v, row_move<0x128>(v));
+    return rows_max(v);
 }
 
-constexpr int KA_WAVES = 4;
-constexpr int KA_ROWS = 16;
 constexpr float KA_LAZY = 8.f;  // the softmax's reference moves when a score is 2^8 beyond it
 
-// Half a page (32 rows) as a lane holds it.
-template <int D, int G>
-struct Half {
-    uint32_t k[2][D / 32];  // [16 rows][words of the lane's row and chunk]
-    u32x4_t v[2];
-    half8_t ksm[2][G], vsm[2][G];  // scales and minima of four rows
+// The kernel for few rows.  A workgroup's waves take units of 16 max(2, PACK) rows of the cache in turn, each with a softmax
+// of its own, and join them in LDS.
+//
+// PACK.  The matrix instruction has 16 columns for the tile's rows; with 4 rows, 12 of them would be empty, and so would
+// be three quarters of all that follows per score.  So 4 (2) tiles of 16 cache rows share one result: the tile's queries stand
+// in columns 4 j .. 4 j + 3 of the operand that meets the j-th of them and the other columns are 0, so that the four products
+// add up to four tiles side by side.  Each column is then a softmax over its own cache rows, and P' meets the values the same
+// way round: of its operand, the columns of other tiles are masked off.
+template <int D, int G, int PACK>
+struct Unit {
+    static constexpr int TILES = PACK == 4 ? 4 : 2, SETS = TILES / PACK, ROWS = 16 * TILES;
+    uint32_t k[TILES][D / 32];  // [words of the lane's row and chunk]
+    u32x4_t v[TILES];
+    half8_t ksm[SETS][G], vsm[SETS][G];  // scales and minima of four rows
 };
 
-template <int D, int G>
-__global__ __launch_bounds__(64 * KA_WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Deal d) {
+template <int D, int G, int PACK, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Deal d) {
     constexpr int g = D / G;
     constexpr int REC = kv4_record_bytes(D, g);
-    constexpr int NT = D / 16;    // tiles of 16 columns
-    constexpr int PITCH = D + 4;  // of a row of partial outputs: the 16 queries of a store fall on different banks
-    __shared__ __attribute__((aligned(16))) float part[KA_WAVES][KA_ROWS][PITCH];
-    __shared__ float state[KA_WAVES][KA_ROWS][2];
+    constexpr int NT = D / 16;        // tiles of 16 columns of the values
+    constexpr int COLS = 16 / PACK;   // of a tile of cache rows
+    constexpr int R = COLS * RT;      // rows of the tile
+    constexpr int PITCH = D + 4;      // of a row of partial outputs: the queries of a store fall on different banks
+    typedef Unit<D, G, PACK> U;
+    static_assert(RT == 1 || PACK == 1);
+    // The queries as the products take them, lane by lane, and as many zeros for the columns that a product leaves out: one
+    // copy for all waves, read where it is used (kept in registers, 64 of them with PACK = 4, other things would be spilled).
+    constexpr int QBYTES = RT * (D / 32) * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t queries[PACK > 1 ? 2 : 1][QBYTES];
+    __shared__ __attribute__((aligned(16))) float part[WAVES][R][PITCH];
+    __shared__ float state[WAVES][R][2];
 
     const Kv4Cache& c = a.c;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Piece pc;
-    if (!deal<KA_ROWS, false>(a, d, blockIdx.x, pc)) return;
-    if (pc.shares > 1 && pc.slot >= 2 << d.log_wgs) return;  // (only where lengths change under the launch)
-    const int b = __builtin_amdgcn_readfirstlane(pc.b), head = __builtin_amdgcn_readfirstlane(pc.head);
-    const int tile = __builtin_amdgcn_readfirstlane(pc.tile), shares = __builtin_amdgcn_readfirstlane(pc.shares);
-    const int share = __builtin_amdgcn_readfirstlane(pc.share), slot = __builtin_amdgcn_readfirstlane(pc.slot);
-    const int first = __builtin_amdgcn_readfirstlane(pc.first), count = __builtin_amdgcn_readfirstlane(pc.count);
-    const int len = __builtin_amdgcn_readfirstlane(pc.len);
+    if (!deal<R, false>(a, d, blockIdx.x, pc)) return;
+    if (pc.shares > 1 && pc.slot >= 2 * d.wgs()) return;  // (only where lengths change under the launch)
+    const int head = pc.head, tile = pc.tile, len = pc.len;
 
-    // This lane's query: row n of the tile.
     const int n = lane & 15, l4 = lane >> 4;
-    const int rows = imin(count * a.share - tile * KA_ROWS, KA_ROWS);
-    const int row = tile * KA_ROWS + imin(n, rows - 1);
-    const int token = row / a.share, qhead = head * a.share + row % a.share;
-    const int limit = len - count + token;  // the last row it sees
-    const int limit_lo = len - count + tile * KA_ROWS / a.share;
-    const int limit_hi = len - count + (tile * KA_ROWS + rows - 1) / a.share;
-    const int all_pages = ceil_div(imin(limit_hi + 1, len) > 0 ? imin(limit_hi + 1, len) : 0, KV4_PAGE);
+    const int col = n & (COLS - 1), part_of = n / COLS;  // the lane's query, and which of PACK tiles of cache rows
+    const int rows = imin(pc.count * a.share - tile * R, R);
+    // Queries of this lane: rows col + 16 rt of the tile; the last cache row that each sees.
+    int limit[RT], token[RT], qhead[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = tile * R + imin(col + 16 * rt, rows - 1);
+        token[rt] = pc.count == 1 ? 0 : row / a.share;
+        qhead[rt] = head * a.share + row - token[rt] * a.share;
+        limit[rt] = len - pc.count + token[rt];
+    }
+    const int limit_hi = len - pc.count + (pc.count == 1 ? 0 : (tile * R + rows - 1) / a.share);
+    const int all_pages = limit_hi < 0 ? 0 : imin(limit_hi / KV4_PAGE + 1, ceil_div(len, KV4_PAGE));
     // (selected pages are for single tokens: limit_hi + 1 = len)
     const int pages = a.selected ? imin(all_pages, a.count) : all_pages;
-    const int p0 = (int)((long)pages * share / shares), p1 = (int)((long)pages * (share + 1) / shares);
-
-    half8_t qf[D / 32];
-    float qsum[G];
-    {
-        const half_t* src = a.q + (long)(first + token) * a.q_ts + (long)qhead * a.q_hs + 8 * l4;
-#pragma unroll
-        for (int i = 0; i < G; i++) qsum[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-            qf[i] = *(const half8_t*)(src + 32 * i);
-#pragma unroll
-            for (int e = 0; e < 8; e++) qsum[32 * i / g] += (float)qf[i][e];
-        }
-#pragma unroll
-        for (int i = 0; i < G; i++) qsum[i] = rows_sum(qsum[i]) * a.scale;
+    int p0 = 0, p1 = pages;
+    if (pc.shares > 1) {
+        const int each = pages / pc.shares, more = pages - each * pc.shares;
+        p0 = pc.share * each + imin(pc.share, more);
+        p1 = p0 + each + (pc.share < more ? 1 : 0);
     }
 
-    float4_t acc[NT];
+    float qsum[RT][G];
 #pragma unroll
-    for (int i = 0; i < NT; i++) acc[i] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;     // the reference of the softmax (of this query), the lane's share of the sum
-    float mins[G], sref[G];           // sum P (m + 8 s) (the lane's share), power of two in P'
+    for (int rt = 0; rt < RT; rt++) {
+        const half_t* src = a.q + (long)(pc.first + token[rt]) * a.q_ts + (long)qhead[rt] * a.q_hs + 8 * l4;
 #pragma unroll
-    for (int i = 0; i < G; i++) mins[i] = 0.f, sref[i] = 0x1p-30f;
+        for (int i = 0; i < G; i++) qsum[rt][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            const half8_t x = *(const half8_t*)(src + 32 * i);
+            if (wave == 0) {
+                *(half8_t*)(queries[0] + (rt * (D / 32) + i) * 1024 + lane * 16) = x;
+                if (PACK > 1) *(half8_t*)(queries[PACK > 1] + i * 1024 + lane * 16) = (half8_t){};
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                qsum[rt][32 * i / g] = __builtin_amdgcn_fdot2((half2_t){x[e], x[e + 1]}, (half2_t){(half_t)1.f, (half_t)1.f},
+                                                              qsum[rt][32 * i / g], false);
+        }
+#pragma unroll
+        for (int i = 0; i < G; i++) qsum[rt][i] = rows_sum(qsum[rt][i]) * a.scale;
+    }
+    const uint8_t* qat[PACK];  // the lane's place in the queries, or in the zeros for a product that leaves its column out
+#pragma unroll
+    for (int j = 0; j < PACK; j++) qat[j] = queries[PACK > 1 && part_of != j ? 1 : 0] + lane * 16;
+    __syncthreads();
+
+    float4_t acc[RT][NT];
+    float m[RT], l[RT];            // the reference of the softmax (of this column), the lane's share of the sum
+    float mins[RT][G];             // sum P (m + 8 s) (the lane's share)
+    float sref[G], sinv[G];        // power of two in P', and 16 over it
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY, l[rt] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; i++) acc[rt][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < G; i++) mins[rt][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < G; i++) sref[i] = 0x1p-30f, sinv[i] = 0x1p34f;
     const half8_t eight[2] = {bit_cast<half8_t>((u32x4_t){0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u}),   // -8 * 2^-24
                               bit_cast<half8_t>((u32x4_t){0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u})};  // -8 * 2^-20
     const float scale24 = a.scale * 0x1p24f;
     const NibbleMasks nm = nibble_masks();
-    const uint32_t voff = (D == 128 ? n : (n & 7)) * 16;
+    uint32_t own[PACK];  // all ones where the column is of the j-th tile
+#pragma unroll
+    for (int j = 0; j < PACK; j++) own[j] = part_of == j ? ~0u : 0u;
+    const uint32_t koff = n * (D / 2) + l4 * (D / 8);
+    const uint32_t voff = 32 * D + l4 * (2 * D) + (D == 128 ? n : (n & 7)) * 16;
+    const uint32_t smoff = 64 * D + (4 * part_of + l4) * 16;
     const uint32_t vsel = D == 64 && n >= 8 ? 0x07060302u : 0x05040100u;
+    constexpr int PER = KV4_PAGE / U::ROWS;  // units of a page
 
-    const int* const table = c.table + (long)b * c.table_stride;
-    const int* const chosen = a.selected ? a.selected + ((long)b * c.H + head) * a.count : nullptr;
+    const int* const table = c.table + (long)pc.b * c.table_stride;
+    const int* const chosen = a.selected ? a.selected + ((long)pc.b * c.H + head) * a.count : nullptr;
     // Pages are looked up 64 at a time: lane i has the i-th one's place in the sequence and in the pool.
     for (int pb = p0; pb < p1; pb += 64) {
         int place = pb + lane, id = -1;
@@ -215,212 +287,283 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv4_attn_kernel(Kv4AttnArgs a, 
             if ((unsigned)id >= (unsigned)c.num_pages) id = -1;
         }
         if (id < 0) place = 0;  // a page that does not exist: its rows lie behind every query's last
-        const int units = 2 * imin(64, p1 - pb);
-        auto load = [&](int u, Half<D, G>& x) {
-            const int pid = __builtin_amdgcn_readlane(id, u >> 1);
-            const uint8_t* const rec = c.pool + ((long)(pid < 0 ? 0 : pid) * c.H + head) * REC;
-            const int r0 = 32 * (u & 1);
+        const int units = PER * imin(64, p1 - pb);
+        U x;
+        // (uniform base, 32-bit offset of the lane, the rest an immediate)
+        auto record = [&](int u) {
+            const int pid = __builtin_amdgcn_readlane(id, u / PER);
+            return c.pool + ((long)(pid < 0 ? 0 : pid) * c.H + head) * REC;
+        };
+        auto load_keys = [&](int u) {
+            const uint8_t* const rec = record(u);
+            const int t0 = PER == 1 ? 0 : u % PER * U::TILES;
+            const uint8_t* const ks = rec + t0 * (8 * D);
+            const uint8_t* const sm = rec + t0 * 64;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint8_t* ks = rec + (r0 + 16 * t + n) * (D / 2) + l4 * (D / 8);
+            for (int t = 0; t < U::TILES; t++) {
                 if constexpr (D == 128) {
-                    const u32x4_t w = *(const u32x4_t*)ks;
+                    const u32x4_t w = __builtin_nontemporal_load((const u32x4_t*)(ks + (koff + t * (8 * D))));
 #pragma unroll
                     for (int i = 0; i < 4; i++) x.k[t][i] = w[i];
                 } else {
-                    const u32x2_t w = *(const u32x2_t*)ks;
+                    const u32x2_t w = __builtin_nontemporal_load((const u32x2_t*)(ks + (koff + t * (8 * D))));
                     x.k[t][0] = w[0];
                     x.k[t][1] = w[1];
                 }
-                const int quad = (r0 + 16 * t) / 4 + l4;
-                x.v[t] = *(const u32x4_t*)(rec + 32 * D + quad * (2 * D) + voff);
-#pragma unroll
-                for (int i = 0; i < G; i++) {
-                    x.ksm[t][i] = *(const half8_t*)(rec + 64 * D + (i * 16 + quad) * 16);
-                    x.vsm[t][i] = *(const half8_t*)(rec + 64 * D + 256 * G + (i * 16 + quad) * 16);
-                }
             }
+#pragma unroll
+            for (int i = 0; i < U::SETS; i++)
+#pragma unroll
+                for (int j = 0; j < G; j++) x.ksm[i][j] = *(const half8_t*)(sm + (smoff + PACK * i * 64 + j * 256));
         };
-        auto consume = [&](int u, const Half<D, G>& x) {
-            const int pid = __builtin_amdgcn_readlane(id, u >> 1);
-            const int pos0 = __builtin_amdgcn_readlane(place, u >> 1) * KV4_PAGE + 32 * (u & 1);
-            float s[8];
+        auto load_values = [&](int u) {
+            const uint8_t* const rec = record(u);
+            const int t0 = PER == 1 ? 0 : u % PER * U::TILES;
+            const uint8_t* const vs = rec + t0 * (8 * D);
+            const uint8_t* const sm = rec + t0 * 64;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                float4_t even[G], odd[G];
+            for (int i = 0; i < U::SETS; i++)
 #pragma unroll
-                for (int i = 0; i < G; i++) even[i] = odd[i] = (float4_t){0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < G; j++) x.vsm[i][j] = *(const half8_t*)(sm + (smoff + 256 * G + PACK * i * 64 + j * 256));
+#pragma unroll
+            for (int t = 0; t < U::TILES; t++)
+                x.v[t] = __builtin_nontemporal_load((const u32x4_t*)(vs + (voff + t * (8 * D))));
+        };
+        // One unit.  The next one's keys are asked for where this one's have met the queries, its values where these have met P.
+        auto consume = [&](int u) {
+            constexpr int NS = 4 * U::SETS;  // scores of a lane and query
+            float s[RT][NS];
+            float4_t even[U::SETS][RT][G], odd[U::SETS][RT][G];
+#pragma unroll
+            for (int i = 0; i < U::SETS; i++)
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int j = 0; j < G; j++) even[i][rt][j] = odd[i][rt][j] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            asm volatile("" ::: "memory");  // the queries are read anew
+#pragma unroll
+            for (int t = 0; t < U::TILES; t++) {
+                const int set = t / PACK, j = t % PACK;
 #pragma unroll
                 for (int p = 0; p < D / 64; p++) {
                     const uint32_t w0 = x.k[t][2 * p], w1 = x.k[t][2 * p + 1], h0 = w0 >> 8, h1 = w1 >> 8;
-                    const u32x4_t lo = {w0 & nm.lo, w1 & nm.lo, h0 & nm.lo, h1 & nm.lo};
-                    const u32x4_t hi = {w0 & nm.hi, w1 & nm.hi, h0 & nm.hi, h1 & nm.hi};
+                    const half8_t lo = bit_cast<half8_t>((u32x4_t){w0 & nm.lo, w1 & nm.lo, h0 & nm.lo, h1 & nm.lo});
+                    const half8_t hi = bit_cast<half8_t>((u32x4_t){w0 & nm.hi, w1 & nm.hi, h0 & nm.hi, h1 & nm.hi});
                     const int ie = 64 * p / g, io = (64 * p + 32) / g;
-                    even[ie] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<half8_t>(lo), qf[2 * p], even[ie], 0, 0, 0);
-                    odd[io] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<half8_t>(hi), qf[2 * p + 1], odd[io], 0, 0, 0);
-                }
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
+                    for (int rt = 0; rt < RT; rt++) {
+                        const half8_t* const q = (const half8_t*)(qat[j] + (rt * (D / 32) + 2 * p) * 1024);
+                        even[set][rt][ie] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, q[0], even[set][rt][ie], 0, 0, 0);
+                        odd[set][rt][io] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, q[64], odd[set][rt][io], 0, 0, 0);
+                    }
+                }
+            }
+            // Where the lane's scores stand: rows pos + 16 PACK set + r.
+            const int pid = __builtin_amdgcn_readlane(id, u / PER);
+            const int pos = __builtin_amdgcn_readlane(place, u / PER) * KV4_PAGE + u % PER * U::ROWS + 16 * part_of + 4 * l4;
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const int last = pid < 0 ? -1 : limit[rt];
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const int set = i / 4, r = i % 4;
                     float codes = 0.f, shift = 0.f;
 #pragma unroll
-                    for (int i = 0; i < G; i++) {
-                        const float sum = odd[i][r] * 0.0625f + even[i][r];
-                        codes += (float)x.ksm[t][i][r] * sum;
-                        shift += (float)x.ksm[t][i][4 + r] * qsum[i];
+                    for (int j = 0; j < G; j++) {
+                        const float sum = odd[set][rt][j][r] * 0.0625f + even[set][rt][j][r];
+                        codes += (float)x.ksm[set][j][r] * sum;
+                        shift += (float)x.ksm[set][j][4 + r] * qsum[rt][j];
                     }
-                    s[4 * t + r] = codes * scale24 + shift;
+                    s[rt][i] = codes * scale24 + shift;
+                    if (pos + 16 * PACK * set + r > last) s[rt][i] = -INFINITY;
+                    top = fmaxf(top, s[rt][i]);
+                }
+                if (rt == RT - 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (u + WAVES < units) load_keys(u + WAVES);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (__ballot(top > m[rt] + KA_LAZY)) {
+                    const float to = fmaxf(rows_max(top), m[rt]);
+                    const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+                    m[rt] = to;
+                    l[rt] *= f;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) acc[rt][i] *= f;
+#pragma unroll
+                    for (int i = 0; i < G; i++) mins[rt][i] *= f;
+                }
+                const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    s[rt][i] = __builtin_amdgcn_exp2f(s[rt][i] - ref);
+                    l[rt] += s[rt][i];
                 }
             }
-            bool vis[8];
+            // P' of every group, as the operand's halves.
+            const int seen_to = RT == 1 ? limit[0] : limit_hi;
+            uint32_t pf[RT][U::SETS][G][2];
 #pragma unroll
-            for (int j = 0; j < 8; j++) vis[j] = true;
-            if (pid < 0 || pos0 + 31 > limit_lo) {  // some row is not there, or not for every query
-                const int last = pid < 0 ? -1 : limit;
+            for (int j = 0; j < G; j++) {
+                float sv[NS], mid[NS], big = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    vis[j] = pos0 + 16 * (j >> 2) + 4 * l4 + (j & 3) <= last;
-                    if (!vis[j]) s[j] = -INFINITY;
+                for (int i = 0; i < NS; i++) {
+                    const int set = i / 4, r = i % 4;
+                    sv[i] = (float)x.vsm[set][j][r];
+                    mid[i] = 8.f * sv[i] + (float)x.vsm[set][j][4 + r];
+                    if (pid < 0 || pos + 16 * PACK * set + r > seen_to) sv[i] = mid[i] = 0.f;  // whatever lies where nobody looks
+                    big = fmaxf(big, sv[i]);
                 }
-            }
-            float top = s[0];
-#pragma unroll
-            for (int j = 1; j < 8; j++) top = fmaxf(top, s[j]);
-            if (__ballot(top > m + KA_LAZY)) {
-                const float to = fmaxf(rows_max(top), m);
-                const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < NT; i++) acc[i] *= f;
-#pragma unroll
-                for (int i = 0; i < G; i++) mins[i] *= f;
-            }
-            const float ref = m == -INFINITY ? 0.f : m;
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[j] = __builtin_amdgcn_exp2f(s[j] - ref);
-                l += p[j];
-            }
-            half8_t pf[G];
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-                float sv[8], mv[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    sv[j] = (float)x.vsm[j >> 2][i][j & 3];
-                    mv[j] = (float)x.vsm[j >> 2][i][4 + (j & 3)];
-                    if (!vis[j]) sv[j] = mv[j] = 0.f;  // whatever lies there
-                }
-                float big = sv[0];
-#pragma unroll
-                for (int j = 1; j < 8; j++) big = fmaxf(big, sv[j]);
-                if (__ballot(big > 8.f * sref[i])) {
+                if (__ballot(big > 8.f * sref[j])) {
                     const float to = bit_cast<float>(bit_cast<uint32_t>(wave_max(big)) & 0x7f800000u) * 2.f;
-                    const float f = sref[i] / to;
-                    sref[i] = to;
+                    const float f = sref[j] / to;
+                    sref[j] = to;
+                    sinv[j] = 16.f / to;
 #pragma unroll
-                    for (int k = i * g / 16; k < (i + 1) * g / 16; k++) acc[k] *= f;
-                }
-                const float inv = 16.f / sref[i];
+                    for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    pf[i][j] = (half_t)(p[j] * (sv[j] * inv));
-                    mins[i] += p[j] * (8.f * sv[j] + mv[j]);
+                        for (int k = j * g / 16; k < (j + 1) * g / 16; k++) acc[rt][k] *= f;
                 }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int i = 0; i < NS; i += 2) {
+                        float x0 = s[rt][i] * (sv[i] * sinv[j]), x1 = s[rt][i + 1] * (sv[i + 1] * sinv[j]);
+                        float y0 = s[rt][i] * mid[i], y1 = s[rt][i + 1] * mid[i + 1];
+                        if (RT > 1) {  // a row that another query sees
+                            const int set = i / 4, r = i % 4;
+                            if (pos + 16 * PACK * set + r > limit[rt]) x0 = y0 = 0.f;
+                            if (pos + 16 * PACK * set + r + 1 > limit[rt]) x1 = y1 = 0.f;
+                        }
+                        mins[rt][j] += y0;
+                        mins[rt][j] += y1;
+                        pf[rt][i / 4][j][i % 4 / 2] = bit_cast<uint32_t>((half2_t){(half_t)x0, (half_t)x1});
+                    }
             }
-            uint32_t lo[4];
-            auto products = [&](int tile0) {
-                uint32_t up[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) up[j] = lo[j] >> 8;
-                const u32x4_t a0 = {lo[0] & nm.lo, lo[1] & nm.lo, lo[2] & nm.lo, lo[3] & nm.lo};
-                const u32x4_t a1 = {lo[0] & nm.hi, lo[1] & nm.hi, lo[2] & nm.hi, lo[3] & nm.hi};
-                const u32x4_t a2 = {up[0] & nm.lo, up[1] & nm.lo, up[2] & nm.lo, up[3] & nm.lo};
-                const u32x4_t a3 = {up[0] & nm.hi, up[1] & nm.hi, up[2] & nm.hi, up[3] & nm.hi};
-                const u32x4_t op[4] = {a0, a1, a2, a3};
+            for (int t = 0; t < U::TILES; t += 2) {
+                const int s0 = t / PACK, s1 = (t + 1) / PACK, j0 = t % PACK, j1 = (t + 1) % PACK;
+                half8_t b[RT][G];
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    acc[tile0 + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<half8_t>(op[k]), pf[16 * (tile0 + k) / g],
-                                                                            acc[tile0 + k], 0, 0, 0);
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    acc[tile0 + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight[k & 1], pf[16 * (tile0 + k) / g], acc[tile0 + k],
-                                                                            0, 0, 0);
-            };
+                    for (int j = 0; j < G; j++) {
+                        u32x4_t w = {pf[rt][s0][j][0], pf[rt][s0][j][1], pf[rt][s1][j][0], pf[rt][s1][j][1]};
+                        if (PACK > 1) w = (u32x4_t){w[0] & own[j0], w[1] & own[j0], w[2] & own[j1], w[3] & own[j1]};
+                        b[rt][j] = bit_cast<half8_t>(w);
+                    }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                lo[j] = __builtin_amdgcn_perm(x.v[j >> 1][2 * (j & 1) + 1], x.v[j >> 1][2 * (j & 1)], vsel);
-            products(0);
-            if constexpr (D == 128) {
+                for (int hf = 0; hf < D / 64; hf++) {  // low halves of the words (D = 64: the lane's half), high halves
+                    const uint32_t sel = hf ? 0x07060302u : vsel;
+                    uint32_t lo[4], up[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    lo[j] = __builtin_amdgcn_perm(x.v[j >> 1][2 * (j & 1) + 1], x.v[j >> 1][2 * (j & 1)], 0x07060302u);
-                products(4);
+                    for (int j = 0; j < 4; j++) {
+                        lo[j] = __builtin_amdgcn_perm(x.v[t + (j >> 1)][2 * (j & 1) + 1], x.v[t + (j >> 1)][2 * (j & 1)], sel);
+                        up[j] = lo[j] >> 8;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t mask = k & 1 ? nm.hi : nm.lo;
+                        const half8_t op = k < 2 ? bit_cast<half8_t>((u32x4_t){lo[0] & mask, lo[1] & mask, lo[2] & mask, lo[3] & mask})
+                                                 : bit_cast<half8_t>((u32x4_t){up[0] & mask, up[1] & mask, up[2] & mask, up[3] & mask});
+                        const int i = 4 * hf + k;
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+                            acc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, b[rt][16 * i / g], acc[rt][i], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int i = 4 * hf + k;
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+                            acc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight[k & 1], b[rt][16 * i / g], acc[rt][i], 0, 0, 0);
+                    }
+                }
             }
         };
-        Half<D, G> x0, x1;
-        int u = wave;
-        if (u < units) {
-            load(u, x0);
-            while (u < units) {
-                if (u + KA_WAVES < units) load(u + KA_WAVES, x1);
-                consume(u, x0);
-                u += KA_WAVES;
-                if (u >= units) break;
-                if (u + KA_WAVES < units) load(u + KA_WAVES, x0);
-                consume(u, x1);
-                u += KA_WAVES;
-            }
+        if (wave < units) {
+            load_keys(wave);
+            load_values(wave);
+        }
+        for (int u = wave; u < units; u += WAVES) {
+            consume(u);
+            __builtin_amdgcn_sched_barrier(0);
+            if (u + WAVES < units) load_values(u + WAVES);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
-    // The wave's output over its rows, then the workgroup's.
-    l = rows_sum(l);
+    // Of the wave: sums over the lanes of a column, then the columns of one query, which have seen different rows.
 #pragma unroll
-    for (int i = 0; i < G; i++) mins[i] = rows_sum(mins[i]);
-    if (n < rows) {
+    for (int rt = 0; rt < RT; rt++) {
+        l[rt] = rows_sum(l[rt]);
+#pragma unroll
+        for (int i = 0; i < G; i++) mins[rt][i] = rows_sum(mins[rt][i]);
 #pragma unroll
         for (int i = 0; i < NT; i++) {
             const int gi = 16 * i / g;
-            const float f = sref[gi] * 0.0625f, fc = f * (i & 1 ? 0x1p20f : 0x1p24f), base = mins[gi];
-            *(float4_t*)&part[wave][n][16 * i + 4 * l4] = (float4_t){acc[i][0] * fc + base, acc[i][1] * fc + base,
-                                                                     acc[i][2] * fc + base, acc[i][3] * fc + base};
+            const float f = sref[gi] * (i & 1 ? 0x1p16f : 0x1p20f);  // over the 16 in P', times 2^20 or 2^24
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[rt][i][e] = acc[rt][i][e] * f + mins[rt][gi];
         }
-        if (l4 == 0) {
-            state[wave][n][0] = m;
-            state[wave][n][1] = l;
+        if constexpr (PACK > 1) {
+            float to = fmaxf(m[rt], row_move<0x128>(m[rt]));          // row_ror:8
+            if (PACK == 4) to = fmaxf(to, row_move<0x124>(to));        // row_ror:4
+            const float f = m[rt] == to ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+            m[rt] = to;
+            l[rt] *= f;
+            l[rt] += row_move<0x128>(l[rt]);
+            if (PACK == 4) l[rt] += row_move<0x124>(l[rt]);
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float v = acc[rt][i][e] * f;
+                    v += row_move<0x128>(v);
+                    if (PACK == 4) v += row_move<0x124>(v);
+                    acc[rt][i][e] = v;
+                }
+        }
+        const int row = n + 16 * rt;
+        if (n < COLS && row < rows) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) *(float4_t*)&part[wave][row][16 * i + 4 * l4] = acc[rt][i];
+            if (l4 == 0) {
+                state[wave][row][0] = m[rt];
+                state[wave][row][1] = l[rt];
+            }
         }
     }
     __syncthreads();
     constexpr int C4 = D / 4;
-    for (int i = threadIdx.x; i < rows * C4; i += 64 * KA_WAVES) {
+    for (int i = threadIdx.x; i < rows * C4; i += 64 * WAVES) {
         const int r = i / C4, c4 = i % C4;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KA_WAVES; w++) mx = fmaxf(mx, state[w][r][0]);
+        for (int w = 0; w < WAVES; w++) mx = fmaxf(mx, state[w][r][0]);
         float sum = 0.f;
         float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < KA_WAVES; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float mw = state[w][r][0];
-            const float f = mw == -INFINITY ? (mx == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mw - mx);
+            const float f = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
             sum += state[w][r][1] * f;
             o += *(const float4_t*)&part[w][r][4 * c4] * f;
         }
-        if (shares == 1) {
-            const int rr = tile * KA_ROWS + r;
+        if (pc.shares == 1) {
+            const int rr = tile * R + r, t = pc.count == 1 ? 0 : rr / a.share;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;  // nothing visible: 0
             half4_t h;
 #pragma unroll
             for (int e = 0; e < 4; e++) h[e] = (half_t)(o[e] * inv);
-            *(half4_t*)(a.out + ((long)(first + rr / a.share) * c.H * a.share + head * a.share + rr % a.share) * D + 4 * c4) = h;
+            *(half4_t*)(a.out + ((long)(pc.first + t) * c.H * a.share + head * a.share + rr - t * a.share) * D + 4 * c4) = h;
         } else {
-            float* const dst = a.ws + (long)slot * KA_ROWS * (D + 2);
+            float* const dst = a.ws + (long)pc.slot * R * (D + 2);
             *(float4_t*)(dst + r * D + 4 * c4) = o;
             if (c4 == 0) {
-                dst[KA_ROWS * D + 2 * r] = mx;
-                dst[KA_ROWS * D + 2 * r + 1] = sum;
+                dst[R * D + 2 * r] = mx;
+                dst[R * D + 2 * r + 1] = sum;
             }
         }
     }
@@ -434,7 +577,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, Deal d) {
     __shared__ float state[LANES][2];
     Piece pc;
     if (!deal<R, true>(a, d, blockIdx.x, pc)) return;
-    if (pc.slot + pc.shares > 2 << d.log_wgs) return;  // (only where lengths change under the launch)
+    if (pc.slot + pc.shares > 2 * d.wgs()) return;  // (only where lengths change under the launch)
     const int r = blockIdx.y;
     const int rr = pc.tile * R + r;
     if (rr >= pc.count * a.share) return;
@@ -478,13 +621,20 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, Deal d) {
     *(half4_t*)(a.out + ((long)(pc.first + rr / a.share) * a.c.H * a.share + pc.head * a.share + rr % a.share) * D + 4 * c4) = h;
 }
 
-constexpr Deal KA_DEAL = {10, 4};
+// Workgroups that a launch's pages are dealt to, and a share's fewest pages: see launch_kv4_attention.
+constexpr Deal KA_DEAL = {2, 16};
+constexpr int KA_ROWS = 32;  // of a tile at the most
 
 }  // namespace
 
-// At most 2^(log_wgs + 1) shares of shared tiles: every one but a tile's last holds `least` pages or more, of which
-// there are 2^log_wgs times as many as in all, and there are fewer shared tiles than that.
-size_t kv4_attention_workspace_bytes(int D) { return (size_t)(2 << KA_DEAL.log_wgs) * KA_ROWS * (D + 2) * sizeof(float); }
+// At most 2 wgs() shares of shared tiles: a tile of p pages has fewer than p / least + 1, there are at most wgs() * least
+// pages in all, and every shared tile has more than `least` of them.
+size_t kv4_attention_workspace_bytes(int T, int B, int share, int D, int pages) {
+    if (pages <= KA_DEAL.least) return 0;
+    const long mean = ((long)T * share + B - 1) / B;
+    const int rows = mean <= 4 ? 4 : mean <= 8 ? 8 : mean <= 16 ? 16 : KA_ROWS;
+    return (size_t)(2 * KA_DEAL.wgs()) * rows * (D + 2) * sizeof(float);
+}
 
 hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, const int* selected, void* workspace, int D, int g,
                                 int share, int count, long q_ts, long q_hs, float sm_scale, hipStream_t st) {
@@ -501,22 +651,35 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
     const int most = selected && count < c.width ? count : c.width;
     const bool split = workspace != nullptr && most > KA_DEAL.least;
     a.ws = split ? (float*)workspace : nullptr;
-    const long tiles = (c.starts ? (long)c.T * share / KA_ROWS + c.B : (long)c.B * (((long)c.each * share + KA_ROWS - 1) / KA_ROWS)) *
-                       c.H;
-    const long wgs = split ? tiles + (1l << KA_DEAL.log_wgs) : tiles;
-    auto go = [&](auto d, auto groups) {
-        hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value>), dim3((unsigned)wgs), dim3(64 * KA_WAVES), 0, st, a, KA_DEAL);
+    // Rows of a sequence and key/value head (of the average one where they differ).
+    const long mean = ((long)c.T * share + c.B - 1) / c.B;
+    auto go = [&](auto d, auto groups, auto pack, auto rt, auto waves) {
+        constexpr int R = 16 / pack.value * rt.value;
+        const long tiles = (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
+        const long wgs = split ? tiles + KA_DEAL.wgs() : tiles;
+        hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value, pack.value, rt.value, waves.value>), dim3((unsigned)wgs),
+                           dim3(64 * waves.value), 0, st, a, KA_DEAL);
         if (!split) return;
-        const long tokens = c.starts ? KA_ROWS : c.each;
-        const unsigned rows = (unsigned)(tokens * share < KA_ROWS ? tokens * share : KA_ROWS);
-        const long shared = tiles < (1l << KA_DEAL.log_wgs) ? tiles : (1l << KA_DEAL.log_wgs);
-        hipLaunchKernelGGL((kv4_join_kernel<d.value, KA_ROWS>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
+        const long tokens = c.starts ? R : c.each;
+        const unsigned rows = (unsigned)(tokens * share < R ? tokens * share : R);
+        const long shared = tiles < KA_DEAL.wgs() ? tiles : KA_DEAL.wgs();
+        hipLaunchKernelGGL((kv4_join_kernel<d.value, R>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
     };
-    if (D == 128 && g == 128) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
-    if (D == 128 && g == 64) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{});
-    if (D == 128 && g == 32) go(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
-    if (D == 64 && g == 64) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    if (D == 64 && g == 32) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    auto by_rows = [&](auto d, auto groups) {
+        if (mean <= 4)
+            go(d, groups, Int<4>{}, Int<1>{}, Int<4>{});
+        else if (mean <= 8)
+            go(d, groups, Int<2>{}, Int<1>{}, Int<4>{});
+        else if (mean <= 16)
+            go(d, groups, Int<1>{}, Int<1>{}, Int<4>{});
+        else
+            go(d, groups, Int<1>{}, Int<2>{}, Int<4>{});
+    };
+    if (D == 128 && g == 128) by_rows(Int<128>{}, Int<1>{});
+    if (D == 128 && g == 64) by_rows(Int<128>{}, Int<2>{});
+    if (D == 128 && g == 32) by_rows(Int<128>{}, Int<4>{});
+    if (D == 64 && g == 64) by_rows(Int<64>{}, Int<1>{});
+    if (D == 64 && g == 32) by_rows(Int<64>{}, Int<2>{});
     return hipGetLastError();
 }
 

@@ -22,6 +22,7 @@ import heapq
 
 import torch
 
+import quant
 from . import capi
 from .capi import _check, _ptr, _stream
 
@@ -84,10 +85,14 @@ def _table_stride(pages):
     return max(pages.stride(0), pages.shape[1]) if pages.shape[0] > 1 else pages.shape[1]
 
 
-def append(k, v, pool, pages, lengths, starts=None, values=False, stream=None):
+def append(k, v, pool, pages, lengths, starts=None, values=False):
     """Quantise the rows k, v fp16 [T, kv_heads, D] (any token and head strides) of new tokens into their pages; they are
     the last rows of their sequences.  With `values` returns (k_hat, v_hat) fp16 [T, kv_heads, D], what the cache holds
     of them (of no defined content where a token has no page); otherwise None."""
+    got = quant.kv4_append(k, v, pool, pages, lengths, starts, values)
+    if got is not None:
+        return tuple(got) if values else None
+    # something is empty, has to be copied first, or is refused
     t, b, g = _check_cache(k, pool, pages, lengths, starts)
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must be alike, got %s %s and %s %s" % (k.dtype, tuple(k.shape), v.dtype, tuple(v.shape)))
@@ -100,15 +105,18 @@ def append(k, v, pool, pages, lengths, starts=None, values=False, stream=None):
     with torch.cuda.device(k.device):
         _check(capi.lib().sq_kv4_append(_ptr(k), _ptr(v), _ptr(hats[0]), _ptr(hats[1]), _ptr(pool), _ptr(pages), _ptr(lengths),
                                         _ptr(starts), t, b, h, d, g, pool.shape[0], pages.shape[1], _table_stride(pages),
-                                        strides, _stream(stream)), "sq_kv4_append")
+                                        strides, _stream()), "sq_kv4_append")
     return hats if values else None
 
 
-def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out=None, stream=None):
+def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out=None):
     """Causal attention of q fp16 [T, heads, D], the last tokens of their sequences (their own rows are in the cache), over
     the cached rows; query head h reads key/value head h // (heads // kv_heads).  selected int32 [sequences, kv_heads,
     count] (one token per sequence): over the rows of these pages only, as select_pages gives them.  Returns fp16
     [T, heads, D]; a token that sees no row gets 0, tokens behind the last sequence's are left as `out` had them."""
+    got = quant.kv4_attention(q, pool, pages, lengths, sm_scale, starts, selected, out)
+    if got is not None:
+        return got if out is None else out
     t, b, g = _check_cache(q, pool, pages, lengths, starts)
     hq, d = q.shape[1:]
     h = pool.shape[1]
@@ -127,20 +135,23 @@ def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out
         out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise ValueError("out must be a contiguous fp16 %s on the device of q" % (tuple(q.shape),))
-    # The workspace holds nothing between calls: one of its own for each, from the stream's (or a captured graph's) memory.
-    ws = torch.empty(capi.lib().sq_kv4_attention_workspace_bytes(d), dtype=torch.uint8, device=q.device) if t else None
+    need = capi.lib().sq_kv4_attention_workspace_bytes(t, b, hq, h, d, pages.shape[1], count)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         _check(capi.lib().sq_kv4_attention(_ptr(q), _ptr(out), _ptr(pool), _ptr(pages), _ptr(lengths), _ptr(starts),
                                            _ptr(selected), t, b, hq, h, d, g, pool.shape[0], pages.shape[1],
                                            _table_stride(pages), count, q.stride(0), q.stride(1), float(sm_scale), _ptr(ws),
-                                           0 if ws is None else ws.numel(), _stream(stream)), "sq_kv4_attention")
+                                           need, _stream()), "sq_kv4_attention")
     return out
 
 
-def select_pages(q, pool, pages, lengths, count, keep_first=1, keep_last=1, stream=None):
+def select_pages(q, pool, pages, lengths, count, keep_first=1, keep_last=1):
     """int32 [sequences, kv_heads, count]: for the next token of each sequence, q fp16 [sequences, heads, D], the places of
     the `count` pages that can hold the highest scores, ascending, -1 behind the last where there are fewer; the first
     keep_first and the last keep_last are always among them."""
+    got = quant.kv4_select(q, pool, pages, lengths, count, keep_first, keep_last)
+    if got is not None:
+        return got
     t, b, g = _check_cache(q, pool, pages, lengths, None)
     hq, d = q.shape[1:]
     h = pool.shape[1]
@@ -158,14 +169,16 @@ def select_pages(q, pool, pages, lengths, count, keep_first=1, keep_last=1, stre
     with torch.cuda.device(q.device):
         _check(capi.lib().sq_kv4_select(_ptr(q), _ptr(selected), _ptr(pool), _ptr(pages), _ptr(lengths), b, hq, h, d, g,
                                         pool.shape[0], width, _table_stride(pages), int(count), int(keep_first),
-                                        int(keep_last), q.stride(0), q.stride(1), _ptr(ws), need, _stream(stream)),
+                                        int(keep_last), q.stride(0), q.stride(1), _ptr(ws), need, _stream()),
                "sq_kv4_select")
     return selected
 
 
-def copy_pages(pool, src, dst, stream=None):
+def copy_pages(pool, src, dst):
     """Copy page src[i] to page dst[i], int32 on the device, in a pool [pages, ...] or in every layer of [layers, pages,
     kv_heads, record].  No page may be a destination twice, or a destination and another pair's source."""
+    if quant.kv4_copy_pages(pool, src, dst):
+        return
     if pool.dim() not in (3, 4) or pool.dtype != torch.uint8 or not pool.is_contiguous() or not pool.is_cuda:
         raise ValueError("the pool must be a contiguous uint8 [pages, kv_heads, record] or [layers, ...] on the device")
     if src.shape != dst.shape or src.dim() != 1 or any(i.dtype != torch.int32 or i.device != pool.device
@@ -174,7 +187,7 @@ def copy_pages(pool, src, dst, stream=None):
     layers, (n, h, rec) = (1, pool.shape) if pool.dim() == 3 else (pool.shape[0], pool.shape[1:])
     with torch.cuda.device(pool.device):
         _check(capi.lib().sq_kv4_copy_pages(_ptr(pool), _ptr(src), _ptr(dst), src.numel(), n, layers, h * rec, n * h * rec,
-                                            _stream(stream)), "sq_kv4_copy_pages")
+                                            _stream()), "sq_kv4_copy_pages")
 
 
 class KV4Cache:

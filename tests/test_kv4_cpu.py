@@ -100,10 +100,13 @@ def test_attention_refuses(L, p):
     for bad in (dict(q=odd), dict(out=odd), dict(qh=100), dict(sel=odd, count=2)):
         assert call(**bad) == capi.SQ_ERR_MISALIGNED, bad
     assert call(g=256) == capi.SQ_ERR_BAD_GROUP
-    assert call(ws=p, size=16) == capi.SQ_ERR_WORKSPACE
+    need = L.sq_kv4_attention_workspace_bytes
+    assert call(ws=p, size=16, width=500, stride=500) == capi.SQ_ERR_WORKSPACE
     assert call(ws=odd, size=1 << 30) == capi.SQ_ERR_WORKSPACE
-    assert L.sq_kv4_attention_workspace_bytes(96) == 0 < L.sq_kv4_attention_workspace_bytes(64) \
-        < L.sq_kv4_attention_workspace_bytes(128)
+    assert call(ws=p, size=need(4, 4, 16, 8, 128, 500, 0) - 1, width=500, stride=500) == capi.SQ_ERR_WORKSPACE
+    assert need(4, 4, 16, 8, 128, 4, 0) == 0 == need(4, 4, 16, 8, 128, 500, 4)  # too short to be dealt out
+    assert need(4, 4, 16, 8, 96, 500, 0) == 0 < need(4, 4, 16, 8, 64, 500, 0) < need(4, 4, 16, 8, 128, 500, 0)
+    assert need(0, 4, 16, 8, 128, 500, 0) == 0 == need(4, 4, 12, 8, 128, 500, 0)
 
 
 def test_select_refuses(L, p):
