@@ -48,6 +48,8 @@ __device__ __forceinline__ void kv4_tokens(const Kv4Cache& c, int b, int& first,
     }
 }
 
+__device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
+
 // Inclusive sum over the lanes of a wave, by data-parallel moves (a shuffle through LDS costs 60 cycles a step).
 __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1

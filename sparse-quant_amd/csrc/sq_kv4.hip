@@ -262,10 +262,12 @@ __global__ __launch_bounds__(256) void kv4_copy_kernel(uint8_t* pool, const int*
 // ------------------------------------------------------------------------------------------------------- select
 //
 // score(page) = max over the head's queries of sum_d max(q_d hi_d, q_d lo_d), hi and lo the page's largest and
-// smallest keys: no key of the page can score higher.  Sums in 64 bits: which of two pages is the better one must not
-// hang on the order of a sum.  A lane owns a page and walks over its bounds; the queries come from LDS, split into
-// their positive and negative parts, so that the choice between hi and lo is two products and no comparison.
-constexpr int SELECT_QUERIES = 8;  // of a round
+// smallest keys: no key of the page can score higher.  Which of two pages is the better one must not hang on the order
+// of a sum: products of fp16 numbers are exact in fp32, their sums are taken in 64 bits.
+// 16 (D = 64: 8) lanes share a page, 8 elements each; the choice between hi and lo goes by the signs of the queries, which
+// a lane keeps as masks of pairs.  A wave takes SELECT_PAGES pages, all their bounds asked for at once.
+constexpr int SELECT_QUERIES = 4;  // of a round
+constexpr int SELECT_PAGES = 16;   // of a wave
 
 struct Kv4SelectArgs {
     Kv4Cache c;
@@ -276,49 +278,73 @@ struct Kv4SelectArgs {
     int share, count, keep_first, keep_last;
 };
 
+typedef short short2_t __attribute__((ext_vector_type(2)));
+
+template <int CTRL>
+__device__ __forceinline__ double row_move(double v) {
+    const u32x2_t u = bit_cast<u32x2_t>(v);
+    return bit_cast<double>((u32x2_t){(uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, 0xF, 0xF, false),
+                                      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, 0xF, 0xF, false)});
+}
+
 template <int D>
 __global__ __launch_bounds__(64) void kv4_score_kernel(Kv4SelectArgs a, int rec_bytes) {
-    __shared__ double qs[SELECT_QUERIES][D][2];
+    constexpr int LPP = D / 8, PPI = 64 / LPP, N = SELECT_PAGES / PPI;
     const Kv4Cache& c = a.c;
     const int lane = threadIdx.x;
     const int head = blockIdx.y % c.H, b = blockIdx.y / c.H;
     const int pages = (kv4_length(c, b) + KV4_PAGE - 1) / KV4_PAGE;
-    const int page = blockIdx.x * 64 + lane;
-    if (pages <= a.count || (int)(blockIdx.x * 64) >= pages) return;
-    int id = page < pages ? c.table[(long)b * c.table_stride + page] : -1;
-    const bool real = (unsigned)id < (unsigned)c.num_pages;
-    if (!real) id = 0;
-    const half8_t* const hi = (const half8_t*)(c.pool + ((long)id * c.H + head) * rec_bytes + rec_bytes - 4 * D);
-    const half8_t* const lo = hi + D / 8;
-    double best = -INFINITY;
+    const int first = blockIdx.x * SELECT_PAGES;
+    if (pages <= a.count || first >= pages) return;
+    const int sub = lane % LPP, slot = lane / LPP;
+    int id = first + lane < pages && lane < SELECT_PAGES ? c.table[(long)b * c.table_stride + first + lane] : -1;
+    u32x4_t hi[N], lo[N];
+    bool real[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        int p = __shfl(id, PPI * i + slot, 64);
+        real[i] = (unsigned)p < (unsigned)c.num_pages;
+        if (!real[i]) p = 0;
+        const uint8_t* const bounds = c.pool + ((long)p * c.H + head) * rec_bytes + rec_bytes - 4 * D + 16 * sub;
+        hi[i] = *(const u32x4_t*)bounds;
+        lo[i] = *(const u32x4_t*)(bounds + 2 * D);
+    }
+    double best[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) best[i] = -INFINITY;
     for (int g0 = 0; g0 < a.share; g0 += SELECT_QUERIES) {
-        const int ng = imin(SELECT_QUERIES, a.share - g0);
-        __syncthreads();
-        for (int i = lane; i < SELECT_QUERIES * D; i += 64) {
-            const int g = i / D, d = i % D;
-            const float x = g < ng ? (float)a.q[(long)b * a.q_ts + (long)(head * a.share + g0 + g) * a.q_hs + d] : 0.f;
-            qs[g][d][0] = fmaxf(x, 0.f);
-            qs[g][d][1] = fminf(x, 0.f);
-        }
-        __syncthreads();
-        double s[SELECT_QUERIES];
+        half8_t q[SELECT_QUERIES];
 #pragma unroll
-        for (int g = 0; g < SELECT_QUERIES; g++) s[g] = 0.0;
-        for (int d8 = 0; d8 < D / 8; d8++) {
-            const half8_t h8 = hi[d8], l8 = lo[d8];
+        for (int g = 0; g < SELECT_QUERIES; g++)  // (a round's queries beyond the last are the last again)
+            q[g] = *(const half8_t*)(a.q + (long)b * a.q_ts + (long)(head * a.share + imin(g0 + g, a.share - 1)) * a.q_hs + 8 * sub);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const double h = (double)(float)h8[e], l = (double)(float)l8[e];
+        for (int g = 0; g < SELECT_QUERIES; g++) {
+            const u32x4_t qb = bit_cast<u32x4_t>(q[g]);
+            uint32_t minus[4];
 #pragma unroll
-                for (int g = 0; g < SELECT_QUERIES; g++)
-                    s[g] += qs[g][8 * d8 + e][0] * h + qs[g][8 * d8 + e][1] * l;
+            for (int j = 0; j < 4; j++) minus[j] = bit_cast<uint32_t>(bit_cast<short2_t>(qb[j]) >> (short)15);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                double s = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const half2_t x = bit_cast<half2_t>((lo[i][j] & minus[j]) | (hi[i][j] & ~minus[j]));
+                    s += (double)((float)x[0] * (float)q[g][2 * j]);
+                    s += (double)((float)x[1] * (float)q[g][2 * j + 1]);
+                }
+                s += row_move<0xB1>(s);                // quad_perm 1,0,3,2
+                s += row_move<0x4E>(s);                // quad_perm 2,3,0,1
+                s += row_move<0x141>(s);               // row_half_mirror: the other quad of eight
+                if (D == 128) s += row_move<0x140>(s);  // row_mirror: the other eight
+                if (s > best[i]) best[i] = s;
             }
         }
-#pragma unroll
-        for (int g = 0; g < SELECT_QUERIES; g++)
-            if (g < ng && s[g] > best) best = s[g];
     }
-    if (page < pages) a.scores[((long)b * c.H + head) * c.width + page] = real ? best : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int page = first + PPI * i + slot;
+        if (sub == 0 && page < pages) a.scores[((long)b * c.H + head) * c.width + page] = real[i] ? best[i] : -INFINITY;
+    }
 }
 
 // A double as an unsigned number of the same order; one that is no number is the lowest.
@@ -467,7 +493,7 @@ hipError_t launch_kv4_select(const Kv4Cache& c, const void* q, void* selected, v
     a.keep_last = keep_last;
     const int heads = c.B * c.H;
     if (c.width > count) {
-        const dim3 grid((c.width + 63) / 64, heads);
+        const dim3 grid((c.width + SELECT_PAGES - 1) / SELECT_PAGES, heads);
         if (D == 128)
             hipLaunchKernelGGL(kv4_score_kernel<128>, grid, dim3(64), 0, st, a, kv4_record_bytes(D, g));
         else

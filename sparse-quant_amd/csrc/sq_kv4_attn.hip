@@ -19,145 +19,11 @@
 // instead of 2.8e-4, the rounding of P' and of the output).  P' is kept inside fp16's range by a power of two per group that
 // follows the scales.
 #include "sq_kernels.h"
-#include "sq_kv4.h"
-
-#include <type_traits>
+#include "sq_kv4_attn.h"
 
 namespace sq {
 
 namespace {
-
-template <int N>
-using Int = std::integral_constant<int, N>;
-
-struct Kv4AttnArgs {
-    Kv4Cache c;
-    const half_t* q;
-    half_t* out;          // [T][share * H][D]
-    const int* selected;  // [B][H][count] or null
-    float* ws;            // partial states, or null: no sequence is split
-    long q_ts, q_hs;      // element strides of q over token and head
-    int share;            // query heads of a key/value head
-    int count;
-    float scale;          // sm_scale * log2(e)
-};
-
-// How a launch's work is dealt.  A tile is R of the rows (token, query head) of a sequence and key/value head; a
-// workgroup takes one tile over a share of its pages.  The share's length follows from the lengths on the device: the pages
-// of all tiles over 256 per_cu workgroups, `least` at the fewest.
-struct Deal {
-    int per_cu, least;
-    __host__ __device__ int wgs() const { return 256 * per_cu; }
-};
-struct Piece {
-    int b, tile, head, share, shares;  // share of how many
-    int slot;                          // where its partial state goes (shares > 1)
-    int first, count, len;             // tokens and rows of the sequence
-};
-
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// A sequence's tokens, rows, pages and tiles.
-struct Sizes {
-    int first, count, len, pages, tiles;
-};
-template <int R>
-__device__ __forceinline__ Sizes sizes_of(const Kv4AttnArgs& a, int b) {
-    Sizes s = {0, 0, 0, 0, 0};
-    if (b < a.c.B) {
-        kv4_tokens(a.c, b, s.first, s.count);
-        s.len = kv4_length(a.c, b);
-        s.pages = ceil_div(s.len, KV4_PAGE);
-        if (a.selected) s.pages = imin(s.pages, a.count);
-        s.tiles = ceil_div(s.count * a.share, R) * a.c.H;
-    }
-    return s;
-}
-
-// The piece of workgroup `index` (SPLIT: of the index-th tile among those that are shared), by every wave alone: lane i
-// looks at sequence 64 k + i.
-template <int R, bool SPLIT>
-__device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int index, Piece& out) {
-    const int lane = threadIdx.x & 63;
-    const int B = a.c.B;
-    Sizes s = sizes_of<R>(a, lane);
-    int least = 1 << 30;
-    if (a.ws) {
-        unsigned long long units = 0;
-        for (int b0 = 0; b0 < B; b0 += 64) {
-            const Sizes t = b0 ? sizes_of<R>(a, b0 + lane) : s;
-            const unsigned long long mine = (unsigned long long)t.tiles * t.pages;
-            units += (unsigned)wave_sum((int)(mine & 0xffff)) + ((unsigned long long)(unsigned)wave_sum((int)(mine >> 16)) << 16);
-        }
-        const unsigned even = (unsigned)ceil_div((int)((units + 255) >> 8), d.per_cu);  // (T * Hq <= 2^30: at most 2^48 pages)
-        least = even > (unsigned)d.least ? (int)even : d.least;
-    }
-    int slots = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        if (b0) s = sizes_of<R>(a, b0 + lane);
-        const int shares = s.pages > least ? ceil_div(s.pages, least) : 1;
-        const int mine = SPLIT ? (shares > 1 ? s.tiles : 0) : s.tiles * shares;
-        const int upto = wave_scan(mine);
-        const int taken = shares > 1 ? s.tiles * shares : 0;
-        const int slots_upto = wave_scan(taken);
-        const unsigned long long past = __ballot(upto > index);
-        if (past) {
-            const int at = __ffsll(past) - 1;
-            const int rest = index - __builtin_amdgcn_readlane(upto - mine, at);
-            out.shares = __builtin_amdgcn_readlane(shares, at);
-            const int tile = SPLIT || out.shares == 1 ? rest : rest / out.shares;
-            out.b = b0 + at;
-            out.share = SPLIT ? 0 : rest - tile * out.shares;
-            out.head = tile % a.c.H;
-            out.tile = tile / a.c.H;
-            out.slot = slots + __builtin_amdgcn_readlane(slots_upto - taken, at) + tile * out.shares + out.share;
-            out.first = __builtin_amdgcn_readlane(s.first, at);
-            out.count = __builtin_amdgcn_readlane(s.count, at);
-            out.len = __builtin_amdgcn_readlane(s.len, at);
-            return true;
-        }
-        index -= __builtin_amdgcn_readlane(upto, 63);
-        slots += __builtin_amdgcn_readlane(slots_upto, 63);
-    }
-    return false;
-}
-
-template <int CTRL>
-__device__ __forceinline__ float row_move(float v) {
-    return bit_cast<float>(__builtin_amdgcn_update_dpp(0, bit_cast<int>(v), CTRL, 0xF, 0xF, false));
-}
-// A value and that of the lane 16 (32) away, on every lane.
-__device__ __forceinline__ void pair16(float v, float& a, float& b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
-    a = bit_cast<float>((uint32_t)r[0]);
-    b = bit_cast<float>((uint32_t)r[1]);
-}
-__device__ __forceinline__ void pair32(float v, float& a, float& b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
-    a = bit_cast<float>((uint32_t)r[0]);
-    b = bit_cast<float>((uint32_t)r[1]);
-}
-__device__ __forceinline__ float rows_sum(float v) {  // over the four lanes of a column
-    float a, b;
-    pair16(v, a, b);
-    pair32(a + b, a, b);
-    return a + b;
-}
-__device__ __forceinline__ float rows_max(float v) {
-    float a, b;
-    pair16(v, a, b);
-    pair32(fmaxf(a, b), a, b);
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, row_move<0x121>(v));  // row_ror:1
-    v = fmaxf(v, row_move<0x122>(v));
-    v = fmaxf(v, row_move<0x124>(v));
-    v = fmaxf(v, row_move<0x128>(v));
-    return rows_max(v);
-}
-
-constexpr float KA_LAZY = 8.f;  // the softmax's reference moves when a score is 2^8 beyond it
 
 // The kernel for few rows.  A workgroup's waves take units of 16 max(2, PACK) rows of the cache in turn, each with a softmax
 // of its own, and join them in LDS.
@@ -569,58 +435,6 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     }
 }
 
-// Shares of a tile's pages, joined: a workgroup per row of a shared tile.
-template <int D, int R>
-__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, Deal d) {
-    constexpr int C4 = D / 4, LANES = 256 / C4;
-    __shared__ __attribute__((aligned(16))) float part[LANES][D];
-    __shared__ float state[LANES][2];
-    Piece pc;
-    if (!deal<R, true>(a, d, blockIdx.x, pc)) return;
-    if (pc.slot + pc.shares > 2 * d.wgs()) return;  // (only where lengths change under the launch)
-    const int r = blockIdx.y;
-    const int rr = pc.tile * R + r;
-    if (rr >= pc.count * a.share) return;
-    const float* const base = a.ws + (long)pc.slot * R * (D + 2);
-    const int c4 = threadIdx.x % C4, part0 = threadIdx.x / C4;
-    float m = -INFINITY, sum = 0.f;
-    float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = part0; s < pc.shares; s += LANES) {
-        const float* const src = base + (long)s * R * (D + 2);
-        const float ms = src[R * D + 2 * r], ls = src[R * D + 2 * r + 1];
-        const float4_t v = *(const float4_t*)(src + r * D + 4 * c4);
-        const float to = fmaxf(m, ms);
-        const float f0 = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to), f1 = ms == to ? 1.f : __builtin_amdgcn_exp2f(ms - to);
-        sum = sum * f0 + ls * f1;
-        o = o * f0 + v * f1;
-        m = to;
-    }
-    *(float4_t*)&part[part0][4 * c4] = o;
-    if (c4 == 0) {
-        state[part0][0] = m;
-        state[part0][1] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x >= C4) return;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < LANES; w++) mx = fmaxf(mx, state[w][0]);
-    sum = 0.f;
-    o = (float4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < LANES; w++) {
-        const float mw = state[w][0];
-        const float f = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
-        sum += state[w][1] * f;
-        o += *(const float4_t*)&part[w][4 * c4] * f;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    half4_t h;
-#pragma unroll
-    for (int e = 0; e < 4; e++) h[e] = (half_t)(o[e] * inv);
-    *(half4_t*)(a.out + ((long)(pc.first + rr / a.share) * a.c.H * a.share + pc.head * a.share + rr % a.share) * D + 4 * c4) = h;
-}
-
 // Workgroups that a launch's pages are dealt to, and a share's fewest pages: see launch_kv4_attention.
 constexpr Deal KA_DEAL = {2, 16};
 constexpr int KA_ROWS = 32;  // of a tile at the most
@@ -630,8 +444,9 @@ constexpr int KA_ROWS = 32;  // of a tile at the most
 // At most 2 wgs() shares of shared tiles: a tile of p pages has fewer than p / least + 1, there are at most wgs() * least
 // pages in all, and every shared tile has more than `least` of them.
 size_t kv4_attention_workspace_bytes(int T, int B, int share, int D, int pages) {
-    if (pages <= KA_DEAL.least) return 0;
     const long mean = ((long)T * share + B - 1) / B;
+    if (mean > KA_ROWS) return kv4_chunk_workspace_bytes(D, pages);
+    if (pages <= KA_DEAL.least) return 0;
     const int rows = mean <= 4 ? 4 : mean <= 8 ? 8 : mean <= 16 ? 16 : KA_ROWS;
     return (size_t)(2 * KA_DEAL.wgs()) * rows * (D + 2) * sizeof(float);
 }
@@ -648,11 +463,15 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
     a.share = share;
     a.count = count;
     a.scale = sm_scale * 1.44269504088896340736f;
+    // Rows of a sequence and key/value head (of the average one where they differ).
+    const long mean = ((long)c.T * share + c.B - 1) / c.B;
+    if (mean > KA_ROWS && !selected) {
+        a.ws = (float*)workspace;
+        return launch_kv4_chunk(a, D, g, st);
+    }
     const int most = selected && count < c.width ? count : c.width;
     const bool split = workspace != nullptr && most > KA_DEAL.least;
     a.ws = split ? (float*)workspace : nullptr;
-    // Rows of a sequence and key/value head (of the average one where they differ).
-    const long mean = ((long)c.T * share + c.B - 1) / c.B;
     auto go = [&](auto d, auto groups, auto pack, auto rt, auto waves) {
         constexpr int R = 16 / pack.value * rt.value;
         const long tiles = (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
@@ -663,7 +482,7 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         const long tokens = c.starts ? R : c.each;
         const unsigned rows = (unsigned)(tokens * share < R ? tokens * share : R);
         const long shared = tiles < KA_DEAL.wgs() ? tiles : KA_DEAL.wgs();
-        hipLaunchKernelGGL((kv4_join_kernel<d.value, R>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
+        hipLaunchKernelGGL((kv4_join_kernel<d.value, R, false>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
     };
     auto by_rows = [&](auto d, auto groups) {
         if (mean <= 4)
