@@ -59,6 +59,20 @@ template <int R, bool SPLIT>
 __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int index, Piece& out) {
     const int lane = threadIdx.x & 63;
     const int B = a.c.B;
+    if (!SPLIT && !a.ws && !a.c.starts) {  // nothing is shared, every sequence has as many tiles: no length is waited for here
+        const int tiles = ceil_div(a.c.each * a.share, R) * a.c.H;
+        out.b = index / tiles;
+        const int tile = index - out.b * tiles;
+        out.tile = tile / a.c.H;
+        out.head = tile - out.tile * a.c.H;
+        out.share = out.slot = 0;
+        out.shares = 1;
+        out.first = out.b * a.c.each;
+        out.count = a.c.each;
+        if (out.b >= B) return false;
+        out.len = kv4_length(a.c, out.b);
+        return true;
+    }
     Sizes s = sizes_of<R>(a, lane);
     int least = 1 << 30;
     if (a.ws) {
@@ -68,8 +82,8 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
             const unsigned long long mine = (unsigned long long)t.tiles * t.pages;
             units += (unsigned)wave_sum((int)(mine & 0xffff)) + ((unsigned long long)(unsigned)wave_sum((int)(mine >> 16)) << 16);
         }
-        const unsigned even = (unsigned)ceil_div((int)((units + 255) >> 8), d.per_cu);  // (T * Hq <= 2^30: at most 2^48 pages)
-        least = even > (unsigned)d.least ? (int)even : d.least;
+        const int even = ceil_div((int)((units + 255) >> 8), d.per_cu);  // (T * Hq <= 2^30: at most 2^48 pages)
+        least = imax(even, d.least);
     }
     int slots = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
@@ -138,51 +152,65 @@ __device__ __forceinline__ float wave_max(float v) {
 
 constexpr float KA_LAZY = 8.f;  // the softmax's reference moves when a score is 2^8 beyond it
 
-// Shares of a tile's pages, joined: a workgroup per row of a shared tile.
-// (LAST: tiles are worked on from the last to the first)
-template <int D, int R, bool LAST>
+// Shares of a tile's pages, joined: a workgroup has ROWS rows of a shared tile, 256 / ROWS threads each, of which D / 4 hold
+// four columns each of every so many-th share.  (LAST: tiles are worked on from the last to the first.)
+template <int D, int R, int ROWS, bool LAST>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, Deal d) {
-    constexpr int C4 = D / 4, LANES = 256 / C4;
-    __shared__ __attribute__((aligned(16))) float part[LANES][D];
-    __shared__ float state[LANES][2];
+    constexpr int C4 = D / 4, LANES = 256 / C4 / ROWS;
+    static_assert(LANES >= 1 && R % ROWS == 0);
+    __shared__ __attribute__((aligned(16))) float part[ROWS][LANES][D];
+    __shared__ float state[ROWS][LANES][2];
     Piece pc;
     if (!deal<R, true>(a, d, blockIdx.x, pc)) return;
     if (pc.slot + pc.shares > 2 * d.wgs()) return;  // (only where lengths change under the launch)
-    const int r = blockIdx.y;
+    const int c4 = threadIdx.x % C4, lane = threadIdx.x / C4 % LANES, sub = threadIdx.x / (C4 * LANES);
+    const int r = blockIdx.y * ROWS + sub;
     const int rr = (LAST ? ceil_div(pc.count * a.share, R) - 1 - pc.tile : pc.tile) * R + r;
-    if (rr >= pc.count * a.share) return;
+    const bool live = rr < pc.count * a.share;
     const float* const base = a.ws + (long)pc.slot * R * (D + 2);
-    const int c4 = threadIdx.x % C4, part0 = threadIdx.x / C4;
     float m = -INFINITY, sum = 0.f;
     float4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = part0; s < pc.shares; s += LANES) {
-        const float* const src = base + (long)s * R * (D + 2);
-        const float ms = src[R * D + 2 * r], ls = src[R * D + 2 * r + 1];
-        const float4_t v = *(const float4_t*)(src + r * D + 4 * c4);
-        const float to = fmaxf(m, ms);
-        const float f0 = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to), f1 = ms == to ? 1.f : __builtin_amdgcn_exp2f(ms - to);
-        sum = sum * f0 + ls * f1;
-        o = o * f0 + v * f1;
-        m = to;
-    }
-    *(float4_t*)&part[part0][4 * c4] = o;
+    constexpr int AHEAD = 4;  // shares whose states are asked for at once
+    if (live)
+        for (int s0 = lane; s0 < pc.shares; s0 += LANES * AHEAD) {
+            float ms[AHEAD], ls[AHEAD];
+            float4_t v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const float* const src = base + (long)imin(s0 + LANES * i, pc.shares - 1) * R * (D + 2);
+                ms[i] = src[R * D + 2 * r];
+                ls[i] = src[R * D + 2 * r + 1];
+                v[i] = *(const float4_t*)(src + r * D + 4 * c4);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (s0 + LANES * i < pc.shares) {
+                    const float to = fmaxf(m, ms[i]);
+                    const float f0 = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
+                    const float f1 = ms[i] == to ? 1.f : __builtin_amdgcn_exp2f(ms[i] - to);
+                    sum = sum * f0 + ls[i] * f1;
+                    o = o * f0 + v[i] * f1;
+                    m = to;
+                }
+        }
+    *(float4_t*)&part[sub][lane][4 * c4] = o;
     if (c4 == 0) {
-        state[part0][0] = m;
-        state[part0][1] = sum;
+        state[sub][lane][0] = m;
+        state[sub][lane][1] = sum;
     }
     __syncthreads();
-    if (threadIdx.x >= C4) return;
+    if (lane != 0 || !live) return;
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < LANES; w++) mx = fmaxf(mx, state[w][0]);
+    for (int w = 0; w < LANES; w++) mx = fmaxf(mx, state[sub][w][0]);
     sum = 0.f;
     o = (float4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < LANES; w++) {
-        const float mw = state[w][0];
+        const float mw = state[sub][w][0];
         const float f = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
-        sum += state[w][1] * f;
-        o += *(const float4_t*)&part[w][4 * c4] * f;
+        sum += state[sub][w][1] * f;
+        o += *(const float4_t*)&part[sub][w][4 * c4] * f;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     half4_t h;

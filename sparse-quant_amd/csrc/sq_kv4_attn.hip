@@ -25,7 +25,7 @@ namespace sq {
 
 namespace {
 
-// The kernel for few rows.  A workgroup's waves take units of 16 max(2, PACK) rows of the cache in turn, each with a softmax
+// The kernel for few rows.  A workgroup's waves take units of a page (PACK = 1: half of one) in turn, each with a softmax
 // of its own, and join them in LDS.
 //
 // PACK.  The matrix instruction has 16 columns for the tile's rows; with 4 rows, 12 of them would be empty, and so would
@@ -35,7 +35,7 @@ namespace {
 // way round: of its operand, the columns of other tiles are masked off.
 template <int D, int G, int PACK>
 struct Unit {
-    static constexpr int TILES = PACK == 4 ? 4 : 2, SETS = TILES / PACK, ROWS = 16 * TILES;
+    static constexpr int TILES = PACK > 1 ? 4 : 2, SETS = TILES / PACK, ROWS = 16 * TILES;
     uint32_t k[TILES][D / 32];  // [words of the lane's row and chunk]
     u32x4_t v[TILES];
     half8_t ksm[SETS][G], vsm[SETS][G];  // scales and minima of four rows
@@ -65,6 +65,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     if (!deal<R, false>(a, d, blockIdx.x, pc)) return;
     if (pc.shares > 1 && pc.slot >= 2 * d.wgs()) return;  // (only where lengths change under the launch)
     const int head = pc.head, tile = pc.tile, len = pc.len;
+    const int* const table = c.table + (long)pc.b * c.table_stride;
+    const int* const chosen = a.selected ? a.selected + ((long)pc.b * c.H + head) * a.count : nullptr;
+    // The first 64 pages, or the places of the selected ones, without waiting for the length.
+    int ahead = -1;
+    if (lane < (chosen ? a.count : c.width)) ahead = chosen ? chosen[lane] : table[lane];
 
     const int n = lane & 15, l4 = lane >> 4;
     const int col = n & (COLS - 1), part_of = n / COLS;  // the lane's query, and which of PACK tiles of cache rows
@@ -142,14 +147,12 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     const uint32_t vsel = D == 64 && n >= 8 ? 0x07060302u : 0x05040100u;
     constexpr int PER = KV4_PAGE / U::ROWS;  // units of a page
 
-    const int* const table = c.table + (long)pc.b * c.table_stride;
-    const int* const chosen = a.selected ? a.selected + ((long)pc.b * c.H + head) * a.count : nullptr;
     // Pages are looked up 64 at a time: lane i has the i-th one's place in the sequence and in the pool.
     for (int pb = p0; pb < p1; pb += 64) {
         int place = pb + lane, id = -1;
         if (place < p1) {
-            if (chosen) place = chosen[place];
-            if ((unsigned)place < (unsigned)all_pages) id = table[place];
+            if (chosen) place = pb == 0 ? ahead : chosen[place];
+            if ((unsigned)place < (unsigned)all_pages) id = pb == 0 && !chosen ? ahead : table[place];
             if ((unsigned)id >= (unsigned)c.num_pages) id = -1;
         }
         if (id < 0) place = 0;  // a page that does not exist: its rows lie behind every query's last
@@ -472,9 +475,12 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
     const int most = selected && count < c.width ? count : c.width;
     const bool split = workspace != nullptr && most > KA_DEAL.least;
     a.ws = split ? (float*)workspace : nullptr;
+    auto tiles_of = [&](int R) {
+        return (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
+    };
     auto go = [&](auto d, auto groups, auto pack, auto rt, auto waves) {
         constexpr int R = 16 / pack.value * rt.value;
-        const long tiles = (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
+        const long tiles = tiles_of(R);
         const long wgs = split ? tiles + KA_DEAL.wgs() : tiles;
         hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value, pack.value, rt.value, waves.value>), dim3((unsigned)wgs),
                            dim3(64 * waves.value), 0, st, a, KA_DEAL);
@@ -482,17 +488,20 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         const long tokens = c.starts ? R : c.each;
         const unsigned rows = (unsigned)(tokens * share < R ? tokens * share : R);
         const long shared = tiles < KA_DEAL.wgs() ? tiles : KA_DEAL.wgs();
-        hipLaunchKernelGGL((kv4_join_kernel<d.value, R, false>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
+        hipLaunchKernelGGL((kv4_join_kernel<d.value, R, 1, false>), dim3((unsigned)shared, rows), dim3(256), 0, st, a, KA_DEAL);
     };
     auto by_rows = [&](auto d, auto groups) {
-        if (mean <= 4)
+        const bool one = !split && tiles_of(4) <= 256;
+        if (mean <= 4 && one)
+            go(d, groups, Int<4>{}, Int<1>{}, Int<8>{});
+        else if (mean <= 4)
             go(d, groups, Int<4>{}, Int<1>{}, Int<4>{});
         else if (mean <= 8)
             go(d, groups, Int<2>{}, Int<1>{}, Int<4>{});
         else if (mean <= 16)
             go(d, groups, Int<1>{}, Int<1>{}, Int<4>{});
         else
-            go(d, groups, Int<1>{}, Int<2>{}, Int<4>{});
+            go(d, groups, Int<1>{}, Int<2>{}, Int<8>{});
     };
     if (D == 128 && g == 128) by_rows(Int<128>{}, Int<1>{});
     if (D == 128 && g == 64) by_rows(Int<128>{}, Int<2>{});

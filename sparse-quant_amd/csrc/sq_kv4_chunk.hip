@@ -184,17 +184,27 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
 #pragma unroll
     for (int i = 0; i < G; i++) mins[i] = 0.f, sref[i] = 0x1p-24f;
 
-    auto block = [&](auto masked, int pos, const Stage& st, int kb) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked)::value;
-        float16_t dot[G];
+    auto dots = [&](const Stage& st, int kb, float16_t (&dot)[G]) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < G; i++)
 #pragma unroll
             for (int v = 0; v < 16; v++) dot[i][v] = 0.f;
+        u32x4_t kf[ST];  // all asked for before the first product
+#pragma unroll
+        for (int i = 0; i < ST; i++) kf[i] = st.k[2 * i + hl][32 * kb + n];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < ST; i++)
-            dot[16 * i / g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(st.k[2 * i + hl][32 * kb + n]), qf[i],
-                                                                     dot[16 * i / g], 0, 0, 0);
+            dot[16 * i / g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(kf[i]), qf[i], dot[16 * i / g], 0, 0, 0);
+    };
+    auto block = [&](auto masked, int pos, const Stage& st, int kb, const float16_t (&dot)[G]) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
+        u32x4_t vf[2][DT];  // and these before the softmax
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int t = 0; t < DT; t++) vf[u][t] = st.v[2 * (2 * kb + u) + hl][32 * t + n];
+        __builtin_amdgcn_sched_barrier(0);
         float s[16], top = -INFINITY;
 #pragma unroll
         for (int qd = 0; qd < 4; qd++) {
@@ -251,8 +261,7 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int t = 0; t < DT; t++)
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(st.v[2 * (2 * kb + u) + hl][32 * t + n]),
-                                                                pf[u][32 * t / g], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(vf[u][t]), pf[u][32 * t / g], acc[t], 0, 0, 0);
     };
 
     if (p0 < p1) {
@@ -281,8 +290,11 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
             }
         }
         if (id >= 0) {  // a page that does not exist is seen by nobody
-            block(masked, p * KV4_PAGE, st, 0);
-            block(masked, p * KV4_PAGE + 32, st, 1);
+            float16_t dot[G];
+            dots(st, 0, dot);
+            block(masked, p * KV4_PAGE, st, 0, dot);
+            dots(st, 1, dot);
+            block(masked, p * KV4_PAGE + 32, st, 1, dot);
         }
         barrier();
     };
@@ -357,7 +369,8 @@ hipError_t launch_kv4_chunk(Kv4AttnArgs a, int D, int g, hipStream_t st) {
         hipLaunchKernelGGL((kv4_chunk_kernel<d.value, groups.value>), dim3((unsigned)wgs), dim3(64 * KC_WAVES), 0, st, a, KC_DEAL);
         if (!split) return;
         const long shared = tiles < KC_DEAL.wgs() ? tiles : KC_DEAL.wgs();
-        hipLaunchKernelGGL((kv4_join_kernel<d.value, KC_ROWS, true>), dim3((unsigned)shared, KC_ROWS), dim3(256), 0, st, a, KC_DEAL);
+        hipLaunchKernelGGL((kv4_join_kernel<d.value, KC_ROWS, 4, true>), dim3((unsigned)shared, KC_ROWS / 4), dim3(256), 0, st, a,
+                           KC_DEAL);
     };
     if (D == 128 && g == 128) go(Int<128>{}, Int<1>{});
     if (D == 128 && g == 64) go(Int<128>{}, Int<2>{});
