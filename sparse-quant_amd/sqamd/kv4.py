@@ -386,14 +386,31 @@ class KV4Cache:
         at = torch.tensor(list(seqs), device=self.table.device)
         return self.table[at], self.lengths[at]
 
+    def layer(self, index, seqs):
+        """One layer's operators for these sequences (an int n: the first n), bound to the cache's tables as they are."""
+        return LayerOf(self.pool[index], *self.batch(seqs))
+
     def append(self, layer, k, v, seqs, starts=None, values=False):
-        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
-        return append(k, v, self.pool[layer], pages, lengths, starts, values)
+        return self.layer(layer, seqs).append(k, v, starts, values)
 
     def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None):
-        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
-        return attention(q, self.pool[layer], pages, lengths, sm_scale, starts, selected, out)
+        return self.layer(layer, seqs).attention(q, sm_scale, starts, selected, out)
 
     def select_pages(self, layer, q, count, seqs, keep_first=1, keep_last=1):
-        pages, lengths = self.batch(seqs) if not isinstance(seqs, tuple) else seqs
-        return select_pages(q, self.pool[layer], pages, lengths, count, keep_first, keep_last)
+        return self.layer(layer, seqs).select_pages(q, count, keep_first, keep_last)
+
+
+class LayerOf:
+    """A pool with the tables of some sequences: append, attention and select_pages without naming them again."""
+
+    def __init__(self, pool, pages, lengths):
+        self.pool, self.pages, self.lengths = pool, pages, lengths
+
+    def append(self, k, v, starts=None, values=False):
+        return append(k, v, self.pool, self.pages, self.lengths, starts, values)
+
+    def attention(self, q, sm_scale, starts=None, selected=None, out=None):
+        return attention(q, self.pool, self.pages, self.lengths, sm_scale, starts, selected, out)
+
+    def select_pages(self, q, count, keep_first=1, keep_last=1):
+        return select_pages(q, self.pool, self.pages, self.lengths, count, keep_first, keep_last)

@@ -14,6 +14,10 @@ default; a layer that has been given a look-up table (`DecoderLayer.lut`, per he
 prefill over the table's blocks (sparse_attention(q, k, v, scaling, lut, LT=True) in the reference's OPT
 attention, test/nvidia/module/opt/modeling_opt_ours.py:435-438).  Either way a prompt's attention is one kernel
 that also fills the cache (sq_lut_attention_strided).
+
+With `new_cache(batch, max_len, kv_bits=4)` the keys and values are held in 4 bits, in pages (kv4.KV4Cache): a layer quantises
+its rows into the cache and attends over what is held there, in prompts as in steps (over a look-up table: the prompt's
+attention is given the values that the cache holds).
 """
 import math
 import time
@@ -21,7 +25,7 @@ import time
 import torch
 from torch import nn
 
-from . import capi, lut_layout
+from . import capi, kv4, lut_layout
 from .block_sparse_attention_lut import sparse_attention
 from .qlinear import WALinear
 
@@ -66,7 +70,8 @@ class DecoderLayer(nn.Module):
         self.capture = None  # a dict: the prefill's q, k, v and attention output are left in it (tests)
 
     def forward(self, x, kc, vc, pos0):
-        """x [B, T, H]; kc, vc [B, heads, Lmax, hd]; writes cache rows pos0 .. pos0+T-1."""
+        """x [B, T, H]; kc, vc [B, heads, Lmax, hd], or kc a layer of a 4-bit cache and vc None; writes cache rows pos0 ..
+        pos0+T-1."""
         b, t, hdim = x.shape
         if self.qkv_proj is not None:
             # the first LayerNorm rides in the q/k/v launch (inside the kernel at decode batch sizes)
@@ -83,7 +88,9 @@ class DecoderLayer(nn.Module):
             k = self.k_proj(flat).view(b, t, self.heads, self.hd).transpose(1, 2)
             v = self.v_proj(flat).view(b, t, self.heads, self.hd).transpose(1, 2)
         scale = 1.0 / math.sqrt(self.hd)
-        if isinstance(pos0, int) and pos0 == 0 and t > 1 and capi.lut_attention_strided_ok(q, k, v, kc, vc) \
+        if vc is None:
+            a = self._attend_4bit(q, k, v, kc, pos0, scale)
+        elif isinstance(pos0, int) and pos0 == 0 and t > 1 and capi.lut_attention_strided_ok(q, k, v, kc, vc) \
                 and (self.lut is None or self.lut.dtype in (torch.int32, torch.int64)):
             # a whole prompt: one kernel reads q, k and v where the projection left them, fills the cache and writes
             # [b, t, hidden] (without a table: every block up to the diagonal)
@@ -116,6 +123,21 @@ class DecoderLayer(nn.Module):
             h = self.fc1(_layernorm(self.ln2, x).reshape(1, b * t, hdim), act="relu")
         return self.fc2(h, residual=x.reshape(1, b * t, hdim)).view(b, t, hdim)
 
+    def _attend_4bit(self, q, k, v, cache, pos0, scale):
+        """q, k, v [B, heads, T, hd] -> [1, B * T, hidden]; the cache's lengths count these rows already."""
+        b, h, t, hd = q.shape
+        q4, k4, v4 = (x.transpose(1, 2).reshape(b * t, h, hd) for x in (q, k, v))
+        if self.lut is not None and isinstance(pos0, int) and pos0 == 0 and t > 1:
+            k_hat, v_hat = (x.view(b, t, h, hd).transpose(1, 2) for x in cache.append(k4, v4, values=True))
+            a = capi.lut_attention_strided(q, k_hat, v_hat, self.lut.contiguous().to(q.device), scale, True, rows_first=True)
+        else:
+            cache.append(k4, v4)
+            a = cache.attention(q4, scale)
+        if self.capture is not None:
+            self.capture.update(q=q.detach().clone(), k=k.detach().clone(), v=v.detach().clone(),
+                                a=a.view(b, t, h, hd).transpose(1, 2).detach().clone())
+        return a.view(1, b * t, h * hd)
+
     def fuse_qkv(self):
         """Serve q, k and v with one launch: layout L1 is row-major in N, so the three weights
         (and their zeros_scales and biases) concatenate along the output dimension."""
@@ -127,6 +149,18 @@ class DecoderLayer(nn.Module):
         fused.bias = torch.cat([p.bias for p in ps], 1).contiguous()
         self.qkv_proj = fused
         self.q_proj = self.k_proj = self.v_proj = None
+
+
+def _per_layer(cache, batch, tokens, pos0):
+    """A cache's layers as DecoderLayer.forward takes them; a 4-bit cache's lengths are counted up to behind the rows that
+    it will write (on the device where the position lives there)."""
+    if not isinstance(cache, kv4.KV4Cache):
+        return cache
+    if isinstance(pos0, int):
+        cache.set_lengths(list(range(batch)), pos0 + tokens)
+    else:
+        cache.lengths[:batch] = pos0 + tokens
+    return [(cache.layer(i, batch), None) for i in range(cache.layers)]
 
 
 class OPTDecoder(nn.Module):
@@ -156,8 +190,16 @@ class OPTDecoder(nn.Module):
             layout = lut_layout.synth_layout(self.heads, nb, density, causal=True, seed=seed + idx)
             layer.lut = lut_layout.layout2lut_single_density(layout[None])[0].to(self.embed.device)
 
-    def new_cache(self, batch, max_len):
+    def new_cache(self, batch, max_len, kv_bits=16, kv_group=64):
         hd = self.hidden // self.heads
+        if kv_bits == 4:
+            pages = (max_len + kv4.PAGE - 1) // kv4.PAGE
+            cache = kv4.KV4Cache(len(self.layers), batch * pages, self.heads, hd, kv_group, batch, max_len, self.embed.device)
+            seqs = [cache.add() for _ in range(batch)]
+            cache.reserve(seqs, max_len)
+            return cache
+        if kv_bits != 16:
+            raise ValueError("the cache is held in 16 or 4 bits, not %r" % (kv_bits,))
         shape = (batch, self.heads, max_len, hd)
         dev = self.embed.device
         return [(torch.zeros(shape, dtype=torch.float16, device=dev), torch.zeros(shape, dtype=torch.float16, device=dev))
@@ -173,7 +215,7 @@ class OPTDecoder(nn.Module):
             if pos_ids is None:
                 pos_ids = torch.arange(pos0, pos0 + t, device=ids.device) + 2
             x = self.embed[ids] + self.pos[pos_ids]
-        for layer, (kc, vc) in zip(self.layers, cache):
+        for layer, (kc, vc) in zip(self.layers, _per_layer(cache, b, t, pos0)):
             x = layer(x, kc, vc, pos0)
         x = _layernorm(self.final_ln, x[:, -1:])
         w = self.lm_head
@@ -194,7 +236,7 @@ class OPTDecoder(nn.Module):
         if getattr(self, "_parts", None) is None:
             self._parts = capi.f16_gemv_parts(self.lm_head.shape[0], self.lm_head.device)
         x = capi.embed_rows(self.embed, self.pos, tok.view(-1), pos_t, 2).view(b, 1, self.hidden)
-        for layer, (kc, vc) in zip(self.layers, cache):
+        for layer, (kc, vc) in zip(self.layers, _per_layer(cache, b, 1, pos_t)):
             x = layer(x, kc, vc, pos_t)
         x = _layernorm(self.final_ln, x.view(b, self.hidden))
         logits = capi.f16_gemv(x, self.lm_head, parts=self._parts)
@@ -204,7 +246,8 @@ class OPTDecoder(nn.Module):
 
 @torch.no_grad()
 def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed=0, fuse_qkv=True,
-            return_tokens=False, lut_density=0.26, scale_std=E2E_SCALE_STD, scale_min=E2E_SCALE_MIN, fused_ends=True):
+            return_tokens=False, lut_density=0.26, scale_std=E2E_SCALE_STD, scale_min=E2E_SCALE_MIN, fused_ends=True,
+            kv_bits=16):
     """Greedy generation on random token ids; returns timing and throughput figures."""
     dev = "cuda"
     model = OPTDecoder(layers=layers, dev=dev, seed=seed, scale_std=scale_std, scale_min=scale_min)
@@ -215,7 +258,7 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     gen.manual_seed(seed + 1)
     ids = torch.randint(0, 50272, (batch, prompt), device=dev, generator=gen)
     max_len = prompt + new_tokens
-    cache = model.new_cache(batch, max_len)
+    cache = model.new_cache(batch, max_len, kv_bits)
 
     model(ids, cache, 0)  # untimed first pass: code objects, library handles and workspaces come into being here
     torch.cuda.synchronize()
@@ -300,7 +343,8 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     lin = lambda n, k: n * k // 2 + (k // g) * n * 4 + batch * k * 2 + batch * n * 2
     rows_avg = prompt + (steps + 1) / 2.0
     per_layer = lin(3 * hidden, hidden) + lin(hidden, hidden) + lin(ffn, hidden) + lin(hidden, ffn) + \
-        2 * batch * hidden * rows_avg * 2
+        (2 * batch * hidden * rows_avg * 2 if kv_bits == 16 else
+         batch * hidden * rows_avg * (1 + 8 / cache.group_size))
     step_bytes = layers * per_layer + vocab * hidden * 2
     step_s = decode_s / steps
     return {
@@ -316,7 +360,8 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
                  "launch" + ("; embeddings, fp16 lm_head + argmax, token feedback as three launches inside the step"
                              if fused_ends else ""),
         "prefill_ms": round(prefill_s * 1e3, 2),
-        "prefill_attention": "dense causal (sq_lut_attention_strided without a table)",
+        "prefill_attention": "dense causal (%s)" % ("sq_lut_attention_strided without a table" if kv_bits == 16 else
+                                                     "sq_kv4_attention over the cache in 4 bits"),
         "prefill_lut_ms": None if prefill_lut_s is None else round(prefill_lut_s * 1e3, 2),
         "prefill_lut_attention": None if prefill_lut_s is None else
         "causal per-head tables in every layer, block density %.2f, D = 128 (sq_lut_attention_strided)" % lut_density,
@@ -338,4 +383,4 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
 if __name__ == "__main__":
     import json
     import sys
-    print(json.dumps(run_e2e(use_graph="--no-graph" not in sys.argv)))
+    print(json.dumps(run_e2e(use_graph="--no-graph" not in sys.argv, kv_bits=4 if "--kv4" in sys.argv else 16)))
