@@ -62,4 +62,27 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 __device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
+// A value and that of the lane 16 (32) away, on every lane.
+__device__ __forceinline__ void pair16(float v, float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+    a = bit_cast<float>((uint32_t)r[0]);
+    b = bit_cast<float>((uint32_t)r[1]);
+}
+__device__ __forceinline__ void pair32(float v, float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+    a = bit_cast<float>((uint32_t)r[0]);
+    b = bit_cast<float>((uint32_t)r[1]);
+}
+__device__ __forceinline__ float rows_sum(float v) {  // over the four lanes of a column
+    float a, b;
+    pair16(v, a, b);
+    pair32(a + b, a, b);
+    return a + b;
+}
+__device__ __forceinline__ float rows_max(float v) {
+    float a, b;
+    pair16(v, a, b);
+    pair32(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
 }  // namespace sq

@@ -1,7 +1,7 @@
 // A key/value cache held in 4 bits: quantising new rows into it, choosing pages by a bound of their scores, copying
 // pages (layout: sq_kv4.h; attention: sq_kv4_attn.hip).
 #include "sq_kernels.h"
-#include "sq_kv4.h"
+#include "sq_kv4_row.h"
 
 #include <type_traits>
 
@@ -11,11 +11,8 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------------- append
 //
-// Per row and group of g elements: m = min x, s = fp16((max x - m) / 15), code = round((x - m) / s) in 0..15, the
-// element then reads as s * code + m.  All steps in fp32 with one rounding each (the division included), so that the
-// codes are those of any IEEE implementation.  An infinity or a NaN in a group makes its scale one: the group reads
-// as NaN.  A workgroup owns one page of one head and with it the page's bounds, so nothing is shared between
-// workgroups and nothing is atomic.
+// A workgroup owns one page of one head and with it the page's bounds, so nothing is shared between workgroups and nothing is
+// atomic (the row itself: sq_kv4_row.h).
 struct Kv4AppendArgs {
     Kv4Cache c;
     const half_t* k;
@@ -25,32 +22,13 @@ struct Kv4AppendArgs {
     long k_ts, k_hs, v_ts, v_hs;  // element strides over token and head
 };
 
-struct Group {
-    float s, m;
-    half_t sh, mh;
-};
-
-// A group's scale and minimum from its extremes; bad: 0, or NaN where an element is no finite number.
-__device__ __forceinline__ Group group_of(float lo, float hi, float bad) {
-    Group r;
-    r.sh = (half_t)((hi - lo) / 15.f + bad);
-    r.mh = (half_t)lo;
-    r.s = (float)r.sh;
-    r.m = lo;
-    return r;
-}
-__device__ __forceinline__ int code_of(float x, const Group& g) {
-    const float c = rintf((x - g.m) / g.s);
-    return g.s > 0.f ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
-}
-
 template <int D, int G, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void kv4_append_kernel(Kv4AppendArgs a) {
     constexpr int g = D / G;
     constexpr int LPR = D / 8;     // lanes of a row
     constexpr int RPW = 64 / LPR;  // rows of a wave
     constexpr int REC = kv4_record_bytes(D, g);
-    __shared__ float ext[WAVES][2][D];
+    __shared__ __attribute__((aligned(16))) half2_t ext[WAVES][2][D / 2];
     const Kv4Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head = blockIdx.x % c.H;
@@ -106,134 +84,83 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_append_kernel(Kv4AppendArgs a)
     const long token0 = first + (pr - begin);  // token of row 0 of the page (it may lie before the first)
 
     const int sub = lane % LPR, slot = lane / LPR;
-    float kmax[8], kmin[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) kmax[e] = -INFINITY, kmin[e] = INFINITY;
-
-    for (int rb = r0 + wave * RPW; rb < r1; rb += WAVES * RPW) {
-        const int row = rb + slot;
-        const bool live = row < r1;
-        const long t = token0 + (live ? row : rb);
-        const int quad = row >> 2, in_quad = row & 3;
-        // Keys: lane `sub` holds elements 8 sub .. 8 sub + 7.
-        {
-            const half8_t x8 = *(const half8_t*)(a.k + t * a.k_ts + head * a.k_hs + 8 * sub);
-            float x[8], lo, hi, bad = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = (float)x8[e];
-                lo = e ? fminf(lo, x[e]) : x[e];
-                hi = e ? fmaxf(hi, x[e]) : x[e];
-                bad += 0.f * x[e];
-                if (live) {
-                    kmax[e] = fmaxf(kmax[e], x[e]);
-                    kmin[e] = fminf(kmin[e], x[e]);
-                }
-            }
-#pragma unroll
-            for (int d = 1; d < g / 8; d <<= 1) {
-                lo = fminf(lo, __shfl_xor(lo, d, 64));
-                hi = fmaxf(hi, __shfl_xor(hi, d, 64));
-                bad += __shfl_xor(bad, d, 64);
-            }
-            const Group gr = group_of(lo, hi, bad);
-            const int cl = sub & 3, h = (sub >> 2) & 1, p = sub >> 3;
-            uint32_t w0 = 0, w1 = 0;
-            half8_t y8;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int code = code_of(x[e], gr);
-                const uint32_t bits = (uint32_t)code << (4 * (4 * (e & 1) + 2 * (e >> 2)));
-                if (e & 2)
-                    w1 |= bits;
-                else
-                    w0 |= bits;
-                y8[e] = (half_t)(gr.s * (float)code + gr.m);
-            }
-            w0 <<= 4 * h;
-            w1 <<= 4 * h;
-            const uint32_t o0 = __shfl_xor((int)w0, 4, 64), o1 = __shfl_xor((int)w1, 4, 64);
-            const uint32_t word = h ? (w1 | o1) : (w0 | o0);
-            if (live) {
-                *(uint32_t*)(rec + row * (D / 2) + (cl * (D / 32) + 2 * p + h) * 4) = word;
-                if (sub % (g / 8) == 0) {
-                    half_t* sm = (half_t*)(rec + 64 * D) + ((sub / (g / 8)) * 16 + quad) * 8 + in_quad;
-                    sm[0] = gr.sh;
-                    sm[4] = gr.mh;
-                }
-                if (a.k_hat) *(half8_t*)(a.k_hat + (t * c.H + head) * D + 8 * sub) = y8;
-            }
-        }
-        // Values: lane `sub` holds the elements of word `sub`.
-        {
-            const half_t* src = a.v + t * a.v_ts + head * a.v_hs + sub;
-            float x[8];
-#pragma unroll
-            for (int n = 0; n < 8; n++) x[n] = (float)src[D == 128 ? 16 * n : 16 * (n & 3) + 8 * (n >> 2)];
-            uint32_t word = 0;
-#pragma unroll
-            for (int gi = 0; gi < G; gi++) {
-                float lo = INFINITY, hi = -INFINITY, bad = 0.f;
-#pragma unroll
-                for (int n = 0; n < 8; n++)
-                    if ((D == 128 ? 16 * n : 16 * (n & 3)) / g == gi) {
-                        lo = fminf(lo, x[n]);
-                        hi = fmaxf(hi, x[n]);
-                        bad += 0.f * x[n];
-                    }
-#pragma unroll
-                for (int d = 1; d < LPR; d <<= 1) {
-                    lo = fminf(lo, __shfl_xor(lo, d, 64));
-                    hi = fmaxf(hi, __shfl_xor(hi, d, 64));
-                    bad += __shfl_xor(bad, d, 64);
-                }
-                const Group gr = group_of(lo, hi, bad);
-#pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    const int off = D == 128 ? 16 * n : 16 * (n & 3) + 8 * (n >> 2);
-                    if ((D == 128 ? 16 * n : 16 * (n & 3)) / g == gi) {
-                        const int code = code_of(x[n], gr);
-                        word |= (uint32_t)code << (4 * n);
-                        if (live && a.v_hat) a.v_hat[(t * c.H + head) * D + off + sub] = (half_t)(gr.s * (float)code + gr.m);
-                    }
-                }
-                if (live && sub == gi) {
-                    half_t* sm = (half_t*)(rec + 64 * D + 256 * G) + (gi * 16 + quad) * 8 + in_quad;
-                    sm[0] = gr.sh;
-                    sm[4] = gr.mh;
-                }
-            }
-            if (live) *(uint32_t*)(rec + 32 * D + (quad * (D / 8) + sub) * 16 + in_quad * 4) = word;
-        }
-    }
-    // Bounds: over the rows of this call, then with those that the page had unless its row 0 is among them.
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-#pragma unroll
-        for (int d = LPR; d < 64; d <<= 1) {
-            kmax[e] = fmaxf(kmax[e], __shfl_xor(kmax[e], d, 64));
-            kmin[e] = fminf(kmin[e], __shfl_xor(kmin[e], d, 64));
-        }
-        if (slot == 0) {
-            ext[wave][0][8 * sub + e] = kmax[e];
-            ext[wave][1][8 * sub + e] = kmin[e];
-        }
-    }
-    __syncthreads();
     half_t* const bounds = (half_t*)(rec + 64 * D + 512 * G);
-    for (int d = threadIdx.x; d < D; d += 64 * WAVES) {
-        float hi = ext[0][0][d], lo = ext[0][1][d];
+    half8_t old_hi, old_lo;  // what the page had, unless its row 0 is among the rows of this call
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            hi = fmaxf(hi, ext[w][0][d]);
-            lo = fminf(lo, ext[w][1][d]);
+    for (int e = 0; e < 8; e++) old_hi[e] = (half_t)-INFINITY, old_lo[e] = (half_t)INFINITY;
+    if (r0 > 0 && threadIdx.x < LPR) {
+        old_hi = *(const half8_t*)(bounds + 8 * sub);
+        old_lo = *(const half8_t*)(bounds + D + 8 * sub);
+    }
+    half2_t top[4], bottom[4];  // of the lane's elements over its rows
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        top[j] = (half2_t){(half_t)-INFINITY, (half_t)-INFINITY}, bottom[j] = (half2_t){(half_t)INFINITY, (half_t)INFINITY};
+
+    // A pass of the workgroup is WAVES * RPW rows; the next one's are asked for ahead.
+    const half_t* const kp = a.k + head * a.k_hs + 8 * sub;
+    const half_t* const vp = a.v + head * a.v_hs + 8 * sub;
+    int row = r0 + wave * RPW + slot;
+    long t = token0 + imin(row, r1 - 1);
+    half8_t k8 = *(const half8_t*)(kp + t * a.k_ts), v8 = *(const half8_t*)(vp + t * a.v_ts);
+#pragma unroll 1
+    while (true) {
+        const int next = row + WAVES * RPW;
+        const long tn = token0 + imin(next, r1 - 1);
+        const half8_t kn = *(const half8_t*)(kp + tn * a.k_ts), vn = *(const half8_t*)(vp + tn * a.v_ts);
+        const RowOut hat = {a.k_hat ? a.k_hat + (t * c.H + head) * D : nullptr, a.v_hat ? a.v_hat + (t * c.H + head) * D : nullptr};
+        kv4_store_row<D, G>(rec, row, k8, v8, row < r1, hat);
+        // (a row behind the last is the last once more)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const half2_t x = {k8[2 * j], k8[2 * j + 1]};
+            top[j] = pair_max(top[j], x);
+            bottom[j] = pair_min(bottom[j], x);
         }
-        if (r0 > 0) {
-            hi = fmaxf(hi, (float)bounds[d]);
-            lo = fminf(lo, (float)bounds[D + d]);
+        if (__ballot(next < r1) == 0) break;
+        row = next, t = tn, k8 = kn, v8 = vn;
+    }
+    // Bounds: over the wave's rows, the waves', and the page's before.
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        auto fold = [&](half2_t v, auto join) {
+            if constexpr (LPR == 8) v = join(v, bit_cast<half2_t>(lane_move<0x128>(bit_cast<uint32_t>(v))));  // row_ror:8
+            float x, y;
+            pair16(bit_cast<float>(v), x, y);
+            v = join(bit_cast<half2_t>(x), bit_cast<half2_t>(y));
+            pair32(bit_cast<float>(v), x, y);
+            return join(bit_cast<half2_t>(x), bit_cast<half2_t>(y));
+        };
+        top[j] = fold(top[j], pair_max);
+        bottom[j] = fold(bottom[j], pair_min);
+    }
+    if constexpr (WAVES > 1) {
+        if (slot == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                ext[wave][0][4 * sub + j] = top[j];
+                ext[wave][1][4 * sub + j] = bottom[j];
+            }
         }
-        bounds[d] = (half_t)hi;
-        bounds[D + d] = (half_t)lo;
+        __syncthreads();
+    }
+    if (threadIdx.x < LPR) {
+        half8_t hi8, lo8;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            half2_t hi = top[j], lo = bottom[j];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) {
+                hi = pair_max(hi, ext[w][0][4 * sub + j]);
+                lo = pair_min(lo, ext[w][1][4 * sub + j]);
+            }
+            hi = pair_max(hi, (half2_t){old_hi[2 * j], old_hi[2 * j + 1]});
+            lo = pair_min(lo, (half2_t){old_lo[2 * j], old_lo[2 * j + 1]});
+            hi8[2 * j] = hi[0], hi8[2 * j + 1] = hi[1];
+            lo8[2 * j] = lo[0], lo8[2 * j + 1] = lo[1];
+        }
+        *(half8_t*)(bounds + 8 * sub) = hi8;
+        *(half8_t*)(bounds + D + 8 * sub) = lo8;
     }
 }
 

@@ -119,29 +119,6 @@ template <int CTRL>
 __device__ __forceinline__ float row_move(float v) {
     return bit_cast<float>(__builtin_amdgcn_update_dpp(0, bit_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
-// A value and that of the lane 16 (32) away, on every lane.
-__device__ __forceinline__ void pair16(float v, float& a, float& b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
-    a = bit_cast<float>((uint32_t)r[0]);
-    b = bit_cast<float>((uint32_t)r[1]);
-}
-__device__ __forceinline__ void pair32(float v, float& a, float& b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
-    a = bit_cast<float>((uint32_t)r[0]);
-    b = bit_cast<float>((uint32_t)r[1]);
-}
-__device__ __forceinline__ float rows_sum(float v) {  // over the four lanes of a column
-    float a, b;
-    pair16(v, a, b);
-    pair32(a + b, a, b);
-    return a + b;
-}
-__device__ __forceinline__ float rows_max(float v) {
-    float a, b;
-    pair16(v, a, b);
-    pair32(fmaxf(a, b), a, b);
-    return fmaxf(a, b);
-}
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, row_move<0x121>(v));  // row_ror:1
     v = fmaxf(v, row_move<0x122>(v));
