@@ -501,14 +501,16 @@ int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* 
  * selected   NULL, or int32 [B][H][count] with T == B and no starts: the token sees only the rows of these pages (their
  *            places in the sequence).  The first min(count, pages of the sequence) entries are read; one outside the
  *            sequence is no page; one that stands there twice counts twice.
+ * k_new, v_new  both NULL, or the rows of the call's tokens, which are appended as by sq_kv4_append (new_strides: its strides)
+ *            and then attended to: for one token per sequence in the same launch.  Not with selected pages.
  * workspace  NULL, or sq_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, of any content: a sequence's pages are
  *            then dealt to several workgroups where there are few, and a second launch joins their shares.  Not shared by
  *            calls that may run at the same time.  The size is 0 where no sequence can be long enough. */
 size_t sq_kv4_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int width, int count);
 int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
                      const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
-                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, void* workspace,
-                     size_t workspace_bytes, void* stream);
+                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, const void* k_new,
+                     const void* v_new, const long* new_strides, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The pages that matter to a sequence's next token: selected int32 [B][H][count] receives the places of the `count` pages
  * of the highest score in ascending order, -1 behind the last where a sequence has fewer.  score = max over the query

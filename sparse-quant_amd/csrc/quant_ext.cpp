@@ -546,7 +546,8 @@ c10::optional<std::vector<at::Tensor>> kv4_append(const at::Tensor& k, const at:
 
 c10::optional<at::Tensor> kv4_attention(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& pages,
                                         const at::Tensor& lengths, double sm_scale, const c10::optional<at::Tensor>& starts,
-                                        const c10::optional<at::Tensor>& selected, const c10::optional<at::Tensor>& into) {
+                                        const c10::optional<at::Tensor>& selected, const c10::optional<at::Tensor>& into,
+                                        const c10::optional<at::Tensor>& k_new, const c10::optional<at::Tensor>& v_new) {
     int g;
     int64_t pitch;
     if (!kv4_fits(q, pool, pages, lengths, starts, g, pitch)) return c10::nullopt;
@@ -557,6 +558,16 @@ c10::optional<at::Tensor> kv4_attention(const at::Tensor& q, const at::Tensor& p
     if (into.has_value() && (into->sizes() != q.sizes() || into->scalar_type() != at::kHalf || into->device() != q.device() ||
                              !into->is_contiguous()))
         return c10::nullopt;
+    long strides[4] = {0, 0, 0, 0};
+    if (k_new.has_value() != v_new.has_value()) return c10::nullopt;
+    if (k_new.has_value()) {
+        if (selected.has_value() || !kv4_rows(*k_new) || !kv4_rows(*v_new) || k_new->device() != q.device() ||
+            v_new->device() != q.device() || k_new->size(0) != T || k_new->size(1) != H || k_new->size(2) != D ||
+            v_new->sizes() != k_new->sizes())
+            return c10::nullopt;
+        const long of[4] = {k_new->stride(0), k_new->stride(1), v_new->stride(0), v_new->stride(1)};
+        std::copy(of, of + 4, strides);
+    }
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(q.device());
     at::Tensor out = into.has_value() ? *into : at::empty({T, Hq, D}, q.options());
@@ -568,7 +579,9 @@ c10::optional<at::Tensor> kv4_attention(const at::Tensor& q, const at::Tensor& p
                                     starts.has_value() ? starts->data_ptr() : nullptr,
                                     selected.has_value() ? selected->data_ptr() : nullptr, (int)T, (int)B, (int)Hq, (int)H, (int)D,
                                     g, (int)pool.size(0), (int)pages.size(1), (int)pitch, count, q.stride(0), q.stride(1),
-                                    (float)sm_scale, need ? ws.data_ptr() : nullptr, need, current_stream(q));
+                                    (float)sm_scale, k_new.has_value() ? k_new->data_ptr() : nullptr,
+                                    k_new.has_value() ? v_new->data_ptr() : nullptr, strides, need ? ws.data_ptr() : nullptr,
+                                    need, current_stream(q));
     if (rc != SQ_OK) return c10::nullopt;
     return out;
 }

@@ -381,6 +381,17 @@ int check_kv4(const void* pool, const void* pages, const void* lengths, const vo
     return SQ_OK;
 }
 
+// Rows of keys and values: strides over token and head of k, then of v.
+int check_kv4_rows(const void* k, const void* v, const long* strides) {
+    if (!k || !v || !strides) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(k) || !aligned16(v)) return SQ_ERR_MISALIGNED;
+    for (int i = 0; i < 4; i++) {
+        if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
+        if (strides[i] % 8 != 0) return SQ_ERR_MISALIGNED;
+    }
+    return SQ_OK;
+}
+
 sq::Kv4Cache kv4_cache(const void* pool, const void* pages, const void* lengths, const void* starts, int T, int B, int H,
                        int num_pages, int width, int page_stride) {
     sq::Kv4Cache c;
@@ -1145,12 +1156,10 @@ int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* 
     const int rc = check_kv4(pool, pages, lengths, starts, T, B, H, D, group_size, num_pages, width, page_stride);
     if (rc != SQ_OK) return rc;
     if (T == 0 || B == 0 || width == 0) return SQ_OK;
-    if (!k || !v || !strides || (k_hat == nullptr) != (v_hat == nullptr)) return SQ_ERR_NULL_POINTER;
-    if (!aligned16(k) || !aligned16(v) || !aligned16(k_hat) || !aligned16(v_hat)) return SQ_ERR_MISALIGNED;
-    for (int i = 0; i < 4; i++) {
-        if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
-        if (strides[i] % 8 != 0) return SQ_ERR_MISALIGNED;
-    }
+    const int rr = check_kv4_rows(k, v, strides);
+    if (rr != SQ_OK) return rr;
+    if ((k_hat == nullptr) != (v_hat == nullptr)) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(k_hat) || !aligned16(v_hat)) return SQ_ERR_MISALIGNED;
     return launch_code(sq::launch_kv4_append(kv4_cache(pool, pages, lengths, starts, T, B, H, num_pages, width, page_stride), k,
                                              v, k_hat, v_hat, D, group_size, strides, static_cast<hipStream_t>(stream)));
 }
@@ -1162,10 +1171,16 @@ size_t sq_kv4_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int 
 
 int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
                      const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
-                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     int page_stride, int count, long q_tstride, long q_hstride, float sm_scale, const void* k_new,
+                     const void* v_new, const long* new_strides, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_kv4(pool, pages, lengths, starts, T, B, H, D, group_size, num_pages, width, page_stride);
     if (rc != SQ_OK) return rc;
+    if ((k_new == nullptr) != (v_new == nullptr)) return SQ_ERR_NULL_POINTER;
+    if (k_new && selected) return SQ_ERR_BAD_SHAPE;
+    if (k_new && T > 0 && B > 0) {
+        const int ra = check_kv4_rows(k_new, v_new, new_strides);
+        if (ra != SQ_OK) return ra;
+    }
     if (Hq <= 0 || Hq % H != 0 || (long)T * Hq > (1L << 30) || q_tstride < 0 || q_hstride < 0) return SQ_ERR_BAD_SHAPE;
     if (selected && (count <= 0 || starts || T != B)) return SQ_ERR_BAD_SHAPE;
     if (T == 0 || B == 0) return SQ_OK;
@@ -1177,8 +1192,8 @@ int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pag
         return SQ_ERR_WORKSPACE;
     return launch_code(sq::launch_kv4_attention(kv4_cache(pool, pages, lengths, starts, T, B, H, num_pages, width, page_stride),
                                                 q, out, static_cast<const int*>(selected), workspace, D, group_size, Hq / H,
-                                                selected ? count : 0, q_tstride, q_hstride, sm_scale,
-                                                static_cast<hipStream_t>(stream)));
+                                                selected ? count : 0, q_tstride, q_hstride, sm_scale, k_new, v_new,
+                                                new_strides, static_cast<hipStream_t>(stream)));
 }
 
 size_t sq_kv4_select_workspace_bytes(int B, int H, int width) {

@@ -142,7 +142,8 @@ hipError_t launch_kv4_select(const Kv4Cache& c, const void* q, void* selected, v
                              long q_ts, long q_hs, int count, int keep_first, int keep_last, hipStream_t st);
 size_t kv4_attention_workspace_bytes(int T, int B, int share, int D, int pages);  // pages: the most of a sequence
 hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, const int* selected, void* workspace, int D, int g,
-                                int share, int count, long q_ts, long q_hs, float sm_scale, hipStream_t st);
+                                int share, int count, long q_ts, long q_hs, float sm_scale, const void* k_new, const void* v_new,
+                                const long* new_strides, hipStream_t st);  // k_new: rows to store first, or null
 
 // sq_lm_head.hip: the ends of a greedy decode step around the W4A16 layers (the end-to-end harness).
 // out[r, :] = embed[tok[r], :] + pos_table[*pos + pos_offset, :] (fp16; indices clamped to their tables).

@@ -19,6 +19,9 @@ struct Kv4AttnArgs {
     int share;            // query heads of a key/value head
     int count;
     float scale;          // sm_scale * log2(e)
+    const half_t* k_new;  // the row of every sequence's one token, stored by the kernel first, or null
+    const half_t* v_new;
+    long k_ts, k_hs, v_ts, v_hs;
 };
 
 // How a launch's work is dealt.  A tile is R of the rows (token, query head) of a sequence and key/value head; a

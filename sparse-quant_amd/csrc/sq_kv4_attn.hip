@@ -20,6 +20,7 @@
 // follows the scales.
 #include "sq_kernels.h"
 #include "sq_kv4_attn.h"
+#include "sq_kv4_row.h"
 
 namespace sq {
 
@@ -41,7 +42,7 @@ struct Unit {
     half8_t ksm[SETS][G], vsm[SETS][G];  // scales and minima of four rows
 };
 
-template <int D, int G, int PACK, int RT, int WAVES>
+template <int D, int G, int PACK, int RT, int WAVES, bool NEW>
 __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Deal d) {
     constexpr int g = D / G;
     constexpr int REC = kv4_record_bytes(D, g);
@@ -351,9 +352,40 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
                 }
             }
         };
-        if (wave < units) {
+        // The new row, if this is the share that sees it: stored by the wave whose unit it is in, before it asks for that
+        // unit; the others do not wait.  (Workgroups with other queries of this head store the same bytes.)
+        const int fresh = NEW && pb + 64 >= p1 && p1 == all_pages && len > 0 && c.lengths[pc.b] == len  // (inside the table)
+                              ? PER * (p1 - pb - 1) + (len - 1) % KV4_PAGE / U::ROWS : -1;
+        const bool mine = fresh >= 0 && fresh % WAVES == wave;
+        if (wave < units && !(mine && fresh == wave)) {
             load_keys(wave);
             load_values(wave);
+        }
+        if (NEW && mine) {
+            const int pid = __builtin_amdgcn_readlane(id, fresh / PER);
+            if (pid >= 0) {
+                uint8_t* const rec = c.pool + ((long)pid * c.H + head) * REC;
+                const int row = (len - 1) % KV4_PAGE, sub = lane % (D / 8);
+                const half8_t k8 = *(const half8_t*)(a.k_new + (long)pc.first * a.k_ts + (long)head * a.k_hs + 8 * sub);
+                const half8_t v8 = *(const half8_t*)(a.v_new + (long)pc.first * a.v_ts + (long)head * a.v_hs + 8 * sub);
+                half8_t* const bounds = (half8_t*)(rec + 64 * D + 512 * G) + sub;
+                half8_t hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; e++) hi[e] = (half_t)-INFINITY, lo[e] = (half_t)INFINITY;
+                if (row > 0) hi = bounds[0], lo = bounds[D / 8];
+                hi = __builtin_elementwise_max(hi, k8);
+                lo = __builtin_elementwise_min(lo, k8);
+                kv4_store_row<D, G>(rec, row, k8, v8, lane < D / 8, RowOut{nullptr, nullptr});
+                if (lane < D / 8) {
+                    bounds[0] = hi;
+                    bounds[D / 8] = lo;
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if (fresh == wave) {
+                load_keys(wave);
+                load_values(wave);
+            }
         }
         for (int u = wave; u < units; u += WAVES) {
             consume(u);
@@ -455,7 +487,8 @@ size_t kv4_attention_workspace_bytes(int T, int B, int share, int D, int pages) 
 }
 
 hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, const int* selected, void* workspace, int D, int g,
-                                int share, int count, long q_ts, long q_hs, float sm_scale, hipStream_t st) {
+                                int share, int count, long q_ts, long q_hs, float sm_scale, const void* k_new, const void* v_new,
+                                const long* new_strides, hipStream_t st) {
     Kv4AttnArgs a;
     a.c = c;
     a.q = (const half_t*)q;
@@ -466,8 +499,21 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
     a.share = share;
     a.count = count;
     a.scale = sm_scale * 1.44269504088896340736f;
+    a.k_new = a.v_new = nullptr;
+    a.k_ts = a.k_hs = a.v_ts = a.v_hs = 0;
     // Rows of a sequence and key/value head (of the average one where they differ).
     const long mean = ((long)c.T * share + c.B - 1) / c.B;
+    if (k_new && !c.starts && c.each == 1 && mean <= KA_ROWS) {
+        a.k_new = (const half_t*)k_new;
+        a.v_new = (const half_t*)v_new;
+        a.k_ts = new_strides[0];
+        a.k_hs = new_strides[1];
+        a.v_ts = new_strides[2];
+        a.v_hs = new_strides[3];
+    } else if (k_new) {
+        const hipError_t e = launch_kv4_append(c, k_new, v_new, nullptr, nullptr, D, g, new_strides, st);
+        if (e != hipSuccess) return e;
+    }
     if (mean > KA_ROWS && !selected) {
         a.ws = (float*)workspace;
         return launch_kv4_chunk(a, D, g, st);
@@ -482,8 +528,12 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         constexpr int R = 16 / pack.value * rt.value;
         const long tiles = tiles_of(R);
         const long wgs = split ? tiles + KA_DEAL.wgs() : tiles;
-        hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value, pack.value, rt.value, waves.value>), dim3((unsigned)wgs),
-                           dim3(64 * waves.value), 0, st, a, KA_DEAL);
+        if (a.k_new)
+            hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value, pack.value, rt.value, waves.value, true>),
+                               dim3((unsigned)wgs), dim3(64 * waves.value), 0, st, a, KA_DEAL);
+        else
+            hipLaunchKernelGGL((kv4_attn_kernel<d.value, groups.value, pack.value, rt.value, waves.value, false>),
+                               dim3((unsigned)wgs), dim3(64 * waves.value), 0, st, a, KA_DEAL);
         if (!split) return;
         const long tokens = c.starts ? R : c.each;
         const unsigned rows = (unsigned)(tokens * share < R ? tokens * share : R);

@@ -60,8 +60,8 @@ SIGNATURES = {
     "sq_kv4_record_bytes": (_i, [_i, _i]),
     "sq_kv4_append": (_i, [_vp] * 8 + [_i] * 8 + [_vp, _vp]),
     "sq_kv4_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 7),
-    "sq_kv4_attention": (_i, [_vp] * 7 + [_i] * 10 + [ctypes.c_long, ctypes.c_long, ctypes.c_float, _vp, ctypes.c_size_t,
-                                                      _vp]),
+    "sq_kv4_attention": (_i, [_vp] * 7 + [_i] * 10 + [ctypes.c_long, ctypes.c_long, ctypes.c_float] + [_vp] * 4 +
+                         [ctypes.c_size_t, _vp]),
     "sq_kv4_select_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
     "sq_kv4_select": (_i, [_vp] * 5 + [_i] * 11 + [ctypes.c_long, ctypes.c_long, _vp, ctypes.c_size_t, _vp]),
     "sq_kv4_copy_pages": (_i, [_vp] * 3 + [_i] * 3 + [ctypes.c_size_t, ctypes.c_size_t, _vp]),

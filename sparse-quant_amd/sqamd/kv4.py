@@ -109,12 +109,14 @@ def append(k, v, pool, pages, lengths, starts=None, values=False):
     return hats if values else None
 
 
-def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out=None):
+def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out=None, k_new=None, v_new=None):
     """Causal attention of q fp16 [T, heads, D], the last tokens of their sequences (their own rows are in the cache), over
     the cached rows; query head h reads key/value head h // (heads // kv_heads).  selected int32 [sequences, kv_heads,
     count] (one token per sequence): over the rows of these pages only, as select_pages gives them.  Returns fp16
-    [T, heads, D]; a token that sees no row gets 0, tokens behind the last sequence's are left as `out` had them."""
-    got = quant.kv4_attention(q, pool, pages, lengths, sm_scale, starts, selected, out)
+    [T, heads, D]; a token that sees no row gets 0, tokens behind the last sequence's are left as `out` had them.
+    k_new, v_new fp16 [T, kv_heads, D]: the tokens' rows are not in the cache yet and are appended first (for one token per
+    sequence in the same launch); not with selected pages."""
+    got = quant.kv4_attention(q, pool, pages, lengths, sm_scale, starts, selected, out, k_new, v_new)
     if got is not None:
         return got if out is None else out
     t, b, g = _check_cache(q, pool, pages, lengths, starts)
@@ -130,6 +132,14 @@ def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out
                 or selected.dim() != 3 or tuple(selected.shape[:2]) != (b, h) or selected.shape[2] < 1:
             raise ValueError("selected must be a contiguous int32 [sequences, kv_heads, count] on the device of q")
         count = selected.shape[2]
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
+    if k_new is not None:
+        if selected is not None:
+            raise ValueError("rows are appended before pages are selected")
+        if k_new.shape != (t, h, d):
+            raise ValueError("rows of shape %s for %d tokens, %d heads of %d" % (tuple(k_new.shape), t, h, d))
+        append(k_new, v_new, pool, pages, lengths, starts)
     q = _readable(q)
     if out is None:
         out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
@@ -140,7 +150,7 @@ def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out
     with torch.cuda.device(q.device):
         _check(capi.lib().sq_kv4_attention(_ptr(q), _ptr(out), _ptr(pool), _ptr(pages), _ptr(lengths), _ptr(starts),
                                            _ptr(selected), t, b, hq, h, d, g, pool.shape[0], pages.shape[1],
-                                           _table_stride(pages), count, q.stride(0), q.stride(1), float(sm_scale), _ptr(ws),
+                                           _table_stride(pages), count, q.stride(0), q.stride(1), float(sm_scale), None, None, None, _ptr(ws),
                                            need, _stream()), "sq_kv4_attention")
     return out
 
@@ -393,8 +403,8 @@ class KV4Cache:
     def append(self, layer, k, v, seqs, starts=None, values=False):
         return self.layer(layer, seqs).append(k, v, starts, values)
 
-    def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None):
-        return self.layer(layer, seqs).attention(q, sm_scale, starts, selected, out)
+    def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None, k_new=None, v_new=None):
+        return self.layer(layer, seqs).attention(q, sm_scale, starts, selected, out, k_new, v_new)
 
     def select_pages(self, layer, q, count, seqs, keep_first=1, keep_last=1):
         return self.layer(layer, seqs).select_pages(q, count, keep_first, keep_last)
@@ -409,8 +419,8 @@ class LayerOf:
     def append(self, k, v, starts=None, values=False):
         return append(k, v, self.pool, self.pages, self.lengths, starts, values)
 
-    def attention(self, q, sm_scale, starts=None, selected=None, out=None):
-        return attention(q, self.pool, self.pages, self.lengths, sm_scale, starts, selected, out)
+    def attention(self, q, sm_scale, starts=None, selected=None, out=None, k_new=None, v_new=None):
+        return attention(q, self.pool, self.pages, self.lengths, sm_scale, starts, selected, out, k_new, v_new)
 
     def select_pages(self, q, count, keep_first=1, keep_last=1):
         return select_pages(q, self.pool, self.pages, self.lengths, count, keep_first, keep_last)

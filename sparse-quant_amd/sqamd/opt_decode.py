@@ -131,8 +131,7 @@ class DecoderLayer(nn.Module):
             k_hat, v_hat = (x.view(b, t, h, hd).transpose(1, 2) for x in cache.append(k4, v4, values=True))
             a = capi.lut_attention_strided(q, k_hat, v_hat, self.lut.contiguous().to(q.device), scale, True, rows_first=True)
         else:
-            cache.append(k4, v4)
-            a = cache.attention(q4, scale)
+            a = cache.attention(q4, scale, k_new=k4, v_new=v4)
         if self.capture is not None:
             self.capture.update(q=q.detach().clone(), k=k.detach().clone(), v=v.detach().clone(),
                                 a=a.view(b, t, h, hd).transpose(1, 2).detach().clone())

@@ -417,6 +417,10 @@ def test_refusals(kv4):
         lambda: kv4.attention(q, pool, pages, lens, 1.0, selected=sel[:1]),
         lambda: kv4.attention(q, pool, pages, lens, 1.0, out=q.float()),
         lambda: kv4.attention(torch.cat([q, q[:1]]), pool, pages, lens, 1.0),
+        lambda: kv4.attention(q, pool, pages, lens, 1.0, k_new=kv),
+        lambda: kv4.attention(q, pool, pages, lens, 1.0, k_new=q, v_new=q),
+        lambda: kv4.attention(q, pool, pages, lens, 1.0, k_new=kv, v_new=kv.float()),
+        lambda: kv4.attention(q, pool, pages, lens, 1.0, selected=sel, k_new=kv, v_new=kv),
         lambda: kv4.append(q, q, pool, pages, lens),
         lambda: kv4.append(kv, kv[:1], pool, pages, lens),
         lambda: kv4.append(kv, kv.float(), pool, pages, lens),
@@ -681,6 +685,46 @@ def test_two_graphs_at_once(kv4):
                     graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("d,g", SIZES)
+@pytest.mark.parametrize("h,share,lens,new", [
+    (2, 4, [1, 64, 65, 640], None), (4, 1, [33, 32, 700, 128], None), (1, 7, [97, 3000], None), (2, 16, [129, 1025], None),
+    (1, 24, [200, 64], None), (1, 40, [300], None), (8, 4, [5000], None), (2, 2, [30, 200], [30, 70]), (1, 3, [0, 70, 129], None),
+], ids=["edges", "unshared", "seven", "sixteen", "two-tiles", "many-rows", "split", "chunks", "none"])
+def test_rows_appended_by_the_attention_itself(kv4, d, g, h, share, lens, new):
+    # the cache and the result are those of an append followed by the attention, bit for bit
+    rng = np.random.default_rng(d + g + share)
+    new = new or [1] * len(lens)
+    pages, total = tables(rng, lens)
+    pool = dev(random_pool(rng, total, h, d, g))
+    t = sum(new)
+    kv = dev(rng.normal(0, 1, (t, 2, h, d)).astype(np.float16))
+    q = dev(rng.normal(0, 1, (t, h * share, d)).astype(np.float16))
+    n, table = dev(np.array(lens, np.int32)), dev(pages)
+    st = None if max(new) == 1 else dev(starts_of(new))
+    other = pool.clone()
+    kv4.append(kv[:, 0], kv[:, 1], pool, table, n, st)
+    want = kv4.attention(q, pool, table, n, 0.1, st)
+    for _ in range(2):  # (once more: the same rows in the same places)
+        got = kv4.attention(q, other, table, n, 0.1, st, k_new=kv[:, 0], v_new=kv[:, 1])
+        assert torch.equal(got, want) and torch.equal(other, pool)
+    odd = kv.clone().flatten()
+    shifted = torch.cat([odd.new_zeros(3), odd])[3:].view(kv.shape)  # rows that have to be copied first
+    assert torch.equal(kv4.attention(q, other, table, n, 0.1, st, k_new=shifted[:, 0], v_new=shifted[:, 1]), want)
+
+
+def test_a_new_row_without_a_page(kv4):
+    d, g, h = 64, 32, 1
+    rng = np.random.default_rng(30)
+    pool = random_pool(rng, 3, h, d, g)
+    pages = np.array([[0, 9], [1, -1], [2, 2]], dtype=np.int32)
+    lens = np.array([100, 65, 129], np.int32)  # a page outside the pool, none, a row beyond the table
+    q, kv = rng.normal(0, 1, (3, 2, d)).astype(np.float16), rng.normal(0, 1, (2, 3, h, d)).astype(np.float16)
+    a, b = dev(pool), dev(pool)
+    got = kv4.attention(dev(q), a, dev(pages), dev(lens), 0.1, k_new=dev(kv[0]), v_new=dev(kv[1]))
+    kv4.append(dev(kv[0]), dev(kv[1]), b, dev(pages), dev(lens))
+    assert torch.equal(a, b) and torch.equal(got, kv4.attention(dev(q), b, dev(pages), dev(lens), 0.1))
 
 
 def test_results_repeat_bit_for_bit(kv4):

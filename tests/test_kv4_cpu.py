@@ -86,9 +86,16 @@ def test_attention_refuses(L, p):
     from sqamd import capi
 
     def call(q=p, out=p, pool=p, pages=p, lengths=p, starts=None, sel=None, T=4, B=4, Hq=16, H=8, D=128, g=64, n=10, width=5,
-             stride=5, count=0, qt=2048, qh=128, ws=None, size=0):
+             stride=5, count=0, qt=2048, qh=128, k=None, v=None, st=None, ws=None, size=0):
         return L.sq_kv4_attention(q, out, pool, pages, lengths, starts, sel, T, B, Hq, H, D, g, n, width, stride, count, qt, qh,
-                                  0.1, ws, size, None)
+                                  0.1, k, v, st, ws, size, None)
+
+    strides = (ctypes.c_long * 4)(1024, 128, 1024, 128)
+    assert call(k=p) == call(v=p, st=strides) == call(k=p, v=p) == capi.SQ_ERR_NULL_POINTER
+    assert call(k=p, v=p, st=strides, sel=p, count=2) == capi.SQ_ERR_BAD_SHAPE
+    assert call(k=ctypes.c_void_p(p.value + 2), v=p, st=strides) == capi.SQ_ERR_MISALIGNED
+    assert call(k=p, v=p, st=(ctypes.c_long * 4)(1024, 128, 1020, 128)) == capi.SQ_ERR_MISALIGNED
+    assert call(k=p, v=p, st=(ctypes.c_long * 4)(1024, -128, 1024, 128)) == capi.SQ_ERR_BAD_SHAPE
 
     odd = ctypes.c_void_p(p.value + 2)
     assert call(T=0) == capi.SQ_OK and call(T=0, B=0) == capi.SQ_OK
