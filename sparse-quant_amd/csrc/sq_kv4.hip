@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void kv4_copy_kernel(uint8_t* pool, const int*
 // 16 (D = 64: 8) lanes share a page, 8 elements each; the choice between hi and lo goes by the signs of the queries, which
 // a lane keeps as masks of pairs.  A wave takes SELECT_PAGES pages, all their bounds asked for at once.
 constexpr int SELECT_QUERIES = 4;  // of a round
-constexpr int SELECT_PAGES = 16;   // of a wave
+constexpr int SELECT_PAGES = 8;    // of a wave
 
 struct Kv4SelectArgs {
     Kv4Cache c;
@@ -210,8 +210,7 @@ typedef short short2_t __attribute__((ext_vector_type(2)));
 template <int CTRL>
 __device__ __forceinline__ double row_move(double v) {
     const u32x2_t u = bit_cast<u32x2_t>(v);
-    return bit_cast<double>((u32x2_t){(uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, 0xF, 0xF, false),
-                                      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, 0xF, 0xF, false)});
+    return bit_cast<double>((u32x2_t){lane_move<CTRL>(u.x), lane_move<CTRL>(u.y)});
 }
 
 template <int D>
@@ -281,7 +280,7 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     return u & 0x8000000000000000ull ? ~u : u | 0x8000000000000000ull;
 }
 
-constexpr int SELECT_THREADS = 1024;
+constexpr int SELECT_THREADS = 512;
 
 // The `count` best pages of a head in ascending order, ties to the lowest; -1 behind the last where there are fewer.
 // The count-th largest key is found digit by digit, from the top, until no other key shares its digits.

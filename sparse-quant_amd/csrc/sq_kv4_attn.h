@@ -120,7 +120,7 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
 
 template <int CTRL>
 __device__ __forceinline__ float row_move(float v) {
-    return bit_cast<float>(__builtin_amdgcn_update_dpp(0, bit_cast<int>(v), CTRL, 0xF, 0xF, false));
+    return bit_cast<float>(__builtin_amdgcn_mov_dpp(bit_cast<int>(v), CTRL, 0xF, 0xF, true));
 }
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, row_move<0x121>(v));  // row_ror:1

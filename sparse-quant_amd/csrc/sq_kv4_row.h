@@ -17,7 +17,7 @@ namespace sq {
 
 template <int CTRL>
 __device__ __forceinline__ uint32_t lane_move(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
 template <int CTRL>
 __device__ __forceinline__ float lane_move(float v) {
