@@ -486,7 +486,7 @@ int sq_kv4_record_bytes(int D, int group_size);
 
 /* Rows k, v fp16 (element (t, h, d) at k[t * strides[0] + h * strides[1] + d], v with strides[2], strides[3]) are
  * quantised into their pages and take part in their pages' bounds; a page that gets its row 0 starts its bounds anew.
- * A page that two sequences of the call name must not get rows from both.  k_hat, v_hat: both NULL, or fp16 [T][H][D]
+ * A page that gets rows stands once in the tables of the call.  k_hat, v_hat: both NULL, or fp16 [T][H][D]
  * that receive what the rows read as from now on (rounded once): what a prompt's own attention is given so that it
  * sees what decoding will see.  Tokens without a page (a negative row, one beyond the table, a page outside the pool)
  * are left out, their k_hat and v_hat as they were. */

@@ -71,7 +71,7 @@ class Rows:
         self.v_rest = flat(np.abs(f["vs"].astype(np.float64) * 8 + f["vm"].astype(np.float64)))
 
 
-def attend(rows, q, scale, seen):
+def attend(rows, q, scale, seen, middles=0.0):
     """q fp64 [D] over the rows named by `seen` (indices, with repetition): (out, tolerance) [D] in 64 bits.
 
     Tolerance.  P' = P s is rounded to fp16 before it meets code - 8: eps/2 = 2^-11 of every term.  A probability is off by
@@ -80,7 +80,8 @@ def attend(rows, q, scale, seen):
     sums.  fp32 sums of the result: of every 32 rows first P s code and then -8 P s are added, 66 additions that each round
     (towards zero as well) 2^-23 of a partial sum of at most sum P s (code + 8) over those rows; what remains of each 32 rows
     is added in one chain of n / 32, 8 additions join partial sums.  The output's own rounding is 2^-11 of it, or 2^-25
-    where it is denormal."""
+    where it is denormal.  middles: what m + 8 s is rounded by, of itself (2^-11
+    for fp16), where it is held in fewer bits."""
     if len(seen) == 0:
         return np.zeros(rows.k.shape[1]), np.zeros(rows.k.shape[1])
     d = rows.k.shape[1]
@@ -94,7 +95,7 @@ def attend(rows, q, scale, seen):
     chain = (8 + min(len(seen), 4096) / 32) * 2.0 ** -23
     tol = 2.0 ** -11 * (np.abs(out) + mid) + (2 * dscore + chain) * (mid + rest) + 2.0 ** -24
     tol += 66 * 2.0 ** -23 * (p @ rows.v_code[seen])
-    return out, tol
+    return out, tol + middles * rest
 
 
 def select(bounds, q, count, keep_first, keep_last):

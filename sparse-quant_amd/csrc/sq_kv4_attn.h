@@ -31,6 +31,7 @@ struct Deal {
     int per_cu, least;
     __host__ __device__ int wgs() const { return 256 * per_cu; }
 };
+constexpr long KA_MOST_PAGES = 1l << 38;  // of all tiles, that `deal` can count: beyond it nothing is shared
 struct Piece {
     int b, tile, head, share, shares;  // share of how many
     int slot;                          // where its partial state goes (shares > 1)
@@ -85,7 +86,7 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
             const unsigned long long mine = (unsigned long long)t.tiles * t.pages;
             units += (unsigned)wave_sum((int)(mine & 0xffff)) + ((unsigned long long)(unsigned)wave_sum((int)(mine >> 16)) << 16);
         }
-        const int even = ceil_div((int)((units + 255) >> 8), d.per_cu);  // (T * Hq <= 2^30: at most 2^48 pages)
+        const int even = ceil_div((int)((units + 255) >> 8), d.per_cu);  // (below KA_MOST_PAGES)
         least = imax(even, d.least);
     }
     int slots = 0;

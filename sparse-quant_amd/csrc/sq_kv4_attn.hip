@@ -353,7 +353,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
             }
         };
         // The new row, if this is the share that sees it: stored by the wave whose unit it is in, before it asks for that
-        // unit; the others do not wait.  (Workgroups with other queries of this head store the same bytes.)
+        // unit; the others do not wait.  (All queries of a head stand in one tile here.)
         const int fresh = NEW && pb + 64 >= p1 && p1 == all_pages && len > 0 && c.lengths[pc.b] == len  // (inside the table)
                               ? PER * (p1 - pb - 1) + (len - 1) % KV4_PAGE / U::ROWS : -1;
         const bool mine = fresh >= 0 && fresh % WAVES == wave;
@@ -519,11 +519,11 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         return launch_kv4_chunk(a, D, g, st);
     }
     const int most = selected && count < c.width ? count : c.width;
-    const bool split = workspace != nullptr && most > KA_DEAL.least;
-    a.ws = split ? (float*)workspace : nullptr;
     auto tiles_of = [&](int R) {
         return (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
     };
+    const bool split = workspace != nullptr && most > KA_DEAL.least && tiles_of(4) < KA_MOST_PAGES / most;
+    a.ws = split ? (float*)workspace : nullptr;
     auto go = [&](auto d, auto groups, auto pack, auto rt, auto waves) {
         constexpr int R = 16 / pack.value * rt.value;
         const long tiles = tiles_of(R);

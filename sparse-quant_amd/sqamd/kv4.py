@@ -81,13 +81,16 @@ def _readable(x):
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _table_stride(pages):
-    return max(pages.stride(0), pages.shape[1]) if pages.shape[0] > 1 else pages.shape[1]
+def _table(pages):
+    """pages with rows that lie apart (a copy where they do not: an expanded row), and their distance."""
+    if pages.shape[0] > 1 and pages.stride(0) < pages.shape[1]:
+        pages = pages.contiguous()
+    return pages, max(pages.stride(0), pages.shape[1]) if pages.shape[0] > 1 else pages.shape[1]
 
 
 def append(k, v, pool, pages, lengths, starts=None, values=False):
     """Quantise the rows k, v fp16 [T, kv_heads, D] (any token and head strides) of new tokens into their pages; they are
-    the last rows of their sequences.  With `values` returns (k_hat, v_hat) fp16 [T, kv_heads, D], what the cache holds
+    the last rows of their sequences (two sequences that get rows must not share the page these go to).  With `values` returns (k_hat, v_hat) fp16 [T, kv_heads, D], what the cache holds
     of them (of no defined content where a token has no page); otherwise None."""
     got = quant.kv4_append(k, v, pool, pages, lengths, starts, values)
     if got is not None:
@@ -102,9 +105,10 @@ def append(k, v, pool, pages, lengths, starts=None, values=False):
     k, v = _readable(k), _readable(v)
     hats = torch.empty((2, t, h, d), dtype=k.dtype, device=k.device).unbind(0) if values else (None, None)
     strides = (ctypes.c_long * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    pages, pitch = _table(pages)
     with torch.cuda.device(k.device):
         _check(capi.lib().sq_kv4_append(_ptr(k), _ptr(v), _ptr(hats[0]), _ptr(hats[1]), _ptr(pool), _ptr(pages), _ptr(lengths),
-                                        _ptr(starts), t, b, h, d, g, pool.shape[0], pages.shape[1], _table_stride(pages),
+                                        _ptr(starts), t, b, h, d, g, pool.shape[0], pages.shape[1], pitch,
                                         strides, _stream()), "sq_kv4_append")
     return hats if values else None
 
@@ -137,21 +141,25 @@ def attention(q, pool, pages, lengths, sm_scale, starts=None, selected=None, out
     if k_new is not None:
         if selected is not None:
             raise ValueError("rows are appended before pages are selected")
-        if k_new.shape != (t, h, d):
-            raise ValueError("rows of shape %s for %d tokens, %d heads of %d" % (tuple(k_new.shape), t, h, d))
+        if k_new.shape != (t, h, d) or k_new.device != q.device:
+            raise ValueError("rows of shape %s for %d tokens, %d heads of %d on the device of q"
+                             % (tuple(k_new.shape), t, h, d))
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()
+                            or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous fp16 %s at a multiple of 16 bytes on the device of q" % (tuple(q.shape),))
+    if k_new is not None:
         append(k_new, v_new, pool, pages, lengths, starts)
     q = _readable(q)
     if out is None:
         out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise ValueError("out must be a contiguous fp16 %s on the device of q" % (tuple(q.shape),))
+    pages, pitch = _table(pages)
     need = capi.lib().sq_kv4_attention_workspace_bytes(t, b, hq, h, d, pages.shape[1], count)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         _check(capi.lib().sq_kv4_attention(_ptr(q), _ptr(out), _ptr(pool), _ptr(pages), _ptr(lengths), _ptr(starts),
-                                           _ptr(selected), t, b, hq, h, d, g, pool.shape[0], pages.shape[1],
-                                           _table_stride(pages), count, q.stride(0), q.stride(1), float(sm_scale), None, None, None, _ptr(ws),
-                                           need, _stream()), "sq_kv4_attention")
+                                           _ptr(selected), t, b, hq, h, d, g, pool.shape[0], pages.shape[1], pitch, count,
+                                           q.stride(0), q.stride(1), float(sm_scale), None, None, None, _ptr(ws), need,
+                                           _stream()), "sq_kv4_attention")
     return out
 
 
@@ -172,14 +180,15 @@ def select_pages(q, pool, pages, lengths, count, keep_first=1, keep_last=1):
     if count < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > count:
         raise ValueError("cannot keep the first %d and the last %d among %d pages" % (keep_first, keep_last, count))
     q = _readable(q)
+    pages, pitch = _table(pages)
     selected = torch.empty((b, h, count), dtype=torch.int32, device=q.device)
     width = pages.shape[1]
     need = capi.lib().sq_kv4_select_workspace_bytes(b, h, width) if width > count else 0
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         _check(capi.lib().sq_kv4_select(_ptr(q), _ptr(selected), _ptr(pool), _ptr(pages), _ptr(lengths), b, hq, h, d, g,
-                                        pool.shape[0], width, _table_stride(pages), int(count), int(keep_first),
-                                        int(keep_last), q.stride(0), q.stride(1), _ptr(ws), need, _stream()),
+                                        pool.shape[0], width, pitch, int(count), int(keep_first), int(keep_last),
+                                        q.stride(0), q.stride(1), _ptr(ws), need, _stream()),
                "sq_kv4_select")
     return selected
 
@@ -206,10 +215,13 @@ class KV4Cache:
     Sequences are numbered 0 .. max_seqs - 1 (`add`, `fork`, `free`).  Rows are given room with `extend` (which also counts
     them) or ahead of time with `reserve`; `append`, `attention` and `select_pages` then work on one layer for a list of
     sequences, or for all of the first n (`seqs` an int).  Pages may be shared between sequences (`fork`): a page is copied
-    before a sequence that shares it gets rows in it.  `lengths` and `table` are the device's view of it and change in place; with
+    before a sequence that shares it gets rows in it, by `reserve` (and so by `extend`), which therefore follows a fork.  `lengths` and `table` are the device's view of it and change in place; with
     rows reserved a captured graph may count `lengths` up itself (`set_lengths` then brings the host's view after it)."""
 
     def __init__(self, layers, num_pages, kv_heads, head_dim, group_size=64, max_seqs=8, max_rows=2048, device="cuda"):
+        if min(layers, num_pages, kv_heads, max_seqs, max_rows) < 1:
+            raise ValueError("a cache of %d layers, %d pages, %d heads, %d sequences of %d rows"
+                             % (layers, num_pages, kv_heads, max_seqs, max_rows))
         self.pool = new_pool(num_pages, kv_heads, head_dim, group_size, layers, device)
         self.layers, self.num_pages, self.max_seqs, self.max_rows = layers, num_pages, max_seqs, max_rows
         self.kv_heads, self.head_dim, self.group_size = kv_heads, head_dim, group_size
@@ -272,7 +284,7 @@ class KV4Cache:
             self._uses[page] += 1
         self._pages[new] = list(used)
         self._write([new])
-        self.set_lengths([new], [rows])
+        self._count([new], [rows])
         return new
 
     def truncate(self, seq, rows):
@@ -285,7 +297,7 @@ class KV4Cache:
         for page in pages[keep:]:
             self._release(page)
         del pages[keep:]
-        self.set_lengths([seq], [rows])
+        self._count([seq], [rows])
 
     def reserve(self, seqs, rows):
         """Pages for the first rows[i] rows of seqs[i], of their own from the row behind the last one on."""
@@ -340,11 +352,17 @@ class KV4Cache:
         self.set_lengths(seqs, total)
 
     def set_lengths(self, seqs, rows):
-        """Count rows that have pages already."""
+        """Count rows that have pages already, new ones pages that no other sequence shares."""
         rows = self._per_sequence(seqs, rows)
         for seq, n in zip(seqs, rows):
-            if not 0 <= n <= len(self._known(seq)) * PAGE:
-                raise ValueError("%d rows on %d pages" % (n, len(self._pages[seq])))
+            pages = self._known(seq)
+            if not 0 <= n <= len(pages) * PAGE:
+                raise ValueError("%d rows on %d pages" % (n, len(pages)))
+            if n > self._rows[seq] and any(self._uses[p] > 1 for p in pages[self._rows[seq] // PAGE:(n + PAGE - 1) // PAGE]):
+                raise ValueError("rows of sequence %d would go to a page that another shares; reserve gives it its own" % seq)
+        self._count(seqs, rows)
+
+    def _count(self, seqs, rows):
         for seq, n in zip(seqs, rows):
             self._rows[seq] = n
         at, n = self._vectors(seqs, rows)
@@ -392,18 +410,30 @@ class KV4Cache:
     def batch(self, seqs):
         """(pages, lengths) of these sequences; views of the cache's own where seqs is an int n (sequences 0 .. n - 1)."""
         if isinstance(seqs, int):
+            if not 0 <= seqs <= self.max_seqs:
+                raise ValueError("%d sequences of a cache for %d" % (seqs, self.max_seqs))
             return self.table[:seqs], self.lengths[:seqs]
-        at = torch.tensor(list(seqs), device=self.table.device)
+        for seq in seqs:
+            self._known(seq)
+        at = torch.tensor(list(seqs), dtype=torch.int64, device=self.table.device)
         return self.table[at], self.lengths[at]
+
+    @staticmethod
+    def _once(seqs):
+        if not isinstance(seqs, int) and len(set(seqs)) != len(seqs):
+            raise ValueError("sequences that get rows stand once each, not %s" % (list(seqs),))
 
     def layer(self, index, seqs):
         """One layer's operators for these sequences (an int n: the first n), bound to the cache's tables as they are."""
         return LayerOf(self.pool[index], *self.batch(seqs))
 
     def append(self, layer, k, v, seqs, starts=None, values=False):
+        self._once(seqs)
         return self.layer(layer, seqs).append(k, v, starts, values)
 
     def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None, k_new=None, v_new=None):
+        if k_new is not None:
+            self._once(seqs)
         return self.layer(layer, seqs).attention(q, sm_scale, starts, selected, out, k_new, v_new)
 
     def select_pages(self, layer, q, count, seqs, keep_first=1, keep_last=1):

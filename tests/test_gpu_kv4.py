@@ -195,7 +195,7 @@ def check_attention(kv4, rng, d, g, h, share, lens, new, equal, magnitude=1.0, s
     compare(out, q, pool, pages, lens, new, d, g, h, share, scale)
 
 
-def compare(out, q, pool, pages, lens, new, d, g, h, share, scale, few=24):
+def compare(out, q, pool, pages, lens, new, d, g, h, share, scale, few=24, middles=0.0):
     """Every output of up to `few` tokens of a sequence (the first, the last and some between)."""
     at = 0
     for b, (n, c) in enumerate(zip(lens, new)):
@@ -205,7 +205,7 @@ def compare(out, q, pool, pages, lens, new, d, g, h, share, scale, few=24):
             for i in tokens:
                 seen = np.arange(max(0, min(n - c + i + 1, max(n, 0))))
                 for j in range(head * share, (head + 1) * share):
-                    want, tol = ko.attend(rows, q[at + i, j].astype(np.float64), scale, seen)
+                    want, tol = ko.attend(rows, q[at + i, j].astype(np.float64), scale, seen, middles)
                     err = np.abs(out[at + i, j] - want)
                     assert np.all(err <= tol), "sequence %d token %d head %d: %.3g of %.3g" % (
                         b, i, j, err[np.argmax(err - tol)], tol[np.argmax(err - tol)])
@@ -250,6 +250,76 @@ def test_scales_of_very_different_size(kv4):
             q = rng.normal(0, 0.01, (c, 4, d)).astype(np.float16)
             out = kv4.attention(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), 0.1).cpu().numpy()
             compare(out.astype(np.float64), q, pool, pages, lens, [c], d, g, h, 4, 0.1)
+
+
+@pytest.mark.parametrize("c,share,middles", [(1, 4, 0.0), (5, 4, 0.0), (70, 4, 2.0 ** -11)], ids=["one", "five", "many"])
+def test_values_far_from_zero(kv4, c, share, middles):
+    # minima of 40 and scales of 0.3: the middle of a group is 30 times its spread (with many rows it is held in fp16)
+    d, g, h = 128, 64, 1
+    rng = np.random.default_rng(31)
+    lens = [700, 130]
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    sm = pool[..., 64 * d:64 * d + 512 * (d // g)].view(np.float16).reshape(total, h, 2, d // g, 16, 2, 4)
+    sm[:, :, 0, :, :, 1] += np.float16(3)
+    sm[:, :, 1, :, :, 1] += np.float16(40)
+    pool[..., 64 * d:64 * d + 512 * (d // g)] = sm.reshape(total, h, -1).view(np.uint8)
+    q = rng.normal(0, 1, (2 * c, share * h, d)).astype(np.float16)
+    out = kv4.attention(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), 0.1).cpu().numpy().astype(np.float64)
+    compare(out, q, pool, pages, lens, [c, c], d, g, h, share, 0.1, middles=middles)
+
+
+@pytest.mark.parametrize("d,g,h,share,tokens", [(64, 32, 2, 1, "one"), (128, 64, 1, 4, "one"), (64, 64, 1, 2, "few"),
+                                                 (128, 128, 1, 1, "chunks"), (64, 32, 2, 6, "drafts")])
+def test_many_sequences(kv4, d, g, h, share, tokens):
+    # more sequences than a wave has lanes: where a workgroup's piece lies is found over several rounds of 64
+    rng = np.random.default_rng(d + share)
+    b = 150
+    lens = rng.integers(0, 200, b).tolist()
+    lens[3], lens[70], lens[149] = 0, 4000, 2500  # two of them are dealt to several workgroups
+    if tokens in ("one", "drafts"):
+        new = [1 if tokens == "one" else 3] * b
+    elif tokens == "few":
+        new = [int(x) for x in rng.integers(0, 6, b)]
+    else:
+        new = [int(min(x, n)) for x, n in zip(rng.integers(60, 150, b), lens)]
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    q = rng.normal(0, 1, (sum(new), h * share, d)).astype(np.float16)
+    out = kv4.attention(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), d ** -0.5,
+                        None if tokens in ("one", "drafts") else dev(starts_of(new))).cpu().numpy().astype(np.float64)
+    few = {"chunks": 8}.get(tokens, 24)
+    compare(out, q, pool, pages, lens, new, d, g, h, share, d ** -0.5, few)
+
+
+def test_append_to_many_sequences(kv4):
+    d, g, h, b = 64, 32, 2, 150
+    rng = np.random.default_rng(33)
+    lens = rng.integers(1, 300, b).tolist()
+    new = [int(min(n, x)) for n, x in zip(lens, rng.integers(0, 100, b))]
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    k, v = (rng.normal(0, 1, (sum(new), h, d)).astype(np.float16) for _ in range(2))
+    dpool = dev(pool)
+    kv4.append(dev(k), dev(v), dpool, dev(pages), dev(np.array(lens, np.int32)), dev(starts_of(new)))
+    want, _ = expect_append(pool, k, v, pages, lens, new, d, g)
+    fields = ko.read(dpool.cpu().numpy(), d, g)
+    for name in want:
+        assert np.array_equal(fields[name], want[name]), name
+
+
+def test_one_table_row_for_several_sequences(kv4):
+    # samples of one prompt: the same pages, lengths of their own; the row need not be repeated in memory
+    d, g, h, share = 64, 64, 2, 4
+    rng = np.random.default_rng(34)
+    pages, total = tables(rng, [500])
+    pool, n = dev(random_pool(rng, total, h, d, g)), dev(np.array([500, 129, 64], np.int32))
+    q = dev(rng.normal(0, 1, (3, h * share, d)).astype(np.float16))
+    one = dev(pages).expand(3, -1)
+    assert torch.equal(kv4.attention(q, pool, one, n, 0.1), kv4.attention(q, pool, one.contiguous(), n, 0.1))
+    assert torch.equal(kv4.select_pages(q, pool, one, n, 3), kv4.select_pages(q, pool, one.contiguous(), n, 3))
+    with pytest.raises(ValueError):
+        kv4.attention(q, pool, one, n[:1].expand(3), 0.1)
 
 
 def test_tokens_that_see_nothing_and_tokens_of_no_sequence(kv4):
@@ -360,6 +430,19 @@ def test_pool_beyond_32_bits(kv4):
     assert torch.equal(kv4.attention(q, pool, dev(np.array([[7, n - 2, 8]], np.int32)), lens, 0.1), want)
 
 
+def test_a_refused_call_appends_nothing(kv4):
+    pool = kv4.new_pool(2, 2, 64, 32, device=DEV).zero_()
+    q, pages, lens = torch.ones((1, 4, 64), dtype=torch.float16, device=DEV), torch.zeros((1, 2), dtype=torch.int32, device=DEV), \
+        torch.ones(1, dtype=torch.int32, device=DEV)
+    room = torch.zeros(300, dtype=torch.float16, device=DEV)
+    for out in (q.float(), q[:, :2], room[4:260].view(1, 4, 64), q.cpu()):
+        with pytest.raises(ValueError):
+            kv4.attention(q, pool, pages, lens, 1.0, out=out, k_new=q[:, :2], v_new=q[:, :2])
+    assert not torch.any(pool)
+    kv4.attention(q, pool, pages, lens, 1.0, out=room[8:264].view(1, 4, 64), k_new=q[:, :2], v_new=q[:, :2])
+    assert torch.any(pool) and torch.all(room[8:264] == 1) and not torch.any(room[:8]) and not torch.any(room[264:])
+
+
 def test_strided_queries_and_other_streams(kv4):
     d, g, h, share = 64, 32, 2, 3
     rng = np.random.default_rng(16)
@@ -458,6 +541,21 @@ def test_select(kv4, d, g, h, share, lens, count, first, last):
             assert got[b, head].tolist() == want + [-1] * (count - len(want))
 
 
+def test_select_from_the_widest_table(kv4):
+    d, g, h, share, width = 64, 32, 1, 2, 16384
+    rng = np.random.default_rng(35)
+    pool = random_pool(rng, 997, h, d, g)
+    pages = rng.integers(0, 997, (2, width)).astype(np.int32)  # equal scores by the dozen
+    lens = [64 * width, 64 * 9000 + 1]
+    q = rng.normal(0, 1, (2, h * share, d)).astype(np.float16)
+    got = kv4.select_pages(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), 100).cpu().numpy()
+    bounds = ko.read(pool, d, g)["bounds"][:, 0]
+    for b, n in enumerate(lens):
+        assert got[b, 0].tolist() == ko.select(bounds[pages[b, :(n + 63) // 64]], q[b], 100, 1, 1)
+    with pytest.raises((ValueError, RuntimeError)):
+        kv4.select_pages(dev(q), dev(pool), dev(np.zeros((2, width + 1), np.int32)), dev(np.array(lens, np.int32)), 100)
+
+
 def test_select_between_equals_and_without_numbers(kv4):
     d, g = 64, 64
     rng = np.random.default_rng(20)
@@ -478,7 +576,7 @@ def test_select_between_equals_and_without_numbers(kv4):
 
 
 @pytest.mark.parametrize("d,g,h,share,lens,count", [(128, 64, 2, 4, [64 * 40 + 3, 64 * 5, 17], 8), (64, 32, 1, 1, [64 * 200], 33),
-                                                     (128, 32, 1, 16, [64 * 9 + 1], 300)])
+                                                     (128, 32, 1, 16, [64 * 9 + 1], 300), (64, 64, 1, 40, [64 * 60, 70], 20)])
 def test_attention_over_selected_pages(kv4, d, g, h, share, lens, count):
     rng = np.random.default_rng(count)
     pages, total = tables(rng, lens)

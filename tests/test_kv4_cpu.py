@@ -200,3 +200,30 @@ def test_bookkeeping_without_copies():
     assert c.free_pages() == 3 and c.pages(more) == [] and c.pages(b) == [3, 4]
     with pytest.raises(RuntimeError):
         c.add()
+
+
+def test_bookkeeping_refuses_what_would_write_into_shared_or_unknown_pages():
+    from sqamd import kv4
+    c = kv4.KV4Cache(1, 10, 1, 64, 64, max_seqs=3, max_rows=300, device="cpu")
+    a = c.add()
+    c.reserve([a], 200)
+    c.set_lengths([a], [70])
+    b = c.fork(a)
+    for seq in (a, b):  # the page of rows 64 to 69 is shared: no more rows in it before one of them has its own
+        with pytest.raises(ValueError):
+            c.set_lengths([seq], 71)
+    c.set_lengths([a], 64)
+    with pytest.raises(ValueError):
+        c.set_lengths([a], 65)
+    c.free(b)
+    c.set_lengths([a], 200)
+    x = torch.zeros((2, 1, 64), dtype=torch.float16)
+    for call in (lambda: c.batch([0, 1]), lambda: c.batch([3]), lambda: c.batch([-1]), lambda: c.batch(4), lambda: c.batch(-1),
+                 lambda: c.append(0, x, x, [a, a]), lambda: c.attention(0, x, 1.0, [a, a], k_new=x, v_new=x)):
+        with pytest.raises(ValueError):
+            call()
+    assert [t.shape[0] for t in c.batch([a, a])] == [2, 2] and c.batch(3)[1].tolist() == [200, 0, 0]
+    for wrong in ((0, 10, 1, 64, 64, 3, 300), (1, 0, 1, 64, 64, 3, 300), (1, 10, 1, 64, 64, 0, 300), (1, 10, 1, 64, 64, 3, 0),
+                  (1, 10, 1, 64, 128, 3, 300), (1, 10, 1, 96, 32, 3, 300)):
+        with pytest.raises(ValueError):
+            kv4.KV4Cache(*wrong, device="cpu")
