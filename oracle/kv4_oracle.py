@@ -67,7 +67,6 @@ class Rows:
         self.k, self.v = flat(values(f["kc"], f["ks"], f["km"])), flat(values(f["vc"], f["vs"], f["vm"]))
         self.k_abs = flat(f["ks"].astype(np.float64) * f["kc"] + np.abs(f["km"].astype(np.float64)))
         self.v_mid = flat(np.abs(f["vs"].astype(np.float64) * (f["vc"] - 8)))
-        self.v_code = flat(f["vs"].astype(np.float64) * (f["vc"] + 8))
         self.v_rest = flat(np.abs(f["vs"].astype(np.float64) * 8 + f["vm"].astype(np.float64)))
 
 
@@ -77,9 +76,9 @@ def attend(rows, q, scale, seen, middles=0.0):
     Tolerance.  P' = P s is rounded to fp16 before it meets code - 8: eps/2 = 2^-11 of every term.  A probability is off by
     twice the error of its exponent (numerator and sum): the score's fp32 sums of D + 16 terms, each rounding (also towards
     zero) 2^-23 of sum |q| (s code + |m|), and 2^-20 for the exponential, its argument in base 2 and the joining of partial
-    sums.  fp32 sums of the result: of every 32 rows first P s code and then -8 P s are added, 66 additions that each round
-    (towards zero as well) 2^-23 of a partial sum of at most sum P s (code + 8) over those rows; what remains of each 32 rows
-    is added in one chain of n / 32, 8 additions join partial sums.  The output's own rounding is 2^-11 of it, or 2^-25
+    sums.  fp32 sums of the result: the terms P s (code - 8) of every 32 rows are added to what there is, 33 additions
+    that each round (towards zero as well) 2^-23 of a partial sum of at most sum P s |code - 8| over those rows; the sums are in
+    one chain of n / 32, 8 additions join partial sums.  The output's own rounding is 2^-11 of it, or 2^-25
     where it is denormal.  middles: what m + 8 s is rounded by, of itself (2^-11
     for fp16), where it is held in fewer bits."""
     if len(seen) == 0:
@@ -94,8 +93,7 @@ def attend(rows, q, scale, seen, middles=0.0):
     dscore = (d + 16) * 2.0 ** -23 * np.max(rows.k_abs[seen] @ np.abs(q)) * abs(scale) + 2.0 ** -20
     chain = (8 + min(len(seen), 4096) / 32) * 2.0 ** -23
     tol = 2.0 ** -11 * (np.abs(out) + mid) + (2 * dscore + chain) * (mid + rest) + 2.0 ** -24
-    tol += 66 * 2.0 ** -23 * (p @ rows.v_code[seen])
-    return out, tol + middles * rest
+    return out, tol + 33 * 2.0 ** -23 * mid + middles * rest
 
 
 def select(bounds, q, count, keep_first, keep_last):

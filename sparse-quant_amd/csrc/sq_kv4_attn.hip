@@ -8,16 +8,16 @@
 // Neither operand is ever dequantised.  Per row j and group: q . k_hat = s (q . code) + m sum(q), and with P' = P s:
 // sum_j P k_hat = sum_j P' code + sum_j P m.  Codes enter the matrix instruction as they are: a nibble masked in
 // place is the denormal fp16 number code * 2^-24 (bits 0..3) or code * 2^-20 (bits 4..7), exact, so eight codes cost a
-// shift and four masks, nothing is subtracted, and the powers of two leave with the fp32 result.
+// shift and four masks, and the powers of two leave with the fp32 result.
 //   S   = K Q^T  v_mfma_f32_16x16x32_f16, A = codes (row = key), B = q: a lane has one query and four keys of 16
 //   O^T = V^T P' A = codes (row = column of V), B = P': the keys that the lane already has, in that order; the two rows
 //                whose codes share a register come together by one byte permutation of two words
-// The sum is one of P' (code - 8) and of P (m + 8 s): a second product of P' with the constant -8 follows the codes' own,
-// within every 32 rows.  The rounding of P' to fp16 then acts on s (code - 8), about the size of v, and not on s code, which
-// is twice that; and the fp32 sums stay as small as the result, where those of positive codes alone, which the matrix
-// instruction rounds towards zero, lose the more of it the longer the cache is (131072 rows: error 5.4e-4 of the result
-// instead of 2.8e-4, the rounding of P' and of the output).  P' is kept inside fp16's range by a power of two per group that
-// follows the scales.
+// The sum is one of P' (code - 8) and of P (m + 8 s): 8 is taken off the values' codes, which is exact among denormals too.
+// The rounding of P' to fp16 then acts on s (code - 8), about the size of v, and not on s code, which is twice that; and the
+// fp32 sums stay as small as the result, where those of positive codes, which the matrix instruction rounds towards zero, lose
+// the more of it the longer the cache is (131072 rows: error 5.4e-4 of the result; 3.7e-4 with the constant -8 as a product of
+// its own after every 32 rows' codes, 2 % faster; 2.9e-4 so, nearly all of it the rounding of P' and of the output).  P' is kept
+// inside fp16's range by a power of two per group that follows the scales.
 #include "sq_kernels.h"
 #include "sq_kv4_attn.h"
 #include "sq_kv4_row.h"
@@ -335,19 +335,13 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const uint32_t mask = k & 1 ? nm.hi : nm.lo;
-                        const half8_t op = k < 2 ? bit_cast<half8_t>((u32x4_t){lo[0] & mask, lo[1] & mask, lo[2] & mask, lo[3] & mask})
-                                                 : bit_cast<half8_t>((u32x4_t){up[0] & mask, up[1] & mask, up[2] & mask, up[3] & mask});
+                        const half8_t op = (k < 2 ? bit_cast<half8_t>((u32x4_t){lo[0] & mask, lo[1] & mask, lo[2] & mask, lo[3] & mask})
+                                                  : bit_cast<half8_t>((u32x4_t){up[0] & mask, up[1] & mask, up[2] & mask, up[3] & mask})) +
+                                           eight[k & 1];
                         const int i = 4 * hf + k;
 #pragma unroll
                         for (int rt = 0; rt < RT; rt++)
                             acc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op, b[rt][16 * i / g], acc[rt][i], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int i = 4 * hf + k;
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-                            acc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight[k & 1], b[rt][16 * i / g], acc[rt][i], 0, 0, 0);
                     }
                 }
             }

@@ -655,7 +655,7 @@ class Mirror:
                     kc, ks, km = (x[:, head] for x in f["k"])
                     vc, vs, vm = (x[:, head] for x in f["v"])
                     r.k, r.v, r.k_abs = ks * kc + km, vs * vc + vm, ks * kc + np.abs(km)
-                    r.v_mid, r.v_rest, r.v_code = np.abs(vs * (vc - 8)), np.abs(8 * vs + vm), vs * (vc + 8)
+                    r.v_mid, r.v_rest = np.abs(vs * (vc - 8)), np.abs(8 * vs + vm)
                     for j in range(2 * head, 2 * head + 2):
                         want, tol = ko.attend(r, q[i, j].astype(np.float64), scale, np.arange(len(r.k)))
                         assert np.all(np.abs(out[i, j] - want) <= tol), (layer, s, j)
