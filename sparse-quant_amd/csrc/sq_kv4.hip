@@ -12,7 +12,10 @@ namespace {
 // ------------------------------------------------------------------------------------------------------- append
 //
 // A workgroup owns one page of one head and with it the page's bounds, so nothing is shared between workgroups and nothing is
-// atomic (the row itself: sq_kv4_row.h).
+// atomic (the row itself: sq_kv4_row.h).  One wave where a sequence gets one row; four otherwise, each with every fourth
+// pass of rows (6421 tokens of 12 prompts, 8 heads in groups of 32: 22.1 / 20.0 / 22.2 / 30.8 us with 2 / 4 / 8 / 16 waves).
+// Bounds: a step of 8 sequences 3.65 us, of which a launch that does nothing is 1.7; the prompts move 61 MB in 18 to 20 us
+// (3.1 to 3.4 TB/s; a copy of as many bytes 12.3) and spend as long on the codes as on the loads.
 struct Kv4AppendArgs {
     Kv4Cache c;
     const half_t* k;
@@ -166,7 +169,9 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_append_kernel(Kv4AppendArgs a)
 
 // --------------------------------------------------------------------------------------------------------- copy
 
-// Pages of all layers, src[i] to dst[i]; a pair with an index outside the pool is left out.
+// Pages of all layers, src[i] to dst[i]; a pair with an index outside the pool is left out.  16 KB of a page per workgroup,
+// four 16-byte loads of a thread under way at once: 195 MB of 8 layers in 39 to 42 us, what a large copy reaches (5 TB/s);
+// one page of 32 layers 3.15 us.
 __global__ __launch_bounds__(256) void kv4_copy_kernel(uint8_t* pool, const int* src, const int* dst, int num_pages,
                                                        int parts, long page_bytes, long layer_bytes) {
     const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -192,7 +197,10 @@ __global__ __launch_bounds__(256) void kv4_copy_kernel(uint8_t* pool, const int*
 // smallest keys: no key of the page can score higher.  Which of two pages is the better one must not hang on the order
 // of a sum: products of fp16 numbers are exact in fp32, their sums are taken in 64 bits.
 // 16 (D = 64: 8) lanes share a page, 8 elements each; the choice between hi and lo goes by the signs of the queries, which
-// a lane keeps as masks of pairs.  A wave takes SELECT_PAGES pages, all their bounds asked for at once.
+// a lane keeps as masks of pairs.  A wave takes SELECT_PAGES pages, all their bounds asked for at once (8 sequences of up
+// to 32768 rows and 8 heads: 7.1 us, up to 17 MB of bounds in pieces of 512 bytes; 125 pages of 8 heads 16.9 us for all three
+// launches with 8 pages a wave, 17.3 with 16).  A launch of its own: with the choice in the same one, by the workgroup that
+// ends last, the two took 8.5 instead of 8.4 and 20 instead of 11 us.
 constexpr int SELECT_QUERIES = 4;  // of a round
 constexpr int SELECT_PAGES = 8;    // of a wave
 
@@ -280,10 +288,12 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     return u & 0x8000000000000000ull ? ~u : u | 0x8000000000000000ull;
 }
 
+// (1024 / 512 / 256: 17.7 / 17.3 / 17.2 us for all three launches at 125 pages, 30.0 / 29.6 / 30.2 at 512)
 constexpr int SELECT_THREADS = 512;
 
 // The `count` best pages of a head in ascending order, ties to the lowest; -1 behind the last where there are fewer.
-// The count-th largest key is found digit by digit, from the top, until no other key shares its digits.
+// The count-th largest key is found digit by digit, from the top, until no other key shares its digits.  4 to 5 us, most of it
+// the barriers of two or three digits.
 __global__ __launch_bounds__(SELECT_THREADS) void kv4_select_kernel(Kv4SelectArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned long long keys[];
     __shared__ unsigned hist[256];

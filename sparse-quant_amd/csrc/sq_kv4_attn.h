@@ -134,7 +134,8 @@ __device__ __forceinline__ float wave_max(float v) {
 constexpr float KA_LAZY = 8.f;  // the softmax's reference moves when a score is 2^8 beyond it
 
 // Shares of a tile's pages, joined: a workgroup has ROWS rows of a shared tile, 256 / ROWS threads each, of which D / 4 hold
-// four columns each of every so many-th share.  (LAST: tiles are worked on from the last to the first.)
+// four columns each of every so many-th share.  (LAST: tiles are worked on from the last to the first.)  3.8 to 4.7 us where
+// a tile has up to a few dozen shares, nearly all of it the launch and two rounds of loads; 18 us for the 35 MB of 1024 tokens.
 template <int D, int R, int ROWS, bool LAST>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, Deal d) {
     constexpr int C4 = D / 4, LANES = 256 / C4 / ROWS;

@@ -29,6 +29,11 @@ namespace {
 // The kernel for few rows.  A workgroup's waves take units of a page (PACK = 1: half of one) in turn, each with a softmax
 // of its own, and join them in LDS.
 //
+// What bounds it: over long caches the stream of records (64 ragged sequences, 221 MB, 49 us = 4.5 TB/s; 131072 rows of one,
+// 151 MB, 37.5 us = 4.0 TB/s), with which the work on the codes just keeps up; over short ones latency, one after the other:
+// launch, lengths and table, records, join (640 rows of one sequence 8.1 us, of eight 9.9 us = 2.4 TB/s); with 20 queries
+// to a key the work per row (5 tokens of 16 sequences 22.5 us).
+//
 // PACK.  The matrix instruction has 16 columns for the tile's rows; with 4 rows, 12 of them would be empty, and so would
 // be three quarters of all that follows per score.  So 4 (2) tiles of 16 cache rows share one result: the tile's queries stand
 // in columns 4 j .. 4 j + 3 of the operand that meets the j-th of them and the other columns are 0, so that the four products
@@ -464,7 +469,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     }
 }
 
-// Workgroups that a launch's pages are dealt to, and a share's fewest pages: see launch_kv4_attention.
+// Workgroups per CU that a launch's pages are dealt to, and a share's fewest pages.  Two (64 ragged sequences / one of
+// 131072 rows: 48.9 / 38.0 us; 59 / 45 with three, 54 / 46 with four: more partial states and no more loads under way than
+// the registers allow).  Sixteen pages, so that up to 1024 rows nothing is shared: with eight, 640 rows of one sequence
+// take 10.5 instead of 8.1 us, of eight 14 instead of 9.9 (the second launch is dearer than what it saves), 5 tokens of
+// 16 sequences 28.7 instead of 22.5.
 constexpr Deal KA_DEAL = {2, 16};
 constexpr int KA_ROWS = 32;  // of a tile at the most
 
@@ -542,6 +551,9 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         else
             go(d, groups, pack, rt, Int<4>{});
     };
+    // Rows of a tile: the fewest that hold the average sequence's, so that few columns of the products are empty.  17 to 32
+    // rows: two operands of queries per unpacked code by 8 waves (5 tokens of 4 query heads 22.5 us, by 4 waves 25.9; two
+    // tiles of 16 rows instead 26.9 and, by 4 waves, 24.3).
     auto by_rows = [&](auto d, auto groups) {
         if (mean <= 4)
             waves_for(d, groups, Int<4>{}, Int<1>{});

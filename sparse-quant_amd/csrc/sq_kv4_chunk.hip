@@ -11,6 +11,10 @@
 // s' = 16 s over a power of two that follows the scales (of the largest so far), so that P' stays inside fp16's range.
 // While a page is worked on, the next one's codes are unpacked into the other half of LDS and the one behind it is on its way to
 // registers; one barrier a page, which does not wait for those.
+//
+// What bounds it: vector instructions, 561 of them beside 32 matrix instructions per wave and page (13.3 a score), which the two
+// waves of a SIMD hardly overlap (heads of 128 in groups of 64, 1024 tokens of 32 heads over 16384 rows: 438 us = 608 TFLOP/s
+// with the join; counters: vector units busy 0.63, matrix units 0.26, LDS 0.34 of 968 thousand cycles, no bank conflicts).  Groups of 128 take 0.84 of the time of groups of 64, of 32 1.5 times.
 #include "sq_kernels.h"
 #include "sq_kv4_attn.h"
 
@@ -352,6 +356,8 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
     }
 }
 
+// Workgroups per CU that the pages are dealt to (1 / 2 / 3 / 4 / 6 / 8: 645 / 449 / 478 / 466 / 473 / 493 us at 1024 tokens
+// over 16384 rows: two fit on a CU, and a share's partial state is 66 KB to write and read), and a share's fewest pages.
 constexpr Deal KC_DEAL = {2, 8};
 
 }  // namespace
