@@ -757,6 +757,53 @@ def test_a_captured_step_follows_lengths_and_tables(kv4):
         assert torch.equal(pool, eager[0]) and torch.equal(n, eager[1])
 
 
+@pytest.mark.parametrize("each,share,d,g", [(40, 4, 128, 64), (3, 4, 64, 32)], ids=["chunk", "drafts"])
+def test_captured_chunks_follow_lengths(kv4, each, share, d, g):
+    # tokens appended and attended to in one graph: shares and joins follow the lengths that a replay finds
+    h, b = 2, 2
+    rng = np.random.default_rng(36)
+    lens = np.array([each, 1500], np.int32)
+    pages, total = tables(rng, lens + 8 * 640, spare=0)
+    pool, n, table = dev(random_pool(rng, total, h, d, g)), dev(lens), dev(pages)
+    kv = torch.empty((2, b * each, h, d), dtype=torch.float16, device=DEV)
+    q = torch.empty((b * each, h * share, d), dtype=torch.float16, device=DEV)
+    call = lambda pool: kv4.attention(q, pool, table, n, 0.1, k_new=kv[0], v_new=kv[1])
+    kv.normal_(), q.normal_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(pool.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    eager = pool.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(pool)
+    for more in (0, each, 640, each, 3000):
+        n += more
+        kv.normal_(), q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call(eager)) and torch.equal(pool, eager), more
+
+
+@pytest.mark.parametrize("tokens,share", [(1, 4), (1, 12), (30, 8)], ids=["packed", "rows", "chunk"])
+def test_attention_without_a_workspace(kv4, tokens, share):
+    # nothing is shared then: one workgroup goes through all of a tile's pages
+    from sqamd import capi
+    d, g, h = 128, 64, 1
+    rng = np.random.default_rng(37)
+    lens = [4000, 70]
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    q = rng.normal(0, 1, (2 * tokens, share, d)).astype(np.float16)
+    dq, dpool, dpages, n = dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32))
+    out, p = torch.empty_like(dq), capi._ptr
+    assert capi.lib().sq_kv4_attention(p(dq), p(out), p(dpool), p(dpages), p(n), None, None, 2 * tokens, 2, h * share, h, d, g, total,
+                                       pages.shape[1], pages.shape[1], 0, share * d, d, d ** -0.5, None, None, None, None, 0,
+                                       capi._stream()) == 0
+    compare(out.cpu().numpy().astype(np.float64), q, pool, pages, lens, [tokens] * 2, d, g, h, share, d ** -0.5)
+
+
 def test_two_graphs_at_once(kv4):
     # each captured call has a workspace of its own: graphs on two streams do not disturb each other
     d, g, h, share = 128, 64, 8, 4
