@@ -301,7 +301,7 @@ class KV4Cache:
 
     def reserve(self, seqs, rows):
         """Pages for the first rows[i] rows of seqs[i], of their own from the row behind the last one on."""
-        rows = self._per_sequence(seqs, rows)
+        seqs, rows = self._per_sequence(seqs, rows)
         fresh = {}   # sequence -> places that get a new page
         for seq, n in zip(seqs, rows):
             pages = self._known(seq)
@@ -344,7 +344,7 @@ class KV4Cache:
 
     def extend(self, seqs, rows):
         """Room for rows[i] (or `rows`) more rows of seqs[i], and count them."""
-        more = self._per_sequence(seqs, rows)
+        seqs, more = self._per_sequence(seqs, rows)
         total = [self.rows(seq) + n for seq, n in zip(seqs, more)]
         if any(n < 0 for n in more):
             raise ValueError("a sequence shrinks by truncate")
@@ -353,7 +353,7 @@ class KV4Cache:
 
     def set_lengths(self, seqs, rows):
         """Count rows that have pages already, new ones pages that no other sequence shares."""
-        rows = self._per_sequence(seqs, rows)
+        seqs, rows = self._per_sequence(seqs, rows)
         for seq, n in zip(seqs, rows):
             pages = self._known(seq)
             if not 0 <= n <= len(pages) * PAGE:
@@ -390,10 +390,11 @@ class KV4Cache:
 
     @staticmethod
     def _per_sequence(seqs, rows):
-        rows = [rows] * len(seqs) if isinstance(rows, int) else list(rows)
+        seqs = [int(seq) for seq in seqs]
+        rows = [rows] * len(seqs) if isinstance(rows, int) else [int(n) for n in rows]
         if len(rows) != len(seqs) or len(set(seqs)) != len(seqs):
-            raise ValueError("%d row counts for the sequences %s" % (len(rows), list(seqs)))
-        return rows
+            raise ValueError("%d row counts for the sequences %s" % (len(rows), seqs))
+        return seqs, rows
 
     def _vectors(self, *lists):
         return torch.tensor(lists, dtype=torch.int32).to(self.pool.device).unbind(0)
@@ -413,27 +414,32 @@ class KV4Cache:
             if not 0 <= seqs <= self.max_seqs:
                 raise ValueError("%d sequences of a cache for %d" % (seqs, self.max_seqs))
             return self.table[:seqs], self.lengths[:seqs]
+        seqs = [int(seq) for seq in seqs]
         for seq in seqs:
             self._known(seq)
-        at = torch.tensor(list(seqs), dtype=torch.int64, device=self.table.device)
+        at = torch.tensor(seqs, dtype=torch.int64, device=self.table.device)
         return self.table[at], self.lengths[at]
 
     @staticmethod
     def _once(seqs):
-        if not isinstance(seqs, int) and len(set(seqs)) != len(seqs):
-            raise ValueError("sequences that get rows stand once each, not %s" % (list(seqs),))
+        """The sequences of a call that stores rows."""
+        if isinstance(seqs, int):
+            return seqs
+        seqs = [int(seq) for seq in seqs]
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("sequences that get rows stand once each, not %s" % (seqs,))
+        return seqs
 
     def layer(self, index, seqs):
         """One layer's operators for these sequences (an int n: the first n), bound to the cache's tables as they are."""
         return LayerOf(self.pool[index], *self.batch(seqs))
 
     def append(self, layer, k, v, seqs, starts=None, values=False):
-        self._once(seqs)
-        return self.layer(layer, seqs).append(k, v, starts, values)
+        return self.layer(layer, self._once(seqs)).append(k, v, starts, values)
 
     def attention(self, layer, q, sm_scale, seqs, starts=None, selected=None, out=None, k_new=None, v_new=None):
         if k_new is not None:
-            self._once(seqs)
+            seqs = self._once(seqs)
         return self.layer(layer, seqs).attention(q, sm_scale, starts, selected, out, k_new, v_new)
 
     def select_pages(self, layer, q, count, seqs, keep_first=1, keep_last=1):

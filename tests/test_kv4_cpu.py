@@ -222,6 +222,11 @@ def test_bookkeeping_refuses_what_would_write_into_shared_or_unknown_pages():
                  lambda: c.append(0, x, x, [a, a]), lambda: c.attention(0, x, 1.0, [a, a], k_new=x, v_new=x)):
         with pytest.raises(ValueError):
             call()
+    c.set_lengths(iter([a]), (n for n in [199]))  # any iterable of numbers
+    c.set_lengths(torch.tensor([a]), torch.tensor([200]))
+    with pytest.raises(ValueError):
+        c.append(0, x, x, torch.tensor([a, a]))
+    assert c.batch(iter([a]))[1].tolist() == [200]
     assert [t.shape[0] for t in c.batch([a, a])] == [2, 2] and c.batch(3)[1].tolist() == [200, 0, 0]
     for wrong in ((0, 10, 1, 64, 64, 3, 300), (1, 0, 1, 64, 64, 3, 300), (1, 10, 1, 64, 64, 0, 300), (1, 10, 1, 64, 64, 3, 0),
                   (1, 10, 1, 64, 128, 3, 300), (1, 10, 1, 96, 32, 3, 300)):
