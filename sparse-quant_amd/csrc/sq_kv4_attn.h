@@ -22,6 +22,7 @@ struct Kv4AttnArgs {
     const half_t* k_new;  // the row of every sequence's one token, stored by the kernel first, or null
     const half_t* v_new;
     long k_ts, k_hs, v_ts, v_hs;
+    int rows_min, rows_max;  // sequences with fewer or more rows (token, query head) per head are another launch's (with starts)
 };
 
 // How a launch's work is dealt.  A tile is R of the rows (token, query head) of a sequence and key/value head; a
@@ -52,7 +53,8 @@ __device__ __forceinline__ Sizes sizes_of(const Kv4AttnArgs& a, int b) {
         s.len = kv4_length(a.c, b);
         s.pages = ceil_div(s.len, KV4_PAGE);
         if (a.selected) s.pages = imin(s.pages, a.count);
-        s.tiles = ceil_div(s.count * a.share, R) * a.c.H;
+        const int rows = s.count * a.share;
+        s.tiles = rows >= a.rows_min && rows <= a.rows_max ? ceil_div(rows, R) * a.c.H : 0;
     }
     return s;
 }

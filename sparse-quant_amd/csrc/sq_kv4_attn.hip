@@ -505,7 +505,8 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
     a.k_new = a.v_new = nullptr;
     a.k_ts = a.k_hs = a.v_ts = a.v_hs = 0;
     // Rows of a sequence and key/value head (of the average one where they differ).
-    const long mean = ((long)c.T * share + c.B - 1) / c.B;
+    long mean = ((long)c.T * share + c.B - 1) / c.B;
+    a.rows_min = 0, a.rows_max = 1 << 30;
     if (k_new && !c.starts && c.each == 1 && mean <= KA_ROWS) {
         a.k_new = (const half_t*)k_new;
         a.v_new = (const half_t*)v_new;
@@ -517,12 +518,22 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         const hipError_t e = launch_kv4_append(c, k_new, v_new, nullptr, nullptr, D, g, new_strides, st);
         if (e != hipSuccess) return e;
     }
+    // Prompts beside single tokens: where sequences differ and the average is up to 1024 rows, the kernel for many rows takes
+    // those with more than KA_ROWS and this one the others, which there would fill a thirtieth of a tile (4 query heads, 1024
+    // tokens over 4096 rows beside 63 sequences of one token: 414 us without, 205 so; beside 7: 177 and 151; 8 prompts of 30
+    // to 58 tokens, where nothing is left for this kernel: 9.4 and 11.2, as chunks over 2000 rows 49 and 55).
+    const bool both = c.starts && !selected && mean > KA_ROWS && mean <= 1024 && share <= KA_ROWS && c.B > 1;
     if (mean > KA_ROWS && !selected) {
         a.ws = (float*)workspace;
-        return launch_kv4_chunk(a, D, g, st);
+        if (both) a.rows_min = KA_ROWS + 1;
+        const hipError_t e = launch_kv4_chunk(a, D, g, st);
+        if (e != hipSuccess || !both) return e;
+        a.rows_min = 0, a.rows_max = KA_ROWS;
+        mean = share;  // most have one token
     }
     const int most = selected && count < c.width ? count : c.width;
     auto tiles_of = [&](int R) {
+        if (both && (long)c.T * share > (long)c.B * KA_ROWS) return (long)c.B * (KA_ROWS / R) * c.H;
         return (c.starts ? (long)c.T * share / R + c.B : (long)c.B * (((long)c.each * share + R - 1) / R)) * c.H;
     };
     const bool split = workspace != nullptr && most > KA_DEAL.least && tiles_of(4) < KA_MOST_PAGES / most;

@@ -292,6 +292,29 @@ def test_many_sequences(kv4, d, g, h, share, tokens):
     compare(out, q, pool, pages, lens, new, d, g, h, share, d ** -0.5, few)
 
 
+@pytest.mark.parametrize("d,g,h,share,singles,others", [
+    (128, 64, 2, 4, 30, [(3000, 400), (70, 9), (40, 8), (5, 0), (9, 9)]), (64, 32, 1, 1, 20, [(1200, 1100), (33, 33), (32, 32), (400, 31), (0, 0)]),
+    (128, 128, 1, 16, 5, [(200, 40), (90, 2), (91, 3)]), (64, 64, 1, 32, 3, [(100, 6), (2500, 1), (60, 2)]),
+    (64, 64, 1, 33, 3, [(100, 6), (2500, 1), (60, 2)])], ids=["four", "one", "sixteen", "widest", "too-wide"])
+def test_prompts_beside_single_tokens(kv4, d, g, h, share, singles, others):
+    # few and many rows in one call: the sequences are dealt to two kernels by their rows, each once
+    rng = np.random.default_rng(38)
+    lens = rng.integers(1, 1500, singles).tolist() + [n for n, _ in others]
+    new = [1] * singles + [c for _, c in others]
+    order = rng.permutation(len(lens))
+    lens, new = [int(lens[i]) for i in order], [int(new[i]) for i in order]
+    assert 32 < (sum(new) * share + len(new) - 1) // len(new) <= 256
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    t = sum(new)
+    q = rng.normal(0, 1, (t + 2, h * share, d)).astype(np.float16)
+    out = torch.full(q.shape, 9.0, dtype=torch.float16, device=DEV)
+    kv4.attention(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), d ** -0.5, dev(starts_of(new)), out=out)
+    out = out.cpu().numpy().astype(np.float64)
+    assert np.all(out[t:] == 9.0)
+    compare(out, q, pool, pages, lens, new, d, g, h, share, d ** -0.5)
+
+
 def test_append_to_many_sequences(kv4):
     d, g, h, b = 64, 32, 2, 150
     rng = np.random.default_rng(33)
