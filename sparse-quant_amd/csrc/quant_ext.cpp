@@ -533,7 +533,14 @@ c10::optional<std::vector<at::Tensor>> kv4_append(const at::Tensor& k, const at:
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(k.device());
     std::vector<at::Tensor> hats;
-    if (values) hats = {at::empty(k.sizes(), k.options()), at::empty(k.sizes(), k.options())};
+    if (values) {  // one allocation for both (an allocation costs the host 1 us of the 5 that a call takes)
+        const at::Tensor both = at::empty({2, k.size(0), k.size(1), k.size(2)}, k.options());
+        for (int i = 0; i < 2; i++) {
+            hats.push_back(at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), both.dtype()));
+            hats[i].unsafeGetTensorImpl()->set_storage_offset(i * k.numel());
+            hats[i].unsafeGetTensorImpl()->set_sizes_contiguous(k.sizes());
+        }
+    }
     const long strides[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
     const int rc = sq_kv4_append(k.data_ptr(), v.data_ptr(), values ? hats[0].data_ptr() : nullptr,
                                  values ? hats[1].data_ptr() : nullptr, pool.data_ptr(), pages.data_ptr(), lengths.data_ptr(),
