@@ -216,7 +216,8 @@ class KV4Cache:
     them) or ahead of time with `reserve`; `append`, `attention` and `select_pages` then work on one layer for a list of
     sequences, or for all of the first n (`seqs` an int).  Pages may be shared between sequences (`fork`): a page is copied
     before a sequence that shares it gets rows in it, by `reserve` (and so by `extend`), which therefore follows a fork.  `lengths` and `table` are the device's view of it and change in place; with
-    rows reserved a captured graph may count `lengths` up itself (`set_lengths` then brings the host's view after it)."""
+    rows reserved a captured graph may count `lengths` up itself (`set_lengths` then brings the host's view after it); rows
+    that it counts beyond the reserved pages, or of a sequence that has ended, are left out."""
 
     def __init__(self, layers, num_pages, kv_heads, head_dim, group_size=64, max_seqs=8, max_rows=2048, device="cuda"):
         if min(layers, num_pages, kv_heads, max_seqs, max_rows) < 1:
@@ -226,7 +227,9 @@ class KV4Cache:
         self.layers, self.num_pages, self.max_seqs, self.max_rows = layers, num_pages, max_seqs, max_rows
         self.kv_heads, self.head_dim, self.group_size = kv_heads, head_dim, group_size
         self.width = (max_rows + PAGE - 1) // PAGE
-        self.table = torch.zeros((max_seqs, self.width), dtype=torch.int32, device=self.pool.device)
+        # Places without a page hold -1, which the kernels know as no page: a sequence whose length is counted on the device
+        # past its pages, or after it has ended, neither stores nor sees rows there.
+        self.table = torch.full((max_seqs, self.width), -1, dtype=torch.int32, device=self.pool.device)
         self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=self.pool.device)
         self._pages = [None] * max_seqs  # of a sequence, in their order; None: no such sequence
         self._rows = [0] * max_seqs
@@ -273,6 +276,7 @@ class KV4Cache:
         self._pages[seq] = None
         self._rows[seq] = 0
         self.lengths[seq:seq + 1].zero_()
+        self.table[seq].fill_(-1)
 
     def fork(self, seq):
         """A new sequence with the rows of `seq`, on the same pages; returns its number."""
@@ -297,6 +301,7 @@ class KV4Cache:
         for page in pages[keep:]:
             self._release(page)
         del pages[keep:]
+        self.table[seq, keep:].fill_(-1)
         self._count([seq], [rows])
 
     def reserve(self, seqs, rows):
@@ -401,7 +406,7 @@ class KV4Cache:
 
     def _write(self, seqs):
         """The device's table of these sequences."""
-        rows = torch.zeros((len(seqs), self.width), dtype=torch.int32)
+        rows = torch.full((len(seqs), self.width), -1, dtype=torch.int32)
         for i, seq in enumerate(seqs):
             rows[i, :len(self._pages[seq])] = torch.tensor(self._pages[seq], dtype=torch.int32)
         self.table[torch.tensor(seqs, device=self.table.device)] = rows.to(self.table.device)

@@ -164,3 +164,34 @@ def test_other_widths_are_refused(opt):
         model.new_cache(1, 64, kv_bits=8)
     with pytest.raises(ValueError):
         model.new_cache(1, 64, kv_bits=4, kv_group=256)
+
+
+def test_steps_past_the_reserved_pages_leave_other_sequences_alone(opt):
+    # the device counts every sequence of the batch: one that has ended, and one at the end of its pages, store nowhere
+    model = small(opt)
+    from sqamd import kv4
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    ids = torch.randint(0, 1000, (3, 60), device=DEV, generator=gen)
+    cache = kv4.KV4Cache(len(model.layers), 8, model.heads, 128, max_seqs=4, max_rows=256, device=DEV)
+    cache.pool.zero_()
+    for _ in range(3):
+        cache.add()
+    cache.reserve([0, 1, 2], 60)
+    model(ids, cache, 0)
+    cache.free(1)
+    cache.reserve([0], 200)          # the first gets the page that was the second's; the third has rows up to 64 only
+    assert cache.pages(0)[1] == 1
+    tok, pos = ids[:, :1].contiguous(), torch.tensor([60], device=DEV)
+    for _ in range(4):
+        model.greedy_step(tok, cache, pos)
+    before = cache.pool.clone()
+    for _ in range(6):               # rows 64 to 69
+        logits = model.greedy_step(tok, cache, pos)
+    assert torch.isfinite(logits[0]).all()
+    # what has changed: six rows of the first sequence's second page and its bounds, in every layer
+    changed = torch.nonzero((cache.pool != before).flatten(2).any(2))
+    assert sorted(set(changed[:, 1].tolist())) == [1] and len(changed) == len(model.layers)
+    new, old = (ko.read(x[:, 1].cpu().numpy(), 128, 64) for x in (cache.pool, before))
+    for name in ("kc", "vc", "ks", "vs", "km", "vm"):
+        assert np.array_equal(new[name][..., 6:, :], old[name][..., 6:, :]), name
+    assert np.any(new["kc"][..., :6, :] != old["kc"][..., :6, :])

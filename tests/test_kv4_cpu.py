@@ -232,3 +232,48 @@ def test_bookkeeping_refuses_what_would_write_into_shared_or_unknown_pages():
                   (1, 10, 1, 64, 128, 3, 300), (1, 10, 1, 96, 32, 3, 300)):
         with pytest.raises(ValueError):
             kv4.KV4Cache(*wrong, device="cpu")
+
+
+@pytest.fixture
+def host_copies(monkeypatch):
+    """Page copies of a pool on the host, so that the bookkeeping around them runs without a GPU."""
+    from sqamd import kv4
+
+    def copy(pool, src, dst):
+        pool[:, dst.long()] = pool[:, src.long()]
+    monkeypatch.setattr(kv4, "copy_pages", copy)
+
+
+def only_own_pages(c):
+    """Every place of the device's table names the sequence's own page there, or none."""
+    for seq, row in enumerate(c.table.tolist()):
+        own = c._pages[seq] or []
+        if row != own + [-1] * (c.width - len(own)):
+            return False
+    return True
+
+
+def test_places_without_a_page_name_none(host_copies):
+    # a place that no sequence owns must not name a page: a length counted on the device past it would reach others' rows
+    from sqamd import kv4
+    c = kv4.KV4Cache(1, 10, 1, 64, 64, max_seqs=3, max_rows=256, device="cpu")
+    assert only_own_pages(c)
+    a, b = c.add(), c.add()
+    c.extend([a, b], [64, 130])
+    assert only_own_pages(c)
+    c.free(b)
+    assert only_own_pages(c)
+    c.extend([a], 64)  # on a page that was b's
+    assert only_own_pages(c)
+    c.extend([a], 70)
+    c.truncate(a, 60)
+    assert c.pages(a) == [0] and only_own_pages(c)
+    b = c.add()
+    f = c.fork(a)
+    assert only_own_pages(c)
+    c.reserve([f, a, b], [200, 61, 64])
+    assert only_own_pages(c)
+    c.truncate(f, 0)
+    c.free(a)
+    c.extend([b], 10)
+    assert only_own_pages(c)
