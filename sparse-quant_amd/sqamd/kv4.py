@@ -215,9 +215,15 @@ class KV4Cache:
     Sequences are numbered 0 .. max_seqs - 1 (`add`, `fork`, `free`).  Rows are given room with `extend` (which also counts
     them) or ahead of time with `reserve`; `append`, `attention` and `select_pages` then work on one layer for a list of
     sequences, or for all of the first n (`seqs` an int).  Pages may be shared between sequences (`fork`): a page is copied
-    before a sequence that shares it gets rows in it, by `reserve` (and so by `extend`), which therefore follows a fork.  `lengths` and `table` are the device's view of it and change in place; with
-    rows reserved a captured graph may count `lengths` up itself (`set_lengths` then brings the host's view after it); rows
-    that it counts beyond the reserved pages, or of a sequence that has ended, are left out."""
+    before a sequence that shares it gets rows in it, by `reserve` (and so by `extend`), which therefore follows a fork.
+    `lengths` and `table` are the device's view of it and change in place.
+
+    With rows reserved the device may count `lengths` up itself, as a captured graph does and every decode step that takes
+    its position from the device.  `counted_on_device` says so, once, before the first such step.  From then on the host asks
+    the device for the rows of these sequences where it needs them (`rows`, `fork`, `truncate`, `reserve`, `extend`), which
+    waits for the current stream; and where `fork`, `truncate` or `set_lengths` leaves them at the end of a shared page it
+    gives them their own at once, since a replayed step cannot be refused.  Rows counted beyond the reserved pages, or of a
+    sequence that has ended, are left out."""
 
     def __init__(self, layers, num_pages, kv_heads, head_dim, group_size=64, max_seqs=8, max_rows=2048, device="cuda"):
         if min(layers, num_pages, kv_heads, max_seqs, max_rows) < 1:
@@ -233,6 +239,7 @@ class KV4Cache:
         self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=self.pool.device)
         self._pages = [None] * max_seqs  # of a sequence, in their order; None: no such sequence
         self._rows = [0] * max_seqs
+        self._device_counts = set()  # sequences (their numbers, whoever has them) whose lengths the device counts as well
         self._uses = [0] * num_pages
         self._free = list(range(num_pages))  # a heap: the lowest page first
 
@@ -243,11 +250,36 @@ class KV4Cache:
             raise ValueError("no sequence %r" % (seq,))
         return self._pages[seq]
 
+    def counted_on_device(self, seqs):
+        """Something on the device counts `lengths` of these sequences from now on (an int n: of the first n, whether they
+        exist or not).  Refused where the next rows would go to a page that another sequence shares."""
+        seqs = [seq for seq in (range(seqs) if isinstance(seqs, int) else map(int, seqs)) if seq not in self._device_counts]
+        for seq in seqs:
+            if not 0 <= seq < self.max_seqs:
+                raise ValueError("no sequence %r" % (seq,))
+            if self._pages[seq] and any(self._uses[page] > 1 for page in self._pages[seq][self._rows[seq] // PAGE:]):
+                raise ValueError("rows of sequence %d would go to a page that another shares; reserve gives it its own" % seq)
+        self._device_counts.update(seqs)
+
+    def _ask_device(self, seqs, beyond=False):
+        """Bring the host's row counts after the device's; more rows than pages hold are an error unless `beyond`."""
+        asked = [seq for seq in seqs if seq in self._device_counts and self._pages[seq] is not None]
+        if not asked:
+            return
+        lengths = self.lengths.tolist()
+        for seq in asked:
+            room = len(self._pages[seq]) * PAGE
+            if lengths[seq] > room and not beyond:
+                raise RuntimeError("the device counted sequence %d to %d rows, of which its pages hold %d: truncate or "
+                                   "set_lengths says how many it keeps" % (seq, lengths[seq], room))
+            self._rows[seq] = max(0, min(lengths[seq], room))
+
     def free_pages(self):
         return len(self._free)
 
     def rows(self, seq):
         self._known(seq)
+        self._ask_device([seq])
         return self._rows[seq]
 
     def pages(self, seq):
@@ -281,7 +313,7 @@ class KV4Cache:
     def fork(self, seq):
         """A new sequence with the rows of `seq`, on the same pages; returns its number."""
         pages = self._known(seq)
-        rows = self._rows[seq]
+        rows = self.rows(seq)
         new = self.add()
         used = pages[:(rows + PAGE - 1) // PAGE]
         for page in used:
@@ -289,32 +321,51 @@ class KV4Cache:
         self._pages[new] = list(used)
         self._write([new])
         self._count([new], [rows])
+        if self._device_counts & {seq, new}:
+            try:
+                self._give({new: (rows, len(used) * PAGE)})
+            except RuntimeError:
+                self.free(new)
+                raise
         return new
 
     def truncate(self, seq, rows):
         """Keep the first `rows` rows of a sequence and release the pages behind them.  (The bounds of the page that becomes
         its last still cover the rows that went, until its row 0 is stored again.)"""
         pages = self._known(seq)
+        self._ask_device([seq], beyond=True)
         if not 0 <= rows <= self._rows[seq]:
             raise ValueError("cannot keep %d of %d rows" % (rows, self._rows[seq]))
         keep = (rows + PAGE - 1) // PAGE
+        own = seq in self._device_counts and rows % PAGE and self._uses[pages[keep - 1]] > 1
+        if own and not self._free and all(self._uses[page] > 1 for page in pages[keep:]):
+            raise RuntimeError("1 page wanted, 0 free of %d" % self.num_pages)
         for page in pages[keep:]:
             self._release(page)
         del pages[keep:]
         self.table[seq, keep:].fill_(-1)
+        if own:
+            self._give({seq: (rows, keep * PAGE)})
         self._count([seq], [rows])
 
     def reserve(self, seqs, rows):
         """Pages for the first rows[i] rows of seqs[i], of their own from the row behind the last one on."""
         seqs, rows = self._per_sequence(seqs, rows)
-        fresh = {}   # sequence -> places that get a new page
         for seq, n in zip(seqs, rows):
-            pages = self._known(seq)
+            self._known(seq)
             if n > self.max_rows:
                 raise ValueError("%d rows in a cache of %d" % (n, self.max_rows))
-            if n > self._rows[seq]:
-                first = self._rows[seq] // PAGE
-                fresh[seq] = [j for j in range(first, (n + PAGE - 1) // PAGE) if j >= len(pages) or self._uses[pages[j]] > 1]
+        self._ask_device(seqs)
+        self._give({seq: (self._rows[seq], n) for seq, n in zip(seqs, rows)})
+
+    def _give(self, wanted):
+        """{sequence: (held, rows)}: pages of its own for the rows from `held`, the last it has, to `rows`."""
+        fresh = {}   # sequence -> places that get a new page
+        for seq, (held, n) in wanted.items():
+            if n > held:
+                pages = self._pages[seq]
+                fresh[seq] = [j for j in range(held // PAGE, (n + PAGE - 1) // PAGE)
+                              if j >= len(pages) or self._uses[pages[j]] > 1]
         # a page shared by sequences of this very call is copied for all but the last of them
         want = []
         shared = dict()
@@ -335,7 +386,7 @@ class KV4Cache:
             page = heapq.heappop(self._free)
             self._uses[page] = 1
             if j < len(pages):
-                if j * PAGE < self._rows[seq]:  # it holds rows
+                if j * PAGE < wanted[seq][0]:  # it holds rows
                     src.append(pages[j])
                     dst.append(page)
                 self._release(pages[j])
@@ -350,7 +401,10 @@ class KV4Cache:
     def extend(self, seqs, rows):
         """Room for rows[i] (or `rows`) more rows of seqs[i], and count them."""
         seqs, more = self._per_sequence(seqs, rows)
-        total = [self.rows(seq) + n for seq, n in zip(seqs, more)]
+        for seq in seqs:
+            self._known(seq)
+        self._ask_device(seqs)
+        total = [self._rows[seq] + n for seq, n in zip(seqs, more)]
         if any(n < 0 for n in more):
             raise ValueError("a sequence shrinks by truncate")
         self.reserve(seqs, total)
@@ -365,6 +419,7 @@ class KV4Cache:
                 raise ValueError("%d rows on %d pages" % (n, len(pages)))
             if n > self._rows[seq] and any(self._uses[p] > 1 for p in pages[self._rows[seq] // PAGE:(n + PAGE - 1) // PAGE]):
                 raise ValueError("rows of sequence %d would go to a page that another shares; reserve gives it its own" % seq)
+        self._give({seq: (n, len(self._pages[seq]) * PAGE) for seq, n in zip(seqs, rows) if seq in self._device_counts})
         self._count(seqs, rows)
 
     def _count(self, seqs, rows):

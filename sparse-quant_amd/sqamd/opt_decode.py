@@ -152,12 +152,13 @@ class DecoderLayer(nn.Module):
 
 def _per_layer(cache, batch, tokens, pos0):
     """A cache's layers as DecoderLayer.forward takes them; a 4-bit cache's lengths are counted up to behind the rows that
-    it will write (on the device where the position lives there)."""
+    it will write (on the device where the position lives there, and the cache is told so)."""
     if not isinstance(cache, kv4.KV4Cache):
         return cache
     if isinstance(pos0, int):
         cache.set_lengths(list(range(batch)), pos0 + tokens)
     else:
+        cache.counted_on_device(batch)
         cache.lengths[:batch] = pos0 + tokens
     return [(cache.layer(i, batch), None) for i in range(cache.layers)]
 
@@ -230,7 +231,8 @@ class OPTDecoder(nn.Module):
         end, pos_t int64 [1] (the cache row the new keys and values go to) is advanced, and with history int64
         [T, B] and step_t int64 [1] the chosen tokens are also written to history[step_t].  Embeddings, final
         LayerNorm, fp16 lm_head and argmax are what forward() computes with torch ops (the embeddings bit for bit;
-        the logits with fp32 sums in another order).  Returns the logits [B, vocab]."""
+        the logits with fp32 sums in another order).  A 4-bit cache's lengths are counted on the device then
+        (KV4Cache.counted_on_device).  Returns the logits [B, vocab]."""
         b = tok.shape[0]
         if getattr(self, "_parts", None) is None:
             self._parts = capi.f16_gemv_parts(self.lm_head.shape[0], self.lm_head.device)

@@ -195,3 +195,51 @@ def test_steps_past_the_reserved_pages_leave_other_sequences_alone(opt):
     for name in ("kc", "vc", "ks", "vs", "km", "vm"):
         assert np.array_equal(new[name][..., 6:, :], old[name][..., 6:, :]), name
     assert np.any(new["kc"][..., :6, :] != old["kc"][..., :6, :])
+
+
+@pytest.mark.parametrize("captured", [False, True], ids=["eager", "captured"])
+def test_steps_then_a_fork(opt, captured):
+    # the device has counted rows that the host did not see: a fork has them all, and steps that go on (replays cannot be
+    # refused) leave it alone
+    model = small(opt)
+    from sqamd import kv4
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    ids = torch.randint(0, 1000, (2, 60), device=DEV, generator=gen)
+    runs = []
+    for forked in (False, True):
+        cache = kv4.KV4Cache(len(model.layers), 16, model.heads, 128, max_seqs=3, max_rows=192, device=DEV)
+        cache.pool.zero_()
+        cache.add(), cache.add()
+        cache.reserve([0, 1], 192)
+        tok, pos = model(ids, cache, 0).argmax(-1), torch.tensor([60], device=DEV)
+        first, step = tok.clone(), lambda: model.greedy_step(tok, cache, pos)
+        if captured:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step()
+            tok.copy_(first)
+            pos.fill_(60)
+            step = graph.replay
+        for _ in range(10):
+            step()
+        if forked:
+            assert cache.rows(0) == 70 and cache.fork(0) == 2 and cache.rows(2) == 70
+            pages = cache.pages(2)
+            assert len(pages) == 2 and pages[0] == cache.pages(0)[0] and pages[1] != cache.pages(0)[1]
+            new, old = (ko.read(cache.pool[:, p].cpu().numpy(), 128, 64) for p in (pages[1], cache.pages(0)[1]))
+            for name in ("kc", "vc", "ks", "vs", "km", "vm"):
+                assert np.array_equal(new[name][..., :6, :], old[name][..., :6, :])
+            kept = cache.pool[:, pages].clone()
+        for _ in range(10):
+            step()
+        assert cache.rows(0) == cache.rows(1) == 80
+        if forked:
+            assert cache.rows(2) == 70 and torch.equal(cache.pool[:, pages], kept)
+        runs.append((tok.clone(), [cache.pool[:, cache.pages(i)[:2]].clone() for i in range(2)]))
+    assert torch.equal(runs[0][0], runs[1][0]) and all(torch.equal(a, b) for a, b in zip(*(r[1] for r in runs)))

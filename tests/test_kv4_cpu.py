@@ -277,3 +277,92 @@ def test_places_without_a_page_name_none(host_copies):
     c.free(a)
     c.extend([b], 10)
     assert only_own_pages(c)
+
+
+def test_rows_that_the_device_counts_are_known_to_the_host(host_copies):
+    # a decode step counts `lengths` up where the host does not see it: what the host does next starts from there
+    from sqamd import kv4, opt_decode
+    c = kv4.KV4Cache(1, 20, 1, 64, 64, max_seqs=4, max_rows=400, device="cpu")
+    a, b = c.add(), c.add()
+    c.reserve([a, b], 200)
+    opt_decode._per_layer(c, 2, 60, 0)                      # a prompt: counted by the host
+    assert c.rows(a) == 60
+    for pos in range(60, 131):                              # steps: by the device
+        opt_decode._per_layer(c, 2, 1, torch.tensor([pos]))
+    assert c.lengths.tolist() == [131, 131, 0, 0] and c.rows(a) == c.rows(b) == 131
+    c.pool.copy_(torch.randint(0, 256, c.pool.shape, dtype=torch.uint8))
+    f = c.fork(a)
+    assert c.rows(f) == 131 and c.lengths[f] == 131 and c.pages(f)[:2] == c.pages(a)[:2]
+    # the step of the first two may be a captured one: the page it goes on writing to is not shared, and no page was lost
+    assert c.pages(f)[2] != c.pages(a)[2] and torch.equal(c.pool[0, c.pages(f)[2]], c.pool[0, c.pages(a)[2]])
+    assert only_own_pages(c)
+    c.extend([a, f], 4)
+    assert c.lengths.tolist() == [135, 131, 135, 0]
+    c.truncate(a, 130)
+    with pytest.raises(ValueError):
+        c.truncate(a, 131)
+    c.lengths[a] = 190
+    c.truncate(a, 180)
+    assert c.rows(a) == 180
+    c.lengths[a] = 193                                      # past its pages, which end at 192
+    for call in (lambda: c.rows(a), lambda: c.fork(a), lambda: c.extend([a], 1), lambda: c.reserve([a], 300)):
+        with pytest.raises(RuntimeError):
+            call()
+    c.truncate(a, 192)
+    c.extend([a], 1)
+    assert c.rows(a) == 193 and only_own_pages(c)
+    c.lengths[b] = 500
+    c.set_lengths([b], 190)
+    assert c.rows(b) == 190
+
+
+def test_the_device_never_counts_into_a_shared_page(host_copies):
+    from sqamd import kv4
+    c = kv4.KV4Cache(1, 6, 1, 64, 64, max_seqs=3, max_rows=256, device="cpu")
+    a = c.add()
+    c.reserve([a], 128)
+    c.set_lengths([a], 70)
+    f = c.fork(a)
+    for n in (1, 2, [f]):
+        with pytest.raises(ValueError):
+            c.counted_on_device(n)
+    with pytest.raises(ValueError):
+        c.counted_on_device([3])
+    c.reserve([f], 71)
+    c.counted_on_device(3)                                  # the third does not exist yet
+    pages, uses = c.pages(a), list(c._uses)
+    g = c.fork(f)
+    assert g == 2 and c.pages(g)[0] == pages[0] and c._uses[c.pages(g)[1]] == c._uses[c.pages(f)[1]] == 1
+    c.free(g)
+    assert c._uses == uses
+    # back into a shared full page: by truncate and by set_lengths
+    c.truncate(f, 64)
+    g = c.fork(f)
+    c.truncate(g, 30)
+    assert c.pages(g)[0] != pages[0] and c.pages(f)[0] == pages[0]
+    c.set_lengths([f], 10)
+    assert c.pages(f)[0] != pages[0] and c.pages(a) == pages and only_own_pages(c)
+
+
+def test_a_shared_page_without_a_free_one_leaves_everything_as_it_was(host_copies):
+    from sqamd import kv4
+    for rows, cut in ((100, None), (128, 100)):
+        c = kv4.KV4Cache(1, 2, 1, 64, 64, max_seqs=2, max_rows=256, device="cpu")
+        c.counted_on_device(2)
+        a = c.add()
+        c.extend([a], rows)
+        if cut:
+            c.fork(a)
+        state = lambda: (c._pages[:], c._rows[:], c._uses[:], c._free[:], c.table.tolist(), c.lengths.tolist())
+        before = state()
+        with pytest.raises(RuntimeError):
+            c.truncate(1, cut) if cut else c.fork(a)
+        assert state() == before
+    c = kv4.KV4Cache(1, 3, 1, 64, 64, max_seqs=2, max_rows=256, device="cpu")
+    c.counted_on_device(2)
+    a = c.add()
+    c.extend([a], 128)
+    f = c.fork(a)
+    c.extend([f], 64)
+    c.truncate(f, 100)  # the page that goes is the one that comes
+    assert c.pages(a) == [0, 1] and c.pages(f) == [0, 2] and c.free_pages() == 0 and only_own_pages(c)
