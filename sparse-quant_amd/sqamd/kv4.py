@@ -410,8 +410,9 @@ class KV4Cache:
         self.reserve(seqs, total)
         self.set_lengths(seqs, total)
 
-    def set_lengths(self, seqs, rows):
-        """Count rows that have pages already, new ones pages that no other sequence shares."""
+    def set_lengths(self, seqs, rows, stored=0):
+        """Count rows that have pages already, new ones pages that no other sequence shares.  stored: the last so many rows of
+        each will be stored, again where they are not new; their pages must not be shared either."""
         seqs, rows = self._per_sequence(seqs, rows)
         for seq, n in zip(seqs, rows):
             pages = self._known(seq)
@@ -419,6 +420,9 @@ class KV4Cache:
                 raise ValueError("%d rows on %d pages" % (n, len(pages)))
             if n > self._rows[seq] and any(self._uses[p] > 1 for p in pages[self._rows[seq] // PAGE:(n + PAGE - 1) // PAGE]):
                 raise ValueError("rows of sequence %d would go to a page that another shares; reserve gives it its own" % seq)
+            if stored and any(self._uses[p] > 1 for p in pages[max(0, n - stored) // PAGE:(n + PAGE - 1) // PAGE]):
+                raise ValueError("rows of sequence %d would be stored again on a page that another shares; truncate and reserve "
+                                 "give it its own" % seq)
         self._give({seq: (n, len(self._pages[seq]) * PAGE) for seq, n in zip(seqs, rows) if seq in self._device_counts})
         self._count(seqs, rows)
 

@@ -156,7 +156,7 @@ def _per_layer(cache, batch, tokens, pos0):
     if not isinstance(cache, kv4.KV4Cache):
         return cache
     if isinstance(pos0, int):
-        cache.set_lengths(list(range(batch)), pos0 + tokens)
+        cache.set_lengths(range(batch), pos0 + tokens, tokens)
     else:
         cache.counted_on_device(batch)
         cache.lengths[:batch] = pos0 + tokens

@@ -366,3 +366,27 @@ def test_a_shared_page_without_a_free_one_leaves_everything_as_it_was(host_copie
     c.extend([f], 64)
     c.truncate(f, 100)  # the page that goes is the one that comes
     assert c.pages(a) == [0, 1] and c.pages(f) == [0, 2] and c.free_pages() == 0 and only_own_pages(c)
+
+
+def test_a_prompt_is_not_stored_again_over_shared_pages(host_copies):
+    from sqamd import kv4, opt_decode
+    c = kv4.KV4Cache(1, 10, 1, 64, 64, max_seqs=2, max_rows=300, device="cpu")
+    a = c.add()
+    c.reserve([a], 200)
+    opt_decode._per_layer(c, 1, 130, 0)
+    opt_decode._per_layer(c, 1, 130, 0)             # again, on pages of its own
+    f = c.fork(a)
+    c.reserve([f], 150)
+    before = c.lengths.tolist(), c.table.tolist()
+    for first, tokens in ((0, 130), (0, 20), (127, 3), (64, 64)):
+        with pytest.raises(ValueError):             # the first two pages are the fork's too
+            opt_decode._per_layer(c, 1, tokens, first)
+    assert (c.lengths.tolist(), c.table.tolist()) == before
+    opt_decode._per_layer(c, 2, 5, 130)             # behind them
+    opt_decode._per_layer(c, 2, 5, 128)             # again
+    opt_decode._per_layer(c, 2, 0, 10)              # nothing is stored
+    assert c.lengths.tolist() == [10, 10]
+    c.truncate(a, 0)
+    c.reserve([a], 130)
+    opt_decode._per_layer(c, 1, 130, 0)
+    assert not set(c.pages(a)) & set(c.pages(f))
