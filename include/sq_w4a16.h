@@ -479,7 +479,8 @@ int sq_greedy_feedback(const void* part_val, const void* part_idx, int parts, in
  *            tokens are the last rows of their sequence: token i of n is row lengths[b] - n + i.
  * All four lie on the device and are read by the kernels: a captured HIP graph follows them.  Whatever they hold, nothing
  * outside the pool, the T tokens and the outputs is touched: a page outside [0, num_pages) does not exist (nothing is
- * stored there, nobody sees its rows), lengths are clamped to [0, 64 width], starts to [0, T].
+ * stored there, nobody sees its rows), nor does one beyond the table (a length may pass 64 width: tokens whose rows the table
+ * has no place for are not stored, and see those that it has); a negative length is 0, starts are clamped to [0, T].
  * D in {64, 128}, group_size in {32, 64, 128} and at most D; strides in elements and multiples of 8; k, v, q, outputs and
  * pool 16-byte aligned.  T == 0 is no work. */
 int sq_kv4_record_bytes(int D, int group_size);

@@ -21,7 +21,7 @@ constexpr int KV4_PAGE = 64;
 __host__ __device__ constexpr int kv4_record_bytes(int D, int g) { return 68 * D + 512 * (D / g); }
 
 // The cache as a kernel sees it.  Whatever the tables and lengths on the device say, nothing outside the pool is
-// read or written: a page outside [0, num_pages) does not exist, a length is clamped to the table's width.
+// read or written: a page outside [0, num_pages) does not exist, and neither do rows that the table has no place for.
 struct Kv4Cache {
     uint8_t* pool;
     const int* table;    // [B][table_stride], `width` entries used
@@ -30,10 +30,12 @@ struct Kv4Cache {
     int B, T, H, num_pages, width, table_stride, each;
 };
 
-__device__ __forceinline__ int kv4_length(const Kv4Cache& c, int b) {
-    const int n = c.lengths[b], most = c.width * KV4_PAGE;
-    return n < 0 ? 0 : (n > most ? most : n);
+// Of a sequence's rows, those that its table has places for.
+__device__ __forceinline__ int kv4_inside(const Kv4Cache& c, int rows) {
+    const int most = c.width * KV4_PAGE;
+    return rows < 0 ? 0 : (rows > most ? most : rows);
 }
+__device__ __forceinline__ int kv4_length(const Kv4Cache& c, int b) { return kv4_inside(c, c.lengths[b]); }
 
 // First token of sequence b and behind its last, inside [0, T].
 __device__ __forceinline__ void kv4_tokens(const Kv4Cache& c, int b, int& first, int& count) {

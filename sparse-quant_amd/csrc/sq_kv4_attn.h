@@ -36,21 +36,23 @@ constexpr long KA_MOST_PAGES = 1l << 38;  // of all tiles, that `deal` can count
 struct Piece {
     int b, tile, head, share, shares;  // share of how many
     int slot;                          // where its partial state goes (shares > 1)
-    int first, count, len;             // tokens and rows of the sequence
+    int first, count, len;             // tokens of the sequence, and its rows inside the table
+    int end;                           // behind the row of its last token (which the table may have no place for)
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// A sequence's tokens, rows, pages and tiles.
+// A sequence's tokens, rows (see Piece), pages and tiles.
 struct Sizes {
-    int first, count, len, pages, tiles;
+    int first, count, len, end, pages, tiles;
 };
 template <int R>
 __device__ __forceinline__ Sizes sizes_of(const Kv4AttnArgs& a, int b) {
-    Sizes s = {0, 0, 0, 0, 0};
+    Sizes s = {0, 0, 0, 0, 0, 0};
     if (b < a.c.B) {
         kv4_tokens(a.c, b, s.first, s.count);
-        s.len = kv4_length(a.c, b);
+        s.end = imax(a.c.lengths[b], 0);
+        s.len = kv4_inside(a.c, s.end);
         s.pages = ceil_div(s.len, KV4_PAGE);
         if (a.selected) s.pages = imin(s.pages, a.count);
         const int rows = s.count * a.share;
@@ -76,7 +78,8 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
         out.first = out.b * a.c.each;
         out.count = a.c.each;
         if (out.b >= B) return false;
-        out.len = kv4_length(a.c, out.b);
+        out.end = imax(a.c.lengths[out.b], 0);
+        out.len = kv4_inside(a.c, out.end);
         return true;
     }
     Sizes s = sizes_of<R>(a, lane);
@@ -113,6 +116,7 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
             out.first = __builtin_amdgcn_readlane(s.first, at);
             out.count = __builtin_amdgcn_readlane(s.count, at);
             out.len = __builtin_amdgcn_readlane(s.len, at);
+            out.end = __builtin_amdgcn_readlane(s.end, at);
             return true;
         }
         index -= __builtin_amdgcn_readlane(upto, 63);

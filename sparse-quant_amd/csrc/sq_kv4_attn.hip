@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     Piece pc;
     if (!deal<R, false>(a, d, blockIdx.x, pc)) return;
     if (pc.shares > 1 && pc.slot >= 2 * d.wgs()) return;  // (only where lengths change under the launch)
-    const int head = pc.head, tile = pc.tile, len = pc.len;
+    const int head = pc.head, tile = pc.tile, len = pc.len, before = pc.end - pc.count;  // (rows before the call's)
     const int* const table = c.table + (long)pc.b * c.table_stride;
     const int* const chosen = a.selected ? a.selected + ((long)pc.b * c.H + head) * a.count : nullptr;
     // The first 64 pages, or the places of the selected ones, without waiting for the length.
@@ -87,11 +87,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
         const int row = tile * R + imin(col + 16 * rt, rows - 1);
         token[rt] = pc.count == 1 ? 0 : row / a.share;
         qhead[rt] = head * a.share + row - token[rt] * a.share;
-        limit[rt] = len - pc.count + token[rt];
+        limit[rt] = before + token[rt];
     }
-    const int limit_hi = len - pc.count + (pc.count == 1 ? 0 : (tile * R + rows - 1) / a.share);
+    const int limit_hi = before + (pc.count == 1 ? 0 : (tile * R + rows - 1) / a.share);
     const int all_pages = limit_hi < 0 ? 0 : imin(limit_hi / KV4_PAGE + 1, ceil_div(len, KV4_PAGE));
-    // (selected pages are for single tokens: limit_hi + 1 = len)
+    // (selected pages are for single tokens: limit_hi is the sequence's last row)
     const int pages = a.selected ? imin(all_pages, a.count) : all_pages;
     int p0 = 0, p1 = pages;
     if (pc.shares > 1) {
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
         };
         // The new row, if this is the share that sees it: stored by the wave whose unit it is in, before it asks for that
         // unit; the others do not wait.  (All queries of a head stand in one tile here.)
-        const int fresh = NEW && pb + 64 >= p1 && p1 == all_pages && len > 0 && c.lengths[pc.b] == len  // (inside the table)
+        const int fresh = NEW && pb + 64 >= p1 && p1 == all_pages && len > 0 && pc.end == len  // (inside the table)
                               ? PER * (p1 - pb - 1) + (len - 1) % KV4_PAGE / U::ROWS : -1;
         const bool mine = fresh >= 0 && fresh % WAVES == wave;
         if (wave < units && !(mine && fresh == wave)) {

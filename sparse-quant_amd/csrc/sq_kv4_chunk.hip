@@ -52,9 +52,10 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
     const int rows = imin(pc.count * a.share - tile * KC_ROWS, KC_ROWS);
     const int row = tile * KC_ROWS + imin(32 * wave + n, rows - 1);
     const int token = row / a.share, qhead = head * a.share + row - token * a.share;
-    const int limit = len - pc.count + token;  // the last row it sees
-    const int limit_lo = len - pc.count + tile * KC_ROWS / a.share;
-    const int limit_hi = len - pc.count + (tile * KC_ROWS + rows - 1) / a.share;
+    const int before = pc.end - pc.count;  // rows before the call's
+    const int limit = before + token;      // the last row it sees
+    const int limit_lo = before + tile * KC_ROWS / a.share;
+    const int limit_hi = before + (tile * KC_ROWS + rows - 1) / a.share;
     const int pages = limit_hi < 0 ? 0 : imin(limit_hi / KV4_PAGE + 1, ceil_div(len, KV4_PAGE));
     int p0 = 0, p1 = pages;
     if (pc.shares > 1) {

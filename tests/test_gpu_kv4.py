@@ -903,3 +903,36 @@ def test_results_repeat_bit_for_bit(kv4):
     q = dev(rng.normal(0, 1, (3, 8, 128)).astype(np.float16))
     first = kv4.attention(q, pool, table, n, 0.1)
     assert all(torch.equal(kv4.attention(q, pool, table, n, 0.1), first) for _ in range(5))
+
+
+@pytest.mark.parametrize("c,h,share,equal", [(4, 2, 1, True), (4, 1, 6, True), (33, 1, 4, True), (40, 2, 4, False), (5, 2, 2, False)],
+                         ids=["packed", "two-tiles", "chunk", "ragged-chunk", "ragged"])
+def test_tokens_beyond_the_table_leave_the_others_where_they_are(kv4, c, h, share, equal):
+    # rows that the table has no place for are not stored and not seen; the call's other tokens are the rows that append
+    # stored, and see what lies up to their own
+    d, g = 128, 64
+    rng = np.random.default_rng(c + share)
+    lens, new = [130, 128 + c, 200, 128 + c // 2, 101], [c, c, c, c, c if equal else 2]
+    pages, total = np.arange(10, dtype=np.int32).reshape(5, 2), 11
+    pool = random_pool(rng, total, h, d, g)
+    q = rng.normal(0, 1, (sum(new), h * share, d)).astype(np.float16)
+    kv = rng.normal(0, 1, (2, sum(new), h, d)).astype(np.float16)
+    st = None if equal else dev(starts_of(new))
+    dpool, args = dev(pool), (dev(pages), dev(np.array(lens, np.int32)))
+    kv4.append(dev(kv[0]), dev(kv[1]), dpool, *args, st)
+    want, written = expect_append(pool, kv[0], kv[1], pages, lens, new, d, g)
+    stored = dpool.cpu().numpy()
+    assert np.array_equal(ko.read(stored, d, g)["kc"], want["kc"]) and written.any()
+    out = kv4.attention(dev(q), dpool, *args, 0.1, st).cpu().numpy().astype(np.float64)
+    both = dev(pool)
+    assert torch.equal(kv4.attention(dev(q), both, *args, 0.1, st, k_new=dev(kv[0]), v_new=dev(kv[1])).double().cpu(),
+                       torch.from_numpy(out)) and torch.equal(both, dpool)
+    at = 0
+    for b, (n, count) in enumerate(zip(lens, new)):
+        for head in range(h):
+            rows = ko.Rows(stored, pages[b], 128, head, d, g)
+            for i in range(count):
+                for j in range(head * share, (head + 1) * share):
+                    expect, tol = ko.attend(rows, q[at + i, j].astype(np.float64), 0.1, np.arange(min(128, n, n - count + i + 1)))
+                    assert not np.sum(np.abs(out[at + i, j] - expect) > tol), (b, i, j)
+        at += count
