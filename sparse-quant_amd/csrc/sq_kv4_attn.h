@@ -91,7 +91,9 @@ __device__ __forceinline__ bool deal(const Kv4AttnArgs& a, const Deal& d, int in
             const unsigned long long mine = (unsigned long long)t.tiles * t.pages;
             units += (unsigned)wave_sum((int)(mine & 0xffff)) + ((unsigned long long)(unsigned)wave_sum((int)(mine >> 16)) << 16);
         }
-        const int even = ceil_div((int)((units + 255) >> 8), d.per_cu);  // (below KA_MOST_PAGES)
+        // (tokens counted once: below KA_MOST_PAGES; starts that let sequences overlap may pass it, and then nothing is shared)
+        const unsigned long long per = (units + 255) >> 8;
+        const int even = ceil_div((int)(per < (1u << 30) ? per : 1u << 30), d.per_cu);
         least = imax(even, d.least);
     }
     int slots = 0;

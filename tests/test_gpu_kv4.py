@@ -936,3 +936,23 @@ def test_tokens_beyond_the_table_leave_the_others_where_they_are(kv4, c, h, shar
                     expect, tol = ko.attend(rows, q[at + i, j].astype(np.float64), 0.1, np.arange(min(128, n, n - count + i + 1)))
                     assert not np.sum(np.abs(out[at + i, j] - expect) > tol), (b, i, j)
         at += count
+
+
+def test_sequences_that_overlap_far_beyond_the_tokens(kv4):
+    # starts that go back and forth: thousands of sequences on the same tokens, more pages in all than 39 bits count.  Which
+    # of them a token's result comes from is open, but one that has its tokens alone gets its own
+    d, g, h, share, t, alone, b, width = 64, 32, 8, 4, 1 << 15, 4096, 4096, 1 << 16
+    rng = np.random.default_rng(40)
+    starts = np.where(np.arange(b + 1) % 2 == 0, t, alone).astype(np.int32)
+    starts[0] = 0
+    lens = np.where(np.arange(b) < 13, 0, 64 * width).astype(np.int32)
+    lens[0] = 1280
+    pool = random_pool(rng, 20, h, d, g)
+    pages = torch.full((b, width), -1, dtype=torch.int32, device=DEV)
+    pages[0, :20] = torch.arange(20, dtype=torch.int32, device=DEV)
+    q = dev(rng.normal(0, 1, (t, h * share, d)).astype(np.float16))
+    out = torch.full_like(q, 9.0)
+    kv4.attention(q, dev(pool), pages, dev(lens), 0.1, dev(starts), out=out)
+    own = out[:alone].cpu().numpy().astype(np.float64)
+    compare(own, q[:alone].cpu().numpy(), pool, pages[:1, :20].cpu().numpy(), [1280], [alone], d, g, h, share, 0.1)
+    assert not torch.any(out[alone:])
