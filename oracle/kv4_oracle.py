@@ -73,7 +73,8 @@ class Rows:
 def attend(rows, q, scale, seen, middles=0.0):
     """q fp64 [D] over the rows named by `seen` (indices, with repetition): (out, tolerance) [D] in 64 bits.
 
-    Tolerance.  P' = P s is rounded to fp16 before it meets code - 8: eps/2 = 2^-11 of every term.  A probability is off by
+    Tolerance.  P' = P s is rounded to fp16 before it meets code - 8: eps/2 = 2^-11 of every term (no allowance is made for
+    denormal ones, below 2^-25 of the largest scale).  A probability is off by
     twice the error of its exponent (numerator and sum): the score's fp32 sums of D + 16 terms, each rounding (also towards
     zero) 2^-23 of sum |q| (s code + |m|), and 2^-20 for the exponential, its argument in base 2 and the joining of partial
     sums.  fp32 sums of the result: the terms P s (code - 8) of every 32 rows are added to what there is, 33 additions

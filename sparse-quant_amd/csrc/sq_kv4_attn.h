@@ -139,7 +139,12 @@ __device__ __forceinline__ float wave_max(float v) {
     return rows_max(v);
 }
 
-constexpr float KA_LAZY = 8.f;  // the softmax's reference moves when a score is 2^8 beyond it
+// The softmax's reference moves when a score is more than KA_LAZY beyond it (in powers of two), so P is at most 2^KA_LAZY, and
+// P' = fp16(P s KA_TOP / sref), sref a power of two above the scales so far, at most 2^15.  The factor is as large as it can be
+// because sref follows the largest scale whatever its row counts for: below 2^-14, where fp16 numbers become denormal, P' is held
+// to 2^-25 only, so that terms P s below 2^(KA_LAZY - 29) sref are held to 2^(KA_LAZY - 40) sref each, not to 2^-11 of themselves.
+constexpr int KA_LAZY = 4;
+constexpr float KA_TOP = 1 << (15 - KA_LAZY);
 
 // Shares of a tile's pages, joined: a workgroup has ROWS rows of a shared tile, 256 / ROWS threads each, of which D / 4 hold
 // four columns each of every so many-th share.  (LAST: tiles are worked on from the last to the first.)  3.8 to 4.7 us where

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
     float4_t acc[RT][NT];
     float m[RT], l[RT];            // the reference of the softmax (of this column), the lane's share of the sum
     float mins[RT][G];             // sum P (m + 8 s) (the lane's share)
-    float sref[G], sinv[G];        // power of two in P', and 16 over it
+    float sref[G], sinv[G];        // power of two in P', and KA_TOP over it
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         m[rt] = -INFINITY, l[rt] = 0.f;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
         for (int i = 0; i < G; i++) mins[rt][i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < G; i++) sref[i] = 0x1p-30f, sinv[i] = 0x1p34f;
+    for (int i = 0; i < G; i++) sref[i] = 0x1p-30f, sinv[i] = KA_TOP * 0x1p30f;
     const half8_t eight[2] = {bit_cast<half8_t>((u32x4_t){0x80088008u, 0x80088008u, 0x80088008u, 0x80088008u}),   // -8 * 2^-24
                               bit_cast<half8_t>((u32x4_t){0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u})};  // -8 * 2^-20
     const float scale24 = a.scale * 0x1p24f;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
                     if (u + WAVES < units) load_keys(u + WAVES);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (__ballot(top > m[rt] + KA_LAZY)) {
+                if (__ballot(top > m[rt] + (float)KA_LAZY)) {
                     const float to = fmaxf(rows_max(top), m[rt]);
                     const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
                     m[rt] = to;
@@ -290,11 +290,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
                     if (pid < 0 || pos + 16 * PACK * set + r > seen_to) sv[i] = mid[i] = 0.f;  // whatever lies where nobody looks
                     big = fmaxf(big, sv[i]);
                 }
-                if (__ballot(big > 8.f * sref[j])) {
+                if (__ballot(big >= sref[j])) {
                     const float to = bit_cast<float>(bit_cast<uint32_t>(wave_max(big)) & 0x7f800000u) * 2.f;
                     const float f = sref[j] / to;
                     sref[j] = to;
-                    sinv[j] = 16.f / to;
+                    sinv[j] = KA_TOP / to;
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
 #pragma unroll
         for (int i = 0; i < NT; i++) {
             const int gi = 16 * i / g;
-            const float f = sref[gi] * (i & 1 ? 0x1p16f : 0x1p20f);  // over the 16 in P', times 2^20 or 2^24
+            const float f = sref[gi] * ((i & 1 ? 0x1p20f : 0x1p24f) / KA_TOP);
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[rt][i][e] = acc[rt][i][e] * f + mins[rt][gi];
         }

@@ -8,7 +8,7 @@
 //   and sum P (m + 8 s) per query and group by vector instructions.  m + 8 s, about the middle of a group, is rounded to fp16,
 //   as the values themselves were that the group was made of (in fp32: 454 instead of 442 us at 2 x 1024 new tokens of 8192
 //   rows, 53 instead of 47 at 8 prompts of 512 tokens with heads of 64).
-// s' = 16 s over a power of two that follows the scales (of the largest so far), so that P' stays inside fp16's range.
+// s' = KA_TOP s over a power of two that follows the scales (of the largest so far), so that P' stays inside fp16's range.
 // While a page is worked on, the next one's codes are unpacked into the other half of LDS and the one behind it is on its way to
 // registers; one barrier a page, which does not wait for those.
 //
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
                 big = fmaxf(big, row_move<0x124>(big));
                 big = fmaxf(big, row_move<0x128>(big));
                 if (big > run) run = bit_cast<float>(bit_cast<uint32_t>(big) & 0x7f800000u) * 2.f;
-                const float inv = 16.f / run;
+                const float inv = KA_TOP / run;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float s = (float)sm[r];
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
 
     float16_t acc[DT];
     // Scores stay in units of 1 / scale (its sign went into the queries); 0 is as good as 1e-30.
-    const float scale = fmaxf(fabsf(a.scale), 1e-30f), lazy = KA_LAZY / scale;
+    const float scale = fmaxf(fabsf(a.scale), 1e-30f), lazy = (float)KA_LAZY / scale;
     float m = -INFINITY, l = 0.f;  // the reference of the softmax, the lane's share of the sum
     float mins[G], sref[G];
 #pragma unroll
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
 #pragma unroll
         for (int t = 0; t < DT; t++) {
             const int gi = 32 * t / g;
-            const float f = sref[gi] * 0.0625f;
+            const float f = sref[gi] * (1.f / KA_TOP);
 #pragma unroll
             for (int qd = 0; qd < 4; qd++) {
                 half4_t h;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(64 * KC_WAVES, 2) void kv4_chunk_kernel(Kv4AttnArgs
 #pragma unroll
         for (int t = 0; t < DT; t++) {
             const int gi = 32 * t / g;
-            const float f = sref[gi] * 0.0625f;
+            const float f = sref[gi] * (1.f / KA_TOP);
 #pragma unroll
             for (int qd = 0; qd < 4; qd++) {
                 float4_t o;

@@ -956,3 +956,36 @@ def test_sequences_that_overlap_far_beyond_the_tokens(kv4):
     own = out[:alone].cpu().numpy().astype(np.float64)
     compare(own, q[:alone].cpu().numpy(), pool, pages[:1, :20].cpu().numpy(), [1280], [alone], d, g, h, share, 0.1)
     assert not torch.any(out[alone:])
+
+
+@pytest.mark.parametrize("d,g,c,share", [(64, 32, 1, 4), (128, 64, 1, 12), (128, 128, 1, 24), (64, 64, 5, 4), (128, 64, 40, 4), (64, 32, 70, 2)],
+                         ids=["packed", "rows", "two-tiles", "drafts", "chunk", "chunk-64"])
+@pytest.mark.parametrize("where", ["first", "middle", "hidden"])
+def test_one_row_of_large_values_that_hardly_counts(kv4, d, g, c, share, where):
+    # values of 60000 in one row of no weight (or that most of the call's tokens do not see) beside rows of 0.01: the small ones
+    # are as exact as they are without it.  Scores come from two elements of a query, so that their own rounding is small
+    rng = np.random.default_rng(41)
+    n = 1000 if where != "hidden" else 64 if c < 64 else 128  # (hidden in a page that the tokens see most of)
+    at = {"first": 3, "middle": 500, "hidden": n - 1}[where]
+    k, v = rng.normal(0, 1, (n, 1, d)), rng.normal(0, 0.01, (n, 1, d))
+    v[at] = 60000 * np.where(np.arange(d) % 2, 1, -1)
+    if where != "hidden":
+        k[at] = 0
+        k[at, 0, 0] = -14
+    q = np.zeros((c, share, d))
+    q[..., 0], q[..., d // 2] = rng.uniform(2.5, 3.5, (c, share)), rng.uniform(-0.5, 0.5, (c, share))
+    k, v, q = (x.astype(np.float16) for x in (k, v, q))
+    pool, pages, lens = kv4.new_pool(16, 1, d, g, device=DEV), np.arange(16, dtype=np.int32)[None], dev(np.array([n], np.int32))
+    pool.zero_()
+    kv4.append(dev(k), dev(v), pool, dev(pages), lens)
+    out = kv4.attention(dev(q), pool, dev(pages), lens, 1.0).cpu().numpy().astype(np.float64)
+    rows = ko.Rows(pool.cpu().numpy(), pages[0], n, 0, d, g)
+    worst = 0.0
+    for i in sorted({0, 1, 2, 30, c - 2, c - 1} & set(range(c))):
+        seen = np.arange(n - c + i + 1)
+        if where == "hidden" and at in seen:
+            continue
+        for j in range(share):
+            want, tol = ko.attend(rows, q[i, j].astype(np.float64), 1.0, seen, 2.0 ** -11 if c * share > 32 else 0.0)
+            worst = max(worst, float(np.max(np.abs(out[i, j] - want) / tol)))
+    assert worst <= 1, worst
