@@ -989,3 +989,27 @@ def test_one_row_of_large_values_that_hardly_counts(kv4, d, g, c, share, where):
             want, tol = ko.attend(rows, q[i, j].astype(np.float64), 1.0, seen, 2.0 ** -11 if c * share > 32 else 0.0)
             worst = max(worst, float(np.max(np.abs(out[i, j] - want) / tol)))
     assert worst <= 1, worst
+
+
+def test_one_sequence_of_a_wider_table(kv4):
+    # views of one row: the row's distance is not read from the table then, the columns may be cut
+    d, g, h, share = 128, 64, 2, 2
+    rng = np.random.default_rng(42)
+    lens = [200, 130, 64]
+    pages, total = tables(rng, lens, width=9)
+    pool, q = random_pool(rng, total, h, d, g), dev(rng.normal(0, 1, (3, h * share, d)).astype(np.float16))
+    kv = dev(rng.normal(0, 1, (2, 3, h, d)).astype(np.float16))
+    n, wide = dev(np.array(lens, np.int32)), dev(pages)
+    for i, cut in ((2, 1), (2, 9), (1, 3), (1, 4), (0, 4)):
+        a, b = dev(pool), dev(pool)
+        views = (wide[i:i + 1, :cut], n[i:i + 1])
+        copies = (dev(pages[i:i + 1, :(lens[i] + 63) // 64]), dev(np.array(lens[i:i + 1], np.int32)))
+        assert views[0].stride(0) == 9
+        assert torch.equal(kv4.attention(q[i:i + 1], a, *views, 0.1), kv4.attention(q[i:i + 1], b, *copies, 0.1))
+        assert torch.equal(kv4.select_pages(q[i:i + 1], a, *views, 2), kv4.select_pages(q[i:i + 1], b, *copies, 2))
+        kv4.append(kv[0, i:i + 1], kv[1, i:i + 1], a, *views)
+        kv4.append(kv[0, i:i + 1], kv[1, i:i + 1], b, *copies)
+        assert torch.equal(a, b) and not torch.equal(a, dev(pool))
+    every = kv4.attention(q, dev(pool), wide, n, 0.1)
+    for i in range(3):
+        assert torch.equal(kv4.attention(q[i:i + 1], dev(pool), wide[i:i + 1], n[i:i + 1], 0.1), every[i:i + 1])
