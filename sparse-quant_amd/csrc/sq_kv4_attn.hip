@@ -518,18 +518,21 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         const hipError_t e = launch_kv4_append(c, k_new, v_new, nullptr, nullptr, D, g, new_strides, st);
         if (e != hipSuccess) return e;
     }
-    // Prompts beside single tokens: where sequences differ and the average is up to 1024 rows, the kernel for many rows takes
-    // those with more than KA_ROWS and this one the others, which there would fill a thirtieth of a tile (4 query heads, 1024
-    // tokens over 4096 rows beside 63 sequences of one token: 414 us without, 205 so; beside 7: 177 and 151; 8 prompts of 30
-    // to 58 tokens, where nothing is left for this kernel: 9.4 and 11.2, as chunks over 2000 rows 49 and 55).
-    const bool both = c.starts && !selected && mean > KA_ROWS && mean <= 1024 && share <= KA_ROWS && c.B > 1;
+    // Prompts beside single tokens: where sequences differ and the average is above KA_ROWS, the kernel for many rows takes those
+    // with more than KA_ROWS and this one the others, which there would fill a thirtieth of a tile (4 query heads; 1024 tokens
+    // over 4096 rows beside 63 sequences of one token: 589 us without, 213 so; 4096 beside 7: 425 and 278).  Where nothing is left
+    // for this kernel its launches are lost: 8 prompts of 30 to 58 tokens 9.4 and 11.2, of 100 to 300 18.9 and 20.8, of 512 64.0
+    // and 66.0.  Up to an average of KA_ROWS this kernel takes all: by both, 64 sequences of 1 to 5 tokens over 2000 rows would
+    // take 82 us instead of 69, 8 of them 21.9 instead of 17.5 (and 256 tokens over 4096 rows beside 63 single ones 123 instead
+    // of 268: the average does not tell these from those).
+    const bool both = c.starts && !selected && mean > KA_ROWS && share <= KA_ROWS && c.B > 1;
     if (mean > KA_ROWS && !selected) {
         a.ws = (float*)workspace;
         if (both) a.rows_min = KA_ROWS + 1;
         const hipError_t e = launch_kv4_chunk(a, D, g, st);
         if (e != hipSuccess || !both) return e;
         a.rows_min = 0, a.rows_max = KA_ROWS;
-        mean = share;  // most have one token
+        mean = share;  // (those with few rows mostly have one token)
     }
     const int most = selected && count < c.width ? count : c.width;
     auto tiles_of = [&](int R) {

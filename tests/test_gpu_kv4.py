@@ -1013,3 +1013,22 @@ def test_one_sequence_of_a_wider_table(kv4):
     every = kv4.attention(q, dev(pool), wide, n, 0.1)
     for i in range(3):
         assert torch.equal(kv4.attention(q[i:i + 1], dev(pool), wide[i:i + 1], n[i:i + 1], 0.1), every[i:i + 1])
+
+
+@pytest.mark.parametrize("d,g,h,share,lens,new", [
+    (128, 64, 2, 4, [2300, 1, 1700, 640, 3000, 5], [2000, 1, 1500, 1, 1, 0]),
+    (64, 32, 1, 1, [4000, 33, 700], [4000, 5, 1]),
+    (128, 128, 1, 16, [900, 400], [900, 1]),
+], ids=["four", "one", "sixteen"])
+def test_long_prompts_beside_single_tokens(kv4, d, g, h, share, lens, new):
+    rng = np.random.default_rng(43)
+    assert sum(new) * share > 1024 * len(new)
+    pages, total = tables(rng, lens)
+    pool = random_pool(rng, total, h, d, g)
+    t = sum(new)
+    q = rng.normal(0, 1, (t + 2, h * share, d)).astype(np.float16)
+    out = torch.full(q.shape, 9.0, dtype=torch.float16, device=DEV)
+    kv4.attention(dev(q), dev(pool), dev(pages), dev(np.array(lens, np.int32)), d ** -0.5, dev(starts_of(new)), out=out)
+    out = out.cpu().numpy().astype(np.float64)
+    assert np.all(out[t:] == 9.0)
+    compare(out, q, pool, pages, lens, new, d, g, h, share, d ** -0.5, few=16)
