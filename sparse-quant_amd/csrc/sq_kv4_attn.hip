@@ -518,14 +518,15 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
         const hipError_t e = launch_kv4_append(c, k_new, v_new, nullptr, nullptr, D, g, new_strides, st);
         if (e != hipSuccess) return e;
     }
-    // Prompts beside single tokens: where sequences differ and the average is above KA_ROWS, the kernel for many rows takes those
-    // with more than KA_ROWS and this one the others, which there would fill a thirtieth of a tile (4 query heads; 1024 tokens
-    // over 4096 rows beside 63 sequences of one token: 589 us without, 213 so; 4096 beside 7: 425 and 278).  Where nothing is left
-    // for this kernel its launches are lost: 8 prompts of 30 to 58 tokens 9.4 and 11.2, of 100 to 300 18.9 and 20.8, of 512 64.0
-    // and 66.0.  Up to an average of KA_ROWS this kernel takes all: by both, 64 sequences of 1 to 5 tokens over 2000 rows would
-    // take 82 us instead of 69, 8 of them 21.9 instead of 17.5 (and 256 tokens over 4096 rows beside 63 single ones 123 instead
-    // of 268: the average does not tell these from those).
-    const bool both = c.starts && !selected && mean > KA_ROWS && share <= KA_ROWS && c.B > 1;
+    // Prompts beside single tokens: where sequences differ and the average is above KA_ROWS and up to 1024 rows, the kernel for many
+    // rows takes those with more than KA_ROWS and this one the others, which there would fill a thirtieth of a tile (4 query
+    // heads; 1024 tokens over 4096 rows beside 63 sequences of one token: 589 us without, 213 so).  Where nothing is left for
+    // this kernel its launches are lost: 8 prompts of 30 to 58 tokens 9.4 and 11.2, of 100 to 300 18.9 and 20.8.
+    // Neither bound tells all calls apart, for the host knows the average alone.  Up to KA_ROWS this kernel takes all: by both, 64
+    // sequences of 1 to 5 tokens over 2000 rows would take 82 us instead of 69, but 256 tokens over 4096 rows beside 63 single
+    // ones 123 instead of 268.  Above 1024 the other takes all: by both, 1024 tokens over 16384 rows beside 5 over 1300 would take
+    // 471 instead of 454 and 8 prompts of 512 66 instead of 64, but 4096 beside 7 single ones 278 instead of 425.
+    const bool both = c.starts && !selected && mean > KA_ROWS && mean <= 1024 && share <= KA_ROWS && c.B > 1;
     if (mean > KA_ROWS && !selected) {
         a.ws = (float*)workspace;
         if (both) a.rows_min = KA_ROWS + 1;
