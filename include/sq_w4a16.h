@@ -488,9 +488,9 @@ int sq_kv4_record_bytes(int D, int group_size);
 /* Rows k, v fp16 (element (t, h, d) at k[t * strides[0] + h * strides[1] + d], v with strides[2], strides[3]) are
  * quantised into their pages and take part in their pages' bounds; a page that gets its row 0 starts its bounds anew.
  * A page that gets rows stands once in the tables of the call.  k_hat, v_hat: both NULL, or fp16 [T][H][D]
- * that receive what the rows read as from now on (rounded once): what a prompt's own attention is given so that it
- * sees what decoding will see.  Tokens without a page (a negative row, one beyond the table, a page outside the pool)
- * are left out, their k_hat and v_hat as they were. */
+ * that receive what the rows read as from now on, rounded to fp16: what a prompt's own attention is given so that it
+ * sees what decoding will see (sq_kv4_attention itself reads them without that rounding).  Tokens without a page (a
+ * negative row, one beyond the table, a page outside the pool) are left out, their k_hat and v_hat as they were. */
 int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* pool, const void* pages, const void* lengths,
                   const void* starts, int T, int B, int H, int D, int group_size, int num_pages, int width, int page_stride,
                   const long* strides, void* stream);
@@ -506,7 +506,9 @@ int sq_kv4_append(const void* k, const void* v, void* k_hat, void* v_hat, void* 
  *            and then attended to: for one token per sequence in the same launch.  Not with selected pages.
  * workspace  NULL, or sq_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, of any content: a sequence's pages are
  *            then dealt to several workgroups where there are few, and a second launch joins their shares.  Not shared by
- *            calls that may run at the same time.  The size is 0 where no sequence can be long enough. */
+ *            calls that may run at the same time.  The size is 0 where the table is too narrow for any sequence to be dealt
+ *            out (16 pages; 8 for more than 32 rows per sequence and key/value head): there one launch does it, and
+ *            short sequences are 2.5 us faster than through a wide table. */
 size_t sq_kv4_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int width, int count);
 int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pages, const void* lengths, const void* starts,
                      const void* selected, int T, int B, int Hq, int H, int D, int group_size, int num_pages, int width,
@@ -517,8 +519,9 @@ int sq_kv4_attention(const void* q, void* out, const void* pool, const void* pag
  * of the highest score in ascending order, -1 behind the last where a sequence has fewer.  score = max over the query
  * heads of h of sum_d max(q_d hi_d, q_d lo_d) with the page's bounds: no key of the page scores higher; sums in 64 bits,
  * equals go to the lowest place, a score that is no number is the lowest.  The first keep_first and the last keep_last
- * pages are always among them (keep_first + keep_last <= count).  q as above, one token per sequence.  width at most
- * 16384, B * H at most 65535.  workspace: sq_kv4_select_workspace_bytes(B, H, width) bytes, 16-byte aligned, of any
+ * pages are always among them (keep_first + keep_last <= count).  Selection and attention over 64 pages take less than
+ * attention over everything from about 100000 rows on, counted over all sequences (8 key/value heads of 128).  q as above,
+ * one token per sequence.  width at most 16384, B * H at most 65535.  workspace: sq_kv4_select_workspace_bytes(B, H, width) bytes, 16-byte aligned, of any
  * content; may be NULL where width <= count.  Not shared by calls that may run at the same time. */
 size_t sq_kv4_select_workspace_bytes(int B, int H, int width);
 int sq_kv4_select(const void* q, void* selected, const void* pool, const void* pages, const void* lengths, int B, int Hq, int H,

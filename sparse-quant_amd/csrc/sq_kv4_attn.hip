@@ -474,6 +474,10 @@ __global__ __launch_bounds__(64 * WAVES) void kv4_attn_kernel(Kv4AttnArgs a, Dea
 // the registers allow).  Sixteen pages, so that up to 1024 rows nothing is shared: with eight, 640 rows of one sequence
 // take 10.5 instead of 8.1 us, of eight 14 instead of 9.9 (the second launch is dearer than what it saves), 5 tokens of
 // 16 sequences 28.7 instead of 22.5.
+// Two things hang on these sixteen pages, and neither fits every call.  Whether a launch shares at all goes by the table's width,
+// which is what the host knows: through a table of more than 16 pages 640 rows of one sequence take 11.0 instead of 8.6 us, of
+// eight 13.3 instead of 10.6 (four waves, a look at all lengths, a second launch that finds nothing).  And once it does, a share
+// has sixteen pages at the fewest: one sequence of 8 heads goes to 8 workgroups at 1024 rows (10.6 us), to 64 at 8000 (16.3).
 constexpr Deal KA_DEAL = {2, 16};
 constexpr int KA_ROWS = 32;  // of a tile at the most
 

@@ -6,15 +6,17 @@
 //   S^T = s (K Q^T) + m sum(q)   v_mfma_f32_32x32x16_f16, A = key codes, B = q: a lane has one query and 16 keys of 32
 //   O^T = (V - 8)^T P'           A = value codes less 8, B = P' = fp16(P s'): what the lane has, in that order
 //   and sum P (m + 8 s) per query and group by vector instructions.  m + 8 s, about the middle of a group, is rounded to fp16,
-//   as the values themselves were that the group was made of (in fp32: 454 instead of 442 us at 2 x 1024 new tokens of 8192
-//   rows, 53 instead of 47 at 8 prompts of 512 tokens with heads of 64).
+//   as the values themselves were that the group was made of: up to 2^-11 of the result where values lie far from zero beside
+//   their spread (in fp32: 454 instead of 442 us at 2 x 1024 new tokens of 8192 rows, 53 instead of 47 at 8 prompts of 512
+//   tokens with heads of 64).
 // s' = KA_TOP s over a power of two that follows the scales (of the largest so far), so that P' stays inside fp16's range.
 // While a page is worked on, the next one's codes are unpacked into the other half of LDS and the one behind it is on its way to
 // registers; one barrier a page, which does not wait for those.
 //
-// What bounds it: vector instructions, 561 of them beside 32 matrix instructions per wave and page (13.3 a score), which the two
-// waves of a SIMD hardly overlap (heads of 128 in groups of 64, 1024 tokens of 32 heads over 16384 rows: 438 us = 608 TFLOP/s
-// with the join; counters: vector units busy 0.63, matrix units 0.26, LDS 0.34 of 968 thousand cycles, no bank conflicts).  Groups of 128 take 0.84 of the time of groups of 64, of 32 1.5 times.
+// What bounds it: vector instructions, by the counters 533 of them beside 32 matrix instructions per wave and page (16.7 for each
+// of a lane's 32 scores), which the two waves of a SIMD hardly overlap (heads of 128 in groups of 64, 1024 tokens of 32 heads over
+// 16384 rows: 440 us = 604 TFLOP/s with the join; vector units busy 0.63, matrix units 0.26, LDS 0.34 of 976 thousand cycles, no
+// bank conflicts).  Groups of 128 take 0.84 of the time of groups of 64, of 32 1.5 times.
 #include "sq_kernels.h"
 #include "sq_kv4_attn.h"
 

@@ -17,7 +17,7 @@ that also fills the cache (sq_lut_attention_strided).
 
 With `new_cache(batch, max_len, kv_bits=4)` the keys and values are held in 4 bits, in pages (kv4.KV4Cache): a layer quantises
 its rows into the cache and attends over what is held there, in prompts as in steps (over a look-up table: the prompt's
-attention is given the values that the cache holds).
+attention is given the values that the cache holds, rounded to fp16).
 """
 import math
 import time
