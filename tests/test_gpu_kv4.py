@@ -1032,3 +1032,19 @@ def test_long_prompts_beside_single_tokens(kv4, d, g, h, share, lens, new):
     out = out.cpu().numpy().astype(np.float64)
     assert np.all(out[t:] == 9.0)
     compare(out, q, pool, pages, lens, new, d, g, h, share, d ** -0.5, few=16)
+
+
+def test_a_row_appended_behind_many_pages(kv4):
+    # more pages in one workgroup than are looked up at once, and the row's page among the last of them
+    d, g, h, b = 64, 32, 8, 130
+    rng = np.random.default_rng(44)
+    lens = (64 * 65 + rng.integers(1, 65, b)).tolist()
+    pages = np.concatenate([np.broadcast_to(rng.permutation(65), (b, 65)), 65 + rng.permutation(b)[:, None]], 1).astype(np.int32)
+    pool = dev(random_pool(rng, 65 + b, h, d, g))
+    kv, q = (dev(rng.normal(0, 1, s).astype(np.float16)) for s in ((2, b, h, d), (b, h, d)))
+    n, table, other = dev(np.array(lens, np.int32)), dev(pages), pool.clone()
+    kv4.append(kv[0], kv[1], pool, table, n)
+    want = kv4.attention(q, pool, table, n, 0.1)
+    assert torch.equal(kv4.attention(q, other, table, n, 0.1, k_new=kv[0], v_new=kv[1]), want) and torch.equal(other, pool)
+    compare(want[:3].cpu().numpy().astype(np.float64), q[:3].cpu().numpy(), pool.cpu().numpy(), pages[:3], lens[:3], [1] * 3, d, g,
+            h, 1, 0.1)

@@ -390,3 +390,73 @@ def test_a_prompt_is_not_stored_again_over_shared_pages(host_copies):
     c.reserve([a], 130)
     opt_decode._per_layer(c, 1, 130, 0)
     assert not set(c.pages(a)) & set(c.pages(f))
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_a_random_life_of_a_cache(host_copies, seed):
+    # every sequence finds its own rows, whatever the others do, with some counted by the host and some by the device; a row is
+    # one byte here, stored where the device's table says
+    import random
+    from sqamd import kv4
+    rng = random.Random(seed)
+    c = kv4.KV4Cache(1, 14, 1, 64, 64, max_seqs=5, max_rows=250, device="cpu")
+    c.counted_on_device(rng.choice([0, 0, 2, 5]))
+    rows = {}
+
+    def store(seq, first, values):
+        for r, value in enumerate(values, first):
+            page = int(c.table[seq, r // 64]) if r // 64 < c.width else -1
+            if page >= 0:
+                c.pool[0, page, 0, r % 64] = value
+
+    def check():
+        assert only_own_pages(c)
+        uses = [0] * c.num_pages
+        for seq, own in rows.items():
+            assert c.rows(seq) == len(own) == int(c.lengths[seq]) <= 64 * len(c.pages(seq))
+            assert [int(c.pool[0, int(c.table[seq, r // 64]), 0, r % 64]) for r in range(len(own))] == own
+            for page in c.pages(seq):
+                uses[page] += 1
+        assert uses == c._uses and sorted(c._free) == [p for p, n in enumerate(uses) if not n]
+
+    for step in range(120):
+        seq = rng.choice(sorted(rows)) if rows else None
+        what = rng.choice(["add", "extend", "extend", "extend", "fork", "truncate", "free", "compact", "reserve", "device", "device"])
+        try:
+            if what == "add":
+                rows[c.add()] = []
+            elif seq is None:
+                continue
+            elif what == "extend":
+                some = sorted(rng.sample(sorted(rows), rng.randint(1, len(rows))))
+                more = [rng.randint(0, 70) for _ in some]
+                c.extend(some, more)
+                for s, n in zip(some, more):
+                    new = [rng.randrange(256) for _ in range(n)]
+                    store(s, len(rows[s]), new)
+                    rows[s] = rows[s] + new
+            elif what == "fork":
+                rows[c.fork(seq)] = list(rows[seq])
+            elif what == "truncate":
+                n = rng.randint(0, len(rows[seq]))
+                c.truncate(seq, n)
+                rows[seq] = rows[seq][:n]
+            elif what == "free":
+                c.free(seq)
+                del rows[seq]
+            elif what == "compact":
+                assert c.compact() == c.num_pages - c.free_pages()
+            elif what == "reserve":
+                c.reserve([seq], rng.randint(0, 250))
+            elif c._device_counts:  # steps of all that the device counts, as a replayed graph takes them
+                room = [64 * len(c.pages(s)) - len(rows[s]) for s in rows if s in c._device_counts]
+                for _ in range(min([rng.randint(0, 20)] + room)):
+                    for s in sorted(c._device_counts):
+                        if s in rows:
+                            value = rng.randrange(256)
+                            store(s, len(rows[s]), [value])
+                            rows[s] = rows[s] + [value]
+                            c.lengths[s] += 1
+        except (RuntimeError, ValueError) as e:
+            assert any(word in str(e) for word in ("wanted", "in use", "in a cache of")), e
+        check()
