@@ -534,6 +534,86 @@ int sq_kv4_select(const void* q, void* selected, const void* pool, const void* p
 int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int num_pages, int layers, size_t page_bytes,
                       size_t layer_bytes, void* stream);
 
+/* Causal attention of a batch of sequences that share a long prefix, which is read once for all of them:
+ *   out[t, h, :] = sum_j P[j] v_j, P = softmax_j(sm_scale q[t, h, :] . k_j) over the P rows of the prefix and the rows of t's
+ * own sequence up to t's; query head h reads key/value head h / (Hq / H).  fp16, softmax and sums in fp32, the probabilities
+ * rounded to fp16 where they meet the values.
+ *   q          element (t, h, d) at q[t * strides[0] + h * strides[1] + d]
+ *   k_prefix, v_prefix  row j of head h at [h * strides[2] + j * strides[3]]; may be NULL where P is 0
+ *   k_cache, v_cache    row j of (sequence b, head h) at [b * strides[4] + h * strides[5] + j * strides[6]], room for Lmax rows
+ *   lengths    int32 [B]: own rows of each sequence, the rows of this call among them
+ *   starts     int32 [B + 1]: sequence b has the tokens starts[b] .. starts[b + 1] - 1 of the call; NULL: T / B each.  Token i
+ *              of n is own row lengths[b] - n + i.
+ *   k_new, v_new  both NULL (the tokens' rows are in the caches), or the rows of the call's tokens, element (t, h, d) at
+ *              [t * strides[7] + h * strides[8] + d], which are stored in the caches and attended to
+ *   out        fp16 [T][Hq][D] contiguous; a token that sees no row gets 0, tokens behind the last sequence's are left as
+ *              they were
+ * lengths and starts lie on the device and are read by the kernels: a captured HIP graph follows them.  Whatever they hold,
+ * nothing outside the given tensors is touched: rows outside [0, Lmax) are neither stored nor seen, starts are clamped to
+ * [0, T].  D in {64, 128}; strides in elements, multiples of 8, those of rows below 2^23; q, rows and out 16-byte aligned.
+ *   workspace  sq_prefix_attention_workspace_bytes(...) bytes (ragged: whether starts is given), 16-byte aligned, of any
+ *              content; not shared by calls that may run at the same time. */
+size_t sq_prefix_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int P, int Lmax, int ragged);
+int sq_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, void* k_cache, void* v_cache,
+                        const void* lengths, const void* starts, const void* k_new, const void* v_new, void* out, int T, int B,
+                        int Hq, int H, int D, int P, int Lmax, const long* strides, float sm_scale, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* A decode step over a key/value cache of R rows a head that evicts by accumulated attention weight, one token per sequence.
+ *   seen       int32 [B] on the device: tokens of each sequence, this one among them (0 or less: nothing is done for it, its
+ *              out is 0 and its slot -1)
+ *   weight     fp32 [B][H][R], position int32 [B][H][R] (the tokens that the rows are of): read and updated
+ *   slot       int32 [B][H] receives the row that the token's key and value (k_new, v_new) are stored in: row seen - 1 where
+ *              seen <= R; otherwise the row of the lowest weight among those with first <= position < seen - last (the lowest
+ *              row among equals; a weight that is no number is the lowest; row 0 where there is none)
+ *   then position[slot] = seen - 1, weight[slot] = 0, the token attends over the first min(seen, R) rows as above, and
+ *   weight[j] += the sum over the query heads of the key/value head of P[j].
+ * A row of the last `last` tokens, the present one among them, or of the first `first` does not go: first + last <= R.
+ * q element (b, h, d) at q[b * strides[0] + h * strides[1] + d], k_new and v_new with strides[2], strides[3], the caches' row j
+ * of (b, h) at [b * strides[4] + h * strides[5] + j * strides[6]]; out fp16 [B][Hq][D].  Types, alignment and workspace as
+ * for sq_prefix_attention. */
+size_t sq_evict_attention_workspace_bytes(int B, int Hq, int H, int D, int R);
+int sq_evict_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, void* weight,
+                       void* position, const void* seen, void* out, void* slot, int B, int Hq, int H, int D, int R, int first,
+                       int last, const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weight that a prompt's queries give to each of its keys:
+ *   w[b][h][j] = sum over the query heads of h and the queries i >= j of P_i[j], P_i = softmax_{j <= i}(sm_scale q_i . k_j)
+ * over all queries of a sequence, or its last `window` (0: all).  q, k fp16, row i of (b, h) at q[b * strides[0] + h *
+ * strides[1] + i * strides[2]], k with strides[3..5]; w fp32 [B][H][S], 0 behind a sequence's rows; lengths int32 [B] on the
+ * device, or NULL: S rows each.  Sums in fp32, their order fixed. */
+size_t sq_attention_weights_workspace_bytes(int B, int Hq, int H, int S, int window);
+int sq_attention_weights(const void* q, const void* k, const void* lengths, void* w, int B, int Hq, int H, int D, int S, int window,
+                         const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Of a prompt's S rows (lengths as above) those that stay in a cache of R rows a head: the R of the highest weight (a weight
+ * that is no number is the lowest, the lower row goes first among equals), its first `first` and last `last` rows (first +
+ * last <= R) in any case; all where there are no more than R.  In their order they are copied to the first rows of the caches, with their
+ * weights and, as positions, their numbers.  rows int32 [B][H][R] names them, -1 behind the last; what the caches hold behind
+ * them stays.  k, v: row j of (b, h) at [b * strides[0] + h * strides[1] + j * strides[2]]; weight fp32 element (b, h, j) at
+ * [b * strides[3] + h * strides[4] + j]; caches with strides[5..7]; cache_weight fp32, cache_position int32 [B][H][R].  The
+ * caches must not overlap the rows that they are filled from. */
+int sq_evict_keep(const void* k, const void* v, const void* weight, const void* lengths, void* k_cache, void* v_cache,
+                  void* cache_weight, void* cache_position, void* rows, int B, int H, int D, int S, int R, int first, int last,
+                  const long* strides, void* stream);
+
+/* Rules on logits x [M][V] (fp16 where elem_bytes is 2, fp32 where it is 4; rows strides[0] elements apart) into y (rows
+ * strides[1] apart; may be x), and the best token of each row (int64 [M]; the lowest among equals, NaN never wins, 0 where there
+ * is none).  In this order, each step rounded once in fp32:
+ *   x > 0 ? x / repetition[m] : x * repetition[m]   tokens that stand in the row's text
+ *   x - frequency[m] * c, then x - presence[m]       tokens that stand c > 0 times in the generated part of it
+ *   x + bias[m][j]                                   tokens that bias_ids[m][j] names (the last j among several)
+ *   -inf                                             tokens whose bit (token % 32 of word token / 32) in mask[m] is 0
+ * ids int64, place i of row m at ids[m * strides[2] + i * strides[3]], i < lengths[m * strides[4]] <= L; generated from place
+ * generated_from[m * strides[5]] on (NULL: all of it).  repetition, frequency and presence fp32 [M], each may be NULL; bias_ids int32
+ * and bias fp32, rows of nb <= 65535 entries strides[6] and strides[7] apart; mask uint32, rows of ceil(V / 32) words strides[8]
+ * apart (0: one for all).  Ids outside [0, V) are none. */
+size_t sq_logit_rules_workspace_bytes(int M, int V);
+int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, const void* lengths, const void* generated_from,
+                   const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,
+                   const void* mask, void* token, int M, int V, int L, int nb, const long* strides, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

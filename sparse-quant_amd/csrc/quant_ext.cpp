@@ -626,6 +626,197 @@ bool kv4_copy_pages(const at::Tensor& pool, const at::Tensor& src, const at::Ten
                              (size_t)(page * n), current_stream(pool)) == SQ_OK;
 }
 
+// Attention behind a shared prefix, the cache that evicts by attention weight, rules on logits (sqamd/prefix.py, evict.py and
+// logits.py, which do what these leave to them: copies of what cannot be read as it lies, and the complaints).
+using Opt = c10::optional<at::Tensor>;
+
+long stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? (long)t.stride(d) : 0; }  // (of one element: any)
+// fp16 rows of 16-byte chunks, the strides of all other dimensions multiples of 8.
+bool rows_fit(const at::Tensor& t, const at::Tensor& like, int64_t dims) {
+    if (!t.is_cuda() || t.device() != like.device() || t.scalar_type() != at::kHalf || t.dim() != dims || t.stride(-1) != 1 ||
+        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u))
+        return false;
+    for (int64_t d = 0; d + 1 < dims; d++)
+        if (stride_of(t, d) % 8 != 0) return false;
+    return true;
+}
+bool pair_fits(const at::Tensor& k, const at::Tensor& v, const at::Tensor& like, int64_t dims) {
+    if (!rows_fit(k, like, dims) || !rows_fit(v, like, dims) || k.sizes() != v.sizes()) return false;
+    for (int64_t d = 0; d + 1 < dims; d++)
+        if (stride_of(k, d) != stride_of(v, d)) return false;
+    return true;
+}
+// ... that are written to: no two of its rows in one place.
+bool apart(const at::Tensor& t) {
+    for (int64_t d = 0; d + 1 < t.dim(); d++)
+        if (t.size(d) > 1 && t.stride(d) < t.size(-1)) return false;
+    return true;
+}
+bool whole(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, at::IntArrayRef sizes) {
+    return t.scalar_type() == type && t.device() == like.device() && t.is_contiguous() && t.sizes() == sizes;
+}
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* pointer(const Opt& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+constexpr int64_t INTS = 1LL << 31;
+
+Opt prefix_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& kc, const at::Tensor& vc,
+                     const at::Tensor& lengths, double sm_scale, const Opt& starts, const Opt& into, const Opt& kn,
+                     const Opt& vn) {
+    if (!rows_fit(q, q, 3) || !pair_fits(kp, vp, q, 3) || !pair_fits(kc, vc, q, 4)) return c10::nullopt;
+    const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), B = kc.size(0), H = kc.size(1), L = kc.size(2), P = kp.size(1);
+    if (kc.size(3) != D || kp.size(0) != H || kp.size(2) != D || H == 0 || Hq % H != 0 || T * Hq >= INTS || L >= INTS || P >= INTS ||
+        !whole(lengths, q, at::kInt, {B}))
+        return c10::nullopt;
+    if (starts.has_value() ? !whole(*starts, q, at::kInt, {B + 1}) : (B ? T % B : T) != 0) return c10::nullopt;
+    if (kn.has_value() != vn.has_value()) return c10::nullopt;
+    if (kn.has_value() && (!pair_fits(*kn, *vn, q, 3) || kn->size(0) != T || kn->size(1) != H || kn->size(2) != D || !apart(kc) || !apart(vc)))
+        return c10::nullopt;
+    if (into.has_value() && !whole(*into, q, at::kHalf, q.sizes())) return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = into.has_value() ? *into : at::empty({T, Hq, D}, q.options());
+    const size_t need = sq_prefix_attention_workspace_bytes((int)T, (int)B, (int)Hq, (int)H, (int)D, (int)P, (int)L, starts.has_value());
+    const at::Tensor ws = scratch(need, q);
+    const long strides[9] = {stride_of(q, 0), stride_of(q, 1), stride_of(kp, 0), stride_of(kp, 1), stride_of(kc, 0), stride_of(kc, 1),
+                             stride_of(kc, 2), kn.has_value() ? stride_of(*kn, 0) : 0, kn.has_value() ? stride_of(*kn, 1) : 0};
+    const int rc = sq_prefix_attention(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), kc.data_ptr(), vc.data_ptr(), lengths.data_ptr(),
+                                       pointer(starts), pointer(kn), pointer(vn), out.data_ptr(), (int)T, (int)B, (int)Hq, (int)H,
+                                       (int)D, (int)P, (int)L, strides, (float)sm_scale, pointer(ws), need, current_stream(q));
+    if (rc != SQ_OK) return c10::nullopt;
+    return out;
+}
+
+c10::optional<std::pair<at::Tensor, at::Tensor>> evict_attention(
+    const at::Tensor& q, const at::Tensor& kn, const at::Tensor& vn, const at::Tensor& kc, const at::Tensor& vc,
+    const at::Tensor& weight, const at::Tensor& position, const at::Tensor& seen, double sm_scale, int64_t first, int64_t last,
+    const Opt& into) {
+    if (!rows_fit(q, q, 3) || !pair_fits(kn, vn, q, 3) || !pair_fits(kc, vc, q, 4) || !apart(kc) || !apart(vc)) return c10::nullopt;
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), H = kc.size(1), R = kc.size(2);
+    if (kc.size(0) != B || kc.size(3) != D || kn.size(0) != B || kn.size(1) != H || kn.size(2) != D || H == 0 || Hq % H != 0 ||
+        B * Hq >= INTS || R >= INTS || first < 0 || last < 1 || first + last > R || !whole(weight, q, at::kFloat, {B, H, R}) ||
+        !whole(position, q, at::kInt, {B, H, R}) || !whole(seen, q, at::kInt, {B}))
+        return c10::nullopt;
+    if (into.has_value() && !whole(*into, q, at::kHalf, q.sizes())) return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(q.device());
+    at::Tensor out = into.has_value() ? *into : at::empty({B, Hq, D}, q.options());
+    at::Tensor slot = at::empty({B, H}, seen.options());
+    const size_t need = sq_evict_attention_workspace_bytes((int)B, (int)Hq, (int)H, (int)D, (int)R);
+    const at::Tensor ws = scratch(need, q);
+    const long strides[7] = {stride_of(q, 0),  stride_of(q, 1),  stride_of(kn, 0), stride_of(kn, 1),
+                             stride_of(kc, 0), stride_of(kc, 1), stride_of(kc, 2)};
+    const int rc = sq_evict_attention(q.data_ptr(), kn.data_ptr(), vn.data_ptr(), kc.data_ptr(), vc.data_ptr(), weight.data_ptr(),
+                                      position.data_ptr(), seen.data_ptr(), out.data_ptr(), slot.data_ptr(), (int)B, (int)Hq, (int)H,
+                                      (int)D, (int)R, (int)first, (int)last, strides, (float)sm_scale, pointer(ws), need,
+                                      current_stream(q));
+    if (rc != SQ_OK) return c10::nullopt;
+    return std::make_pair(out, slot);
+}
+
+Opt evict_weights(const at::Tensor& q, const at::Tensor& k, double sm_scale, int64_t window, const Opt& lengths) {
+    if (!rows_fit(q, q, 4) || !rows_fit(k, q, 4)) return c10::nullopt;
+    const int64_t B = q.size(0), Hq = q.size(1), S = q.size(2), D = q.size(3), H = k.size(1);
+    if (k.size(0) != B || k.size(2) != S || k.size(3) != D || H == 0 || Hq % H != 0 || B * Hq >= INTS || S >= INTS || window < 0 ||
+        window >= INTS || (lengths.has_value() && !whole(*lengths, q, at::kInt, {B})))
+        return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(q.device());
+    at::Tensor w = at::empty({B, H, S}, q.options().dtype(at::kFloat));
+    const size_t need = sq_attention_weights_workspace_bytes((int)B, (int)Hq, (int)H, (int)S, (int)window);
+    const at::Tensor ws = scratch(need, q);
+    const long strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2)};
+    const int rc = sq_attention_weights(q.data_ptr(), k.data_ptr(), pointer(lengths), w.data_ptr(), (int)B, (int)Hq, (int)H, (int)D,
+                                        (int)S, (int)window, strides, (float)sm_scale, pointer(ws), need, current_stream(q));
+    if (rc != SQ_OK) return c10::nullopt;
+    return w;
+}
+
+Opt evict_keep(const at::Tensor& k, const at::Tensor& v, const at::Tensor& weight, const at::Tensor& kc, const at::Tensor& vc,
+               const at::Tensor& cweight, const at::Tensor& cposition, int64_t first, int64_t last, const Opt& lengths) {
+    if (!pair_fits(k, v, k, 4) || !pair_fits(kc, vc, k, 4) || !apart(kc) || !apart(vc)) return c10::nullopt;
+    const int64_t B = k.size(0), H = k.size(1), S = k.size(2), D = k.size(3), R = kc.size(2);
+    if (kc.size(0) != B || kc.size(1) != H || kc.size(3) != D || S >= INTS || R >= INTS || R < 1 || first < 0 || last < 0 ||
+        first + last > R || weight.scalar_type() != at::kFloat || weight.device() != k.device() || weight.dim() != 3 ||
+        weight.size(0) != B || weight.size(1) != H || weight.size(2) != S || stride_of(weight, 2) > 1 ||
+        (S > 1 && weight.stride(2) != 1) || !whole(cweight, k, at::kFloat, {B, H, R}) ||
+        !whole(cposition, k, at::kInt, {B, H, R}) || (lengths.has_value() && !whole(*lengths, k, at::kInt, {B})))
+        return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(k.device());
+    at::Tensor rows = at::empty({B, H, R}, cposition.options());
+    const long strides[8] = {stride_of(k, 0),      stride_of(k, 1),  stride_of(k, 2),  stride_of(weight, 0),
+                             stride_of(weight, 1), stride_of(kc, 0), stride_of(kc, 1), stride_of(kc, 2)};
+    const int rc = sq_evict_keep(k.data_ptr(), v.data_ptr(), weight.data_ptr(), pointer(lengths), kc.data_ptr(), vc.data_ptr(),
+                                 cweight.data_ptr(), cposition.data_ptr(), rows.data_ptr(), (int)B, (int)H, (int)D, (int)S, (int)R,
+                                 (int)first, (int)last, strides, current_stream(k));
+    if (rc != SQ_OK) return c10::nullopt;
+    return rows;
+}
+
+c10::optional<std::pair<at::Tensor, at::Tensor>> logit_rules(const at::Tensor& x, const Opt& ids, const Opt& lengths,
+                                                              const Opt& generated, const Opt& repetition, const Opt& presence,
+                                                              const Opt& frequency, const Opt& bias_ids, const Opt& bias,
+                                                              const Opt& mask, const Opt& into, const Opt& token_into) {
+    const bool half = x.scalar_type() == at::kHalf;
+    if (!x.is_cuda() || x.dim() != 2 || (!half && x.scalar_type() != at::kFloat)) return c10::nullopt;
+    const int64_t M = x.size(0), V = x.size(1);
+    if (V < 1 || V >= INTS || M >= INTS || (V > 1 && x.stride(1) != 1)) return c10::nullopt;
+    auto alike = [&](const at::Tensor& t, at::ScalarType type, int64_t dims) {
+        return t.scalar_type() == type && t.device() == x.device() && t.dim() == dims && (dims == 0 || t.size(0) == M);
+    };
+    long strides[9] = {stride_of(x, 0), 0, 0, 0, 0, 0, 0, 0, 0};
+    int64_t L = 0, nb = 0;
+    if (ids.has_value()) {
+        if (!alike(*ids, at::kLong, 2) || ids->size(1) >= INTS) return c10::nullopt;
+        L = ids->size(1);
+        strides[2] = stride_of(*ids, 0), strides[3] = stride_of(*ids, 1);
+    }
+    for (int i = 0; i < 2; i++) {
+        const Opt& t = i ? generated : lengths;
+        if (!t.has_value()) continue;
+        if (!alike(*t, at::kLong, 1)) return c10::nullopt;
+        strides[4 + i] = stride_of(*t, 0);
+    }
+    for (const Opt* t : {&repetition, &presence, &frequency})
+        if (t->has_value() && (!alike(**t, at::kFloat, 1) || !(*t)->is_contiguous() || !ids.has_value())) return c10::nullopt;
+    if (bias_ids.has_value() != bias.has_value()) return c10::nullopt;
+    if (bias.has_value()) {
+        if (!alike(*bias_ids, at::kInt, 2) || !alike(*bias, at::kFloat, 2) || bias_ids->sizes() != bias->sizes() ||
+            bias->size(1) > 65535 || stride_of(*bias, 1) > 1 || stride_of(*bias_ids, 1) > 1 ||
+            (bias->size(1) > 1 && (bias->stride(1) != 1 || bias_ids->stride(1) != 1)))
+            return c10::nullopt;
+        nb = bias->size(1);
+        strides[6] = stride_of(*bias_ids, 0), strides[7] = stride_of(*bias, 0);
+    }
+    if (mask.has_value()) {
+        const int64_t words = (V + 31) / 32;
+        if (mask->scalar_type() != at::kInt || mask->device() != x.device() || mask->dim() != 2 ||
+            (mask->size(0) != M && mask->size(0) != 1) || mask->size(1) != words || (words > 1 && mask->stride(1) != 1))
+            return c10::nullopt;
+        strides[8] = stride_of(*mask, 0);
+    }
+    if (into.has_value() && (into->scalar_type() != x.scalar_type() || into->device() != x.device() || into->sizes() != x.sizes() ||
+                             (V > 1 && into->stride(1) != 1) || (M > 1 && into->stride(0) < V)))
+        return c10::nullopt;
+    if (token_into.has_value() && !whole(*token_into, x, at::kLong, {M})) return c10::nullopt;
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard guard(x.device());
+    at::Tensor out = into.has_value() ? *into : at::empty({M, V}, x.options());
+    at::Tensor token = token_into.has_value() ? *token_into : at::empty({M}, x.options().dtype(at::kLong));
+    strides[1] = stride_of(out, 0);
+    const size_t need = sq_logit_rules_workspace_bytes((int)M, (int)V);
+    const at::Tensor ws = scratch(need, x);
+    const int rc = sq_logit_rules(x.data_ptr(), out.data_ptr(), half ? 2 : 4, pointer(ids), pointer(lengths), pointer(generated),
+                                  pointer(repetition), pointer(presence), pointer(frequency), pointer(bias_ids), pointer(bias),
+                                  pointer(mask), token.data_ptr(), (int)M, (int)V, (int)L, (int)nb, strides, pointer(ws), need,
+                                  current_stream(x));
+    if (rc != SQ_OK) return c10::nullopt;
+    return std::make_pair(out, token);
+}
+
 // Same with an explicit kernel id (SQ_ALGO_* | tuning word << 8); for tests and benchmarks.
 at::Tensor gemm_awq_algo(at::Tensor I, at::Tensor W, at::Tensor W_zeros_scales, const int N, const int group_size,
                          const int algo) {
@@ -787,6 +978,11 @@ PYBIND11_MODULE(quant, m) {
     m.def("kv4_attention", &kv4_attention);
     m.def("kv4_select", &kv4_select);
     m.def("kv4_copy_pages", &kv4_copy_pages);
+    m.def("prefix_attention", &prefix_attention);
+    m.def("evict_attention", &evict_attention);
+    m.def("evict_weights", &evict_weights);
+    m.def("evict_keep", &evict_keep);
+    m.def("logit_rules", &logit_rules);
     m.def("gemm_awq_silu_dot_ut", &gemm_awq_silu_dot_ut, py::arg("I"), py::arg("W1") = py::none(),
           py::arg("W2") = py::none(), py::arg("ZS1") = py::none(), py::arg("ZS2") = py::none(),
           py::arg("W13") = py::none(), py::arg("ZS13") = py::none(), py::arg("M"), py::arg("N"), py::arg("K"),

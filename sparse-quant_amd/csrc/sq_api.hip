@@ -392,6 +392,20 @@ int check_kv4_rows(const void* k, const void* v, const long* strides) {
     return SQ_OK;
 }
 
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+bool heads_ok(int Hq, int H, int D) { return H > 0 && Hq > 0 && Hq % H == 0 && (D == 64 || D == 128); }
+
+constexpr long ROW_STRIDE_MAX = 1L << 23;  // elements: 64 rows stay inside 32 bits of bytes
+
+int check_strides(const long* strides, int n) {
+    for (int i = 0; i < n; i++) {
+        if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
+        if (strides[i] % 8 != 0) return SQ_ERR_MISALIGNED;
+    }
+    return SQ_OK;
+}
+
 sq::Kv4Cache kv4_cache(const void* pool, const void* pages, const void* lengths, const void* starts, int T, int B, int H,
                        int num_pages, int width, int page_stride) {
     sq::Kv4Cache c;
@@ -1229,6 +1243,187 @@ int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int n
     if (!aligned16(pool) || ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3u)) return SQ_ERR_MISALIGNED;
     return launch_code(sq::launch_kv4_copy_pages(pool, static_cast<const int*>(src), static_cast<const int*>(dst), n, num_pages,
                                                  layers, (long)page_bytes, (long)layer_bytes, static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_prefix_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int P, int Lmax, int ragged) {
+    if (!heads_ok(Hq, H, D) || T <= 0 || B <= 0 || P < 0 || Lmax < 0) return 0;
+    return sq::prefix_attention_workspace_bytes(T, B, H, Hq / H, D, P, Lmax, ragged != 0);
+}
+
+int sq_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, void* k_cache, void* v_cache,
+                        const void* lengths, const void* starts, const void* k_new, const void* v_new, void* out, int T, int B,
+                        int Hq, int H, int D, int P, int Lmax, const long* strides, float sm_scale, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    if (!heads_ok(Hq, H, D) || T < 0 || B < 0 || P < 0 || Lmax < 0) return SQ_ERR_BAD_SHAPE;
+    if ((long)T * Hq > (1L << 28) || (long)B * Hq > (1L << 24) || P > (1 << 30) || Lmax > (1 << 30)) return SQ_ERR_BAD_SHAPE;
+    if (!starts && B > 0 && T % B != 0) return SQ_ERR_BAD_SHAPE;
+    if (T == 0 || B == 0) return SQ_OK;
+    if (!q || !out || !lengths || !strides || (P > 0 && (!k_prefix || !v_prefix)) || (Lmax > 0 && (!k_cache || !v_cache)) ||
+        (k_new == nullptr) != (v_new == nullptr))
+        return SQ_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(out) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_cache) ||
+        !aligned16(v_cache) || !aligned16(k_new) || !aligned16(v_new) || !aligned4(lengths) || !aligned4(starts))
+        return SQ_ERR_MISALIGNED;
+    const int rc = check_strides(strides, k_new ? 9 : 7);
+    if (rc != SQ_OK) return rc;
+    if (strides[3] >= ROW_STRIDE_MAX || strides[6] >= ROW_STRIDE_MAX) return SQ_ERR_BAD_SHAPE;
+    const size_t need = sq_prefix_attention_workspace_bytes(T, B, Hq, H, D, P, Lmax, starts != nullptr);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return SQ_ERR_WORKSPACE;
+    sq::PrefixAttn t = {};
+    t.q = static_cast<const sq::half_t*>(q);
+    t.kp = static_cast<const sq::half_t*>(k_prefix);
+    t.vp = static_cast<const sq::half_t*>(v_prefix);
+    t.kc = static_cast<sq::half_t*>(k_cache);
+    t.vc = static_cast<sq::half_t*>(v_cache);
+    t.kn = static_cast<const sq::half_t*>(k_new);
+    t.vn = static_cast<const sq::half_t*>(v_new);
+    t.o = static_cast<sq::half_t*>(out);
+    t.lengths = static_cast<const int*>(lengths);
+    t.starts = static_cast<const int*>(starts);
+    t.q_ts = strides[0], t.q_hs = strides[1], t.p_hs = strides[2], t.p_rs = strides[3];
+    t.c_bs = strides[4], t.c_hs = strides[5], t.c_rs = strides[6];
+    if (k_new) t.n_ts = strides[7], t.n_hs = strides[8];
+    t.T = T, t.B = B, t.H = H, t.share = Hq / H, t.P = P, t.Lmax = Lmax, t.each = T / B;
+    return launch_code(sq::launch_prefix_attention(t, D, sm_scale, workspace, static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_evict_attention_workspace_bytes(int B, int Hq, int H, int D, int R) {
+    if (!heads_ok(Hq, H, D) || B <= 0 || R <= 0) return 0;
+    return sq::evict_attention_workspace_bytes(B, H, Hq / H, D, R);
+}
+
+int sq_evict_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, void* weight,
+                       void* position, const void* seen, void* out, void* slot, int B, int Hq, int H, int D, int R, int first,
+                       int last, const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!heads_ok(Hq, H, D) || B < 0 || R <= 0 || first < 0 || last < 1 || (long)first + last > R) return SQ_ERR_BAD_SHAPE;
+    if ((long)B * Hq > (1L << 22) || R > (1 << 24)) return SQ_ERR_BAD_SHAPE;
+    if (B == 0) return SQ_OK;
+    if (!q || !k_new || !v_new || !k_cache || !v_cache || !weight || !position || !seen || !out || !slot || !strides)
+        return SQ_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) ||
+        !aligned4(weight) || !aligned4(position) || !aligned4(seen) || !aligned4(slot))
+        return SQ_ERR_MISALIGNED;
+    const int rc = check_strides(strides, 7);
+    if (rc != SQ_OK) return rc;
+    if (strides[6] >= ROW_STRIDE_MAX) return SQ_ERR_BAD_SHAPE;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < sq_evict_attention_workspace_bytes(B, Hq, H, D, R))
+        return SQ_ERR_WORKSPACE;
+    sq::EvictStep t = {};
+    t.q = static_cast<const sq::half_t*>(q);
+    t.kn = static_cast<const sq::half_t*>(k_new);
+    t.vn = static_cast<const sq::half_t*>(v_new);
+    t.kc = static_cast<sq::half_t*>(k_cache);
+    t.vc = static_cast<sq::half_t*>(v_cache);
+    t.weight = static_cast<float*>(weight);
+    t.position = static_cast<int*>(position);
+    t.seen = static_cast<const int*>(seen);
+    t.o = static_cast<sq::half_t*>(out);
+    t.slot = static_cast<int*>(slot);
+    t.q_bs = strides[0], t.q_hs = strides[1], t.n_bs = strides[2], t.n_hs = strides[3];
+    t.c_bs = strides[4], t.c_hs = strides[5], t.c_rs = strides[6];
+    t.B = B, t.H = H, t.share = Hq / H, t.R = R, t.first = first, t.last = last;
+    return launch_code(sq::launch_evict_attention(t, D, sm_scale, workspace, static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_attention_weights_workspace_bytes(int B, int Hq, int H, int S, int window) {
+    if (!heads_ok(Hq, H, 64) || B <= 0 || S <= 0 || window < 0) return 0;
+    return sq::attention_weights_workspace_bytes(B, H, Hq / H, S, window);
+}
+
+int sq_attention_weights(const void* q, const void* k, const void* lengths, void* w, int B, int Hq, int H, int D, int S, int window,
+                         const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!heads_ok(Hq, H, D) || B < 0 || S < 0 || window < 0) return SQ_ERR_BAD_SHAPE;
+    if ((long)B * Hq > (1L << 22) || (long)B * Hq * S > (1L << 34) || (long)S * (Hq / H) > (1L << 30)) return SQ_ERR_BAD_SHAPE;
+    if (B == 0 || S == 0) return SQ_OK;
+    if (!q || !k || !w || !strides) return SQ_ERR_NULL_POINTER;
+    if (!aligned16(q) || !aligned16(k) || !aligned4(w) || !aligned4(lengths)) return SQ_ERR_MISALIGNED;
+    const int rc = check_strides(strides, 6);
+    if (rc != SQ_OK) return rc;
+    if (strides[5] >= ROW_STRIDE_MAX) return SQ_ERR_BAD_SHAPE;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < sq_attention_weights_workspace_bytes(B, Hq, H, S, window))
+        return SQ_ERR_WORKSPACE;
+    sq::WeighArgs t = {};
+    t.q = static_cast<const sq::half_t*>(q);
+    t.k = static_cast<const sq::half_t*>(k);
+    t.lengths = static_cast<const int*>(lengths);
+    t.w = static_cast<float*>(w);
+    t.q_bs = strides[0], t.q_hs = strides[1], t.q_rs = strides[2];
+    t.k_bs = strides[3], t.k_hs = strides[4], t.k_rs = strides[5];
+    t.B = B, t.H = H, t.share = Hq / H, t.S = S, t.window = window;
+    return launch_code(sq::launch_attention_weights(t, D, sm_scale, workspace, static_cast<hipStream_t>(stream)));
+}
+
+int sq_evict_keep(const void* k, const void* v, const void* weight, const void* lengths, void* k_cache, void* v_cache,
+                  void* cache_weight, void* cache_position, void* rows, int B, int H, int D, int S, int R, int first, int last,
+                  const long* strides, void* stream) {
+    if (!heads_ok(H, H, D) || B < 0 || S < 0 || R <= 0 || first < 0 || last < 0 || (long)first + last > R) return SQ_ERR_BAD_SHAPE;
+    if ((long)B * H > 65535 || R > (1 << 24) || S > (1 << 30)) return SQ_ERR_BAD_SHAPE;
+    if (B == 0) return SQ_OK;
+    if (!k_cache || !v_cache || !cache_weight || !cache_position || !rows || !strides || (S > 0 && (!k || !v || !weight)))
+        return SQ_ERR_NULL_POINTER;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned4(weight) || !aligned4(lengths) ||
+        !aligned4(cache_weight) || !aligned4(cache_position) || !aligned4(rows))
+        return SQ_ERR_MISALIGNED;
+    const long of[6] = {strides[0], strides[1], strides[2], strides[5], strides[6], strides[7]};
+    const int rc = check_strides(of, 6);
+    if (rc != SQ_OK) return rc;
+    if (strides[3] < 0 || strides[4] < 0) return SQ_ERR_BAD_SHAPE;
+    sq::EvictKeep t = {};
+    t.k = static_cast<const sq::half_t*>(k);
+    t.v = static_cast<const sq::half_t*>(v);
+    t.weight = static_cast<const float*>(weight);
+    t.lengths = static_cast<const int*>(lengths);
+    t.kc = static_cast<sq::half_t*>(k_cache);
+    t.vc = static_cast<sq::half_t*>(v_cache);
+    t.cweight = static_cast<float*>(cache_weight);
+    t.cposition = static_cast<int*>(cache_position);
+    t.rows = static_cast<int*>(rows);
+    t.k_bs = strides[0], t.k_hs = strides[1], t.k_rs = strides[2], t.w_bs = strides[3], t.w_hs = strides[4];
+    t.c_bs = strides[5], t.c_hs = strides[6], t.c_rs = strides[7];
+    t.B = B, t.H = H, t.S = S, t.R = R, t.first = first, t.last = last;
+    return launch_code(sq::launch_evict_keep(t, D, static_cast<hipStream_t>(stream)));
+}
+
+size_t sq_logit_rules_workspace_bytes(int M, int V) { return M > 0 && V > 0 ? sq::logit_rules_workspace_bytes(M, V) : 0; }
+
+int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, const void* lengths, const void* generated_from,
+                   const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,
+                   const void* mask, void* token, int M, int V, int L, int nb, const long* strides, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    if (M < 0 || M > 65535 || V <= 0 || V > (1 << 30) || L < 0 || nb < 0 || nb > 65535 || (elem_bytes != 2 && elem_bytes != 4))
+        return SQ_ERR_BAD_SHAPE;
+    if (M == 0) return SQ_OK;
+    if (!x || !y || !token || !strides || (nb > 0 && (!bias_ids || !bias)) ||
+        (L > 0 && (repetition || presence || frequency) && !ids))
+        return SQ_ERR_NULL_POINTER;
+    const uintptr_t e = (uintptr_t)elem_bytes - 1;
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & e) || !aligned4(repetition) || !aligned4(presence) ||
+        !aligned4(frequency) || !aligned4(bias_ids) || !aligned4(bias) || !aligned4(mask) ||
+        ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(generated_from) |
+          reinterpret_cast<uintptr_t>(token)) & 7u))
+        return SQ_ERR_MISALIGNED;
+    for (int i = 0; i < 9; i++)
+        if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
+    if (M > 1 && strides[1] < V) return SQ_ERR_BAD_SHAPE;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < sq_logit_rules_workspace_bytes(M, V)) return SQ_ERR_WORKSPACE;
+    sq::LogitRules t = {};
+    t.x = x, t.y = y;
+    t.ids = static_cast<const long long*>(ids);
+    t.lengths = static_cast<const long long*>(lengths);
+    t.generated = static_cast<const long long*>(generated_from);
+    if (L > 0) {
+        t.repetition = static_cast<const float*>(repetition);
+        t.presence = static_cast<const float*>(presence);
+        t.frequency = static_cast<const float*>(frequency);
+    }
+    t.bias_ids = static_cast<const int*>(bias_ids);
+    t.bias = static_cast<const float*>(bias);
+    t.mask = static_cast<const unsigned*>(mask);
+    t.token = static_cast<long long*>(token);
+    t.x_rs = strides[0], t.y_rs = strides[1], t.id_rs = strides[2], t.id_ps = strides[3], t.len_s = strides[4], t.gen_s = strides[5];
+    t.bid_rs = strides[6], t.b_rs = strides[7], t.mask_rs = strides[8];
+    t.M = M, t.V = V, t.L = L, t.nb = nb;
+    return launch_code(sq::launch_logit_rules(t, elem_bytes, workspace, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -42,7 +42,7 @@
 // hidden] output: the element-wise copies around the kernel cost three times its own time (8 prompts of 512 tokens, 32
 // heads of 128, per layer: six copies of 21 us and 35 -> 42 in all; without a table, against torch's attention and its
 // copies, 157 -> 59).
-#include "sq_common.h"
+#include "sq_attn_tile.h"
 #include "sq_kernels.h"
 
 #include <type_traits>
@@ -60,24 +60,6 @@ struct LutAttnArgs {
     float qk_scale;  // sm_scale * log2(e)
     float lazy;      // log2 of how far a score may exceed the reference maximum
 };
-
-// Chunk permutations inside a tile row of D halves (D / 8 chunks of 16 bytes).
-// K is read 128 bits wide by 32 lanes = rows at one chunk: 16 consecutive rows (256 bytes of LDS banks) must differ.
-template <int D>
-__device__ __forceinline__ int k_swz(int row) {
-    return D == 128 ? (row & 15) : ((row & 7) ^ ((row >> 3) & 1));
-}
-// V is read 64 bytes of a row by 8 lanes, four consecutive rows by a transposing read: the rows' 64-byte pieces must differ.
-template <int D>
-__device__ __forceinline__ int v_swz(int row) {
-    return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
-}
-
-typedef short short4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ short4_t lds_read_tr(const uint8_t* p) {
-    typedef __attribute__((address_space(3))) short4_t* lp;
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-}
 
 // KG = 1: two waves, steps of 32 keys.  KG = 2: four waves, steps of 64 keys, wave (qg, kg) on keys 32 kg .. + 31 of each
 // with a softmax state of its own; the two states of a query meet at the end.

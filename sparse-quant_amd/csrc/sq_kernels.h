@@ -145,6 +145,84 @@ hipError_t launch_kv4_attention(const Kv4Cache& c, const void* q, void* out, con
                                 int share, int count, long q_ts, long q_hs, float sm_scale, const void* k_new, const void* v_new,
                                 const long* new_strides, hipStream_t st);  // k_new: rows to store first, or null
 
+// sq_prefix_attn.hip: causal attention of a batch behind a shared prefix.  Tensors fp16, strides in elements.
+struct PrefixAttn {
+    const half_t* q;            // (token, head)
+    const half_t *kp, *vp;      // prefix (head, row)
+    half_t *kc, *vc;            // own rows (sequence, head, row)
+    const half_t *kn, *vn;      // the call's rows (token, head), stored first; null: they are in the cache
+    half_t* o;                  // [T][share * H][D]
+    const int *lengths, *starts;
+    long q_ts, q_hs, p_hs, p_rs, c_bs, c_hs, c_rs, n_ts, n_hs;
+    int T, B, H, share, P, Lmax, each;  // each: tokens of a sequence where starts is null
+};
+// How it is cut: packed rows against the prefix (a), tiles of a sequence against its rows, or the prefix and its rows (b).
+struct PrefixPlan {
+    float* po;  // partial outputs [H][parts][T * share][D], then (maximum, sum) of each
+    float2* pml;
+    int packed, qg, rows;                                  // rows of a tile: 32 qg
+    int tiles_a, parts_a, steps_a, tiles_b, parts_b, steps_b;  // steps of 64 keys of a part
+    int units_a, units_b, grid_a, grid_b;
+};
+size_t prefix_attention_workspace_bytes(int T, int B, int H, int share, int D, int P, int Lmax, bool ragged);
+hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, void* workspace, hipStream_t st);
+
+// sq_evict.hip: a cache that evicts by accumulated attention weight.
+struct EvictStep {
+    const half_t *q, *kn, *vn;  // (sequence, head)
+    half_t *kc, *vc;            // (sequence, head, row)
+    float* weight;              // [B][H][R]
+    int* position;              // [B][H][R]
+    const int* seen;            // [B]
+    half_t* o;                  // [B][share * H][D]
+    int* slot;                  // [B][H]
+    long q_bs, q_hs, n_bs, n_hs, c_bs, c_hs, c_rs;
+    int B, H, share, R, first, last;
+};
+size_t evict_attention_workspace_bytes(int B, int H, int share, int D, int R);
+hipError_t launch_evict_attention(const EvictStep& t, int D, float sm_scale, void* workspace, hipStream_t st);
+
+struct EvictKeep {
+    const half_t *k, *v;        // (sequence, head, row), S rows
+    const float* weight;        // (sequence, head), rows adjacent
+    const int* lengths;         // [B], or null: S each
+    half_t *kc, *vc;            // (sequence, head, row), R rows
+    float* cweight;             // [B][H][R]
+    int* cposition;             // [B][H][R]
+    int* rows;                  // [B][H][R]
+    long k_bs, k_hs, k_rs, w_bs, w_hs, c_bs, c_hs, c_rs;
+    int B, H, S, R, first, last;
+};
+hipError_t launch_evict_keep(const EvictKeep& t, int D, hipStream_t st);
+
+// sq_weigh.hip: the attention weight that a prompt's queries give to each of its keys.
+struct WeighArgs {
+    const half_t *q, *k;        // (sequence, head, row)
+    const int* lengths;         // [B], or null: S each
+    float* w;                   // [B][H][S]
+    long q_bs, q_hs, q_rs, k_bs, k_hs, k_rs;
+    int B, H, share, S, window;  // window: the last so many queries
+};
+size_t attention_weights_workspace_bytes(int B, int H, int share, int S, int window);
+hipError_t launch_attention_weights(const WeighArgs& t, int D, float sm_scale, void* workspace, hipStream_t st);
+
+// sq_logits.hip: penalties, biases and a mask on logits, and the best token.
+struct LogitRules {
+    const void* x;              // [M] rows of V, x_rs apart
+    void* y;
+    const long long* ids;       // (row, place)
+    const long long *lengths, *generated;  // by row, strides below
+    const float *repetition, *presence, *frequency;  // [M] each, or null
+    const int* bias_ids;        // [M] rows of nb, adjacent
+    const float* bias;
+    const unsigned* mask;       // [M] rows of words, mask_rs apart
+    long long* token;
+    long x_rs, y_rs, id_rs, id_ps, len_s, gen_s, bid_rs, b_rs, mask_rs;
+    int M, V, L, nb;
+};
+size_t logit_rules_workspace_bytes(int M, int V);
+hipError_t launch_logit_rules(const LogitRules& t, int elem_bytes, void* workspace, hipStream_t st);
+
 // sq_lm_head.hip: the ends of a greedy decode step around the W4A16 layers (the end-to-end harness).
 // out[r, :] = embed[tok[r], :] + pos_table[*pos + pos_offset, :] (fp16; indices clamped to their tables).
 hipError_t launch_embed_rows(const void* embed, const void* pos_table, const void* tok, const void* pos, long long pos_offset,

@@ -30,7 +30,7 @@ PROBES_PATH = os.path.join(PKG_ROOT, "libsq_probes.so")
 HIP_SOURCES = ["sq_api.hip", "sq_dequant.hip", "sq_repack.hip", "sq_quantize.hip", "sq_gemv2.hip", "sq_gemv_seq.hip", "sq_skinny.hip", "sq_skinny2.hip",
                "sq_skinny3.hip", "sq_gemm.hip", "sq_gemm2.hip", "sq_gemm_ring.hip", "sq_attn.hip", "sq_decode_attn.hip", "sq_layernorm.hip",
                "sq_lm_head.hip", "sq_kv4.hip", "sq_kv4_attn.hip",
-               "sq_kv4_chunk.hip"]
+               "sq_kv4_chunk.hip", "sq_prefix_attn.hip", "sq_evict.hip", "sq_weigh.hip", "sq_logits.hip"]
 PROBE_SOURCES = ["sq_probes.hip"]  # diagnostic kernels, a library of their own (include/sq_probes.h)
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
              # keep the compiler from forming packed-fp32 instructions
@@ -52,6 +52,9 @@ PER_FILE_FLAGS = {
     "sq_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "sq_kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "sq_kv4_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "sq_prefix_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "sq_evict.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "sq_weigh.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -65,6 +65,15 @@ SIGNATURES = {
     "sq_kv4_select_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
     "sq_kv4_select": (_i, [_vp] * 5 + [_i] * 11 + [ctypes.c_long, ctypes.c_long, _vp, ctypes.c_size_t, _vp]),
     "sq_kv4_copy_pages": (_i, [_vp] * 3 + [_i] * 3 + [ctypes.c_size_t, ctypes.c_size_t, _vp]),
+    "sq_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 8),
+    "sq_prefix_attention": (_i, [_vp] * 10 + [_i] * 7 + [_vp, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "sq_evict_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 5),
+    "sq_evict_attention": (_i, [_vp] * 10 + [_i] * 7 + [_vp, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "sq_attention_weights_workspace_bytes": (ctypes.c_size_t, [_i] * 5),
+    "sq_attention_weights": (_i, [_vp] * 4 + [_i] * 6 + [_vp, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "sq_evict_keep": (_i, [_vp] * 9 + [_i] * 7 + [_vp, _vp]),
+    "sq_logit_rules_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "sq_logit_rules": (_i, [_vp, _vp, _i] + [_vp] * 10 + [_i] * 4 + [_vp, _vp, ctypes.c_size_t, _vp]),
     "sq_embed_rows": (_i, [_vp, _vp, _vp, _vp, ctypes.c_longlong, _vp, _i, _i, ctypes.c_longlong, ctypes.c_longlong, _vp]),
     "sq_f16_gemv_parts": (_i, [_i]),
     "sq_f16_gemv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
