@@ -5,7 +5,7 @@
 // its own among them, and every row's weight grows by what the token's heads give it:
 //   P = softmax_j(scale q . k_j),  out = sum_j P_j v_j,  weight_j += sum over the query heads of the key/value head of P_j
 // The probabilities are known only behind the last row, so the scores wait in the workspace (4 bytes of a row's 512 at D = 128).
-#include "sq_attn_tile.h"
+#include "sq_attn_rows.h"
 #include "sq_kernels.h"
 
 #include <algorithm>
@@ -15,16 +15,15 @@ namespace sq {
 
 namespace {
 
-constexpr int EV_STEP = 64;   // rows of a step
-constexpr int EV_TILE = 32;   // query heads of a workgroup
-constexpr int EV_WAVES = 2;
+constexpr int EV_TILE = 32;  // query heads of a workgroup
 
 struct EvictArgs {
     EvictStep t;
     float* scores;  // [B][H][share][pitch], in units of log2
     float* po;      // [B][H][parts][share][D]
     float2* pml;    // [B][H][parts][share]
-    int pitch, parts, steps, tiles;
+    int pitch, parts, blocks, tiles;
+    Divisor by_parts, by_tiles, by_heads;
     float qk_scale;
 };
 
@@ -47,246 +46,102 @@ __device__ __forceinline__ uint64_t wave_min64(uint64_t v) {
 }
 
 template <int D>
-__global__ __launch_bounds__(64 * EV_WAVES, 1) void evict_attn_kernel(EvictArgs a) {
-    constexpr int ROW = D * 2;
-    constexpr int TILE = EV_STEP * ROW;
-    constexpr int SB = 2 * TILE;
-    constexpr int NK = D / 16;
-    constexpr int DT = D / 32;
-    constexpr int NL = TILE / 1024 / EV_WAVES;
-    constexpr int RPL = 1024 / ROW;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SB];
-    __shared__ uint64_t least[EV_WAVES];
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-
+__global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
+    typedef RowsAttn<D> R;
+    constexpr int CPR = R::CPR;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS];
+    __shared__ float2 stat[RA_WAVES * RA_BLOCK];
+    __shared__ uint64_t least[RA_WAVES];
     const EvictStep& t = a.t;
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 31, lc = lane >> 5;
-    const int part = blockIdx.x % a.parts;
-    const int tile = blockIdx.x / a.parts % a.tiles;
-    const int bh = blockIdx.x / a.parts / a.tiles;
-    const int b = bh / t.H, h = bh - b * t.H;
+    const int rest = a.by_parts(blockIdx.x);
+    const int part = blockIdx.x - rest * a.parts;
+    const int bh = a.by_tiles(rest);
+    const int tile = rest - bh * a.tiles;
+    const int b = a.by_heads(bh), h = bh - b * t.H;
     const int seen = t.seen[b];
     const int n = imin(seen, t.R);  // rows attended
-    const int s0 = part * a.steps;
-    const int s1 = imin(s0 + a.steps, ceil_div(n, EV_STEP));
-    if (s0 >= s1) return;  // (also where nothing was seen: the second launch writes zeros)
+    const int blk0 = part * a.blocks, blk1 = imin(blk0 + a.blocks, ceil_div(n, RA_BLOCK));
+    if (blk0 >= blk1) return;  // (also where nothing was seen: the second launch writes zeros)
 
     const int rows = imin(EV_TILE, t.share - tile * EV_TILE);
     const int g = tile * EV_TILE + imin(ln, rows - 1);
-    half8_t qf[NK];
-    {
-        const half_t* qp = t.q + (long)b * t.q_bs + (long)(h * t.share + g) * t.q_hs + 8 * lc;
-#pragma unroll
-        for (int s = 0; s < NK; s++) qf[s] = *(const half8_t*)(qp + 16 * s);
-    }
-    const long c_at = (long)b * t.c_bs + (long)h * t.c_hs;
-    const half_t* const kb = t.kc + c_at;
-    const half_t* const vb = t.vc + c_at;
-    const int rs = (int)t.c_rs * 2;
-    const int lrow = lane / (D / 8), lchunk = lane % (D / 8);
-    const int row_w = RPL * NL * wave + lrow;
-    auto issue = [&](int s, int slot) {
-        const int at = s * EV_STEP;
-        const uint8_t* const kbase = uniform((const uint8_t*)kb + (long)at * rs);
-        const uint8_t* const vbase = uniform((const uint8_t*)vb + (long)at * rs);
-        const uint32_t l0 = lds0 + slot * SB + wave * (NL * 1024);
-#pragma unroll
-        for (int j = 0; j < NL; j++) {  // rows past the end re-read the last one (their scores are masked)
-            const int r = row_w + RPL * j;
-            load_to_lds_x4(kbase, (uint32_t)(imin(r, n - 1 - at) * rs + ((lchunk ^ k_swz<D>(r)) * 16)), l0 + j * 1024);
-        }
-#pragma unroll
-        for (int j = 0; j < NL; j++) {
-            const int r = row_w + RPL * j;
-            load_to_lds_x4(vbase, (uint32_t)(imin(r, n - 1 - at) * rs + ((lchunk ^ v_swz<D>(r)) * 16)), l0 + TILE + j * 1024);
-        }
-    };
-    issue(s0, 0);
-
-    // The new row, a chunk of it per thread.
-    constexpr int CPR = D / 8;
-    const int chunk = tid % CPR;
+    R r;
+    r.load_query(t.q + (long)b * t.q_bs + (long)(h * t.share + g) * t.q_hs + 8 * lc);
+    // The new row, a chunk of it per lane.
+    const int chunk = lane % CPR;
     const long n_at = (long)b * t.n_bs + (long)h * t.n_hs + 8 * chunk;
-    u32x4_t fresh_k = *(const u32x4_t*)(t.kn + n_at);
-    u32x4_t fresh_v = *(const u32x4_t*)(t.vn + n_at);
+    const u32x4_t fresh_k = *(const u32x4_t*)(t.kn + n_at);
+    const u32x4_t fresh_v = *(const u32x4_t*)(t.vn + n_at);
     // Where it goes.
     int slot = seen - 1;
     if (seen > t.R) {
         const float* const w = t.weight + (long)bh * t.R;
         const int* const pos = t.position + (long)bh * t.R;
         uint64_t best = ~0ull;
-        for (int r = tid; r < t.R; r += 64 * EV_WAVES) {
-            const int p = pos[r];
-            const uint32_t o = p >= t.first && p < seen - t.last ? order_of(w[r]) : ~0u;
-            const uint64_t key = ((uint64_t)o << 32) | (uint32_t)r;
+#pragma unroll 4
+        for (int i = tid; i < t.R; i += 256) {
+            const int p = pos[i];
+            const uint32_t o = p >= t.first && p < seen - t.last ? order_of(w[i]) : ~0u;
+            const uint64_t key = ((uint64_t)o << 32) | (uint32_t)i;
             best = key < best ? key : best;
         }
         best = wave_min64(best);
         if (lane == 0) least[wave] = best;
         __syncthreads();
-        uint64_t v = least[0];
 #pragma unroll
-        for (int i = 1; i < EV_WAVES; i++) v = least[i] < v ? least[i] : v;
-        slot = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+        for (int i = 0; i < RA_WAVES; i++) best = least[i] < best ? least[i] : best;
+        slot = __builtin_amdgcn_readfirstlane((int)(uint32_t)best);
     }
-
-    int kread[NK], vread[DT];
-#pragma unroll
-    for (int s = 0; s < NK; s++) kread[s] = (32 * wave + ln) * ROW + (((2 * s + lc) ^ k_swz<D>(ln)) * 16);
-    {
-        const int key = 4 * lc + ((lane & 15) >> 2);
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-            vread[dt] = TILE + (32 * wave + key) * ROW + (((4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(key)) * 16) +
-                        8 * (lane & 1);
-    }
-
-    float ref = 0.f, top = -INFINITY, l_i = 0.f;
-    constexpr float LAZY = 8.f;
-    float16_t acc[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) acc[dt][v] = 0.f;
-    float* const scores = a.scores + ((long)bh * t.share + g) * a.pitch;
+    const long c_at = (long)b * t.c_bs + (long)h * t.c_hs;
+    float* const scores = a.scores + ((long)bh * t.share + g) * a.pitch + 4 * lc;
     const bool valid = ln < rows;
-
-    auto visit = [&](int s, auto slot_, bool more) {
-        constexpr int SLOT = decltype(slot_)::value;
-        uint8_t* l = lds + SLOT * SB;
-        const int at = s * EV_STEP;
-        const bool here = slot >= at && slot < at + EV_STEP;
-        if (here || at + EV_STEP > n) {
-            if (here) {  // the new row takes its place
-                const int r = slot - at;
-                if (tid < CPR) {
-                    *(u32x4_t*)(l + r * ROW + ((chunk ^ k_swz<D>(r)) * 16)) = fresh_k;
-                    *(u32x4_t*)(l + TILE + r * ROW + ((chunk ^ v_swz<D>(r)) * 16)) = fresh_v;
-                    if (tile == 0) {
-                        *(u32x4_t*)(t.kc + c_at + (long)slot * t.c_rs + 8 * chunk) = fresh_k;
-                        *(u32x4_t*)(t.vc + c_at + (long)slot * t.c_rs + 8 * chunk) = fresh_v;
-                    }
-                }
-                if (tid == 0 && tile == 0) t.slot[bh] = slot;
+    r.template run<true>(
+        lds, blk0 + wave, blk1, a.qk_scale,
+        [&](int blk, bool value, uint32_t at) {
+            const half_t* const base = (value ? t.vc : t.kc) + c_at;
+            const int first = blk * RA_BLOCK;
+            if (first + RA_BLOCK <= n)
+                R::request((const uint8_t*)(base + (long)first * t.c_rs), (uint32_t)t.c_rs * 2, value, at);
+            else  // rows past the end re-read the last one
+                R::request_each(value, at, [&](int i) { return base + (long)imin(first + i, n - 1) * t.c_rs; });
+        },
+        [&](int blk, int& first, int& full, int& last) {
+            first = blk * RA_BLOCK;
+            full = n;
+            last = n - 1;
+        },
+        [&](int blk, uint8_t* tile_at) {
+            const int i = slot - blk * RA_BLOCK;
+            if (i >= 0 && i < RA_BLOCK && lane < CPR) {  // the new row takes its place
+                R::put(tile_at, false, i, chunk, fresh_k);
+                if (tile == 0) *(u32x4_t*)(t.kc + c_at + (long)slot * t.c_rs + 8 * chunk) = fresh_k;
+                if (tile == 0 && lane == 0) t.slot[bh] = slot;
             }
-            // values behind the last row meet probabilities of 0: they must be numbers
-            for (int i = imax(n - at, 0) + tid / CPR; i < EV_STEP; i += 64 * EV_WAVES / CPR)
-                *(u32x4_t*)(l + TILE + i * ROW + ((chunk ^ v_swz<D>(i)) * 16)) = (u32x4_t){0u, 0u, 0u, 0u};
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        if (more) issue(s + 1, 1 - SLOT);
-        __builtin_amdgcn_sched_barrier(0);
-        float16_t st;
-#pragma unroll
-        for (int v = 0; v < 16; v++) st[v] = 0.f;
-        half8_t kf[NK];
-#pragma unroll
-        for (int i = 0; i < NK; i++) kf[i] = *(const half8_t*)(l + kread[i]);
-#pragma unroll
-        for (int i = 0; i < NK; i++) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qf[i], st, 0, 0, 0);
-        const int k0 = at + 32 * wave + 4 * lc;
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const int key = k0 + 8 * (v >> 2) + (v & 3);
-            st[v] = key < n ? st[v] * a.qk_scale : -INFINITY;
-        }
-        if (valid) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                *(float4_t*)(scores + k0 + 8 * i) = (float4_t){st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]};
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            st[v] -= ref;
-            mx = fmaxf(mx, st[v]);
-        }
-        if (__builtin_amdgcn_ballot_w64(mx > top) != 0) {
-            const float mq = fmaxf(mx, __shfl_xor(mx, 32));
-            const bool upd = mq > top;
-            const float delta = upd ? mq : 0.f;
-            const float alpha = (upd && top != -INFINITY) ? __builtin_amdgcn_exp2f(-delta) : 1.f;
-            ref += delta;
-            top = upd ? LAZY : top;
-            l_i *= alpha;
-#pragma unroll
-            for (int v = 0; v < 16; v++) st[v] -= delta;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) acc[dt][v] *= alpha;
-        }
-        // The sum is that of the unrounded exponentials: the weights are divided by it and keep 32 bits.
-        half8_t pk[2];
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const float p = __builtin_amdgcn_exp2f(st[v]);
-            l_i += p;
-            pk[v >> 3][v & 7] = (half_t)p;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const u32x2_t lo = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + 16 * i * ROW));
-                const u32x2_t hi = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + (16 * i + 8) * ROW));
-                u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(vt), pk[i], acc[dt], 0, 0, 0);
+        },
+        [&](int blk, uint8_t* tile_at) {
+            const int i = slot - blk * RA_BLOCK;
+            if (i >= 0 && i < RA_BLOCK && lane < CPR) {
+                R::put(tile_at, true, i, chunk, fresh_v);
+                if (tile == 0) *(u32x4_t*)(t.vc + c_at + (long)slot * t.c_rs + 8 * chunk) = fresh_v;
             }
-    };
-    auto landed = []() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+            const int past = n - blk * RA_BLOCK;
+            if (past < RA_BLOCK) R::clear_from(tile_at, past);
+        },
+        [&](int blk, const float16_t& st) {
+            if (valid) {
 #pragma unroll
-    for (int s = 0; s < NK; s++) {
-        u32x4_t x = bit_cast<u32x4_t>(qf[s]);
-        asm volatile("" : "+v"(x));
-        qf[s] = bit_cast<half8_t>(x);
-    }
-    asm volatile("" : "+v"(fresh_k), "+v"(fresh_v));
-    for (int s = s0; s < s1; s += 2) {
-        landed();
-        visit(s, std::integral_constant<int, 0>{}, s + 1 < s1);
-        if (s + 1 >= s1) break;
-        landed();
-        visit(s + 1, std::integral_constant<int, 1>{}, s + 2 < s1);
-    }
-
-    l_i += __shfl_xor(l_i, 32);
-    float m_i = top == -INFINITY ? -INFINITY : ref;
-    __syncthreads();
-    constexpr int OWN = DT / 2;
-    float4_t* red = reinterpret_cast<float4_t*>(lds);                       // [wave][OWN][4][64]
-    float2* stat = reinterpret_cast<float2*>(lds + EV_WAVES * OWN * 4096);  // [wave][64]
-#pragma unroll
-    for (int d = 0; d < OWN; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float4_t x;
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = wave == 0 ? acc[OWN + d][4 * i + j] : acc[d][4 * i + j];
-            red[((wave * OWN + d) * 4 + i) * 64 + lane] = x;
-        }
-    stat[wave * 64 + lane] = make_float2(m_i, l_i);
-    __syncthreads();
-    const float2 ps = stat[(wave ^ 1) * 64 + lane];
-    const float mm = fmaxf(m_i, ps.x);
-    const float w_own = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - mm);
-    const float w_peer = ps.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ps.x - mm);
-    if (!valid) return;
-    const long slot_at = ((long)bh * a.parts + part) * t.share + g;
-#pragma unroll
-    for (int d = 0; d < OWN; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4_t o = red[(((wave ^ 1) * OWN + d) * 4 + i) * 64 + lane];
-            float4_t x;
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = (wave == 0 ? acc[d][4 * i + j] : acc[OWN + d][4 * i + j]) * w_own + o[j] * w_peer;
-            *(float4_t*)(a.po + slot_at * D + 32 * (d + wave * OWN) + 8 * i + 4 * lc) = x;
-        }
-    if (lc == 0 && wave == 0) a.pml[slot_at] = make_float2(mm, l_i * w_own + ps.y * w_peer);
+                for (int i = 0; i < 4; i++)
+                    *(float4_t*)(scores + blk * RA_BLOCK + 8 * i) = (float4_t){st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]};
+            }
+        });
+    r.join(lds, stat, rows, [&](int i, int col, float4_t o, float m, float l) {
+        const long at = ((long)bh * a.parts + part) * t.share + tile * EV_TILE + i;
+        *(float4_t*)(a.po + at * D + col) = o;
+        if (col == 0) a.pml[at] = make_float2(m, l);
+    });
 }
 
 // The parts of a (sequence, key/value head): its outputs (first chunk of rows), and the weights of a chunk of rows.
@@ -309,7 +164,7 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
         if (tid == 0) t.slot[bh] = -1;
         return;
     }
-    const int parts = ceil_div(ceil_div(n, EV_STEP), a.steps);
+    const int parts = ceil_div(ceil_div(n, RA_BLOCK), a.blocks);
     float acc[EJ_ROWS / 256];
 #pragma unroll
     for (int i = 0; i < EJ_ROWS / 256; i++) acc[i] = 0.f;
@@ -322,7 +177,7 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
             for (int s = 0; s < parts; s++) m = fmaxf(m, ml[(long)s * t.share].x);
             for (int s = 0; s < parts; s++) {
                 const float2 x = ml[(long)s * t.share];
-                l += x.x == -INFINITY ? 0.f : x.y * __builtin_amdgcn_exp2f(x.x - m);
+                l += x.y * share_of(x, m);
             }
             state[g] = make_float2(m, 1.f / l);
         }
@@ -343,9 +198,7 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
                 for (int c = lane; c < D; c += 64) {
                     float o = 0.f;
                     for (int s = 0; s < parts; s++) {
-                        const float m = a.pml[at + (long)s * t.share].x;
-                        const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - st.x);
-                        o += a.po[(at + (long)s * t.share) * D + c] * w;
+                        o += a.po[(at + (long)s * t.share) * D + c] * share_of(a.pml[at + (long)s * t.share], st.x);
                     }
                     out[(g0 + g) * D + c] = (half_t)(o * st.y);
                 }
@@ -369,12 +222,16 @@ constexpr int EV_WGS = 512;
 
 EvictArgs plan(int B, int H, int share, int R) {
     EvictArgs a = {};
-    a.pitch = (R + 63) / 64 * 64;
+    a.pitch = (R + 31) / 32 * 32;
     a.tiles = (share + EV_TILE - 1) / EV_TILE;
     const long units = (long)B * H * a.tiles;
-    const int steps = a.pitch / 64;
-    a.steps = (int)std::max<long>((units * steps + EV_WGS - 1) / EV_WGS, 1);
-    a.parts = (steps + a.steps - 1) / a.steps;
+    const int rounds = (a.pitch / RA_BLOCK + RA_WAVES - 1) / RA_WAVES;  // of the waves over the rows
+    const int each = (int)std::max<long>((units * rounds + EV_WGS - 1) / EV_WGS, 1);
+    a.blocks = each * RA_WAVES;
+    a.parts = (rounds + each - 1) / each;
+    a.by_parts = Divisor::of(a.parts);
+    a.by_tiles = Divisor::of(a.tiles);
+    a.by_heads = Divisor::of(H);
     return a;
 }
 
@@ -505,10 +362,10 @@ hipError_t launch_evict_attention(const EvictStep& t, int D, float sm_scale, voi
     a.pml = (float2*)(a.po + (size_t)t.B * t.H * t.share * a.parts * D);
     const dim3 grid(t.B * t.H * a.tiles * a.parts), join(t.B * t.H, (t.R + EJ_ROWS - 1) / EJ_ROWS);
     if (D == 64) {
-        hipLaunchKernelGGL((evict_attn_kernel<64>), grid, dim3(64 * EV_WAVES), 0, st, a);
+        hipLaunchKernelGGL((evict_attn_kernel<64>), grid, dim3(256), 0, st, a);
         hipLaunchKernelGGL((evict_join_kernel<64>), join, dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((evict_attn_kernel<128>), grid, dim3(64 * EV_WAVES), 0, st, a);
+        hipLaunchKernelGGL((evict_attn_kernel<128>), grid, dim3(256), 0, st, a);
         hipLaunchKernelGGL((evict_join_kernel<128>), join, dim3(256), 0, st, a);
     }
     return hipGetLastError();

@@ -156,14 +156,6 @@ struct PrefixAttn {
     long q_ts, q_hs, p_hs, p_rs, c_bs, c_hs, c_rs, n_ts, n_hs;
     int T, B, H, share, P, Lmax, each;  // each: tokens of a sequence where starts is null
 };
-// How it is cut: packed rows against the prefix (a), tiles of a sequence against its rows, or the prefix and its rows (b).
-struct PrefixPlan {
-    float* po;  // partial outputs [H][parts][T * share][D], then (maximum, sum) of each
-    float2* pml;
-    int packed, qg, rows;                                  // rows of a tile: 32 qg
-    int tiles_a, parts_a, steps_a, tiles_b, parts_b, steps_b;  // steps of 64 keys of a part
-    int units_a, units_b, grid_a, grid_b;
-};
 size_t prefix_attention_workspace_bytes(int T, int B, int H, int share, int D, int P, int Lmax, bool ragged);
 hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, void* workspace, hipStream_t st);
 

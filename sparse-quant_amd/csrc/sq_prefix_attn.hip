@@ -9,7 +9,7 @@
 // belong to, are packed into tiles and meet the prefix as one dense product without masks; each sequence's rows meet its own
 // cache apart; a second launch joins the parts.  Where a sequence has many rows itself (a prompt) nothing is gained by packing:
 // its tiles go through the prefix and on through their own rows, and write the result.
-#include "sq_attn_tile.h"
+#include "sq_attn_rows.h"
 #include "sq_kernels.h"
 
 #include <algorithm>
@@ -21,6 +21,16 @@ namespace {
 
 constexpr int PA_STEP = 64;  // keys of a step
 
+// How a call is cut: packed rows against the prefix (a), tiles of a sequence against its rows, or the prefix and its rows (b).
+struct PrefixPlan {
+    float* po;  // partial outputs [H][parts][T * share][D], then (maximum, sum) of each
+    float2* pml;
+    int packed, qa, qb, rows_b;                                // tiles of 32 qa and 32 qb rows
+    int tiles_a, parts_a, steps_a, tiles_b, parts_b, steps_b;  // steps of 64 keys of a part
+    int units_a, units_b, grid_a, grid_b;
+    Divisor by_share, by_tiles_a, by_parts_a, by_tiles_b, by_parts_b;
+};
+
 struct PrefixArgs {
     PrefixAttn t;
     PrefixPlan p;
@@ -29,11 +39,6 @@ struct PrefixArgs {
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
-
-// All bits of the halves of a word that are infinities or NaN.
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
-}
 
 // Tokens of sequence b of the call: [first, first + count), whatever `starts` holds inside [0, T].
 __device__ __forceinline__ void tokens_of(const PrefixAttn& t, int b, int& first, int& count) {
@@ -106,155 +111,209 @@ struct Reach {
 __device__ __forceinline__ Reach reach_of(const PrefixAttn& t, const PrefixPlan& p, const Tile& tl) {
     Reach r;
     r.before = imax(t.lengths[tl.b], 0) - tl.count;
-    const int row0 = tl.tile * p.rows;
-    const int row1 = imin(row0 + p.rows, tl.count * t.share) - 1;
-    r.own = imin(imax(r.before + row1 / t.share + 1, 0), t.Lmax);
-    r.own_first = imin(imax(r.before + row0 / t.share + 1, 0), t.Lmax);
+    const int row0 = tl.tile * p.rows_b;
+    const int row1 = imin(row0 + p.rows_b, tl.count * t.share) - 1;
+    r.own = imin(imax(r.before + p.by_share(row1) + 1, 0), t.Lmax);
+    r.own_first = imin(imax(r.before + p.by_share(row0) + 1, 0), t.Lmax);
     r.pre_steps = p.packed ? 0 : ceil_div(t.P, PA_STEP);
     r.steps = r.pre_steps + ceil_div(r.own, PA_STEP);
     return r;
 }
 
-// QG groups of 32 rows, KG groups of keys: wave (qg, kg) has rows 32 qg .. + 31 and a KG-th of the keys of a step.
-template <int D, int QG, int KG>
-__global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_kernel(PrefixArgs a) {
-    constexpr int NW = QG * KG;
+// A piece of work: rows of a key/value head against a range of steps.
+struct Work {
+    int head, part, row0, rows;  // rows row0 .. row0 + rows - 1 of the head's T * share
+    int s0, s1;                  // steps
+    bool shared;                 // against the prefix alone
+    Tile tl;
+    Reach rc;
+};
+
+__device__ __forceinline__ const half_t* prefix_row(const PrefixAttn& t, const Work& w, bool value, int key) {
+    return (value ? t.vp : t.kp) + (long)w.head * t.p_hs + (long)key * t.p_rs;
+}
+__device__ __forceinline__ const half_t* cache_row(const PrefixAttn& t, const Work& w, bool value, int key) {
+    return (value ? t.vc : t.kc) + (long)w.tl.b * t.c_bs + (long)w.head * t.c_hs + (long)key * t.c_rs;
+}
+// Own rows from here on are the call's: they are taken from there, other workgroups are storing them to the cache.
+__device__ __forceinline__ int fresh_from(const PrefixAttn& t, const Work& w) { return t.kn ? w.rc.before : t.Lmax; }
+__device__ __forceinline__ const half_t* own_row(const PrefixAttn& t, const Work& w, bool value, int key) {
+    const int fresh = fresh_from(t, w);
+    if (key >= fresh) return (value ? t.vn : t.kn) + (long)(w.tl.first + key - fresh) * t.n_ts + (long)w.head * t.n_hs;
+    return cache_row(t, w, value, key);
+}
+
+// Infinities and NaN among the values must reach the rows that see them and no others, and 0 times them is no 0: in steps
+// with a causal mask they count as 0 in the product, and are added behind the last step to the rows that see them.
+template <int D>
+__device__ __forceinline__ bool clear_odd(uint8_t* tile, int rows, int first, int stride) {
+    bool odd = false;
+#pragma unroll 1
+    for (int i = first; i < rows * (D / 8); i += stride) {
+        half8_t x = *(half8_t*)(tile + i * 16);
+        bool any = false;
+#pragma unroll
+        for (int v = 0; v < 8; v++) {
+            const bool finite = __builtin_fabsf((float)x[v]) <= 65504.f;
+            any |= !finite;
+            x[v] = finite ? x[v] : (half_t)0.f;
+        }
+        if (any) *(half8_t*)(tile + i * 16) = x;
+        odd |= any;
+    }
+    return odd;
+}
+template <int D>
+__device__ __forceinline__ void add_odd(const PrefixAttn& t, const Work& w, int last, float16_t (&acc)[D / 32]) {
+    const int lc = (threadIdx.x & 63) >> 5;
+    const int k0 = imax(imax(w.s0 - w.rc.pre_steps, 0) * PA_STEP, w.rc.own_first / PA_STEP * PA_STEP);
+    const int k1 = imin((w.s1 - w.rc.pre_steps) * PA_STEP, w.rc.own);
+#pragma unroll 1
+    for (int key = k0; key < k1; key++) {
+        const half_t* const v = own_row(t, w, true, key) + 4 * lc;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const half4_t h = *(const half4_t*)(v + 32 * dt + 8 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    acc[dt][4 * i + j] += key <= last && !(__builtin_fabsf((float)h[j]) <= 65504.f) ? (float)h[j] : 0.f;
+            }
+    }
+}
+
+// Four columns of a row's sums: the result, or a part of it.
+template <int D>
+__device__ __forceinline__ void store_row(const PrefixArgs& a, const Work& w, int row, int col, float4_t o, float m, float l) {
+    const PrefixAttn& t = a.t;
+    const PrefixPlan& p = a.p;
+    if (p.parts_a + p.parts_b == 1) {
+        const int token = p.by_share(row);
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: 0
+        half4_t h;
+#pragma unroll
+        for (int j = 0; j < 4; j++) h[j] = (half_t)(o[j] * inv);
+        *(half4_t*)(t.o + ((long)token * (t.H * t.share) + w.head * t.share + row - token * t.share) * D + col) = h;
+    } else {
+        const long slot = ((long)w.head * (p.parts_a + p.parts_b) + w.part) * ((long)t.T * t.share) + row;
+        *(float4_t*)(p.po + slot * D + col) = o;
+        if (col == 0) p.pml[slot] = make_float2(m, l);
+    }
+}
+
+// Up to 32 rows: the waves go round the keys.
+template <int D>
+__device__ __forceinline__ void few_rows(const PrefixArgs& a, const Work& w, uint8_t* lds, float2* stat) {
+    typedef RowsAttn<D> R;
+    const PrefixAttn& t = a.t;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = w.row0 + imin(lane & 31, w.rows - 1);
+    const int token = a.p.by_share(row);
+    R r;
+    r.load_query(t.q + (long)token * t.q_ts + (long)(w.head * t.share + row - token * t.share) * t.q_hs + 8 * (lane >> 5));
+    const int limit = imin(w.rc.before + token - w.tl.first, t.Lmax - 1);  // the last own row that it sees
+    const int pre = w.shared ? 2 * w.s1 : 2 * w.rc.pre_steps;              // blocks of the prefix
+    const int plain_own = imin(w.rc.own, fresh_from(t, w));
+    const int end = imin(2 * w.s1, w.shared ? ceil_div(t.P, RA_BLOCK) : pre + ceil_div(w.rc.own, RA_BLOCK));
+    bool odd = false;
+    r.template run<false>(
+        lds, 2 * w.s0 + wave, end, a.qk_scale,
+        [&](int blk, bool value, uint32_t at) {
+            const bool is_pre = blk < pre;
+            const int n = (is_pre ? blk : blk - pre) * RA_BLOCK;
+            if (n + RA_BLOCK <= (is_pre ? t.P : plain_own))
+                R::request((const uint8_t*)(is_pre ? prefix_row(t, w, value, n) : cache_row(t, w, value, n)),
+                           (uint32_t)(is_pre ? t.p_rs : t.c_rs) * 2, value, at);
+            else
+                R::request_each(value, at, [&](int i) {  // rows past the end re-read the last one
+                    return is_pre ? prefix_row(t, w, value, imin(n + i, t.P - 1)) : own_row(t, w, value, imin(n + i, w.rc.own - 1));
+                });
+        },
+        [&](int blk, int& n, int& full, int& last) {
+            const bool is_pre = blk < pre;
+            n = (is_pre ? blk : blk - pre) * RA_BLOCK;
+            full = is_pre ? t.P : w.rc.own_first;
+            last = is_pre ? t.P - 1 : limit;
+        },
+        [](int, uint8_t*) {},
+        [&](int blk, uint8_t* tile) {
+            const bool is_pre = blk < pre;
+            const int n = (is_pre ? blk : blk - pre) * RA_BLOCK;
+            const int past = (is_pre ? t.P : w.rc.own) - n;
+            if (past < RA_BLOCK) R::clear_from(tile, imax(past, 0));
+            if (!is_pre && n + RA_BLOCK > w.rc.own_first && w.rc.own_first < w.rc.own) odd |= clear_odd<D>(tile, RA_BLOCK, lane, 64);
+        },
+        [](int, const float16_t&) {});
+    if (!w.shared && w.rc.own_first < w.rc.own && __syncthreads_or(odd) && wave == 0) add_odd<D>(t, w, limit, r.acc);
+    r.join(lds, stat, w.rows, [&](int i, int col, float4_t o, float m, float l) { store_row<D>(a, w, w.row0 + i, col, o, m, l); });
+}
+
+// 32 QG rows: wave (qg, kg) has rows 32 qg .. + 31 and a KG-th of the keys of a step; the steps' tiles are shared, in two stages.
+template <int D, int QG>
+__device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, uint8_t* lds) {
+    constexpr int KG = 4 / QG;
     constexpr int KS = PA_STEP / (32 * KG);  // 32-key blocks of a wave and step
     constexpr int ROW = D * 2;               // bytes of a tile row
     constexpr int TILE = PA_STEP * ROW;
     constexpr int SB = 2 * TILE;             // a stage: K tile, V tile
     constexpr int NK = D / 16;
     constexpr int DT = D / 32;
-    constexpr int NL = TILE / 1024 / NW;     // direct loads per wave, operand and stage
+    constexpr int NL = TILE / 1024 / 4;      // direct loads per wave, operand and stage
     constexpr int RPL = 1024 / ROW;          // tile rows per load
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SB];
+    constexpr int CPR = D / 8;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-
     const PrefixAttn& t = a.t;
-    const PrefixPlan& p = a.p;
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 31, lc = lane >> 5;
     const int qg = wave / KG, kg = wave % KG;
-
-    // ---- which piece of work this is
-    int index = blockIdx.x;
-    int head, part, row0, rows, s0, s1;  // rows row0 .. row0 + rows - 1 of the head's T * share; steps s0 .. s1 - 1
-    Tile tl = {0, 0, 0, 0};
-    Reach rc = {0, 0, 0, 0, 0};
-    const bool shared = index < p.grid_a;
-    if (shared) {
-        const int per = p.grid_a >> 3;
-        const int work = (index & 7) * per + (index >> 3);  // an eighth of the list per XCD: a prefix piece's tiles share an L2
-        if (work >= p.units_a) return;
-        const int tile = work % p.tiles_a;
-        part = work / p.tiles_a % p.parts_a;
-        head = work / p.tiles_a / p.parts_a;
-        row0 = tile * p.rows;
-        rows = imin(p.rows, t.T * t.share - row0);
-        s0 = part * p.steps_a;
-        s1 = imin(s0 + p.steps_a, ceil_div(t.P, PA_STEP));
-    } else if ((index -= p.grid_a) < p.grid_b) {
-        const int per = p.grid_b >> 3;
-        const int work = (index & 7) * per + (index >> 3);
-        if (work >= p.units_b) return;
-        const int b_part = work / p.tiles_b % p.parts_b;
-        head = work / p.tiles_b / p.parts_b;
-        if (!tile_of(t, p.rows, p.tiles_b - 1 - work % p.tiles_b, tl)) return;
-        rc = reach_of(t, p, tl);
-        row0 = tl.first * t.share + tl.tile * p.rows;
-        rows = imin(p.rows, tl.count * t.share - tl.tile * p.rows);
-        s0 = b_part * p.steps_b;
-        s1 = imin(s0 + p.steps_b, rc.steps);
-        if (s0 >= s1 && b_part > 0) return;  // (the first part also stands for rows that see nothing)
-        part = p.parts_a + b_part;
-    } else {
-        // the call's own rows into the cache, a token per wave
-        index -= p.grid_b;
-        const int token = index * NW + wave;
-        if (token >= t.T) return;
-        const int b = sequence_of(t, token);
-        if (b < 0) return;
-        int first, count;
-        tokens_of(t, b, first, count);
-        const int at = t.lengths[b] - count + token - first;
-        if (at < 0 || at >= t.Lmax) return;
-        constexpr int CPR = D / 8;
-        for (int i = lane; i < t.H * CPR; i += 64) {
-            const int h = i / CPR, c = 8 * (i % CPR);
-            const long from = (long)token * t.n_ts + (long)h * t.n_hs + c;
-            const long to = (long)b * t.c_bs + (long)h * t.c_hs + (long)at * t.c_rs + c;
-            *(u32x4_t*)(t.kc + to) = *(const u32x4_t*)(t.kn + from);
-            *(u32x4_t*)(t.vc + to) = *(const u32x4_t*)(t.vn + from);
-        }
-        return;
-    }
-
-    const bool idle = 32 * qg >= rows;  // (a sequence's tile may be shorter than the workgroup's)
-    const int row = row0 + imin(32 * qg + ln, rows - 1);
-    const int token = row / t.share;
-    const int qhead = head * t.share + row - token * t.share;
-    const int limit = imin(rc.before + token - tl.first, t.Lmax - 1);  // the last own row that it sees
-    // own rows from here on come from the call's rows, not from the cache, which other workgroups are storing them to
-    const int fresh = t.kn ? rc.before : t.Lmax;
-
+    const bool idle = 32 * qg >= w.rows;
+    const int row = w.row0 + imin(32 * qg + ln, w.rows - 1);
+    const int token = a.p.by_share(row);
+    const int limit = imin(w.rc.before + token - w.tl.first, t.Lmax - 1);
     half8_t qf[NK];
     {
-        const half_t* qp = t.q + (long)token * t.q_ts + (long)qhead * t.q_hs + 8 * lc;
+        const half_t* qp = t.q + (long)token * t.q_ts + (long)(w.head * t.share + row - token * t.share) * t.q_hs + 8 * lc;
 #pragma unroll
         for (int s = 0; s < NK; s++) qf[s] = *(const half8_t*)(qp + 16 * s);
     }
-
-    const half_t* const kp = t.kp + (long)head * t.p_hs;
-    const half_t* const vp = t.vp + (long)head * t.p_hs;
-    const long own_at = (long)tl.b * t.c_bs + (long)head * t.c_hs;
-    const half_t* const ko = t.kc + own_at;
-    const half_t* const vo = t.vc + own_at;
-    const long new_at = (long)tl.first * t.n_ts + (long)head * t.n_hs;
-
-    const int pre_steps = shared ? s1 : rc.pre_steps;
-    const int lrow = lane / (D / 8), lchunk = lane % (D / 8);
+    const int pre_steps = w.shared ? w.s1 : w.rc.pre_steps;
+    const int plain_own = imin(w.rc.own, fresh_from(t, w));
+    const int lrow = lane / CPR, lchunk = lane % CPR;
     const int row_w = RPL * NL * wave + lrow;  // of this lane's first load in the tile
-    auto issue = [&](int s, int slot) {
+    auto issue = [&](int s, uint32_t stage) {
         const bool pre = s < pre_steps;
         const int n = (pre ? s : s - pre_steps) * PA_STEP;
-        const int end = pre ? t.P : rc.own;
-        const int rs = (int)(pre ? t.p_rs : t.c_rs) * 2;
-        const half_t* const kb = pre ? kp : ko;
-        const half_t* const vb = pre ? vp : vo;
-        const uint32_t l0 = lds0 + slot * SB + wave * (NL * 1024);
-        if (n + PA_STEP <= (pre ? end : imin(end, fresh))) {
-            const uint8_t* const kbase = uniform((const uint8_t*)kb + (long)n * rs);
-            const uint8_t* const vbase = uniform((const uint8_t*)vb + (long)n * rs);
+        const uint32_t l0 = lds0 + stage + wave * (NL * 1024);
+        if (n + PA_STEP <= (pre ? t.P : plain_own)) {
+            const uint32_t rs = (uint32_t)(pre ? t.p_rs : t.c_rs) * 2;
+            const uint8_t* const kb = uniform((const uint8_t*)(pre ? prefix_row(t, w, false, n) : cache_row(t, w, false, n)));
+            const uint8_t* const vb = uniform((const uint8_t*)(pre ? prefix_row(t, w, true, n) : cache_row(t, w, true, n)));
+            uint32_t off = row_w * rs;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int r = row_w + RPL * j;
-                load_to_lds_x4(kbase, (uint32_t)(r * rs + ((lchunk ^ k_swz<D>(r)) * 16)), l0 + j * 1024);
+                load_to_lds_x4(kb, off + ((lchunk ^ k_swz<D>(r)) * 16), l0 + j * 1024);
+                load_to_lds_x4(vb, off + ((lchunk ^ v_swz<D>(r)) * 16), l0 + TILE + j * 1024);
+                off += RPL * rs;
             }
-#pragma unroll
+        } else {  // rows past the end re-read the last one
+#pragma unroll 1
             for (int j = 0; j < NL; j++) {
                 const int r = row_w + RPL * j;
-                load_to_lds_x4(vbase, (uint32_t)(r * rs + ((lchunk ^ v_swz<D>(r)) * 16)), l0 + TILE + j * 1024);
-            }
-        } else {  // rows past the end re-read the last one (their scores are masked)
-#pragma unroll
-            for (int j = 0; j < NL; j++) {
-                const int r = row_w + RPL * j;
-                const int key = imin(n + r, end - 1);
-                const bool is_new = !pre && key >= fresh;
-                const uint8_t* const kr = is_new ? (const uint8_t*)(t.kn + new_at + (long)(key - fresh) * t.n_ts)
-                                                 : (const uint8_t*)kb + (long)key * rs;
-                const uint8_t* const vr = is_new ? (const uint8_t*)(t.vn + new_at + (long)(key - fresh) * t.n_ts)
-                                                 : (const uint8_t*)vb + (long)key * rs;
-                load_to_lds_x4(kr + (lchunk ^ k_swz<D>(r)) * 16, l0 + j * 1024);
-                load_to_lds_x4(vr + (lchunk ^ v_swz<D>(r)) * 16, l0 + TILE + j * 1024);
+                const int key = imin(n + r, (pre ? t.P : w.rc.own) - 1);
+                const half_t* const k = pre ? prefix_row(t, w, false, key) : own_row(t, w, false, key);
+                const half_t* const v = pre ? prefix_row(t, w, true, key) : own_row(t, w, true, key);
+                load_to_lds_x4((const uint8_t*)k + ((lchunk ^ k_swz<D>(r)) * 16), l0 + j * 1024);
+                load_to_lds_x4((const uint8_t*)v + ((lchunk ^ v_swz<D>(r)) * 16), l0 + TILE + j * 1024);
             }
         }
     };
-    if (s0 < s1) issue(s0, 0);
+    if (w.s0 < w.s1) issue(w.s0, 0);
 
-    // LDS byte offsets of the operand reads.
+    // LDS byte offsets of the operand reads (of the other stage: with SB flipped).
     int kread[NK], vread[DT];
 #pragma unroll
     for (int s = 0; s < NK; s++) kread[s] = (32 * KS * kg + ln) * ROW + (((2 * s + lc) ^ k_swz<D>(ln)) * 16);
@@ -268,26 +327,37 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
 
     // Reference maximum of the row (0 while unset), the score above it at which it moves (any score while unset), and
     // this lane's share of the row sum.
-    constexpr float LAZY = 8.f;
     float ref = 0.f, top = -INFINITY, l_i = 0.f;
     float16_t acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[dt][v] = 0.f;
-
-    // Keys 16 i .. + 15 of this wave's, columns 32 dt .. + 31.
-    auto values = [&](const uint8_t* l, int i, int dt) {
-        const u32x2_t lo = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + 16 * i * ROW));
-        const u32x2_t hi = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + (16 * i + 8) * ROW));
-        return (u32x4_t){lo.x, lo.y, hi.x, hi.y};
-    };
-    auto visit = [&](int s, auto slot_, bool more) {
-        constexpr int SLOT = decltype(slot_)::value;
-        const uint8_t* l = lds + SLOT * SB;
-        if (more) issue(s + 1, 1 - SLOT);
-        if (idle) return;
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+        u32x4_t x = bit_cast<u32x4_t>(qf[s]);
+        asm volatile("" : "+v"(x));
+        qf[s] = bit_cast<half8_t>(x);
+    }
+    bool odd = false;
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (int s = w.s0; s < w.s1; s++, stage ^= SB) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + 1 < w.s1) issue(s + 1, stage ^ SB);
+        const bool pre = s < pre_steps;
+        const int n = (pre ? s : s - pre_steps) * PA_STEP;
+        // Masks (only where the step touches the end of the rows or the causal diagonal; the test is uniform).
+        const bool masked = n + PA_STEP > (pre ? t.P : w.rc.own_first);
+        if (masked) {
+            uint8_t* const vt = lds + stage + TILE;
+            for (int i = imax((pre ? t.P : w.rc.own) - n, 0) * CPR + tid; i < PA_STEP * CPR; i += 256)
+                *(u32x4_t*)(vt + i * 16) = (u32x4_t){0u, 0u, 0u, 0u};
+            if (!pre) odd |= clear_odd<D>(vt, imin(w.rc.own - n, PA_STEP), tid, 256);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        if (idle) continue;
+        const uint8_t* const l = lds + stage;
         float16_t st[KS];
 #pragma unroll
         for (int b = 0; b < KS; b++) {
@@ -303,12 +373,8 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
         for (int b = 0; b < KS; b++)
 #pragma unroll
             for (int v = 0; v < 16; v++) st[b][v] = __builtin_fmaf(st[b][v], a.qk_scale, -ref);
-        const bool pre = s < pre_steps;
-        const int n = (pre ? s : s - pre_steps) * PA_STEP;
-        // Masks (only where the step touches the end of the rows or the causal diagonal; the test is uniform).
-        const bool masked = n + PA_STEP > (pre ? t.P : rc.own_first);
-        const int last = pre ? t.P - 1 : limit;
         if (masked) {
+            const int last = pre ? t.P - 1 : limit;
 #pragma unroll
             for (int b = 0; b < KS; b++)
 #pragma unroll
@@ -317,7 +383,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
                     st[b][v] = key <= last ? st[b][v] : -INFINITY;
                 }
         }
-        // The reference maximum moves only when a score exceeds it by more than 2^LAZY (or when it is still unset): until
+        // The reference maximum moves only when a score exceeds it by more than 2^8 (or when it is still unset): until
         // then p = exp2(score) stays inside fp16 and nothing needs rescaling.
         float mx = -INFINITY;
 #pragma unroll
@@ -330,7 +396,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
             const float delta = upd ? mq : 0.f;
             const float alpha = (upd && top != -INFINITY) ? __builtin_amdgcn_exp2f(-delta) : 1.f;
             ref += delta;
-            top = upd ? LAZY : top;
+            top = upd ? 8.f : top;
             l_i *= alpha;
 #pragma unroll
             for (int b = 0; b < KS; b++)
@@ -354,77 +420,38 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
                 pk[2 * b + (v >> 3)][(v & 7) + 1] = pp.y;
             }
         l_i += rs;
-        uint32_t odd = 0;  // whether a value that some row must not see is no finite number
 #pragma unroll
         for (int i = 0; i < 2 * KS; i++)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                u32x4_t vt = values(l, i, dt);
-                if (masked) {
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t m = not_finite(vt[w]);
-                        odd |= m;
-                        vt[w] &= ~m;
-                    }
-                }
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(vt), pk[i], acc[dt], 0, 0, 0);
+                const u32x2_t lo = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + 16 * i * ROW));
+                const u32x2_t hi = bit_cast<u32x2_t>(lds_read_tr(l + vread[dt] + (16 * i + 8) * ROW));
+                const u32x4_t x = {lo.x, lo.y, hi.x, hi.y};
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(x), pk[i], acc[dt], 0, 0, 0);
             }
-        // Infinities and NaN reach the rows that see them and no others: a product of its own for each of the keys, of which
-        // these rows take their part (0 times them is no 0).
-        if (masked && __builtin_amdgcn_ballot_w64(odd != 0) != 0) {
-#pragma unroll
-            for (int i = 0; i < 2 * KS; i++)
-#pragma unroll 1
-                for (int e = 0; e < 16; e++) {
-                    const bool mine = ((e >> 2) & 1) == lc;
-                    const int el = (e & 3) + 4 * (e >> 3);
-                    const bool visible = n + 32 * KS * kg + 16 * i + e <= last;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        u32x4_t vt = values(l, i, dt);
-#pragma unroll
-                        for (int w = 0; w < 4; w++)
-                            vt[w] = mine && (el >> 1) == w ? vt[w] & not_finite(vt[w]) & (el & 1 ? 0xffff0000u : 0xffffu) : 0u;
-                        float16_t x;
-#pragma unroll
-                        for (int v = 0; v < 16; v++) x[v] = 0.f;
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(vt), pk[i], x, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 16; v++) acc[dt][v] += visible ? x[v] : 0.f;
-                    }
-                }
-        }
-    };
-
-    auto landed = []() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-#pragma unroll
-    for (int s = 0; s < NK; s++) {
-        u32x4_t x = bit_cast<u32x4_t>(qf[s]);
-        asm volatile("" : "+v"(x));
-        qf[s] = bit_cast<half8_t>(x);
     }
-    for (int s = s0; s < s1; s += 2) {
-        landed();
-        visit(s, std::integral_constant<int, 0>{}, s + 1 < s1);
-        if (s + 1 >= s1) break;
-        landed();
-        visit(s + 1, std::integral_constant<int, 1>{}, s + 2 < s1);
-    }
+    if (!w.shared && w.rc.own_first < w.rc.own && __syncthreads_or(odd) && kg == 0) add_odd<D>(t, w, limit, acc);
 
     // ---- the row's state: over its two lanes, then over the key groups
     l_i += __shfl_xor(l_i, 32);
     float m_i = top == -INFINITY ? -INFINITY : ref;
-    float w_own = 1.f;
-    constexpr int OWN = KG == 2 ? DT / 2 : DT;  // column tiles that a wave finishes
+    const bool valid = 32 * qg + ln < w.rows;
     __syncthreads();
-    float4_t other[OWN][4];
-    float w_peer = 0.f;
-    if constexpr (KG == 2) {
+    if constexpr (KG == 1) {
+        if (valid) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    store_row<D>(a, w, row, 32 * dt + 8 * i + 4 * lc,
+                                 (float4_t){acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]}, m_i, l_i);
+        }
+    } else {
         // each wave hands half of its columns to the other key group's wave and finishes the others
-        float4_t* red = reinterpret_cast<float4_t*>(lds);                        // [wave][OWN][4][64]
-        float2* stat = reinterpret_cast<float2*>(lds + NW * OWN * 4096);         // [wave][64]
-        static_assert(NW * OWN * 4096 + NW * 512 <= 2 * SB, "fits");
+        constexpr int OWN = DT / 2;
+        float4_t* red = reinterpret_cast<float4_t*>(lds);                 // [wave][OWN][4][64]
+        float2* state = reinterpret_cast<float2*>(lds + 4 * OWN * 4096);  // [wave][64]
+        static_assert(4 * OWN * 4096 + 4 * 512 <= 2 * SB, "fits");
 #pragma unroll
         for (int d = 0; d < OWN; d++)
 #pragma unroll
@@ -434,49 +461,100 @@ __global__ __launch_bounds__(64 * QG * KG, QG == 1 ? 1 : 2) void prefix_attn_ker
                 for (int j = 0; j < 4; j++) x[j] = kg == 0 ? acc[OWN + d][4 * i + j] : acc[d][4 * i + j];
                 red[((wave * OWN + d) * 4 + i) * 64 + lane] = x;
             }
-        stat[wave * 64 + lane] = make_float2(m_i, l_i);
+        state[wave * 64 + lane] = make_float2(m_i, l_i);
         __syncthreads();
         const int peer = wave ^ 1;
-        const float2 ps = stat[peer * 64 + lane];
-        const float mm = fmaxf(m_i, ps.x);
-        w_own = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - mm);
-        w_peer = ps.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ps.x - mm);
-        l_i = l_i * w_own + ps.y * w_peer;
-        m_i = mm;
+        const float2 mine = make_float2(m_i, l_i), theirs = state[peer * 64 + lane];
+        const float m = fmaxf(mine.x, theirs.x);
+        const float f = share_of(mine, m), g = share_of(theirs, m);
+        const float l = mine.y * f + theirs.y * g;
+        if (valid) {
 #pragma unroll
-        for (int d = 0; d < OWN; d++)
+            for (int d = 0; d < OWN; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) other[d][i] = red[((peer * OWN + d) * 4 + i) * 64 + lane];
+                for (int i = 0; i < 4; i++) {
+                    const float4_t o = red[((peer * OWN + d) * 4 + i) * 64 + lane];
+                    float4_t x;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[j] = (kg == 0 ? acc[d][4 * i + j] : acc[OWN + d][4 * i + j]) * f + o[j] * g;
+                    store_row<D>(a, w, row, 32 * (d + kg * OWN) + 8 * i + 4 * lc, x, m, l);
+                }
+        }
     }
-    const bool valid = 32 * qg + ln < rows;
-    const bool direct = p.parts_a + p.parts_b == 1;
-    const float inv = direct ? (l_i == 0.f ? 0.f : 1.f / l_i) : 1.f;  // a row that sees nothing: 0
-    const long slot = ((long)head * (p.parts_a + p.parts_b) + part) * ((long)t.T * t.share) + row;
-    const long o_at = ((long)token * (t.H * t.share) + qhead) * D;
-    if (!valid) return;
-#pragma unroll
-    for (int d = 0; d < OWN; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float4_t x;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (KG == 2)
-                    x[j] = ((kg == 0 ? acc[d][4 * i + j] : acc[OWN + d][4 * i + j]) * w_own + other[d][i][j] * w_peer) * inv;
-                else
-                    x[j] = acc[d][4 * i + j] * inv;
-            }
-            const int col = 32 * (d + (KG == 2 && kg ? OWN : 0)) + 8 * i + 4 * lc;
-            if (direct) {
-                half4_t h;
-#pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = (half_t)x[j];
-                *(half4_t*)(t.o + o_at + col) = h;
-            } else {
-                *(float4_t*)(p.po + slot * D + col) = x;
+}
+
+template <int D, int QG>
+__device__ __forceinline__ void attend(const PrefixArgs& a, const Work& w, uint8_t* lds, float2* stat) {
+    if constexpr (QG == 1) few_rows<D>(a, w, lds, stat);
+    else many_rows<D, QG>(a, w, lds);
+}
+
+// QA, QB: groups of 32 rows of the tiles against the prefix (0: none) and of a sequence's.
+template <int D, int QA, int QB>
+__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PrefixArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[RowsAttn<D>::LDS];
+    __shared__ float2 stat[4 * 32];
+    static_assert(RowsAttn<D>::LDS == 4 * PA_STEP * D * 2);
+    const PrefixAttn& t = a.t;
+    const PrefixPlan& p = a.p;
+    int index = blockIdx.x;
+    Work w = {};
+    if constexpr (QA > 0) {
+        if (index < p.grid_a) {
+            const int work = (index & 7) * (p.grid_a >> 3) + (index >> 3);  // an eighth of the list per XCD: a prefix piece's tiles share an L2
+            if (work >= p.units_a) return;
+            const int rest = p.by_tiles_a(work);
+            w.row0 = (work - rest * p.tiles_a) * (32 * QA);
+            w.head = p.by_parts_a(rest);
+            w.part = rest - w.head * p.parts_a;
+            w.rows = imin(32 * QA, t.T * t.share - w.row0);
+            w.s0 = w.part * p.steps_a;
+            w.s1 = imin(w.s0 + p.steps_a, ceil_div(t.P, PA_STEP));
+            w.shared = true;
+            if constexpr (QA != QB) {
+                attend<D, QA>(a, w, lds, stat);
+                return;
             }
         }
-    if (!direct && lc == 0 && kg == 0) p.pml[slot] = make_float2(m_i, l_i);
+        index -= p.grid_a;
+    }
+    if (index < p.grid_b) {
+      if (!w.shared) {
+        const int work = (index & 7) * (p.grid_b >> 3) + (index >> 3);
+        if (work >= p.units_b) return;
+        const int rest = p.by_tiles_b(work);
+        w.head = p.by_parts_b(rest);
+        const int part = rest - w.head * p.parts_b;
+        if (!tile_of(t, 32 * QB, p.tiles_b - 1 - (work - rest * p.tiles_b), w.tl)) return;
+        w.rc = reach_of(t, p, w.tl);
+        w.row0 = w.tl.first * t.share + w.tl.tile * (32 * QB);
+        w.rows = imin(32 * QB, w.tl.count * t.share - w.tl.tile * (32 * QB));
+        w.s0 = part * p.steps_b;
+        w.s1 = imin(w.s0 + p.steps_b, w.rc.steps);
+        if (w.s0 >= w.s1 && part > 0) return;  // (the first part also stands for rows that see nothing)
+        w.part = p.parts_a + part;
+      }
+        attend<D, QB>(a, w, lds, stat);
+        return;
+    }
+    // the call's own rows into the cache, a token per wave
+    const int lane = threadIdx.x & 63;
+    const int token = (index - p.grid_b) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (token >= t.T) return;
+    const int b = sequence_of(t, token);
+    if (b < 0) return;
+    int first, count;
+    tokens_of(t, b, first, count);
+    const int at = t.lengths[b] - count + token - first;
+    if (at < 0 || at >= t.Lmax) return;
+    constexpr int CPR = D / 8;
+    for (int i = lane; i < t.H * CPR; i += 64) {
+        const int h = i / CPR, c = 8 * (i % CPR);
+        const long from = (long)token * t.n_ts + (long)h * t.n_hs + c;
+        const long to = (long)b * t.c_bs + (long)h * t.c_hs + (long)at * t.c_rs + c;
+        *(u32x4_t*)(t.kc + to) = *(const u32x4_t*)(t.kn + from);
+        *(u32x4_t*)(t.vc + to) = *(const u32x4_t*)(t.vn + from);
+    }
 }
 
 // The parts of a row (token, query head), a row per wave.
@@ -499,7 +577,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
     if (tl.b < 0) return;
     tokens_of(t, tl.b, tl.first, tl.count);
     const int row = token * t.share + qhead - head * t.share;
-    tl.tile = (row - tl.first * t.share) / p.rows;
+    tl.tile = (row - tl.first * t.share) / p.rows_b;
     const Reach rc = reach_of(t, p, tl);
     const int total = p.parts_a + p.parts_b;
     const int parts = p.parts_a + imin(imax(ceil_div(rc.steps, p.steps_b), 1), p.parts_b);
@@ -514,7 +592,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
         mx = fmaxf(mx, m);
-        const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+        const float w = share_of(ml, mx);
         float ls = ml.y * w;
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) ls += __shfl_xor(ls, x);
@@ -550,27 +628,35 @@ constexpr int PA_WGS = 512;
 
 PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool ragged) {
     PrefixPlan p = {};
-    const long rows = (long)T * share;          // of a key/value head
-    const long each = (rows + B - 1) / B;       // of a sequence, on average
-    p.packed = P > 0 && B > 1 && each < 64;
-    const long most = p.packed ? rows : each;
-    p.qg = most <= 32 ? 1 : most <= 64 ? 2 : 4;
-    p.rows = 32 * p.qg;
+    const long rows = (long)T * share;     // of a key/value head
+    const long each = (rows + B - 1) / B;  // of a sequence, on average
+    const bool packed = P > 0 && B > 1 && each <= 32;
+    p.packed = packed;
+    p.qa = !packed ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    p.qb = each <= 32 ? 1 : each <= 64 ? 2 : 4;
+    p.rows_b = 32 * p.qb;
     const int pre = div_up(P, PA_STEP), own = div_up(Lmax, PA_STEP);
-    if (p.packed) {
-        p.tiles_a = div_up(rows, p.rows);
+    if (packed) {
+        p.tiles_a = div_up(rows, 32 * p.qa);
         const long steps = (long)H * p.tiles_a * pre;
         p.steps_a = std::max(div_up(steps, PA_WGS), 1);
+        if (p.qa == 1) p.steps_a = (p.steps_a + 1) / 2 * 2;
         p.parts_a = div_up(pre, p.steps_a);
-        p.units_a = (long)H * p.parts_a * p.tiles_a;
+        p.units_a = H * p.parts_a * p.tiles_a;
     }
-    p.tiles_b = ragged ? (int)(rows / p.rows + B) : B * div_up((long)(T / B) * share, p.rows);
-    const int steps_b = own + (p.packed ? 0 : pre);
+    p.tiles_b = ragged ? (int)(rows / p.rows_b + B) : B * div_up((long)(T / B) * share, p.rows_b);
+    const int steps_b = own + (packed ? 0 : pre);
     p.steps_b = std::max(div_up((long)p.tiles_b * H * steps_b, PA_WGS), 1);
+    if (p.qb == 1) p.steps_b = (p.steps_b + 1) / 2 * 2;
     p.parts_b = std::max(div_up(steps_b, p.steps_b), 1);
-    p.units_b = (long)H * p.parts_b * p.tiles_b;
+    p.units_b = H * p.parts_b * p.tiles_b;
     p.grid_a = pad8(p.units_a);
     p.grid_b = pad8(p.units_b);
+    p.by_share = Divisor::of(share);
+    p.by_tiles_a = Divisor::of(std::max(p.tiles_a, 1));
+    p.by_parts_a = Divisor::of(std::max(p.parts_a, 1));
+    p.by_tiles_b = Divisor::of(std::max(p.tiles_b, 1));
+    p.by_parts_b = Divisor::of(p.parts_b);
     return p;
 }
 
@@ -588,18 +674,22 @@ hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, v
     const int parts = a.p.parts_a + a.p.parts_b;
     a.p.po = (float*)workspace;
     a.p.pml = (float2*)(a.p.po + (size_t)parts * t.H * t.T * t.share * D);
-#define SQ_PREFIX_LAUNCH(D_, QG_, KG_)                                                                                     \
-    hipLaunchKernelGGL((prefix_attn_kernel<D_, QG_, KG_>),                                                                 \
-                       dim3(a.p.grid_a + a.p.grid_b + (t.kn ? (t.T + QG_ * KG_ - 1) / (QG_ * KG_) : 0)), dim3(64 * QG_ * KG_), 0, \
-                       st, a)
-    if (D == 64) {
-        if (a.p.qg == 1) SQ_PREFIX_LAUNCH(64, 1, 2);
-        else if (a.p.qg == 2) SQ_PREFIX_LAUNCH(64, 2, 2);
-        else SQ_PREFIX_LAUNCH(64, 4, 1);
+    const dim3 pieces(a.p.grid_a + a.p.grid_b + (t.kn ? (t.T + 3) / 4 : 0));
+#define SQ_PREFIX_LAUNCH(QA_, QB_)                                                                  \
+    if (D == 64) hipLaunchKernelGGL((prefix_attn_kernel<64, QA_, QB_>), pieces, dim3(256), 0, st, a); \
+    else hipLaunchKernelGGL((prefix_attn_kernel<128, QA_, QB_>), pieces, dim3(256), 0, st, a)
+    if (a.p.qa == 1) {
+        SQ_PREFIX_LAUNCH(1, 1);
+    } else if (a.p.qa == 2) {
+        SQ_PREFIX_LAUNCH(2, 1);
+    } else if (a.p.qa == 4) {
+        SQ_PREFIX_LAUNCH(4, 1);
+    } else if (a.p.qb == 1) {
+        SQ_PREFIX_LAUNCH(0, 1);
+    } else if (a.p.qb == 2) {
+        SQ_PREFIX_LAUNCH(0, 2);
     } else {
-        if (a.p.qg == 1) SQ_PREFIX_LAUNCH(128, 1, 2);
-        else if (a.p.qg == 2) SQ_PREFIX_LAUNCH(128, 2, 2);
-        else SQ_PREFIX_LAUNCH(128, 4, 1);
+        SQ_PREFIX_LAUNCH(0, 4);
     }
 #undef SQ_PREFIX_LAUNCH
     hipError_t e = hipGetLastError();
