@@ -13,6 +13,7 @@ from the device, so that a captured HIP graph follows it.  Nothing here has a co
 import torch
 
 import quant
+from . import capi
 from .prefix import _alike, _check_ints, _check_written, _readable, _rows_like
 
 
@@ -136,3 +137,51 @@ def _overlap(a, b):
         return False
     (a0, a1), (b0, b1) = _extent(a), _extent(b)
     return a0 < b1 and b0 < a1
+
+
+class EvictCache:
+    """A model's cache of `rows` rows a head in every layer: a prompt's rows of the highest weights stay, by all its queries or
+    its last `window`, and later tokens take the places of those of the lowest.  The first keep_first and the last keep_last
+    tokens are never given up.  `seen` counts the sequences' tokens on the device; `OPTDecoder` keeps it, or whoever drives the
+    layers by hand.  It takes one prompt, at the beginning, and then single tokens."""
+
+    def __init__(self, layers, batch, kv_heads, head_dim, rows, keep_first=4, keep_last=None, window=None, device="cuda"):
+        keep_last = max(1, rows // 4) if keep_last is None else keep_last
+        if min(layers, batch, kv_heads, rows) < 1 or head_dim not in (64, 128) or (window is not None and window < 1):
+            raise ValueError("a cache of %d layers, %d sequences, %d heads of %d, %d rows" % (layers, batch, kv_heads, head_dim, rows))
+        _check_kept(keep_first, keep_last, rows, 1)
+        self.layers, self.batch, self.rows = layers, batch, rows
+        self.keep_first, self.keep_last, self.window = keep_first, keep_last, window
+        shape = (layers, batch, kv_heads, rows)
+        self.k = torch.zeros(shape + (head_dim,), dtype=torch.float16, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.weight = torch.zeros(shape, dtype=torch.float32, device=device)
+        self.position = torch.zeros(shape, dtype=torch.int32, device=device)
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)
+
+    def set_position(self, batch, pos0, tokens):
+        """The next `tokens` tokens of the first `batch` sequences are those of positions pos0 on: an int, or (one token) an
+        int64 tensor of one element on the device."""
+        if batch > self.batch:
+            raise ValueError("%d sequences in a cache for %d" % (batch, self.batch))
+        if tokens != 1 and not (isinstance(pos0, int) and pos0 == 0):
+            raise ValueError("a cache that evicts takes a prompt at the beginning, and then single tokens")
+        if isinstance(pos0, int) and pos0 < 0:
+            raise ValueError("position %d" % pos0)
+        self.seen[:batch] = pos0 + tokens
+
+    def attention(self, layer, q, k, v, sm_scale):
+        """q, k, v fp16 [B, heads, T, D] of a prompt, or of the next token -> [B, T, heads, D]; their rows are stored."""
+        b, h, t, d = q.shape
+        cache = self.k[layer, :b], self.v[layer, :b], self.weight[layer, :b], self.position[layer, :b]
+        if t == 1:
+            q, k, v = (x[:, :, 0] for x in (q, k, v))
+            return attention(q, k, v, *cache, self.seen[:b], sm_scale, self.keep_first, self.keep_last)[0].view(b, 1, h, d)
+        if k.shape[1] == h and capi.lut_attention_strided_ok(q, k, v):
+            out = capi.lut_attention_strided(q, k, v, None, sm_scale, True, rows_first=True)
+        else:
+            out = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True, scale=sm_scale,
+                                                                   enable_gqa=k.shape[1] != h).transpose(1, 2)
+        weight = attention_weights(q, k, sm_scale, self.window)
+        keep(k, v, weight, *cache, self.keep_first, self.keep_last)
+        return out

@@ -1,6 +1,7 @@
 """Rules on logits in front of the choice of a token: penalties for repeated tokens, biases by token, a grammar's mask.
 
     apply_rules   the logits under the rules, and each row's best token
+    Rules         what a decoder applies at every step
 
 The reference leaves these to its caller (test/nvidia/module/opt/modeling_opt_ours.py:1229 returns the lm_head's logits);
 nothing here has a counterpart there.
@@ -74,3 +75,18 @@ def _check(logits, ids, lengths, generated_from, repetition, presence, frequency
     check("token", token, torch.int64, m)
     if token is not None and not token.is_contiguous():
         raise ValueError("token must be contiguous")
+
+
+class Rules:
+    """What `apply_rules` is given at every step of a batch, all but the texts (OPTDecoder.greedy_step): tensors on the device,
+    which may be changed in place between the steps, as a grammar's mask is."""
+
+    def __init__(self, repetition=None, presence=None, frequency=None, generated_from=None, bias_ids=None, bias=None, mask=None):
+        self.repetition, self.presence, self.frequency, self.generated_from = repetition, presence, frequency, generated_from
+        self.bias_ids, self.bias, self.mask = bias_ids, bias, mask
+
+    def apply(self, logits, ids=None, lengths=None, out=None, token=None):
+        if not any(x is not None for x in (self.repetition, self.presence, self.frequency)):
+            ids = lengths = None  # nobody asks for the texts
+        return apply_rules(logits, ids, lengths, self.generated_from if ids is not None else None, self.repetition, self.presence,
+                           self.frequency, self.bias_ids, self.bias, self.mask, out, token)

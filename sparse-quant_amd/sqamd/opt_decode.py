@@ -18,6 +18,11 @@ that also fills the cache (sq_lut_attention_strided).
 With `new_cache(batch, max_len, kv_bits=4)` the keys and values are held in 4 bits, in pages (kv4.KV4Cache): a layer quantises
 its rows into the cache and attends over what is held there, in prompts as in steps (over a look-up table: the prompt's
 attention is given the values that the cache holds, rounded to fp16).
+
+Two more caches take the place of the plain one: `prefix_cache(ids, batch, max_len)` runs a prefix that all sequences begin
+with once and holds its rows once (prefix.PrefixCache), `new_cache(batch, max_len, rows=...)` holds no more than so many rows a
+head and evicts by accumulated attention weight (evict.EvictCache).  `greedy_step(..., rules=...)` chooses the next token under
+rules on the logits (logits.Rules).
 """
 import math
 import time
@@ -25,7 +30,7 @@ import time
 import torch
 from torch import nn
 
-from . import capi, kv4, lut_layout
+from . import capi, evict, kv4, lut_layout, prefix
 from .block_sparse_attention_lut import sparse_attention
 from .qlinear import WALinear
 
@@ -70,8 +75,8 @@ class DecoderLayer(nn.Module):
         self.capture = None  # a dict: the prefill's q, k, v and attention output are left in it (tests)
 
     def forward(self, x, kc, vc, pos0):
-        """x [B, T, H]; kc, vc [B, heads, Lmax, hd], or kc a layer of a 4-bit cache and vc None; writes cache rows pos0 ..
-        pos0+T-1."""
+        """x [B, T, H]; kc, vc [B, heads, Lmax, hd], or kc a layer of a 4-bit cache and vc None, or kc a PrefixCache or an
+        EvictCache and vc the layer's number; writes cache rows pos0 .. pos0+T-1."""
         b, t, hdim = x.shape
         if self.qkv_proj is not None:
             # the first LayerNorm rides in the q/k/v launch (inside the kernel at decode batch sizes)
@@ -88,7 +93,15 @@ class DecoderLayer(nn.Module):
             k = self.k_proj(flat).view(b, t, self.heads, self.hd).transpose(1, 2)
             v = self.v_proj(flat).view(b, t, self.heads, self.hd).transpose(1, 2)
         scale = 1.0 / math.sqrt(self.hd)
-        if vc is None:
+        if isinstance(vc, int):  # a cache that attends for its layers, and the layer's number
+            if self.lut is not None and t > 1:
+                raise ValueError("a prompt over a look-up table needs the plain or the 4-bit cache")
+            a = kc.attention(vc, q, k, v, scale)
+            if self.capture is not None:
+                self.capture.update(q=q.detach().clone(), k=k.detach().clone(), v=v.detach().clone(),
+                                    a=a.transpose(1, 2).detach().clone())
+            a = a.reshape(1, b * t, hdim)
+        elif vc is None:
             a = self._attend_4bit(q, k, v, kc, pos0, scale)
         elif isinstance(pos0, int) and pos0 == 0 and t > 1 and capi.lut_attention_strided_ok(q, k, v, kc, vc) \
                 and (self.lut is None or self.lut.dtype in (torch.int32, torch.int64)):
@@ -153,6 +166,9 @@ class DecoderLayer(nn.Module):
 def _per_layer(cache, batch, tokens, pos0):
     """A cache's layers as DecoderLayer.forward takes them; a 4-bit cache's lengths are counted up to behind the rows that
     it will write (on the device where the position lives there, and the cache is told so)."""
+    if isinstance(cache, (prefix.PrefixCache, evict.EvictCache)):
+        cache.set_position(batch, pos0, tokens)
+        return [(cache, i) for i in range(cache.layers)]
     if not isinstance(cache, kv4.KV4Cache):
         return cache
     if isinstance(pos0, int):
@@ -190,8 +206,26 @@ class OPTDecoder(nn.Module):
             layout = lut_layout.synth_layout(self.heads, nb, density, causal=True, seed=seed + idx)
             layer.lut = lut_layout.layout2lut_single_density(layout[None])[0].to(self.embed.device)
 
-    def new_cache(self, batch, max_len, kv_bits=16, kv_group=64):
+    def prefix_cache(self, ids, batch, max_len):
+        """A cache for `batch` sequences that all begin with the tokens ids [P], which are run here, once; sequences take up to
+        max_len rows, the prefix's among them.  Positions go on behind it: the first prompt is forward(ids, cache, P)."""
+        ids = ids.view(1, -1)
+        p = ids.shape[1]
+        if not 0 < p < max_len:
+            raise ValueError("a prefix of %d rows in sequences of up to %d" % (p, max_len))
+        rows = self.new_cache(1, p)
+        self(ids, rows, 0)
+        return prefix.PrefixCache([k[0] for k, _ in rows], [v[0] for _, v in rows], batch, max_len - p)
+
+    def new_cache(self, batch, max_len, kv_bits=16, kv_group=64, rows=None, keep_first=4, keep_last=None, window=None):
+        """A cache for `batch` sequences of up to max_len rows.  rows: it holds no more than so many a head and evicts by
+        accumulated attention weight (keep_first, keep_last, window: as evict.EvictCache takes them)."""
         hd = self.hidden // self.heads
+        if rows is not None:
+            if kv_bits != 16:
+                raise ValueError("a cache that evicts is held in 16 bits, not %r" % (kv_bits,))
+            return evict.EvictCache(len(self.layers), batch, self.heads, hd, rows, keep_first, keep_last, window,
+                                    self.embed.device)
         if kv_bits == 4:
             pages = (max_len + kv4.PAGE - 1) // kv4.PAGE
             cache = kv4.KV4Cache(len(self.layers), batch * pages, self.heads, hd, kv_group, batch, max_len, self.embed.device)
@@ -225,14 +259,16 @@ class OPTDecoder(nn.Module):
         return torch.matmul(x, self.lm_head.t())  # [B, 1, vocab]
 
     @torch.no_grad()
-    def greedy_step(self, tok, cache, pos_t, history=None, step_t=None):
+    def greedy_step(self, tok, cache, pos_t, history=None, step_t=None, rules=None):
         """One greedy decode step for up to 8 sequences with nothing but library launches, so that a HIP graph
         holds the whole of it: tok int64 [B, 1] is read at the start and replaced by the chosen tokens at the
         end, pos_t int64 [1] (the cache row the new keys and values go to) is advanced, and with history int64
         [T, B] and step_t int64 [1] the chosen tokens are also written to history[step_t].  Embeddings, final
         LayerNorm, fp16 lm_head and argmax are what forward() computes with torch ops (the embeddings bit for bit;
         the logits with fp32 sums in another order).  A 4-bit cache's lengths are counted on the device then
-        (KV4Cache.counted_on_device).  Returns the logits [B, vocab]."""
+        (KV4Cache.counted_on_device).  rules (logits.Rules): the token is the best one under them, and the logits are returned
+        as they leave them; the texts that penalties look at are the first step_t rows of history, which then hold the prompts
+        and the tokens chosen so far, tok among them.  Returns the logits [B, vocab]."""
         b = tok.shape[0]
         if getattr(self, "_parts", None) is None:
             self._parts = capi.f16_gemv_parts(self.lm_head.shape[0], self.lm_head.device)
@@ -240,16 +276,26 @@ class OPTDecoder(nn.Module):
         for layer, (kc, vc) in zip(self.layers, _per_layer(cache, b, 1, pos_t)):
             x = layer(x, kc, vc, pos_t)
         x = _layernorm(self.final_ln, x.view(b, self.hidden))
-        logits = capi.f16_gemv(x, self.lm_head, parts=self._parts)
-        capi.greedy_feedback(self._parts, b, tok.view(-1), pos=pos_t, history=history, step=step_t)
+        if rules is None:
+            logits = capi.f16_gemv(x, self.lm_head, parts=self._parts)
+            capi.greedy_feedback(self._parts, b, tok.view(-1), pos=pos_t, history=history, step=step_t)
+            return logits
+        logits = capi.f16_gemv(x, self.lm_head)
+        texts = history is not None and step_t is not None
+        _, best = rules.apply(logits, history.t() if texts else None, step_t.expand(b) if texts else None, out=logits)
+        # the token itself as the only candidate: its feedback is the launch that a step without rules ends with
+        one = torch.zeros((8, 1), dtype=torch.float32, device=x.device), torch.zeros((8, 1), dtype=torch.int32, device=x.device)
+        one[1][:b, 0] = best
+        capi.greedy_feedback(one, b, tok.view(-1), pos=pos_t, history=history, step=step_t)
         return logits
 
 
 @torch.no_grad()
 def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed=0, fuse_qkv=True,
             return_tokens=False, lut_density=0.26, scale_std=E2E_SCALE_STD, scale_min=E2E_SCALE_MIN, fused_ends=True,
-            kv_bits=16):
-    """Greedy generation on random token ids; returns timing and throughput figures."""
+            kv_bits=16, shared=0, rows=None):
+    """Greedy generation on random token ids; returns timing and throughput figures.  shared: so many tokens in front of every
+    prompt are the same and held once; rows: the cache holds no more than so many rows a head."""
     dev = "cuda"
     model = OPTDecoder(layers=layers, dev=dev, seed=seed, scale_std=scale_std, scale_min=scale_min)
     if fuse_qkv:
@@ -258,10 +304,18 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     gen = torch.Generator(device=dev)
     gen.manual_seed(seed + 1)
     ids = torch.randint(0, 50272, (batch, prompt), device=dev, generator=gen)
-    max_len = prompt + new_tokens
-    cache = model.new_cache(batch, max_len, kv_bits)
+    if (shared or rows) and (kv_bits != 16 or (shared and rows)):
+        raise ValueError("a shared prefix, a cache that evicts and a 4-bit cache are three different caches")
+    if shared or rows:
+        lut_density = None
+    begin = shared
+    max_len = begin + prompt + new_tokens
+    if shared:
+        cache = model.prefix_cache(torch.randint(0, 50272, (shared,), device=dev, generator=gen), batch, max_len)
+    else:
+        cache = model.new_cache(batch, max_len, kv_bits, rows=rows)
 
-    model(ids, cache, 0)  # untimed first pass: code objects, library handles and workspaces come into being here
+    model(ids, cache, begin)  # untimed first pass: code objects, library handles and workspaces come into being here
     torch.cuda.synchronize()
     # The same prefill with the attention of every layer through the LUT kernel (causal tables of the
     # reference's OPT density); the dense pass that follows rewrites the cache, decode starts from that one.
@@ -276,7 +330,7 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
         prefill_lut_s = time.perf_counter() - t0
         model.set_prefill_lut(prompt, None)
     t0 = time.perf_counter()
-    logits = model(ids, cache, 0)
+    logits = model(ids, cache, begin)
     nxt = logits.argmax(-1)
     torch.cuda.synchronize()
     prefill_s = time.perf_counter() - t0
@@ -284,7 +338,7 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     # One decode step with device-side position so that it can be replayed as a graph.  fused_ends: embeddings,
     # lm_head, argmax and the feedback of the chosen token are library launches inside the step (greedy_step);
     # otherwise they are torch ops, three of them between two replays.
-    pos_t = torch.tensor([prompt], device=dev, dtype=torch.long)
+    pos_t = torch.tensor([begin + prompt], device=dev, dtype=torch.long)
     tok = nxt.clone()
     out_tok = torch.empty_like(tok)
     fused_ends = fused_ends and batch <= 8
@@ -302,7 +356,7 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     def rewind():
         # the warm-up and the capture run a step each: put token, position and step counter back
         tok.copy_(first_tok)
-        pos_t.fill_(prompt)
+        pos_t.fill_(begin + prompt)
         if step_t is not None:
             step_t.zero_()
 
@@ -342,7 +396,9 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
     # rows read once (average over the timed steps), the fp16 lm_head.
     hidden, ffn, g, vocab = model.hidden, model.layers[0].fc1.out_features, 128, model.lm_head.shape[0]
     lin = lambda n, k: n * k // 2 + (k // g) * n * 4 + batch * k * 2 + batch * n * 2
-    rows_avg = prompt + (steps + 1) / 2.0
+    rows_avg = prompt + (steps + 1) / 2.0 + begin / batch  # (a shared prefix is read once for all)
+    if rows:
+        rows_avg = min(rows_avg, rows)
     per_layer = lin(3 * hidden, hidden) + lin(hidden, hidden) + lin(ffn, hidden) + lin(hidden, ffn) + \
         (2 * batch * hidden * rows_avg * 2 if kv_bits == 16 else
          batch * hidden * rows_avg * (1 + 8 / cache.group_size))
@@ -355,13 +411,15 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
             " (smaller than the single-linear benchmark's |N(0,0.02)|+1e-3 so that 32 random layers stay finite in fp16)"
             if scale_std < 0.02 else " (the single-linear benchmark's distribution)"),
         "batch": batch, "prompt": prompt, "new_tokens": new_tokens, "layers": layers,
+        **({"shared_prefix": shared} if shared else {}), **({"cache_rows": rows} if rows else {}),
         "launch": "hip-graph replay" if graph is not None else "eager",
         "fused": "bias+relu+residual in the GEMM store" + ("; q/k/v one launch" if fuse_qkv else "") +
                  "; both LayerNorms inside the q/k/v and fc1 kernels at decode; decode attention appends K/V in the same "
                  "launch" + ("; embeddings, fp16 lm_head + argmax, token feedback as three launches inside the step"
                              if fused_ends else ""),
         "prefill_ms": round(prefill_s * 1e3, 2),
-        "prefill_attention": "dense causal (%s)" % ("sq_lut_attention_strided without a table" if kv_bits == 16 else
+        "prefill_attention": "dense causal (%s)" % ("sq_prefix_attention" if shared else
+                                                     "sq_lut_attention_strided without a table" if kv_bits == 16 else
                                                      "sq_kv4_attention over the cache in 4 bits"),
         "prefill_lut_ms": None if prefill_lut_s is None else round(prefill_lut_s * 1e3, 2),
         "prefill_lut_attention": None if prefill_lut_s is None else
@@ -384,4 +442,10 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
 if __name__ == "__main__":
     import json
     import sys
-    print(json.dumps(run_e2e(use_graph="--no-graph" not in sys.argv, kv_bits=4 if "--kv4" in sys.argv else 16)))
+
+
+    def number(flag):
+        return int(sys.argv[sys.argv.index(flag) + 1]) if flag in sys.argv else 0
+
+    print(json.dumps(run_e2e(use_graph="--no-graph" not in sys.argv, kv_bits=4 if "--kv4" in sys.argv else 16,
+                             shared=number("--shared"), rows=number("--rows") or None)))

@@ -98,3 +98,42 @@ def attention(q, k_prefix, v_prefix, k_cache, v_cache, lengths, sm_scale, starts
         raise ValueError("prefix attention of %d tokens over %s behind %s: too large, or rows too far apart"
                          % (t, tuple(k_cache.shape), tuple(k_prefix.shape)))
     return got if out is None else out
+
+
+class PrefixCache:
+    """A model's keys and values behind a shared prefix: its rows in every layer, held once, and room for `max_rows` own rows of
+    each of `batch` sequences.  k_prefix, v_prefix: a tensor [kv_heads, P, D] of each layer.  `lengths` counts the sequences' own
+    rows on the device; `OPTDecoder` keeps it, or whoever drives the layers by hand (rows of the present call among them)."""
+
+    def __init__(self, k_prefix, v_prefix, batch, max_rows):
+        if not k_prefix or len(k_prefix) != len(v_prefix) or batch < 1 or max_rows < 1:
+            raise ValueError("a cache of %d layers, %d sequences of %d rows" % (len(k_prefix), batch, max_rows))
+        h, p, d = k_prefix[0].shape
+        if any(x.shape != (h, p, d) for x in (*k_prefix, *v_prefix)):
+            raise ValueError("the prefix has as many rows in every layer")
+        self.k_prefix, self.v_prefix = list(k_prefix), list(v_prefix)
+        self.layers, self.batch, self.max_rows, self.prefix_rows = len(k_prefix), batch, max_rows, p
+        shape = (self.layers, batch, h, max_rows, d)
+        self.k = torch.zeros(shape, dtype=torch.float16, device=k_prefix[0].device)
+        self.v = torch.zeros_like(self.k)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.k.device)
+
+    def set_position(self, batch, pos0, tokens):
+        """The next `tokens` rows of the first `batch` sequences are those of positions pos0 on (the prefix's counted): an int, or
+        an int64 tensor of one element on the device."""
+        if batch > self.batch:
+            raise ValueError("%d sequences in a cache for %d" % (batch, self.batch))
+        if isinstance(pos0, int):
+            if pos0 < self.prefix_rows or pos0 + tokens > self.prefix_rows + self.max_rows:
+                raise ValueError("positions %d .. %d in a cache of %d rows behind a prefix of %d"
+                                 % (pos0, pos0 + tokens - 1, self.max_rows, self.prefix_rows))
+            self.lengths[:batch] = pos0 + tokens - self.prefix_rows
+        else:
+            self.lengths[:batch] = pos0 + (tokens - self.prefix_rows)
+
+    def attention(self, layer, q, k, v, sm_scale):
+        """q, k, v fp16 [B, heads, T, D] of the next tokens -> [B, T, heads, D]; their rows are stored."""
+        b, h, t, d = q.shape
+        q, k, v = (x.transpose(1, 2).reshape(b * t, x.shape[1], d) for x in (q, k, v))
+        return attention(q, self.k_prefix[layer], self.v_prefix[layer], self.k[layer, :b], self.v[layer, :b], self.lengths[:b],
+                         sm_scale, k_new=k, v_new=v).view(b, t, h, d)
