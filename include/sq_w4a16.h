@@ -608,7 +608,7 @@ int sq_evict_keep(const void* k, const void* v, const void* weight, const void* 
  * generated_from[m * strides[5]] on (NULL: all of it).  repetition, frequency and presence fp32 [M], each may be NULL; bias_ids int32
  * and bias fp32, rows of nb <= 65535 entries strides[6] and strides[7] apart; mask uint32, rows of ceil(V / 32) words strides[8]
  * apart (0: one for all).  Ids outside [0, V) are none. */
-size_t sq_logit_rules_workspace_bytes(int M, int V);
+size_t sq_logit_rules_workspace_bytes(int M, int V, int L, int nb);
 int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, const void* lengths, const void* generated_from,
                    const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,
                    const void* mask, void* token, int M, int V, int L, int nb, const long* strides, void* workspace,

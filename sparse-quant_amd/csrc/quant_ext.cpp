@@ -807,7 +807,7 @@ c10::optional<std::pair<at::Tensor, at::Tensor>> logit_rules(const at::Tensor& x
     at::Tensor out = into.has_value() ? *into : at::empty({M, V}, x.options());
     at::Tensor token = token_into.has_value() ? *token_into : at::empty({M}, x.options().dtype(at::kLong));
     strides[1] = stride_of(out, 0);
-    const size_t need = sq_logit_rules_workspace_bytes((int)M, (int)V);
+    const size_t need = sq_logit_rules_workspace_bytes((int)M, (int)V, (int)L, (int)nb);
     const at::Tensor ws = scratch(need, x);
     const int rc = sq_logit_rules(x.data_ptr(), out.data_ptr(), half ? 2 : 4, pointer(ids), pointer(lengths), pointer(generated),
                                   pointer(repetition), pointer(presence), pointer(frequency), pointer(bias_ids), pointer(bias),

@@ -1384,7 +1384,9 @@ int sq_evict_keep(const void* k, const void* v, const void* weight, const void* 
     return launch_code(sq::launch_evict_keep(t, D, static_cast<hipStream_t>(stream)));
 }
 
-size_t sq_logit_rules_workspace_bytes(int M, int V) { return M > 0 && V > 0 ? sq::logit_rules_workspace_bytes(M, V) : 0; }
+size_t sq_logit_rules_workspace_bytes(int M, int V, int L, int nb) {
+    return M > 0 && V > 0 && L >= 0 && nb >= 0 ? sq::logit_rules_workspace_bytes(M, V, L, nb) : 0;
+}
 
 int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, const void* lengths, const void* generated_from,
                    const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,
@@ -1405,7 +1407,8 @@ int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, cons
     for (int i = 0; i < 9; i++)
         if (strides[i] < 0) return SQ_ERR_BAD_SHAPE;
     if (M > 1 && strides[1] < V) return SQ_ERR_BAD_SHAPE;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < sq_logit_rules_workspace_bytes(M, V)) return SQ_ERR_WORKSPACE;
+    const size_t need = sq_logit_rules_workspace_bytes(M, V, L, nb);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return SQ_ERR_WORKSPACE;
     sq::LogitRules t = {};
     t.x = x, t.y = y;
     t.ids = static_cast<const long long*>(ids);

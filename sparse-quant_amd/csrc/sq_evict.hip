@@ -217,6 +217,8 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
     }
 }
 
+// Workgroups that keep's places are cut for.
+constexpr int KEEP_WGS = 512;
 // Workgroups that the caches' rows are cut for: two per CU.
 constexpr int EV_WGS = 512;
 
@@ -346,6 +348,165 @@ __global__ __launch_bounds__(256) void keep_gather_kernel(EvictKeep t) {
     }
 }
 
+// The same for prompts whose weights fit LDS, and the rows copied by the same workgroup: several share a head where there are
+// few, and each of them makes the choice.  (With the weights in registers the code is a copy of each loop for every one of them,
+// and fetching it takes longer than the loops.)  The threshold is found between the
+// lowest and the highest weight, of whose distance every pass looks at 11 bits: counted by the weights' own digits, most of
+// them fall on a few counters (the numbers of one power of two have one), and LDS takes them one at a time.
+constexpr int KEEP_LIST = 4096;  // places of a workgroup
+
+constexpr int KEEP_MOST = 32 * KEEP_THREADS;  // rows of a prompt
+
+template <int D>
+__global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(EvictKeep t, int each) {
+    constexpr int WAVES = KEEP_THREADS / 64;
+    __shared__ int bins[KEEP_BINS];
+    extern __shared__ uint32_t keys[];  // a thread reads its own
+    __shared__ uint32_t counts[KEEP_MOST / 64];  // of a wave's 64 rows: above the threshold (from bit 16 on), equal to it
+    __shared__ uint32_t sums[WAVES];
+    __shared__ uint32_t found[4];
+    __shared__ int list[KEEP_LIST];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int bh = blockIdx.y, b = bh / t.H, h = bh - b * t.H;
+    const int j0 = blockIdx.x * each, j1 = imin(j0 + each, t.R);  // the places that are this workgroup's
+    int n = t.lengths ? t.lengths[b] : t.S;
+    n = n < 0 ? 0 : imin(n, t.S);
+    int* const rows = t.rows + (long)bh * t.R;
+    const float* const w = t.weight + (long)b * t.w_bs + (long)h * t.w_hs;
+    if (n <= t.R) {
+        for (int j = j0 + tid; j < j1; j += KEEP_THREADS) {
+            rows[j] = j < n ? j : -1;
+            list[j - j0] = j < n ? j : -1;
+        }
+    } else {
+        uint32_t low = ~0u, high = 0u;
+        const int last = n - t.last, groups = ceil_div(n, KEEP_THREADS);
+#pragma unroll 4
+        for (int r = tid; r < n; r += KEEP_THREADS) {
+            const bool forced = r < t.first || r >= last;
+            const uint32_t key = forced ? ~0u : order_of(w[r]);
+            keys[r] = key;
+            low = !forced && key < low ? key : low;
+            high = !forced && key > high ? key : high;
+        }
+        if (tid == 0) found[0] = ~0u, found[1] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t l = __shfl_xor((int)low, x), g = __shfl_xor((int)high, x);
+            low = l < low ? l : low;
+            high = g > high ? g : high;
+        }
+        if (lane == 0) {
+            atomicMin(&found[0], low);
+            atomicMax(&found[1], high);
+        }
+        __syncthreads();
+        low = found[0], high = found[1];
+        int need = t.R - imin(t.first, n) - t.last;  // of the keys in [low, high] the highest
+        if (need <= 0) low = high = ~0u;             // (only the forced ones)
+        while (low < high) {
+            const int shift = imax(32 - __builtin_clz(high - low) - 11, 0);
+            for (int i = tid; i < KEEP_BINS; i += KEEP_THREADS) bins[i] = 0;
+            __syncthreads();
+#pragma unroll 4
+            for (int r = tid; r < n; r += KEEP_THREADS) {
+                const uint32_t key = keys[r];
+                if (key >= low && key <= high) atomicAdd(&bins[(key - low) >> shift], 1);
+            }
+            __syncthreads();
+            // counts from the highest bin down: thread i has bins 2047 - 2 i and 2046 - 2 i
+            const int hi = bins[KEEP_BINS - 1 - 2 * tid], lo = bins[KEEP_BINS - 2 - 2 * tid];
+            int upto = hi + lo;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) {
+                const int v = __shfl_up(upto, x);
+                if (lane >= x) upto += v;
+            }
+            if (lane == 63) sums[wave] = upto;
+            __syncthreads();
+            for (int i = 0; i < wave; i++) upto += sums[i];
+            const int before = upto - hi - lo;
+            if (before < need && upto >= need) {
+                const bool first = before + hi >= need;
+                found[2] = KEEP_BINS - (first ? 1 : 2) - 2 * tid;
+                found[3] = need - before - (first ? 0 : hi);
+            }
+            __syncthreads();
+            const uint32_t from = low + (found[2] << shift);
+            need = (int)found[3];
+            const uint32_t to = from + ((1u << shift) - 1);
+            high = to < high ? to : high;
+            low = from;
+        }
+        // rows above the threshold (the forced ones are), of those equal to it the first `need`: how many each wave's 64 have
+        if (low == ~0u) low = ~0u - 1, need = 0;
+        const uint64_t below = (1ull << lane) - 1;
+        for (int i = 0; i < groups; i++) {
+            const int r = i * KEEP_THREADS + tid;
+            const uint32_t key = r < n ? keys[r] : 0u;
+            const uint64_t above = __ballot(r < n && key > low), equal = __ballot(r < n && key == low);
+            if (lane == 0) counts[i * WAVES + wave] = ((uint32_t)__popcll(above) << 16) | (uint32_t)__popcll(equal);
+        }
+        __syncthreads();
+        uint32_t upto = tid < groups * WAVES ? counts[tid] : 0u;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t v = __shfl_up((int)upto, x);
+            if (lane >= x) upto += v;
+        }
+        if (lane == 63) sums[wave] = upto;
+        __syncthreads();
+        if (tid < groups * WAVES) {
+            for (int i = 0; i < wave; i++) upto += sums[i];
+            counts[tid] = upto - counts[tid];
+        }
+        __syncthreads();
+        for (int i = 0; i < groups; i++) {
+            const int r = i * KEEP_THREADS + tid;
+            const uint32_t key = r < n ? keys[r] : 0u;
+            const bool is_above = r < n && key > low, is_equal = r < n && key == low;
+            const uint64_t above = __ballot(is_above), equal = __ballot(is_equal);
+            const uint32_t front = counts[i * WAVES + wave];
+            const int e = (int)(front & 0xffffu) + __popcll(equal & below);
+            const int place = (int)(front >> 16) + __popcll(above & below) + imin(e, need);
+            if (is_above || (is_equal && e < need)) {
+                if (blockIdx.x == 0) rows[place] = r;
+                if (place >= j0 && place < j1) list[place - j0] = r;
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int CPR = D / 8, RPP = KEEP_THREADS / CPR, AHEAD = 4;  // rows of a pass, passes under way
+    const int c = tid % CPR;
+    for (int i0 = tid / CPR; i0 < j1 - j0; i0 += AHEAD * RPP) {
+        u32x4_t k[AHEAD], v[AHEAD];
+        int r[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            r[u] = i0 + u * RPP < j1 - j0 ? list[i0 + u * RPP] : -1;
+            const long from = (long)b * t.k_bs + (long)h * t.k_hs + (long)imax(r[u], 0) * t.k_rs + 8 * c;
+            if (r[u] >= 0) {
+                k[u] = __builtin_nontemporal_load((const u32x4_t*)(t.k + from));
+                v[u] = __builtin_nontemporal_load((const u32x4_t*)(t.v + from));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            if (r[u] < 0) continue;
+            const int j = j0 + i0 + u * RPP;
+            const long to = (long)b * t.c_bs + (long)h * t.c_hs + (long)j * t.c_rs + 8 * c;
+            *(u32x4_t*)(t.kc + to) = k[u];
+            *(u32x4_t*)(t.vc + to) = v[u];
+            if (c == 0) {
+                t.cweight[(long)bh * t.R + j] = w[r[u]];
+                t.cposition[(long)bh * t.R + j] = r[u];
+            }
+        }
+    }
+}
+
 }  // namespace
 
 size_t evict_attention_workspace_bytes(int B, int H, int share, int D, int R) {
@@ -372,9 +533,25 @@ hipError_t launch_evict_attention(const EvictStep& t, int D, float sm_scale, voi
 }
 
 hipError_t launch_evict_keep(const EvictKeep& t, int D, hipStream_t st) {
-    hipLaunchKernelGGL(keep_select_kernel, dim3(t.B * t.H), dim3(KEEP_THREADS), 0, st, t);
+    const int heads = t.B * t.H;
+    if (t.S <= KEEP_MOST) {
+        // two workgroups a CU, of 256 places or more: each makes the whole choice
+        const int share = std::max((t.R + KEEP_LIST - 1) / KEEP_LIST, std::min((KEEP_WGS + heads - 1) / heads, (t.R + 255) / 256));
+        const int each = (t.R + share - 1) / share;
+        const dim3 grid((t.R + each - 1) / each, heads);
+        const int lds = t.S * 4;
+        if (lds > 32 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(D == 64 ? (const void*)keep_kernel<64> : (const void*)keep_kernel<128>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, KEEP_MOST * 4);
+            if (e != hipSuccess) return e;
+        }
+        if (D == 64) hipLaunchKernelGGL((keep_kernel<64>), grid, dim3(KEEP_THREADS), lds, st, t, each);
+        else hipLaunchKernelGGL((keep_kernel<128>), grid, dim3(KEEP_THREADS), lds, st, t, each);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(keep_select_kernel, dim3(heads), dim3(KEEP_THREADS), 0, st, t);
     const int per = 256 / (D / 8);
-    const dim3 grid((t.R + per - 1) / per, t.B * t.H);
+    const dim3 grid((t.R + per - 1) / per, heads);
     if (D == 64)
         hipLaunchKernelGGL((keep_gather_kernel<64>), grid, dim3(256), 0, st, t);
     else

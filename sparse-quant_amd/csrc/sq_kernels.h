@@ -212,7 +212,7 @@ struct LogitRules {
     long x_rs, y_rs, id_rs, id_ps, len_s, gen_s, bid_rs, b_rs, mask_rs;
     int M, V, L, nb;
 };
-size_t logit_rules_workspace_bytes(int M, int V);
+size_t logit_rules_workspace_bytes(int M, int V, int L, int nb);
 hipError_t launch_logit_rules(const LogitRules& t, int elem_bytes, void* workspace, hipStream_t st);
 
 // sq_lm_head.hip: the ends of a greedy decode step around the W4A16 layers (the end-to-end harness).

@@ -72,7 +72,7 @@ SIGNATURES = {
     "sq_attention_weights_workspace_bytes": (ctypes.c_size_t, [_i] * 5),
     "sq_attention_weights": (_i, [_vp] * 4 + [_i] * 6 + [_vp, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
     "sq_evict_keep": (_i, [_vp] * 9 + [_i] * 7 + [_vp, _vp]),
-    "sq_logit_rules_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "sq_logit_rules_workspace_bytes": (ctypes.c_size_t, [_i] * 4),
     "sq_logit_rules": (_i, [_vp, _vp, _i] + [_vp] * 10 + [_i] * 4 + [_vp, _vp, ctypes.c_size_t, _vp]),
     "sq_embed_rows": (_i, [_vp, _vp, _vp, _vp, ctypes.c_longlong, _vp, _i, _i, ctypes.c_longlong, ctypes.c_longlong, _vp]),
     "sq_f16_gemv_parts": (_i, [_i]),

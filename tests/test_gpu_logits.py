@@ -42,7 +42,8 @@ def call(logits, x, d, **kw):
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
-@pytest.mark.parametrize("m,v", [(1, 1), (2, 7), (3, 33), (1, 2048), (5, 2049), (2, 10007), (300, 9000), (1, 50272)])
+@pytest.mark.parametrize("m,v", [(1, 1), (2, 7), (3, 33), (1, 2048), (5, 2049), (2, 10007), (300, 9000), (1, 50272), (2, 65528),
+                                 (2, 65529), (40, 70001)])
 @pytest.mark.parametrize("length,nb,mask_rows", [(0, 0, 0), (1, 0, 0), (300, 5, 1), (0, 700, 0), (40, 0, 2)])
 def test_rules(logits, dtype, m, v, length, nb, mask_rows):
     rng = np.random.default_rng(v + length)
@@ -58,6 +59,19 @@ def test_rules(logits, dtype, m, v, length, nb, mask_rows):
     size = 8 * 2.0 ** -24 * (np.abs(exact) + 80) + np.finfo(dtype).eps / 2 * np.abs(exact)
     assert (np.abs(y.astype(np.float64) - exact)[fin] <= size[fin]).all() and np.array_equal(np.isfinite(y), fin)
     assert np.array_equal(token.cpu().numpy(), so.best_token(steps))
+
+
+@pytest.mark.parametrize("length,nb", [(16383, 512), (16384, 5), (300, 513), (70000, 6), (20, 33000)])
+def test_long_texts_and_many_biases(logits, length, nb):
+    # one token fills the text: its count passes what a half word, then what a word's half holds
+    rng = np.random.default_rng(length)
+    m, v = 2, 5000
+    x, d = make(rng, m, v, length, nb, np.float32, 0)
+    d["ids"][0], d["lengths"][:], d["generated"][:] = 77, length, 1
+    d["frequency"][:] = 2.0 ** -10
+    y, token = call(logits, dev(x), d)
+    want = so.logit_rules(x, dtype=np.float32, **d)
+    assert np.array_equal(y.cpu().numpy(), want) and np.array_equal(token.cpu().numpy(), so.best_token(want))
 
 
 def test_ties_nan_and_rows_without_a_token(logits):

@@ -107,7 +107,7 @@ def test_logit_rules_refuse_before_any_launch(L):
     for name in ("ids", "lengths", "gen", "rep", "pres", "freq", "bias_ids", "bias", "mask", "token"):
         assert call(**{name: odd}) == capi.SQ_ERR_MISALIGNED, name
     assert call(x=odd, elem=4) == capi.SQ_ERR_MISALIGNED
-    assert call(ws=None) == call(size=4) == capi.SQ_ERR_WORKSPACE
+    assert call(ws=None) == call(size=4) == call(ws=odd) == capi.SQ_ERR_WORKSPACE
     assert call(M=0) == capi.SQ_OK
 
 
