@@ -23,11 +23,15 @@ __device__ __forceinline__ short4_t lds_read_tr(const uint8_t* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
 }
 
-// A pointer that is the same in all lanes, in scalar registers.
+// A pointer that is the same in all lanes, in scalar registers, for the direct loads.  A memory instruction may read a scalar
+// register five wait states after a vector instruction has written it (v_readfirstlane is one), and the compiler does not
+// count them in front of inline assembly: they are here.
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
     const uint64_t u = (uint64_t)(uintptr_t)p;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
-    return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+    uint64_t both = ((uint64_t)hi << 32) | lo;
+    asm volatile("s_nop 4" : "+s"(both));
+    return (const uint8_t*)(uintptr_t)both;
 }
 
 }  // namespace sq
