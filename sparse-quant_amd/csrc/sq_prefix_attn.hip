@@ -21,13 +21,14 @@ namespace {
 
 constexpr int PA_STEP = 64;  // keys of a step
 
-// How a call is cut: packed rows against the prefix (a), tiles of a sequence against its rows, or the prefix and its rows (b).
+// How a call is cut.  Packed: rows of all sequences against pieces of the prefix (a), a sequence's against pieces of its own rows
+// (b).  Otherwise tiles of a sequence's rows against the prefix and its own rows, as `Deal` has it.
 struct PrefixPlan {
-    float* po;  // partial outputs [H][parts][T * share][D], then (maximum, sum) of each
+    float* po;  // partial outputs, then (maximum, sum) of each
     float2* pml;
     int packed, qa, qb, rows_b;                                // tiles of 32 qa and 32 qb rows
     int tiles_a, parts_a, steps_a, tiles_b, parts_b, steps_b;  // steps of 64 keys of a part
-    int units_a, units_b, grid_a, grid_b;
+    int units_a, units_b, grid_a, grid_b, most;                // most: parts that a tile may be cut into
     Divisor by_share, by_tiles_a, by_parts_a, by_tiles_b, by_parts_b;
 };
 
@@ -120,11 +121,50 @@ __device__ __forceinline__ Reach reach_of(const PrefixAttn& t, const PrefixPlan&
     return r;
 }
 
+// Tiles that go through the prefix and on through their own rows.  A launch has room for PA_SLOTS workgroups at a time and the
+// tiles take about as long as each other: those of the full rounds are a workgroup's each, the rest, which would leave most of
+// the last round empty, is cut into as many parts as fill it (616 tiles: 2 rounds, now 1 and a fifth).
+constexpr int PA_SLOTS = 512;
+struct Deal {
+    int tiles;              // of a head
+    int full, rest, parts;  // tiles of full rounds, the others, and the parts of each of those
+};
+__host__ __device__ __forceinline__ Deal deal_of(int tiles, int heads, int most) {
+    Deal d;
+    const int all = tiles * heads;
+    d.tiles = tiles;
+    d.full = all / PA_SLOTS * PA_SLOTS;
+    d.rest = all - d.full;
+    d.parts = d.rest ? PA_SLOTS / d.rest : 1;
+    d.parts = d.parts < 1 ? 1 : d.parts > most ? most : d.parts;
+    return d;
+}
+__device__ __forceinline__ Deal deal_of(const PrefixAttn& t, const PrefixPlan& p) {
+    int tiles = p.tiles_b;
+    if (t.starts) {
+        const int lane = threadIdx.x & 63;
+        tiles = 0;
+        for (int b0 = 0; b0 < t.B; b0 += 64) {
+            int first = 0, count = 0;
+            if (b0 + lane < t.B) tokens_of(t, b0 + lane, first, count);
+            int sum = ceil_div(count * t.share, p.rows_b);
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+            // (starts of any content may let sequences overlap: what the launch has no workgroups for is left out)
+            tiles = imin(tiles + sum, p.tiles_b);
+        }
+        tiles = __builtin_amdgcn_readfirstlane(tiles);
+    }
+    return deal_of(tiles, t.H, p.most);
+}
+
 // A piece of work: rows of a key/value head against a range of steps.
 struct Work {
-    int head, part, row0, rows;  // rows row0 .. row0 + rows - 1 of the head's T * share
-    int s0, s1;                  // steps
-    bool shared;                 // against the prefix alone
+    int head, row0, rows;  // rows row0 .. row0 + rows - 1 of the head's T * share
+    int s0, s1;            // steps
+    bool shared;           // against the prefix alone
+    bool direct;           // all that the rows see: the result; otherwise a part of it, row r at place + r of the parts
+    long place;
     Tile tl;
     Reach rc;
 };
@@ -187,18 +227,16 @@ __device__ __forceinline__ void add_odd(const PrefixAttn& t, const Work& w, int 
 template <int D>
 __device__ __forceinline__ void store_row(const PrefixArgs& a, const Work& w, int row, int col, float4_t o, float m, float l) {
     const PrefixAttn& t = a.t;
-    const PrefixPlan& p = a.p;
-    if (p.parts_a + p.parts_b == 1) {
-        const int token = p.by_share(row);
+    if (w.direct) {
+        const int token = a.p.by_share(row);
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: 0
         half4_t h;
 #pragma unroll
         for (int j = 0; j < 4; j++) h[j] = (half_t)(o[j] * inv);
         *(half4_t*)(t.o + ((long)token * (t.H * t.share) + w.head * t.share + row - token * t.share) * D + col) = h;
     } else {
-        const long slot = ((long)w.head * (p.parts_a + p.parts_b) + w.part) * ((long)t.T * t.share) + row;
-        *(float4_t*)(p.po + slot * D + col) = o;
-        if (col == 0) p.pml[slot] = make_float2(m, l);
+        *(float4_t*)(a.p.po + (w.place + row) * D + col) = o;
+        if (col == 0) a.p.pml[w.place + row] = make_float2(m, l);
     }
 }
 
@@ -500,40 +538,69 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PrefixArgs a) {
     int index = blockIdx.x;
     Work w = {};
     if constexpr (QA > 0) {
+        // (a part's place: [head][parts_a, then parts_b][T * share])
+        const int parts = p.parts_a + p.parts_b, all = t.T * t.share;
         if (index < p.grid_a) {
-            const int work = (index & 7) * (p.grid_a >> 3) + (index >> 3);  // an eighth of the list per XCD: a prefix piece's tiles share an L2
+            const int work = (index & 7) * (p.grid_a >> 3) + (index >> 3);  // an eighth of the list per XCD: a piece's tiles share an L2
             if (work >= p.units_a) return;
             const int rest = p.by_tiles_a(work);
             w.row0 = (work - rest * p.tiles_a) * (32 * QA);
             w.head = p.by_parts_a(rest);
-            w.part = rest - w.head * p.parts_a;
-            w.rows = imin(32 * QA, t.T * t.share - w.row0);
-            w.s0 = w.part * p.steps_a;
+            const int part = rest - w.head * p.parts_a;
+            w.rows = imin(32 * QA, all - w.row0);
+            w.s0 = part * p.steps_a;
             w.s1 = imin(w.s0 + p.steps_a, ceil_div(t.P, PA_STEP));
             w.shared = true;
+            w.place = ((long)w.head * parts + part) * all;
             if constexpr (QA != QB) {
                 attend<D, QA>(a, w, lds, stat);
                 return;
             }
         }
         index -= p.grid_a;
-    }
-    if (index < p.grid_b) {
-      if (!w.shared) {
-        const int work = (index & 7) * (p.grid_b >> 3) + (index >> 3);
-        if (work >= p.units_b) return;
-        const int rest = p.by_tiles_b(work);
-        w.head = p.by_parts_b(rest);
-        const int part = rest - w.head * p.parts_b;
-        if (!tile_of(t, 32 * QB, p.tiles_b - 1 - (work - rest * p.tiles_b), w.tl)) return;
+        if (index < p.grid_b) {
+            if (!w.shared) {
+                const int work = (index & 7) * (p.grid_b >> 3) + (index >> 3);
+                if (work >= p.units_b) return;
+                const int rest = p.by_tiles_b(work);
+                w.head = p.by_parts_b(rest);
+                const int part = rest - w.head * p.parts_b;
+                if (!tile_of(t, 32 * QB, p.tiles_b - 1 - (work - rest * p.tiles_b), w.tl)) return;
+                w.rc = reach_of(t, p, w.tl);
+                w.row0 = w.tl.first * t.share + w.tl.tile * (32 * QB);
+                w.rows = imin(32 * QB, w.tl.count * t.share - w.tl.tile * (32 * QB));
+                w.s0 = part * p.steps_b;
+                w.s1 = imin(w.s0 + p.steps_b, w.rc.steps);
+                if (w.s0 >= w.s1 && part > 0) return;  // (the first part also stands for rows that see nothing)
+                w.place = ((long)w.head * parts + p.parts_a + part) * all;
+            }
+            attend<D, QB>(a, w, lds, stat);
+            return;
+        }
+    } else if (index < p.grid_b) {
+        const Deal d = deal_of(t, p);
+        int at = index, part = 0;
+        if (index < d.full) {
+            at = (index & 7) * (d.full >> 3) + (index >> 3);  // an eighth of the list per XCD: a head's tiles share an L2
+        } else {
+            at = index - d.full;
+            if (at >= d.rest * d.parts) return;
+            part = at / d.rest;
+            at += d.full - part * d.rest;
+        }
+        w.head = at / d.tiles;
+        if (!tile_of(t, 32 * QB, at - w.head * d.tiles, w.tl)) return;
         w.rc = reach_of(t, p, w.tl);
         w.row0 = w.tl.first * t.share + w.tl.tile * (32 * QB);
         w.rows = imin(32 * QB, w.tl.count * t.share - w.tl.tile * (32 * QB));
-        w.s0 = part * p.steps_b;
-        w.s1 = imin(w.s0 + p.steps_b, w.rc.steps);
-        if (w.s0 >= w.s1 && part > 0) return;  // (the first part also stands for rows that see nothing)
-        w.part = p.parts_a + part;
-      }
+        w.s1 = w.rc.steps;
+        w.direct = index < d.full || d.parts == 1;
+        if (!w.direct) {
+            const int each = ceil_div(w.rc.steps, d.parts);
+            w.s0 = imin(part * each, w.rc.steps);
+            w.s1 = imin(w.s0 + each, w.rc.steps);
+            w.place = (long)((at - d.full) * d.parts + part) * (32 * QB) - w.row0;
+        }
         attend<D, QB>(a, w, lds, stat);
         return;
     }
@@ -557,55 +624,40 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PrefixArgs a) {
     }
 }
 
-// The parts of a row (token, query head), a row per wave.
+// The parts of a row, `apart` places from each other, by a wave: its output.
 template <int D>
-__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
-    const PrefixAttn& t = a.t;
-    const PrefixPlan& p = a.p;
+__device__ __forceinline__ void join_row(const PrefixPlan& p, long place, long apart, int parts, half_t* out) {
     constexpr int EPL = D / 64;
     typedef float vec_t __attribute__((ext_vector_type(EPL)));
     typedef half_t hvec_t __attribute__((ext_vector_type(EPL)));
     const int lane = threadIdx.x & 63;
-    const int index = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int heads = t.H * t.share;
-    const int token = index / heads;
-    if (token >= t.T) return;
-    const int qhead = index - token * heads;
-    const int head = qhead / t.share;
-    Tile tl;
-    tl.b = sequence_of(t, token);
-    if (tl.b < 0) return;
-    tokens_of(t, tl.b, tl.first, tl.count);
-    const int row = token * t.share + qhead - head * t.share;
-    tl.tile = (row - tl.first * t.share) / p.rows_b;
-    const Reach rc = reach_of(t, p, tl);
-    const int total = p.parts_a + p.parts_b;
-    const int parts = p.parts_a + imin(imax(ceil_div(rc.steps, p.steps_b), 1), p.parts_b);
-    const long rows = (long)t.T * t.share;
-    const long slot = (long)head * total * rows + row;
     float m = -INFINITY, l = 0.f;
     vec_t o = {};
     for (int s0 = 0; s0 < parts; s0 += 64) {
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (s0 + lane < parts) ml = p.pml[slot + (s0 + lane) * rows];
+        if (s0 + lane < parts) ml = p.pml[place + (s0 + lane) * apart];
+        const int n = imin(parts - s0, 64);
+        vec_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = *(const vec_t*)(p.po + (place + (s0 + imin(j, n - 1)) * apart) * D + EPL * lane);
         float mx = ml.x;
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+        for (int y = 1; y < 64; y <<= 1) mx = fmaxf(mx, __shfl_xor(mx, y));
         mx = fmaxf(mx, m);
         const float w = share_of(ml, mx);
         float ls = ml.y * w;
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) ls += __shfl_xor(ls, x);
+        for (int y = 1; y < 64; y <<= 1) ls += __shfl_xor(ls, y);
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
         l = l * f + ls;
         o *= f;
         m = mx;
-        const int n = imin(parts - s0, 64);
+#pragma unroll 1
         for (int s = 0; s < n; s += 8) {
-            vec_t x[8];
+            if (s > 0) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                x[j] = *(const vec_t*)(p.po + (slot + (s0 + imin(s + j, n - 1)) * rows) * D + EPL * lane);
+                for (int j = 0; j < 8; j++) x[j] = *(const vec_t*)(p.po + (place + (s0 + imin(s + j, n - 1)) * apart) * D + EPL * lane);
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (s + j < n) o += x[j] * bit_cast<float>(__builtin_amdgcn_readlane(bit_cast<int>(w), s + j));
@@ -615,14 +667,64 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
     hvec_t h;
 #pragma unroll
     for (int i = 0; i < EPL; i++) h[i] = (half_t)(o[i] * inv);
-    *(hvec_t*)(t.o + ((long)token * heads + qhead) * D + EPL * lane) = h;
+    *(hvec_t*)(out + EPL * lane) = h;
+}
+
+// Packed: a row (token, query head) per wave.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
+    const PrefixAttn& t = a.t;
+    const PrefixPlan& p = a.p;
+    const int index = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int heads = t.H * t.share;
+    const int token = index / heads;
+    if (token >= t.T) return;
+    const int qhead = index - token * heads, head = p.by_share(qhead);
+    Tile tl;
+    tl.b = sequence_of(t, token);
+    if (tl.b < 0) return;
+    tokens_of(t, tl.b, tl.first, tl.count);
+    const int row = token * t.share + qhead - head * t.share;
+    tl.tile = (row - tl.first * t.share) / p.rows_b;
+    const Reach rc = reach_of(t, p, tl);
+    const int total = p.parts_a + p.parts_b;
+    const long rows = (long)t.T * t.share;
+    join_row<D>(p, (long)head * total * rows + row, rows, p.parts_a + imin(imax(ceil_div(rc.steps, p.steps_b), 1), p.parts_b),
+                t.o + (long)index * D);
+}
+
+// Otherwise: 16 rows of a tile that was cut, four per wave.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_join_tiles_kernel(PrefixArgs a) {
+    const PrefixAttn& t = a.t;
+    const PrefixPlan& p = a.p;
+    const Deal d = deal_of(t, p);
+    const int at = blockIdx.y;
+    if (d.parts == 1 || at >= d.rest) return;
+    const int head = (d.full + at) / d.tiles;
+    Tile tl;
+    if (!tile_of(t, p.rows_b, d.full + at - head * d.tiles, tl)) return;
+    const int row0 = tl.first * t.share + tl.tile * p.rows_b;
+    const int rows = imin(p.rows_b, tl.count * t.share - tl.tile * p.rows_b);
+    for (int i = 0; i < 4; i++) {
+        const int r = blockIdx.x * 16 + 4 * i + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (r >= rows) return;
+        const int token = p.by_share(row0 + r);
+        join_row<D>(p, (long)at * d.parts * p.rows_b + r, p.rows_b, d.parts,
+                    t.o + ((long)token * (t.H * t.share) + head * t.share + row0 + r - token * t.share) * D);
+    }
 }
 
 int div_up(long a, long b) { return (int)((a + b - 1) / b); }
 int pad8(long n) { return (int)((n + 7) / 8 * 8); }
 
-// Workgroups that the pieces of a launch are cut for: two per CU.
-constexpr int PA_WGS = 512;
+// Workgroups that packed rows' pieces are cut for.  Against the prefix a piece writes its rows' sums: two pieces per three CUs
+// for tiles of 128 rows (64 sequences of 32 heads behind 8192 rows, 8 key/value heads: 62 us with 512 pieces, 47 with 256, 44
+// with 128; behind 16384: 67, 55, 57 and 51 with 192), more where a tile has up to 32.
+constexpr int PA_WGS_MANY = 160, PA_WGS_FEW = 256;
+// Against their own rows, of different numbers and up to the caches' room: four per CU (ragged up to 1000 rows 46.1 us with 512,
+// 42.8 with 1024, 48 with 4096).
+constexpr int PA_WGS_OWN = 1024;
 
 }  // namespace
 
@@ -639,19 +741,25 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
     if (packed) {
         p.tiles_a = div_up(rows, 32 * p.qa);
         const long steps = (long)H * p.tiles_a * pre;
-        p.steps_a = std::max(div_up(steps, PA_WGS), 1);
+        p.steps_a = std::max(div_up(steps, p.qa == 1 ? PA_WGS_FEW : PA_WGS_MANY), 1);
         if (p.qa == 1) p.steps_a = (p.steps_a + 1) / 2 * 2;
         p.parts_a = div_up(pre, p.steps_a);
         p.units_a = H * p.parts_a * p.tiles_a;
     }
     p.tiles_b = ragged ? (int)(rows / p.rows_b + B) : B * div_up((long)(T / B) * share, p.rows_b);
-    const int steps_b = own + (packed ? 0 : pre);
-    p.steps_b = std::max(div_up((long)p.tiles_b * H * steps_b, PA_WGS), 1);
-    if (p.qb == 1) p.steps_b = (p.steps_b + 1) / 2 * 2;
-    p.parts_b = std::max(div_up(steps_b, p.steps_b), 1);
-    p.units_b = H * p.parts_b * p.tiles_b;
+    if (packed) {
+        p.steps_b = std::max(div_up((long)p.tiles_b * H * own, PA_WGS_OWN), 1);
+        p.steps_b = (p.steps_b + 1) / 2 * 2;  // (four waves' blocks of 32)
+        p.parts_b = std::max(div_up(own, p.steps_b), 1);
+        p.units_b = H * p.parts_b * p.tiles_b;
+        p.grid_b = pad8(p.units_b);
+    } else {
+        p.steps_b = p.parts_b = 1;
+        p.most = std::max(std::min((own + pre) / 4, p.qb == 1 ? 64 : 8), 1);  // parts of four steps or more
+        const int all = p.tiles_b * H;
+        p.grid_b = ragged ? all / PA_SLOTS * PA_SLOTS + PA_SLOTS : all / PA_SLOTS * PA_SLOTS + all % PA_SLOTS * deal_of(p.tiles_b, H, p.most).parts;
+    }
     p.grid_a = pad8(p.units_a);
-    p.grid_b = pad8(p.units_b);
     p.by_share = Divisor::of(share);
     p.by_tiles_a = Divisor::of(std::max(p.tiles_a, 1));
     p.by_parts_a = Divisor::of(std::max(p.parts_a, 1));
@@ -660,10 +768,19 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
     return p;
 }
 
+namespace {
+// Rows that parts have room for.
+size_t part_rows(const PrefixPlan& p, int T, int H, int share, bool ragged) {
+    if (p.packed) return (size_t)(p.parts_a + p.parts_b) * H * T * share;
+    const Deal d = deal_of(p.tiles_b, H, p.most);
+    if (!ragged) return d.parts == 1 ? 0 : (size_t)d.rest * d.parts * p.rows_b;
+    // (fewer tiles than the launch has room for may be cut into more parts, of up to PA_SLOTS in all)
+    return p.most == 1 ? 0 : (size_t)std::min<long>(PA_SLOTS, (long)p.tiles_b * H * p.most) * p.rows_b;
+}
+}  // namespace
+
 size_t prefix_attention_workspace_bytes(int T, int B, int H, int share, int D, int P, int Lmax, bool ragged) {
-    const PrefixPlan p = prefix_plan(T, B, H, share, P, Lmax, ragged);
-    const size_t parts = p.parts_a + p.parts_b;
-    return parts == 1 ? 0 : parts * H * T * share * (D + 2) * sizeof(float);
+    return part_rows(prefix_plan(T, B, H, share, P, Lmax, ragged), T, H, share, ragged) * (D + 2) * sizeof(float);
 }
 
 hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, void* workspace, hipStream_t st) {
@@ -671,9 +788,9 @@ hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, v
     a.t = t;
     a.p = prefix_plan(t.T, t.B, t.H, t.share, t.P, t.Lmax, t.starts != nullptr);
     a.qk_scale = sm_scale * 1.44269504f;
-    const int parts = a.p.parts_a + a.p.parts_b;
+    const size_t rows = part_rows(a.p, t.T, t.H, t.share, t.starts != nullptr);
     a.p.po = (float*)workspace;
-    a.p.pml = (float2*)(a.p.po + (size_t)parts * t.H * t.T * t.share * D);
+    a.p.pml = (float2*)(a.p.po + rows * D);
     const dim3 pieces(a.p.grid_a + a.p.grid_b + (t.kn ? (t.T + 3) / 4 : 0));
 #define SQ_PREFIX_LAUNCH(QA_, QB_)                                                                  \
     if (D == 64) hipLaunchKernelGGL((prefix_attn_kernel<64, QA_, QB_>), pieces, dim3(256), 0, st, a); \
@@ -693,12 +810,16 @@ hipError_t launch_prefix_attention(const PrefixAttn& t, int D, float sm_scale, v
     }
 #undef SQ_PREFIX_LAUNCH
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || parts == 1) return e;
-    const dim3 grid(div_up((long)t.T * t.H * t.share, 4));
-    if (D == 64)
-        hipLaunchKernelGGL((prefix_join_kernel<64>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((prefix_join_kernel<128>), grid, dim3(256), 0, st, a);
+    if (e != hipSuccess || rows == 0) return e;
+    if (a.p.packed) {
+        const dim3 grid(div_up((long)t.T * t.H * t.share, 4));
+        if (D == 64) hipLaunchKernelGGL((prefix_join_kernel<64>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((prefix_join_kernel<128>), grid, dim3(256), 0, st, a);
+    } else {
+        const dim3 grid(a.p.rows_b / 16, std::min(PA_SLOTS - 1, a.p.tiles_b * t.H));
+        if (D == 64) hipLaunchKernelGGL((prefix_join_tiles_kernel<64>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((prefix_join_tiles_kernel<128>), grid, dim3(256), 0, st, a);
+    }
     return hipGetLastError();
 }
 
