@@ -100,9 +100,10 @@ struct RowsAttn {
     // all rows see, and the last that this lane's row sees; scored(block, st) is given the scores in units of log2 (this lane's
     // row, keys 8 i + 4 (lane / 32) + 0..3).  EXACT: the sum is that of the unrounded exponentials, otherwise of those that meet
     // the values.
-    template <bool EXACT, class Issue, class Seen, class Keys, class Values, class Scored>
-    __device__ __forceinline__ void run(uint8_t* lds, int blk, int blk1, float qk_scale, Issue issue, Seen seen, Keys keys,
-                                        Values values, Scored scored) {
+    // prepare() is called by all waves, behind the first requests.
+    template <bool EXACT, class Prepare, class Issue, class Seen, class Keys, class Values, class Scored>
+    __device__ __forceinline__ void run(uint8_t* lds, int blk, int blk1, float qk_scale, Prepare prepare, Issue issue, Seen seen,
+                                        Keys keys, Values values, Scored scored) {
         const int lane = threadIdx.x & 63, ln = lane & 31, lc = lane >> 5;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         uint8_t* const kt = lds + wave * 2 * TILE;
@@ -113,9 +114,12 @@ struct RowsAttn {
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[dt][v] = 0.f;
+        if (blk < blk1) {
+            issue(blk, false, kt0);
+            issue(blk, true, kt0 + TILE);
+        }
+        prepare();
         if (blk >= blk1) return;
-        issue(blk, false, kt0);
-        issue(blk, true, kt0 + TILE);
         const int vkey = 4 * lc + ((lane & 15) >> 2);  // + 16 s + 8 i, which leave v_swz unchanged
         const int vchunk = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
         const uint8_t* const vread = vt + vkey * ROW + 8 * (lane & 1);

@@ -45,6 +45,40 @@ __device__ __forceinline__ uint64_t wave_min64(uint64_t v) {
     return v;
 }
 
+// A sequence that has seen nothing.
+template <int D>
+__device__ __forceinline__ void nothing_seen(const EvictStep& t, int bh) {
+    half_t* const out = t.o + (long)bh * t.share * D;
+    for (int i = threadIdx.x; i < t.share * D; i += 256) out[i] = (half_t)0.f;
+    if (threadIdx.x == 0) t.slot[bh] = -1;
+}
+
+// What the query heads g0 .. g0 + heads - 1 give to the rows r0 .. r0 + EJ_ROWS - 1 is added to their weights; state holds the
+// heads' maximum (in units of log2) and the reciprocal of their sum.  The row of the slot begins anew, with the first heads.
+constexpr int EJ_ROWS = 1024;
+__device__ __forceinline__ void add_weights(const EvictArgs& a, int bh, int r0, int n, int seen, int slot, const float2* state, int g0,
+                                            int heads) {
+    const EvictStep& t = a.t;
+    const int r = r0 + 4 * threadIdx.x;
+    if (r >= n) return;
+    float* const w = t.weight + (long)bh * t.R + r;
+    float4_t sum;
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum[j] = r + j < n && !(r + j == slot && g0 == 0) ? w[j] : 0.f;
+    const float* const from = a.scores + ((long)bh * t.share + g0) * a.pitch + r;
+#pragma unroll 4
+    for (int g = 0; g < heads; g++) {
+        const float4_t s = *(const float4_t*)(from + (long)g * a.pitch);
+        const float2 st = state[g];
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum[j] += __builtin_amdgcn_exp2f(s[j] - st.x) * st.y;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (r + j < n) w[j] = sum[j];
+    if (slot >= r && slot < r + 4) t.position[(long)bh * t.R + slot] = seen - 1;
+}
+
 template <int D>
 __global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
     typedef RowsAttn<D> R;
@@ -52,6 +86,7 @@ __global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS];
     __shared__ float2 stat[RA_WAVES * RA_BLOCK];
     __shared__ uint64_t least[RA_WAVES];
+    __shared__ float2 state[EV_TILE];
     const EvictStep& t = a.t;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -64,7 +99,10 @@ __global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
     const int seen = t.seen[b];
     const int n = imin(seen, t.R);  // rows attended
     const int blk0 = part * a.blocks, blk1 = imin(blk0 + a.blocks, ceil_div(n, RA_BLOCK));
-    if (blk0 >= blk1) return;  // (also where nothing was seen: the second launch writes zeros)
+    if (blk0 >= blk1) {  // (where there is a second launch it writes the zeros of a sequence that has seen nothing)
+        if (a.parts == 1 && a.tiles == 1) nothing_seen<D>(t, bh);
+        return;
+    }
 
     const int rows = imin(EV_TILE, t.share - tile * EV_TILE);
     const int g = tile * EV_TILE + imin(ln, rows - 1);
@@ -75,31 +113,41 @@ __global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
     const long n_at = (long)b * t.n_bs + (long)h * t.n_hs + 8 * chunk;
     const u32x4_t fresh_k = *(const u32x4_t*)(t.kn + n_at);
     const u32x4_t fresh_v = *(const u32x4_t*)(t.vn + n_at);
-    // Where it goes.
-    int slot = seen - 1;
-    if (seen > t.R) {
-        const float* const w = t.weight + (long)bh * t.R;
-        const int* const pos = t.position + (long)bh * t.R;
-        uint64_t best = ~0ull;
-#pragma unroll 4
-        for (int i = tid; i < t.R; i += 256) {
-            const int p = pos[i];
-            const uint32_t o = p >= t.first && p < seen - t.last ? order_of(w[i]) : ~0u;
-            const uint64_t key = ((uint64_t)o << 32) | (uint32_t)i;
-            best = key < best ? key : best;
-        }
-        best = wave_min64(best);
-        if (lane == 0) least[wave] = best;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < RA_WAVES; i++) best = least[i] < best ? least[i] : best;
-        slot = __builtin_amdgcn_readfirstlane((int)(uint32_t)best);
-    }
+    int slot = seen - 1;  // where it goes
     const long c_at = (long)b * t.c_bs + (long)h * t.c_hs;
     float* const scores = a.scores + ((long)bh * t.share + g) * a.pitch + 4 * lc;
     const bool valid = ln < rows;
     r.template run<true>(
         lds, blk0 + wave, blk1, a.qk_scale,
+        [&]() {
+            if (seen <= t.R) return;
+            const float* const w = t.weight + (long)bh * t.R;
+            const int* const pos = t.position + (long)bh * t.R;
+            uint64_t best = ~0ull;
+#pragma unroll 1
+            for (int i0 = tid; i0 < t.R; i0 += 8 * 256) {
+                int p[8];
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const int i = imin(i0 + u * 256, t.R - 1);  // (the last one again behind the last)
+                    p[u] = pos[i];
+                    v[u] = w[i];
+                }
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const uint32_t o = p[u] >= t.first && p[u] < seen - t.last ? order_of(v[u]) : ~0u;
+                    const uint64_t key = ((uint64_t)o << 32) | (uint32_t)imin(i0 + u * 256, t.R - 1);
+                    best = key < best ? key : best;
+                }
+            }
+            best = wave_min64(best);
+            if (lane == 0) least[wave] = best;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < RA_WAVES; i++) best = least[i] < best ? least[i] : best;
+            slot = __builtin_amdgcn_readfirstlane((int)(uint32_t)best);
+        },
         [&](int blk, bool value, uint32_t at) {
             const half_t* const base = (value ? t.vc : t.kc) + c_at;
             const int first = blk * RA_BLOCK;
@@ -137,90 +185,94 @@ __global__ __launch_bounds__(256, 2) void evict_attn_kernel(EvictArgs a) {
                     *(float4_t*)(scores + blk * RA_BLOCK + 8 * i) = (float4_t){st[4 * i], st[4 * i + 1], st[4 * i + 2], st[4 * i + 3]};
             }
         });
+    const bool whole = a.parts == 1 && a.tiles == 1;  // nothing is left for a second launch
+    half_t* const out = t.o + (long)bh * t.share * D;
     r.join(lds, stat, rows, [&](int i, int col, float4_t o, float m, float l) {
+        if (whole) {
+            half4_t x;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = (half_t)(o[j] / l);
+            *(half4_t*)(out + i * D + col) = x;
+            if (col == 0) state[i] = make_float2(m, 1.f / l);
+            return;
+        }
         const long at = ((long)bh * a.parts + part) * t.share + tile * EV_TILE + i;
         *(float4_t*)(a.po + at * D + col) = o;
         if (col == 0) a.pml[at] = make_float2(m, l);
     });
+    if (whole) {
+        __syncthreads();  // (the scores are in L2, and so is what the waves wrote)
+        for (int r0 = 0; r0 < n; r0 += EJ_ROWS) add_weights(a, bh, r0, n, seen, slot, state, 0, rows);
+    }
 }
 
 // The parts of a (sequence, key/value head): its outputs (first chunk of rows), and the weights of a chunk of rows.
-constexpr int EJ_ROWS = 1024;
 constexpr int EJ_HEADS = 64;  // whose maxima and sums are held at once
 
 template <int D>
 __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
     __shared__ float2 state[EJ_HEADS];
     const EvictStep& t = a.t;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int bh = blockIdx.x, b = bh / t.H;
+    const int tid = threadIdx.x;
+    const int bh = blockIdx.x, b = a.by_heads(bh);
     const int r0 = blockIdx.y * EJ_ROWS;
     const int seen = t.seen[b];
     const int n = imin(seen, t.R);
     if (r0 >= n && r0 > 0) return;
-    half_t* const out = t.o + (long)bh * t.share * D;
     if (seen <= 0) {
-        for (int i = tid; i < t.share * D; i += 256) out[i] = (half_t)0.f;
-        if (tid == 0) t.slot[bh] = -1;
+        nothing_seen<D>(t, bh);
         return;
     }
+    half_t* const out = t.o + (long)bh * t.share * D;
+    const int slot = t.slot[bh];
     const int parts = ceil_div(ceil_div(n, RA_BLOCK), a.blocks);
-    float acc[EJ_ROWS / 256];
-#pragma unroll
-    for (int i = 0; i < EJ_ROWS / 256; i++) acc[i] = 0.f;
     for (int g0 = 0; g0 < t.share; g0 += EJ_HEADS) {
         const int heads = imin(EJ_HEADS, t.share - g0);
+        const long first = (long)bh * a.parts * t.share + g0;
         __syncthreads();
-        for (int g = tid; g < heads; g += 256) {
-            const float2* ml = a.pml + (long)bh * a.parts * t.share + g0 + g;
-            float m = -INFINITY, l = 0.f;
-            for (int s = 0; s < parts; s++) m = fmaxf(m, ml[(long)s * t.share].x);
-            for (int s = 0; s < parts; s++) {
-                const float2 x = ml[(long)s * t.share];
-                l += x.y * share_of(x, m);
-            }
-            state[g] = make_float2(m, 1.f / l);
-        }
-        __syncthreads();
-        for (int g = 0; g < heads; g++) {
-            const float2 st = state[g];
-            const float* s = a.scores + ((long)bh * t.share + g0 + g) * a.pitch;
+        // a wave per head, lane s looks at part s
+        for (int g = tid >> 6; g < heads; g += 4) {
+            float2 all = make_float2(-INFINITY, 0.f);
+            for (int s0 = 0; s0 < parts; s0 += 64) {
+                const int s = s0 + (tid & 63);
+                const float2 x = s < parts ? a.pml[first + (long)s * t.share + g] : make_float2(-INFINITY, 0.f);
+                float m = fmaxf(x.x, all.x);
 #pragma unroll
-            for (int i = 0; i < EJ_ROWS / 256; i++) {
-                const int r = r0 + 256 * i + tid;
-                if (r < n) acc[i] += __builtin_amdgcn_exp2f(s[r] - st.x) * st.y;
+                for (int y = 1; y < 64; y <<= 1) m = fmaxf(m, __shfl_xor(m, y));
+                float l = x.y * share_of(x, m);
+#pragma unroll
+                for (int y = 1; y < 64; y <<= 1) l += __shfl_xor(l, y);
+                all = make_float2(m, all.y * share_of(all, m) + l);
             }
+            if ((tid & 63) == 0) state[g] = make_float2(all.x, 1.f / all.y);
         }
+        __syncthreads();
+        add_weights(a, bh, r0, n, seen, slot, state, g0, heads);
         if (blockIdx.y == 0) {
-            for (int g = wave; g < heads; g += 4) {
+            for (int i = tid; i < heads * (D / 4); i += 256) {
+                const int g = i / (D / 4), c = 4 * (i % (D / 4));
                 const float2 st = state[g];
-                const long at = (long)bh * a.parts * t.share + g0 + g;
-                for (int c = lane; c < D; c += 64) {
-                    float o = 0.f;
-                    for (int s = 0; s < parts; s++) {
-                        o += a.po[(at + (long)s * t.share) * D + c] * share_of(a.pml[at + (long)s * t.share], st.x);
-                    }
-                    out[(g0 + g) * D + c] = (half_t)(o * st.y);
+                float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int s = 0; s < parts; s++) {
+                    const long at = first + (long)s * t.share + g;
+                    o += *(const float4_t*)(a.po + at * D + c) * share_of(a.pml[at], st.x);
                 }
-            }
-        }
-    }
-    const int slot = t.slot[bh];
+                half4_t x;
 #pragma unroll
-    for (int i = 0; i < EJ_ROWS / 256; i++) {
-        const int r = r0 + 256 * i + tid;
-        if (r < n) {
-            float* w = t.weight + (long)bh * t.R + r;
-            *w = r == slot ? acc[i] : *w + acc[i];
-            if (r == slot) t.position[(long)bh * t.R + r] = seen - 1;
+                for (int j = 0; j < 4; j++) x[j] = (half_t)(o[j] * st.y);
+                *(half4_t*)(out + (g0 + g) * D + c) = x;
+            }
         }
     }
 }
 
 // Workgroups that keep's places are cut for.
 constexpr int KEEP_WGS = 512;
-// Workgroups that the caches' rows are cut for: two per CU.
-constexpr int EV_WGS = 512;
+// Workgroups that the caches' rows are cut for: one per CU, so that a chip full of heads needs no second launch (us, with 256 / 512 /
+// 1024: 8 x 32 heads x 512 rows 16.6 / 19.6 / 24.1; 32 x 8 x 4000 107.5 / 109.4 / 109.0; 2 x 32 x 2000 22.4 / 22.3 / 27.9; 4 x 8 x 4000
+// 24.7 / 24.6 / 31.5).
+constexpr int EV_WGS = 256;
 
 EvictArgs plan(int B, int H, int share, int R) {
     EvictArgs a = {};
@@ -522,13 +574,12 @@ hipError_t launch_evict_attention(const EvictStep& t, int D, float sm_scale, voi
     a.po = a.scores + (size_t)t.B * t.H * t.share * a.pitch;
     a.pml = (float2*)(a.po + (size_t)t.B * t.H * t.share * a.parts * D);
     const dim3 grid(t.B * t.H * a.tiles * a.parts), join(t.B * t.H, (t.R + EJ_ROWS - 1) / EJ_ROWS);
-    if (D == 64) {
-        hipLaunchKernelGGL((evict_attn_kernel<64>), grid, dim3(256), 0, st, a);
-        hipLaunchKernelGGL((evict_join_kernel<64>), join, dim3(256), 0, st, a);
-    } else {
-        hipLaunchKernelGGL((evict_attn_kernel<128>), grid, dim3(256), 0, st, a);
-        hipLaunchKernelGGL((evict_join_kernel<128>), join, dim3(256), 0, st, a);
-    }
+    if (D == 64) hipLaunchKernelGGL((evict_attn_kernel<64>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((evict_attn_kernel<128>), grid, dim3(256), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || (a.parts == 1 && a.tiles == 1)) return e;
+    if (D == 64) hipLaunchKernelGGL((evict_join_kernel<64>), join, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((evict_join_kernel<128>), join, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

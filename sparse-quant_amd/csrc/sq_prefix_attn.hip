@@ -257,7 +257,7 @@ __device__ __forceinline__ void few_rows(const PrefixArgs& a, const Work& w, uin
     const int end = imin(2 * w.s1, w.shared ? ceil_div(t.P, RA_BLOCK) : pre + ceil_div(w.rc.own, RA_BLOCK));
     bool odd = false;
     r.template run<false>(
-        lds, 2 * w.s0 + wave, end, a.qk_scale,
+        lds, 2 * w.s0 + wave, end, a.qk_scale, []() {},
         [&](int blk, bool value, uint32_t at) {
             const bool is_pre = blk < pre;
             const int n = (is_pre ? blk : blk - pre) * RA_BLOCK;
