@@ -417,6 +417,7 @@ __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(EvictKeep t, int eac
     __shared__ uint32_t counts[KEEP_MOST / 64];  // of a wave's 64 rows: above the threshold (from bit 16 on), equal to it
     __shared__ uint32_t sums[WAVES];
     __shared__ uint32_t found[4];
+    __shared__ uint64_t left[64];
     __shared__ int list[KEEP_LIST];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -484,6 +485,8 @@ __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(EvictKeep t, int eac
                 const bool first = before + hi >= need;
                 found[2] = KEEP_BINS - (first ? 1 : 2) - 2 * tid;
                 found[3] = need - before - (first ? 0 : hi);
+                found[1] = first ? hi : lo;
+                found[0] = 0;
             }
             __syncthreads();
             const uint32_t from = low + (found[2] << shift);
@@ -491,6 +494,29 @@ __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(EvictKeep t, int eac
             const uint32_t to = from + ((1u << shift) - 1);
             high = to < high ? to : high;
             low = from;
+            const int count = (int)found[1];
+            if (shift == 0 || count > 64) continue;
+            // few are left: each is compared with all of them
+            for (int r = tid; r < n; r += KEEP_THREADS) {
+                const uint32_t key = keys[r];
+                if (key >= low && key <= high) left[atomicAdd(&found[0], 1u)] = ((uint64_t)key << 32) | (uint32_t)~r;
+            }
+            __syncthreads();
+            if (tid < count) {
+                const uint64_t mine = left[tid];
+                int better = 0, higher = 0;
+                for (int i = 0; i < count; i++) {
+                    better += left[i] > mine;
+                    higher += (left[i] >> 32) > (mine >> 32);
+                }
+                if (better == need - 1) {  // the last that stays
+                    found[2] = (uint32_t)(mine >> 32);
+                    found[3] = need - higher;
+                }
+            }
+            __syncthreads();
+            low = high = found[2];
+            need = (int)found[3];
         }
         // rows above the threshold (the forced ones are), of those equal to it the first `need`: how many each wave's 64 have
         if (low == ~0u) low = ~0u - 1, need = 0;

@@ -164,6 +164,13 @@ __global__ __launch_bounds__(THREADS) void logit_slice_kernel(LogitArgs a) {
         v[u] = row.load(e, t.V);
         allowed[u] = row.allowed(e, t.V);
     }
+    // The first tokens of the text as well (a lane's eight), and its first bias.
+    constexpr int AHEAD = 8;
+    const int* const bias_ids = t.bias_ids + (long)m * t.bid_rs;
+    long long id[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) id[u] = tid + u * THREADS < row.n ? row.ids[(long)(tid + u * THREADS) * t.id_ps] : -1;
+    int named = tid < t.nb ? bias_ids[tid] : -1;
     const bool marks = row.n > 0 || t.nb > 0;
     auto enlist = [&](int at, Word was) {
         if (was == 0) list[atomicAdd(&listed, 1u)] = (unsigned short)at;
@@ -176,19 +183,19 @@ __global__ __launch_bounds__(THREADS) void logit_slice_kernel(LogitArgs a) {
     }
     auto place = [&](long long id) { return id >= 0 && id < t.V && id >= base && id < base + W ? (int)(id - base) : -1; };
     if (t.nb > 0) {
-        const int* const ids = t.bias_ids + (long)m * t.bid_rs;
         for (int i = tid; i < t.nb; i += THREADS) {
-            const int at = place(ids[i]);
+            const int at = place(named);
             if (at >= 0) enlist(at, atomicMax(&words[at], (Word)(i + 1) << HALF));
+            named = i + THREADS < t.nb ? bias_ids[i + THREADS] : -1;
         }
         __syncthreads();
     }
     if (row.n > 0) {
-        constexpr int AHEAD = 8;
         for (int i0 = tid; i0 < row.n; i0 += AHEAD * THREADS) {
-            long long id[AHEAD];
+            if (i0 != tid) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; u++) id[u] = i0 + u * THREADS < row.n ? row.ids[(long)(i0 + u * THREADS) * t.id_ps] : -1;
+                for (int u = 0; u < AHEAD; u++) id[u] = i0 + u * THREADS < row.n ? row.ids[(long)(i0 + u * THREADS) * t.id_ps] : -1;
+            }
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 const int at = place(id[u]);

@@ -329,10 +329,13 @@ __global__ __launch_bounds__(256, RG == 1 ? 4 : 2) void weigh_keys_kernel(WeighP
     if (lc == 0 && key < t.S) out[key] = key < n ? sum : 0.f;
 }
 
-// Workgroups that the keys are cut for in the first pass where there are few rows: eight per CU.
-constexpr int WG_WGS = 2048;
-constexpr int WG_PAIRS = 128;
-// Workgroups below which a tile of the second pass is 32 keys wide instead of 128.
+// Workgroups that the keys are cut for in the first pass where there are few rows.  The second pass joins the parts, each time it
+// needs a row: the last 64 queries of ragged prompts of up to 8191 rows, 4 x 8 heads (us): 45.7 with 512, 46.5 with 1024, 53.1
+// with 2048, 67.3 with 4096; one such prompt 25.2, 29.5, 39.6, 39.6.
+constexpr int WG_WGS = 512;
+constexpr int WG_PAIRS = 128;  // (8 x 32 heads x 2048: 425 us with 64, 413 with 128)
+// Workgroups below which a tile of the second pass is 32 keys wide instead of 128 (8 heads x 4096 keys, 4 query heads each: 263 us
+// instead of 346; 8191 keys and 64 queries of one prompt 57 instead of 30: its tiles are shorter than their beginning).
 constexpr int WG_NARROW = 512;
 
 WeighPlan plan(int B, int H, int share, int S, int window) {
