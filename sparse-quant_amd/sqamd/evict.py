@@ -101,10 +101,8 @@ def keep(k, v, weight, k_cache, v_cache, cache_weight, cache_position, keep_firs
     last keep_last are always among them.  They keep their order; their weights and places in the prompt become the cache's
     weights and positions.  Returns the places, int32 [B, kv_heads, rows], -1 behind the last.  The caches must not overlap k
     and v."""
-    for cache in (k_cache, v_cache):
-        for x in (k, v):
-            if torch.is_tensor(cache) and torch.is_tensor(x) and _overlap(cache, x):
-                raise ValueError("rows cannot be kept in the memory that they are read from")
+    if any(_overlap(cache, x) for cache in (k_cache, v_cache) for x in (k, v)) or _overlap(cache_weight, weight):
+        raise ValueError("rows cannot be kept in the memory that they are read from")
     got = quant.evict_keep(k, v, weight, k_cache, v_cache, cache_weight, cache_position, keep_first, keep_last, lengths)
     if got is not None:
         return got

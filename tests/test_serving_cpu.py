@@ -126,6 +126,9 @@ def test_python_refuses_what_is_not_on_the_device():
         evict.keep(kc, kc, torch.zeros(2, 2, 8), kc.clone(), kc.clone(), torch.zeros(2, 2, 8), torch.zeros(2, 2, 8, dtype=torch.int32), 1, 2)
     with pytest.raises(ValueError, match="memory"):
         evict.keep(kc, kc, torch.zeros(2, 2, 8), kc[:, :, :4], kc.clone(), torch.zeros(2, 2, 4), torch.zeros(2, 2, 4, dtype=torch.int32), 1, 2)
+    w = torch.zeros(2, 2, 8)
+    with pytest.raises(ValueError, match="memory"):
+        evict.keep(kc, kc, w, kc.clone()[:, :, :4], kc.clone(), w[:, :, :4], torch.zeros(2, 2, 4, dtype=torch.int32), 1, 2)
     with pytest.raises(ValueError):
         logits.apply_rules(torch.zeros(2, 10))
 
