@@ -801,6 +801,13 @@ c10::optional<std::pair<at::Tensor, at::Tensor>> logit_rules(const at::Tensor& x
     if (into.has_value() && (into->scalar_type() != x.scalar_type() || into->device() != x.device() || into->sizes() != x.sizes() ||
                              (V > 1 && into->stride(1) != 1) || (M > 1 && into->stride(0) < V)))
         return c10::nullopt;
+    if (into.has_value() && x.numel() > 0) {  // in place, or apart
+        auto end = [&](const at::Tensor& t) {
+            return (uintptr_t)t.data_ptr() + ((M - 1) * (M > 1 ? t.stride(0) : 0) + V) * t.element_size();
+        };
+        const uintptr_t a = (uintptr_t)x.data_ptr(), b = (uintptr_t)into->data_ptr();
+        if (a == b ? stride_of(x, 0) != stride_of(*into, 0) : a < end(*into) && b < end(x)) return c10::nullopt;
+    }
     if (token_into.has_value() && !whole(*token_into, x, at::kLong, {M})) return c10::nullopt;
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());

@@ -26,8 +26,8 @@ def apply_rules(logits, ids=None, lengths=None, generated_from=None, repetition=
         -inf                                                     tokens whose bit is 0
 
     Ids outside the vocabulary are none.  The best token is that of the returned logits: the lowest among equals, NaN never
-    wins, 0 where none is above -inf.  out (which may be logits) and token receive the results where they are given.  All on the
-    device and read by the kernels, so that a captured HIP graph follows them."""
+    wins, 0 where none is above -inf.  out (which may be logits, or apart from them) and token receive the results where they
+    are given.  All on the device and read by the kernels, so that a captured HIP graph follows them."""
     got = quant.logit_rules(logits, ids, lengths, generated_from, repetition, presence, frequency, bias_ids, bias, mask, out, token)
     if got is not None:
         return got if out is None and token is None else (got[0] if out is None else out, got[1] if token is None else token)
@@ -37,7 +37,7 @@ def apply_rules(logits, ids=None, lengths=None, generated_from=None, repetition=
     rows = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
     got = quant.logit_rules(rows, ids, lengths, generated_from, *given, out, token)
     if got is None:
-        raise ValueError("rules on logits %s: too large, or out overlaps itself" % (tuple(logits.shape),))
+        raise ValueError("rules on logits %s: too large, or out overlaps them in another place" % (tuple(logits.shape),))
     return got if out is None and token is None else (got[0] if out is None else out, got[1] if token is None else token)
 
 

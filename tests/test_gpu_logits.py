@@ -157,7 +157,8 @@ def test_refusals(logits):
            ((x,), {"repetition": one}), ((x, ids), {"repetition": one.half()}), ((x, ids), {"presence": one[:1]}),
            ((x,), {"bias_ids": b}), ((x,), {"bias_ids": b, "bias": b}), ((x,), {"mask": mask[:, :3]}), ((x,), {"mask": mask.long()}),
            ((x,), {"out": x.float()}), ((x,), {"out": x[:1].expand(2, -1)}), ((x,), {"token": one}), ((x[:, :0],), {}),
-           ((x,), {"mask": torch.zeros((3, 4), dtype=torch.int32, device=DEV)})]
+           ((x,), {"mask": torch.zeros((3, 4), dtype=torch.int32, device=DEV)}),
+           ((x.view(-1)[:198].view(2, 99),), {"out": x.view(-1)[1:199].view(2, 99)}), ((x[:, :50],), {"out": x.view(-1)[:100].view(2, 50)})]
     for args, kw in bad:
         with pytest.raises(ValueError):
             logits.apply_rules(*args, **kw)
