@@ -716,6 +716,8 @@ __global__ __launch_bounds__(256) void prefix_join_tiles_kernel(PrefixArgs a) {
 }
 
 int div_up(long a, long b) { return (int)((a + b - 1) / b); }
+// Steps of a piece where `steps` in all are cut for so many workgroups.
+int cut(long steps, int wgs, int most) { return (int)std::max<long>(std::min<long>((steps + wgs - 1) / wgs, most), 1); }
 int pad8(long n) { return (int)((n + 7) / 8 * 8); }
 
 // Workgroups that packed rows' pieces are cut for.  Against the prefix a piece writes its rows' sums: two pieces per three CUs
@@ -741,14 +743,14 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
     if (packed) {
         p.tiles_a = div_up(rows, 32 * p.qa);
         const long steps = (long)H * p.tiles_a * pre;
-        p.steps_a = std::max(div_up(steps, p.qa == 1 ? PA_WGS_FEW : PA_WGS_MANY), 1);
+        p.steps_a = cut(steps, p.qa == 1 ? PA_WGS_FEW : PA_WGS_MANY, pre);
         if (p.qa == 1) p.steps_a = (p.steps_a + 1) / 2 * 2;
         p.parts_a = div_up(pre, p.steps_a);
         p.units_a = H * p.parts_a * p.tiles_a;
     }
     p.tiles_b = ragged ? (int)(rows / p.rows_b + B) : B * div_up((long)(T / B) * share, p.rows_b);
     if (packed) {
-        p.steps_b = std::max(div_up((long)p.tiles_b * H * own, PA_WGS_OWN), 1);
+        p.steps_b = cut((long)p.tiles_b * H * own, PA_WGS_OWN, own);
         p.steps_b = (p.steps_b + 1) / 2 * 2;  // (four waves' blocks of 32)
         p.parts_b = std::max(div_up(own, p.steps_b), 1);
         p.units_b = H * p.parts_b * p.tiles_b;
