@@ -550,7 +550,8 @@ int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int n
  *              they were
  * lengths and starts lie on the device and are read by the kernels: a captured HIP graph follows them.  Whatever they hold,
  * nothing outside the given tensors is touched: rows outside [0, Lmax) are neither stored nor seen, starts are clamped to
- * [0, T].  D in {64, 128}; strides in elements, multiples of 8, those of rows below 2^23; q, rows and out 16-byte aligned.
+ * [0, T].  D in {64, 128}; strides in elements, multiples of 8, those of rows below 2^23; q, rows and out 16-byte aligned;
+ * T Hq <= 2^25, B Hq <= 2^22.
  *   workspace  sq_prefix_attention_workspace_bytes(...) bytes (ragged: whether starts is given), 16-byte aligned, of any
  *              content; not shared by calls that may run at the same time. */
 size_t sq_prefix_attention_workspace_bytes(int T, int B, int Hq, int H, int D, int P, int Lmax, int ragged);
@@ -581,7 +582,7 @@ int sq_evict_attention(const void* q, const void* k_new, const void* v_new, void
  *   w[b][h][j] = sum over the query heads of h and the queries i >= j of P_i[j], P_i = softmax_{j <= i}(sm_scale q_i . k_j)
  * over all queries of a sequence, or its last `window` (0: all).  q, k fp16, row i of (b, h) at q[b * strides[0] + h *
  * strides[1] + i * strides[2]], k with strides[3..5]; w fp32 [B][H][S], 0 behind a sequence's rows; lengths int32 [B] on the
- * device, or NULL: S rows each.  Sums in fp32, their order fixed. */
+ * device, or NULL: S rows each.  Sums in fp32, their order fixed.  B Hq S <= 2^30. */
 size_t sq_attention_weights_workspace_bytes(int B, int Hq, int H, int S, int window);
 int sq_attention_weights(const void* q, const void* k, const void* lengths, void* w, int B, int Hq, int H, int D, int S, int window,
                          const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
@@ -607,7 +608,8 @@ int sq_evict_keep(const void* k, const void* v, const void* weight, const void* 
  * ids int64, place i of row m at ids[m * strides[2] + i * strides[3]], i < lengths[m * strides[4]] <= L; generated from place
  * generated_from[m * strides[5]] on (NULL: all of it).  repetition, frequency and presence fp32 [M], each may be NULL; bias_ids int32
  * and bias fp32, rows of nb <= 65535 entries strides[6] and strides[7] apart; mask uint32, rows of ceil(V / 32) words strides[8]
- * apart (0: one for all).  Ids outside [0, V) are none. */
+ * apart (0: one for all).  Ids outside [0, V) are none.  y is x, with the same strides, or does not overlap it.  M <= 65535; V and
+ * L up to 2^30. */
 size_t sq_logit_rules_workspace_bytes(int M, int V, int L, int nb);
 int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, const void* lengths, const void* generated_from,
                    const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,

@@ -667,7 +667,7 @@ Opt prefix_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor
                      const Opt& vn) {
     if (!rows_fit(q, q, 3) || !pair_fits(kp, vp, q, 3) || !pair_fits(kc, vc, q, 4)) return c10::nullopt;
     const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), B = kc.size(0), H = kc.size(1), L = kc.size(2), P = kp.size(1);
-    if (kc.size(3) != D || kp.size(0) != H || kp.size(2) != D || H == 0 || Hq % H != 0 || T * Hq >= INTS || L >= INTS || P >= INTS ||
+    if (kc.size(3) != D || kp.size(0) != H || kp.size(2) != D || H == 0 || Hq % H != 0 || T * Hq >= INTS || B * Hq >= INTS || L >= INTS || P >= INTS ||
         !whole(lengths, q, at::kInt, {B}))
         return c10::nullopt;
     if (starts.has_value() ? !whole(*starts, q, at::kInt, {B + 1}) : (B ? T % B : T) != 0) return c10::nullopt;

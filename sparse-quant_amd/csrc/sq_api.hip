@@ -1255,7 +1255,8 @@ int sq_prefix_attention(const void* q, const void* k_prefix, const void* v_prefi
                         int Hq, int H, int D, int P, int Lmax, const long* strides, float sm_scale, void* workspace,
                         size_t workspace_bytes, void* stream) {
     if (!heads_ok(Hq, H, D) || T < 0 || B < 0 || P < 0 || Lmax < 0) return SQ_ERR_BAD_SHAPE;
-    if ((long)T * Hq > (1L << 28) || (long)B * Hq > (1L << 24) || P > (1 << 30) || Lmax > (1 << 30)) return SQ_ERR_BAD_SHAPE;
+    if ((long)T * Hq > (1L << 25) || (long)B * Hq > (1L << 22) || P > (1 << 30) || Lmax > (1 << 30))  // (2^32 threads a launch)
+        return SQ_ERR_BAD_SHAPE;
     if (!starts && B > 0 && T % B != 0) return SQ_ERR_BAD_SHAPE;
     if (T == 0 || B == 0) return SQ_OK;
     if (!q || !out || !lengths || !strides || (P > 0 && (!k_prefix || !v_prefix)) || (Lmax > 0 && (!k_cache || !v_cache)) ||
@@ -1333,7 +1334,7 @@ size_t sq_attention_weights_workspace_bytes(int B, int Hq, int H, int S, int win
 int sq_attention_weights(const void* q, const void* k, const void* lengths, void* w, int B, int Hq, int H, int D, int S, int window,
                          const long* strides, float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
     if (!heads_ok(Hq, H, D) || B < 0 || S < 0 || window < 0) return SQ_ERR_BAD_SHAPE;
-    if ((long)B * Hq > (1L << 22) || (long)B * Hq * S > (1L << 34) || (long)S * (Hq / H) > (1L << 30)) return SQ_ERR_BAD_SHAPE;
+    if ((long)B * Hq > (1L << 22) || (long)B * Hq * S > (1L << 30)) return SQ_ERR_BAD_SHAPE;  // (2^32 threads a launch)
     if (B == 0 || S == 0) return SQ_OK;
     if (!q || !k || !w || !strides) return SQ_ERR_NULL_POINTER;
     if (!aligned16(q) || !aligned16(k) || !aligned4(w) || !aligned4(lengths)) return SQ_ERR_MISALIGNED;
@@ -1392,7 +1393,7 @@ int sq_logit_rules(const void* x, void* y, int elem_bytes, const void* ids, cons
                    const void* repetition, const void* presence, const void* frequency, const void* bias_ids, const void* bias,
                    const void* mask, void* token, int M, int V, int L, int nb, const long* strides, void* workspace,
                    size_t workspace_bytes, void* stream) {
-    if (M < 0 || M > 65535 || V <= 0 || V > (1 << 30) || L < 0 || nb < 0 || nb > 65535 || (elem_bytes != 2 && elem_bytes != 4))
+    if (M < 0 || M > 65535 || V <= 0 || V > (1 << 30) || L < 0 || L > (1 << 30) || nb < 0 || nb > 65535 || (elem_bytes != 2 && elem_bytes != 4))
         return SQ_ERR_BAD_SHAPE;
     if (M == 0) return SQ_OK;
     if (!x || !y || !token || !strides || (nb > 0 && (!bias_ids || !bias)) ||

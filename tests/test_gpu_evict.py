@@ -119,6 +119,19 @@ def test_nothing_seen_and_large_scores(evict):
     assert (np.abs(out.float().cpu().numpy() - want[0]) <= TOL * want[1] + 1e-6).all()
 
 
+@pytest.mark.parametrize("b,heads,room", [(2, 4, 700), (80, 8, 100), (2, 80, 100)])
+def test_the_result_in_the_place_of_the_queries(evict, b, heads, room):
+    rng = np.random.default_rng(b + heads)
+    h, d = heads // 4 if heads < 80 else 2, 64
+    seen = np.full(b, 2 * room, np.int32)
+    cache = [dev(x) for x in state(rng, b, h, room, d, seen, 2, 5)]
+    twin = [x.clone() for x in cache]
+    q, kn, vn = dev(normal(rng, b, heads, d)), dev(normal(rng, b, h, d)), dev(normal(rng, b, h, d))
+    want, _ = evict.attention(q, kn, vn, *cache, dev(seen), 0.125, 2, 5)
+    got, _ = evict.attention(q, kn, vn, *twin, dev(seen), 0.125, 2, 5, out=q)
+    assert got is q and torch.equal(q, want) and all(torch.equal(a, c) for a, c in zip(cache, twin))
+
+
 def test_strided_rows_and_caches(evict):
     rng = np.random.default_rng(3)
     b, heads, h, room, d = 2, 4, 2, 70, 64

@@ -217,6 +217,16 @@ def test_two_streams_at_once(prefix):
     assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
 
 
+@pytest.mark.parametrize("b,new,p", [(16, 1, 700), (1, 1, 2000), (3, 200, 300)])
+def test_the_result_in_the_place_of_the_queries(prefix, b, new, p):
+    rng = np.random.default_rng(b)
+    q, rows = dev(normal(rng, b * new, 8, 64)), [dev(normal(rng, 2, p, 64)) for _ in range(2)]
+    caches = [dev(normal(rng, b, 2, 320, 64)) for _ in range(2)]
+    lengths = torch.full((b,), 300, dtype=torch.int32, device=DEV)
+    want = prefix.attention(q, *rows, *caches, lengths, 0.125)
+    assert prefix.attention(q, *rows, *caches, lengths, 0.125, out=q) is q and torch.equal(q, want)
+
+
 def test_refusals(prefix):
     q = torch.zeros((4, 4, 64), dtype=torch.float16, device=DEV)
     kp = torch.zeros((2, 10, 64), dtype=torch.float16, device=DEV)

@@ -33,7 +33,8 @@ def test_prefix_attention_refuses_before_any_launch(L):
         return L.sq_prefix_attention(q, kp, vp, kc, vc, lengths, starts, kn, vn, out, T, B, Hq, H, D, P, Lmax, strides, 1.0, ws, size, None)
 
     for kw in ({"D": 96}, {"Hq": 3}, {"H": 0}, {"T": 5}, {"T": -4}, {"B": -1}, {"P": -1}, {"Lmax": -1}, {"P": 1 << 30, "Lmax": (1 << 30) + 1},
-               {"T": 1 << 27, "B": 1 << 27}, {"strides": longs(*ok[:3], 1 << 23, *ok[4:])}, {"strides": longs(*ok[:6], -8, *ok[7:])}):
+               {"T": 1 << 27, "B": 1 << 27}, {"T": (1 << 23) + 4}, {"T": 1 << 22, "B": 1 << 22},
+               {"strides": longs(*ok[:3], 1 << 23, *ok[4:])}, {"strides": longs(*ok[:6], -8, *ok[7:])}):
         assert call(**kw) == capi.SQ_ERR_BAD_SHAPE, kw
     for name in ("q", "kp", "vp", "kc", "vc", "lengths", "out", "vn", "strides"):
         assert call(**{name: None}) == capi.SQ_ERR_NULL_POINTER, name
@@ -69,7 +70,8 @@ def test_evict_refuses_before_any_launch(L):
     def weights(q=p, k=p, lengths=None, w=p, B=2, Hq=4, H=2, D=64, S=50, window=0, strides=longs(*[1024] * 6), ws=p, size=1 << 40):
         return L.sq_attention_weights(q, k, lengths, w, B, Hq, H, D, S, window, strides, 1.0, ws, size, None)
 
-    for kw in ({"D": 80}, {"Hq": 3}, {"window": -1}, {"S": -1}, {"S": 1 << 30, "B": 16}, {"strides": longs(*[1024] * 5, 1 << 23)}):
+    for kw in ({"D": 80}, {"Hq": 3}, {"window": -1}, {"S": -1}, {"S": 1 << 30, "B": 16}, {"S": (1 << 27) + 1},
+               {"strides": longs(*[1024] * 5, 1 << 23)}):
         assert weights(**kw) == capi.SQ_ERR_BAD_SHAPE, kw
     for name in ("q", "k", "w", "strides"):
         assert weights(**{name: None}) == capi.SQ_ERR_NULL_POINTER, name
@@ -99,7 +101,8 @@ def test_logit_rules_refuse_before_any_launch(L):
         return L.sq_logit_rules(x, y, elem, ids, lengths, gen, rep, pres, freq, bias_ids, bias, mask, token, M, V, nids, nb, strides, ws,
                                 size, None)
 
-    for kw in ({"elem": 3}, {"V": 0}, {"M": -1}, {"M": 65536}, {"nids": -1}, {"nb": 65536}, {"strides": longs(100, 99, *ok[2:])},
+    for kw in ({"elem": 3}, {"V": 0}, {"M": -1}, {"M": 65536}, {"nids": -1}, {"nids": (1 << 30) + 1}, {"nb": 65536},
+               {"strides": longs(100, 99, *ok[2:])},
                {"strides": longs(-1, *ok[1:])}):
         assert call(**kw) == capi.SQ_ERR_BAD_SHAPE, kw
     for name in ("x", "y", "ids", "bias", "bias_ids", "token", "strides"):
