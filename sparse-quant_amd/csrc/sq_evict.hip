@@ -267,8 +267,6 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EvictArgs a) {
     }
 }
 
-// Workgroups that keep's places are cut for.
-constexpr int KEEP_WGS = 512;
 // Workgroups that the caches' rows are cut for: one per CU, so that a chip full of heads needs no second launch (us, with 256 / 512 /
 // 1024: 8 x 32 heads x 512 rows 16.6 / 19.6 / 24.1; 32 x 8 x 4000 107.5 / 109.4 / 109.0; 2 x 32 x 2000 22.4 / 22.3 / 27.9; 4 x 8 x 4000
 // 24.7 / 24.6 / 31.5).
@@ -400,12 +398,16 @@ __global__ __launch_bounds__(256) void keep_gather_kernel(EvictKeep t) {
     }
 }
 
-// The same for prompts whose weights fit LDS, and the rows copied by the same workgroup: several share a head where there are
-// few, and each of them makes the choice.  (With the weights in registers the code is a copy of each loop for every one of them,
+// The same for prompts whose weights fit LDS, and the rows copied by the same workgroup (in two launches 16 x 8 heads of 20000 rows
+// take 95 us instead of 69, 8 x 8 of 512 places 24.5 instead of 17.4): several share a head where there are few, and each of
+// them makes the choice.  (With the weights in registers the code is a copy of each loop for every one of them,
 // and fetching it takes longer than the loops.)  The threshold is found between the
 // lowest and the highest weight, of whose distance every pass looks at 11 bits: counted by the weights' own digits, most of
 // them fall on a few counters (the numbers of one power of two have one), and LDS takes them one at a time.
 constexpr int KEEP_LIST = 4096;  // places of a workgroup
+// Workgroups that the places are cut for, of 256 places or more each (us, with 128 / 256 / 512 / 1024: 16 x 8 heads, 20000 rows into 2000
+// 94 / 68.7 / 69.7 / 81; 32 x 8, 2000 into 500 28.3 / 28.3 / 31.9 / 31.7; 8 x 8, into 512, with 128 / 256 / 1024 places 23.6 / 17.4 / 17.4).
+constexpr int KEEP_WGS = 256;
 
 constexpr int KEEP_MOST = 32 * KEEP_THREADS;  // rows of a prompt
 
@@ -612,7 +614,7 @@ hipError_t launch_evict_attention(const EvictStep& t, int D, float sm_scale, voi
 hipError_t launch_evict_keep(const EvictKeep& t, int D, hipStream_t st) {
     const int heads = t.B * t.H;
     if (t.S <= KEEP_MOST) {
-        // two workgroups a CU, of 256 places or more: each makes the whole choice
+        // (every workgroup of a head makes the whole choice)
         const int share = std::max((t.R + KEEP_LIST - 1) / KEEP_LIST, std::min((KEEP_WGS + heads - 1) / heads, (t.R + 255) / 256));
         const int each = (t.R + share - 1) / share;
         const dim3 grid((t.R + each - 1) / each, heads);

@@ -720,13 +720,22 @@ int div_up(long a, long b) { return (int)((a + b - 1) / b); }
 int cut(long steps, int wgs, int most) { return (int)std::max<long>(std::min<long>((steps + wgs - 1) / wgs, most), 1); }
 int pad8(long n) { return (int)((n + 7) / 8 * 8); }
 
-// Workgroups that packed rows' pieces are cut for.  Against the prefix a piece writes its rows' sums: two pieces per three CUs
-// for tiles of 128 rows (64 sequences of 32 heads behind 8192 rows, 8 key/value heads: 62 us with 512 pieces, 47 with 256, 44
-// with 128; behind 16384: 67, 55, 57 and 51 with 192), more where a tile has up to 32.
-constexpr int PA_WGS_MANY = 160, PA_WGS_FEW = 256;
+// Workgroups that packed rows' pieces are cut for (us).  Against the prefix a piece writes its rows' sums, and up to 256 rows the
+// prefix's bytes bound it: two pieces per three CUs (64 sequences of 32 heads behind 8192 rows, 8 key/value heads: 42.0 with 160,
+// 44.8 with 256, 56 with 512).  Beyond, behind a long prefix, the products do: one per CU (64 x 4 tokens behind 4096 rows
+// 50.5 with 160, 47.5 with 256, 57 with 512; 64 x 8 88, 70 and 76; behind 1024 32.6 and 37.6).
+constexpr int PA_WGS_MANY = 160, PA_WGS_FULL = 256, PA_WGS_FEW = 256;
 // Against their own rows, of different numbers and up to the caches' room: four per CU (ragged up to 1000 rows 46.1 us with 512,
 // 42.8 with 1024, 48 with 4096).
 constexpr int PA_WGS_OWN = 1024;
+// Packing pays where the prefix is long: it costs a second launch and the rows' sums, and saves each sequence's tile the way through
+// the prefix (from L2).  Packed / not, us, 32 heads over 8: 64 x 1 token behind 512 rows 23.5 / 20.3, 1024 23.5 / 26.6, 8192
+// 44 / 125; 64 x 8 behind 1024 45 / 32, 2048 52 / 45, 4096 70 / 74; where the tiles do not fill the chip 16 x 1 behind 64 12.2 / 9.0,
+// 256 12.7 / 12.3, 1024 13.8 / 16.2; 16 x 8 16.9 / 11.8, 17.9 / 19.3, 19.2 / 23.6.  More than 32 rows of a sequence (64 x 16 tokens
+// behind 4096) 107 / 102.
+bool pack(int P, int B, long each, long tiles) {
+    return B > 1 && each <= 32 && P > (tiles >= PA_SLOTS ? 512 + 64 * each : 128);
+}
 
 }  // namespace
 
@@ -734,16 +743,18 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
     PrefixPlan p = {};
     const long rows = (long)T * share;     // of a key/value head
     const long each = (rows + B - 1) / B;  // of a sequence, on average
-    const bool packed = P > 0 && B > 1 && each <= 32;
+    const bool packed = pack(P, B, each, (long)B * H);
     p.packed = packed;
     p.qa = !packed ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    p.qb = each <= 32 ? 1 : each <= 64 ? 2 : 4;
+    // (tiles of 128 rows where that makes more than 64 of them: 1 x 32 tokens behind 4096 rows 27.1 us instead of 22.3 with 64,
+    // 8 x 32 44.5 and 42.0, 8 x 64 58 and 62.5, 16 x 128 159 and 190)
+    p.qb = each <= 32 ? 1 : each <= 64 || (rows + 127) / 128 * H <= 64 ? 2 : 4;
     p.rows_b = 32 * p.qb;
     const int pre = div_up(P, PA_STEP), own = div_up(Lmax, PA_STEP);
     if (packed) {
         p.tiles_a = div_up(rows, 32 * p.qa);
         const long steps = (long)H * p.tiles_a * pre;
-        p.steps_a = cut(steps, p.qa == 1 ? PA_WGS_FEW : PA_WGS_MANY, pre);
+        p.steps_a = cut(steps, p.qa == 1 ? PA_WGS_FEW : p.tiles_a > 2 && P >= 2048 ? PA_WGS_FULL : PA_WGS_MANY, pre);
         if (p.qa == 1) p.steps_a = (p.steps_a + 1) / 2 * 2;
         p.parts_a = div_up(pre, p.steps_a);
         p.units_a = H * p.parts_a * p.tiles_a;
@@ -757,7 +768,11 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
         p.grid_b = pad8(p.units_b);
     } else {
         p.steps_b = p.parts_b = 1;
-        p.most = std::max(std::min((own + pre) / 4, p.qb == 1 ? 64 : 8), 1);  // parts of four steps or more
+        // Parts of four steps or more; many of them take longer to join than to go through (us, 8 heads x 4: 1 token behind 8192 rows
+        // 18.4 with up to 8 parts, 13.6 with 24, 17.4 with 64, behind 16384 34.4, 21.8 and 24.4; 64 tokens 37.7 with 8, 31.2 with 16;
+        // 2 x 64 behind 4096, of four steps each, 29.8 and 33.3).
+        const int steps = own + pre;
+        p.most = std::max(p.qb == 1 ? std::min(steps / 4, 24) : std::max(std::min(steps / 4, 8), std::min(steps / 8, 16)), 1);
         const int all = p.tiles_b * H;
         p.grid_b = ragged ? all / PA_SLOTS * PA_SLOTS + PA_SLOTS : all / PA_SLOTS * PA_SLOTS + all % PA_SLOTS * deal_of(p.tiles_b, H, p.most).parts;
     }
