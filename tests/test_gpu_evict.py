@@ -209,7 +209,7 @@ def test_weights_of_many_heads(evict):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("s,room,first,last", [(1, 1, 0, 0), (10, 16, 2, 3), (17, 16, 2, 3), (100, 16, 16, 0), (1500, 64, 4, 60),
                                                (5000, 1000, 4, 100), (3000, 2999, 0, 0),
-                                               (20, 6, 2, 4), (5000, 4500, 0, 1), (33000, 500, 4, 100)])
+                                               (20, 6, 2, 4), (5000, 4500, 0, 1), (32768, 300, 0, 7), (33000, 500, 4, 100)])
 @pytest.mark.parametrize("kind", ["spread", "few", "odd"])
 def test_keep(evict, d, s, room, first, last, kind):
     rng = np.random.default_rng(s + room)

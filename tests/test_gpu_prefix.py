@@ -83,6 +83,15 @@ def test_many_sequences_packed_into_tiles(prefix):
     run(prefix, rng, 100, 3, 1, 128, 130, lens[:100], [1] * 100, 31, ragged=True)
 
 
+@pytest.mark.parametrize("b,heads,h,new,p", [(70, 8, 8, 1, 500), (70, 8, 8, 1, 700), (520, 4, 1, 2, 900), (20, 8, 1, 4, 2100), (9, 4, 2, 16, 129),
+                                             (2, 8, 2, 32, 300), (5, 16, 8, 60, 100)])
+def test_either_side_of_each_way(prefix, b, heads, h, new, p):
+    # packed or not (many sequences, short prefixes), many pieces of a long prefix, tiles of 64 and 128 rows
+    rng = np.random.default_rng(b + p)
+    lens = [int(x) for x in rng.integers(new, new + 70, b)]
+    run(prefix, rng, b, heads, h, 64, p, lens, [new] * b, new + 70, ragged=bool(b % 2))
+
+
 def test_lengths_that_fit_nothing(prefix):
     # no rows, negative lengths, more tokens than rows, more rows than room
     rng = np.random.default_rng(2)
