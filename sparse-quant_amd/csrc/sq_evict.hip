@@ -5,6 +5,11 @@
 // its own among them, and every row's weight grows by what the token's heads give it:
 //   P = softmax_j(scale q . k_j),  out = sum_j P_j v_j,  weight_j += sum over the query heads of the key/value head of P_j
 // The probabilities are known only behind the last row, so the scores wait in the workspace (4 bytes of a row's 512 at D = 128).
+//
+// What bounds it: the bytes, 4.6 TB/s of them (32 sequences x 8 heads x 4000 rows of 128, four query heads each: 487 MB in 106 us);
+// where there are few the chain of launch, first rows, the lowest weight, softmax, join and weights (8 sequences of 32 heads x 512
+// rows, 57 MB in 12.8 us, one launch).  The weights are looked through behind the first requests, by every workgroup of a head, which
+// costs 8 bytes a row from L2 and saves a launch in front.
 #include "sq_attn_rows.h"
 #include "sq_kernels.h"
 
@@ -399,14 +404,15 @@ __global__ __launch_bounds__(256) void keep_gather_kernel(EvictKeep t) {
 }
 
 // The same for prompts whose weights fit LDS, and the rows copied by the same workgroup (in two launches 16 x 8 heads of 20000 rows
-// take 95 us instead of 69, 8 x 8 of 512 places 24.5 instead of 17.4): several share a head where there are few, and each of
+// take 95 us instead of 69, 8 x 32 of 512 rows 24.5 instead of 17.4): several share a head where there are few, and each of
 // them makes the choice.  (With the weights in registers the code is a copy of each loop for every one of them,
 // and fetching it takes longer than the loops.)  The threshold is found between the
 // lowest and the highest weight, of whose distance every pass looks at 11 bits: counted by the weights' own digits, most of
 // them fall on a few counters (the numbers of one power of two have one), and LDS takes them one at a time.
 constexpr int KEEP_LIST = 4096;  // places of a workgroup
 // Workgroups that the places are cut for, of 256 places or more each (us, with 128 / 256 / 512 / 1024: 16 x 8 heads, 20000 rows into 2000
-// 94 / 68.7 / 69.7 / 81; 32 x 8, 2000 into 500 28.3 / 28.3 / 31.9 / 31.7; 8 x 8, into 512, with 128 / 256 / 1024 places 23.6 / 17.4 / 17.4).
+// 94 / 68.7 / 69.7 / 81; 32 x 8, 2000 into 500 28.3 / 28.3 / 31.9 / 31.7; 8 x 32, 512 into 256, two workgroups of 128
+// places a head instead of one 23.6 / 17.4).
 constexpr int KEEP_WGS = 256;
 
 constexpr int KEEP_MOST = 32 * KEEP_THREADS;  // rows of a prompt

@@ -9,6 +9,14 @@
 // belong to, are packed into tiles and meet the prefix as one dense product without masks; each sequence's rows meet its own
 // cache apart; a second launch joins the parts.  Where a sequence has many rows itself (a prompt) nothing is gained by packing:
 // its tiles go through the prefix and on through their own rows, and write the result.
+//
+// What bounds it: one token of each sequence the bytes, long ones at 3.1 TB/s with the second launch (64 ragged sequences of up to
+// 1000 rows behind 8192, 32 heads over 8 of 128: 131 MB in 42 us, 31 of the first launch and 5.6 of the second), short ones
+// the chain of launch, first rows, softmax, join (8 sequences behind 512 rows 12.3 us, the host's two launches 9 of them);
+// prompts the vector instructions of the softmax beside the products, which overlap in part (16 ragged ones of up to 512 tokens
+// behind 4096 rows: 141 GFLOP in 176 us, 0.8 PFLOP/s; per 32 x 32 scores 16 products of 32 cycles, and 16 exponentials of 8
+// with about five other instructions of 4 each).  Four waves of 32 rows on two workgroups a CU: products and exponentials of
+// different waves fill each other's gaps better than one wave's own interleaved (202 us as it was then, 226 to 243 interleaved).
 #include "sq_attn_rows.h"
 #include "sq_kernels.h"
 
@@ -734,7 +742,7 @@ constexpr int PA_WGS_OWN = 1024;
 // 256 12.7 / 12.3, 1024 13.8 / 16.2; 16 x 8 16.9 / 11.8, 17.9 / 19.3, 19.2 / 23.6.  More than 32 rows of a sequence (64 x 16 tokens
 // behind 4096) 107 / 102.
 bool pack(int P, int B, long each, long tiles) {
-    return B > 1 && each <= 32 && P > (tiles >= PA_SLOTS ? 512 + 64 * each : 128);
+    return B > 1 && each <= 32 && P > (tiles >= PA_SLOTS ? 512 + 64 * each : PA_STEP);
 }
 
 }  // namespace
@@ -774,7 +782,7 @@ PrefixPlan prefix_plan(int T, int B, int H, int share, int P, int Lmax, bool rag
         const int steps = own + pre;
         p.most = std::max(p.qb == 1 ? std::min(steps / 4, 24) : std::max(std::min(steps / 4, 8), std::min(steps / 8, 16)), 1);
         const int all = p.tiles_b * H;
-        p.grid_b = ragged ? all / PA_SLOTS * PA_SLOTS + PA_SLOTS : all / PA_SLOTS * PA_SLOTS + all % PA_SLOTS * deal_of(p.tiles_b, H, p.most).parts;
+        p.grid_b = all / PA_SLOTS * PA_SLOTS + (ragged ? PA_SLOTS : all % PA_SLOTS * deal_of(p.tiles_b, H, p.most).parts);
     }
     p.grid_a = pad8(p.units_a);
     p.by_share = Divisor::of(share);
