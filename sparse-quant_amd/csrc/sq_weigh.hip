@@ -152,9 +152,10 @@ __global__ __launch_bounds__(256, 4) void weigh_rows_kernel(WeighPlan a) {
 #pragma unroll
             for (int e = 0; e < 32; e++) mx = fmaxf(mx, st[e >> 4][e & 15]);
             const float delta = mx == -INFINITY ? 0.f : unset ? mx : fmaxf(mx, 0.f);
+            // (while it is unset the sum is 0, or NaN where a score was, and 2^-delta of a first score below -128 is infinite)
+            sum = unset ? sum : sum * __builtin_amdgcn_exp2f(-delta);
             unset = unset && mx == -INFINITY;
             ref += delta;
-            sum *= __builtin_amdgcn_exp2f(-delta);  // (0 while it was unset)
             more = 0.f;
 #pragma unroll
             for (int e = 0; e < 32; e++) more += __builtin_amdgcn_exp2f(st[e >> 4][e & 15] - delta);

@@ -267,3 +267,45 @@ def test_refusals(evict):
             evict.keep(*(good[:i] + [y] + good[i + 1:]))
     with pytest.raises(ValueError):
         evict.keep(*good, lengths=n.long())
+
+
+def large_tol(q, k, scale, n):
+    """A score is off by D 2^-24 sum |q k| scale and a few 2^-24 of itself; it and the logarithm of its row's sum bear on a weight,
+    and sums of up to n exponentials (2^-23 each) by n 2^-24."""
+    share = q.shape[1] // k.shape[1]
+    size = max((np.abs(q[:, g].astype(np.float64)) @ np.abs(k[:, g // share].astype(np.float64)).transpose(0, 2, 1)).max()
+               for g in range(q.shape[1])) * scale
+    return (2 * (q.shape[-1] + 8) * size + n + 64) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("s,window", [(1, None), (5, None), (40, 3), (200, None), (300, 70)])
+@pytest.mark.parametrize("kind", ["opposed", "low", "large", "first"])
+def test_weights_of_large_scores(evict, d, s, window, kind):
+    # a lane's first score far below 0 (less than -128 in units of log2), all scores there, scores of any kind up to hundreds
+    rng = np.random.default_rng(s + d)
+    b, heads, h = 2, 4, 2
+    q, k = normal(rng, b, heads, s, d), normal(rng, b, h, s, d)
+    if kind == "opposed":  # a row's own key is what it likes least
+        q = (-24 * k.repeat(heads // h, 1).astype(np.float32) + q).astype(np.float16)
+    if kind == "low":
+        q, k = (q / 8 - 5).astype(np.float16), (k / 8 + 5).astype(np.float16)
+    if kind == "large":
+        q *= 16
+    if kind == "first":  # the first keys alone
+        q, k[:, :, :3] = (q - 3).astype(np.float16), 8.0
+    lens = np.array([s, max(1, s - 2)], np.int32)
+    scale = 1 / np.sqrt(d)
+    want = so.attention_weights(q, k, lens, scale, window)
+    got = evict.attention_weights(dev(q), dev(k), scale, window, dev(lens)).cpu().numpy()
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= large_tol(q, k, scale, 2 * s) * want + 1e-9).all(), (np.abs(got - want) / (want + 1e-9)).max()
+
+
+def test_weights_under_keys_that_are_no_numbers(evict):
+    # whole steps of them in front of others: every row sees them, and no sum begins anew behind them
+    rng = np.random.default_rng(7)
+    q, k = normal(rng, 1, 2, 200, 64), normal(rng, 1, 2, 200, 64)
+    k[:, 1, :70] = np.nan
+    got = evict.attention_weights(dev(q), dev(k), 0.125).cpu().numpy()
+    assert np.isfinite(got[0, 0]).all() and np.isnan(got[0, 1]).all()
