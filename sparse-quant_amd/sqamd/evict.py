@@ -141,7 +141,9 @@ class EvictCache:
     """A model's cache of `rows` rows a head in every layer: a prompt's rows of the highest weights stay, by all its queries or
     its last `window`, and later tokens take the places of those of the lowest.  The first keep_first and the last keep_last
     tokens are never given up.  `seen` counts the sequences' tokens on the device; `OPTDecoder` keeps it, or whoever drives the
-    layers by hand.  It takes one prompt, at the beginning, and then single tokens."""
+    layers by hand.  It takes one prompt, at the beginning, and then single tokens, each once: a step changes the weights and may
+    give up a row, so that running it again (a warm-up in front of a capture, say) leaves its token there twice.  A prompt at
+    position 0 begins anew."""
 
     def __init__(self, layers, batch, kv_heads, head_dim, rows, keep_first=4, keep_last=None, window=None, device="cuda"):
         keep_last = max(1, rows // 4) if keep_last is None else keep_last
@@ -159,7 +161,8 @@ class EvictCache:
 
     def set_position(self, batch, pos0, tokens):
         """The next `tokens` tokens of the first `batch` sequences are those of positions pos0 on: an int, or (one token) an
-        int64 tensor of one element on the device."""
+        int64 tensor of one element on the device.  Positions are not compared with those that came before: each step is for
+        the position behind the last one's."""
         if batch > self.batch:
             raise ValueError("%d sequences in a cache for %d" % (batch, self.batch))
         if tokens != 1 and not (isinstance(pos0, int) and pos0 == 0):

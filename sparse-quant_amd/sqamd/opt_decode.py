@@ -219,7 +219,8 @@ class OPTDecoder(nn.Module):
 
     def new_cache(self, batch, max_len, kv_bits=16, kv_group=64, rows=None, keep_first=4, keep_last=None, window=None):
         """A cache for `batch` sequences of up to max_len rows.  rows: it holds no more than so many a head and evicts by
-        accumulated attention weight (keep_first, keep_last, window: as evict.EvictCache takes them)."""
+        accumulated attention weight (keep_first, keep_last, window: as evict.EvictCache takes them); max_len bounds nothing
+        then, and no step may be run twice over it."""
         hd = self.hidden // self.heads
         if rows is not None:
             if kv_bits != 16:
@@ -354,7 +355,7 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
             out_tok.copy_(lg.argmax(-1))
 
     def rewind():
-        # the warm-up and the capture run a step each: put token, position and step counter back
+        # the warm-up has run a step: put token, position and step counter back
         tok.copy_(first_tok)
         pos_t.fill_(begin + prompt)
         if step_t is not None:
@@ -373,6 +374,10 @@ def run_e2e(batch=8, prompt=512, new_tokens=128, layers=32, use_graph=True, seed
         with torch.cuda.graph(graph, stream=side):  # same stream as the warm-up: per-stream workspaces exist
             step()
         rewind()
+        if rows:
+            # the next step writes the rows of most caches again; of one that evicts a row has gone, the token's has come and
+            # the others' weights have grown: the prompt's rows and weights again
+            model(ids, cache, begin)
     generated = [tok.clone()]
     torch.cuda.synchronize()
     t0 = time.perf_counter()

@@ -245,3 +245,24 @@ def test_end_to_end_figures(opt):
         assert got[what] == list(kw.values())[0] and got["logits_finite"] and torch.equal(got["tokens"], eager["tokens"])
     with pytest.raises(ValueError):
         opt.run_e2e(batch=1, prompt=8, new_tokens=2, layers=1, shared=4, rows=4)
+
+
+def test_end_to_end_over_a_cache_that_evicts_from_the_prompt_on(opt, monkeypatch):
+    # fewer rows than the prompt has: a step in front of the first would leave its token's row and its weights in the cache
+    caches, plain = [], opt.OPTDecoder.new_cache
+
+    def new_cache(self, *args, **kw):
+        caches.append(plain(self, *args, **kw))
+        return caches[-1]
+
+    monkeypatch.setattr(opt.OPTDecoder, "new_cache", new_cache)
+    for rows in (24, 44):  # (44: more than the prompt's, but not than all)
+        got = [opt.run_e2e(batch=2, prompt=40, new_tokens=9, layers=2, rows=rows, use_graph=graph, return_tokens=True)["tokens"]
+               for graph in (True, False)]
+        a, b = caches[-2:]
+        assert torch.equal(*got)
+        assert torch.equal(a.position, b.position) and torch.equal(a.weight, b.weight) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+        for i in range(2):
+            for j in range(2):
+                kept = a.position[i, j].cpu().numpy()
+                assert all(len(set(kept[h])) == rows for h in range(kept.shape[0]))  # no token twice
