@@ -385,6 +385,7 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
         asm volatile("" : "+v"(x));
         qf[s] = bit_cast<half8_t>(x);
     }
+    const bool causal = !w.shared && w.rc.own_first < w.rc.own;  // (or all rows of the tile see all own rows up to the last)
     bool odd = false;
     uint32_t stage = 0;
 #pragma unroll 1
@@ -399,7 +400,7 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
             uint8_t* const vt = lds + stage + TILE;
             for (int i = imax((pre ? t.P : w.rc.own) - n, 0) * CPR + tid; i < PA_STEP * CPR; i += 256)
                 *(u32x4_t*)(vt + i * 16) = (u32x4_t){0u, 0u, 0u, 0u};
-            if (!pre) odd |= clear_odd<D>(vt, imin(w.rc.own - n, PA_STEP), tid, 256);
+            if (!pre && causal) odd |= clear_odd<D>(vt, imin(w.rc.own - n, PA_STEP), tid, 256);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         if (idle) continue;
@@ -476,7 +477,7 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
                 acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<half8_t>(x), pk[i], acc[dt], 0, 0, 0);
             }
     }
-    if (!w.shared && w.rc.own_first < w.rc.own && __syncthreads_or(odd) && kg == 0) add_odd<D>(t, w, limit, acc);
+    if (causal && __syncthreads_or(odd) && kg == 0) add_odd<D>(t, w, limit, acc);
 
     // ---- the row's state: over its two lanes, then over the key groups
     l_i += __shfl_xor(l_i, 32);

@@ -255,3 +255,31 @@ def test_refusals(prefix):
             prefix.attention(*args, **kw)
     empty = prefix.attention(q[:0], kp, kp, kc[:0], kc[:0], n[:0], 1.0)
     assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("heads,h,new,before,p", [
+    (2, 2, [65], 0, 70), (2, 2, [65], 30, 0), (70, 1, [1], 40, 70), (64, 8, [129], 20, 65), (2, 2, [70, 129], 5, 10), (2, 2, [100], 90, 0)])
+def test_infinities_and_nan_in_front_of_a_tile_of_one_token(prefix, heads, h, new, before, p):
+    # the last tile's rows are one token's (or tokens that see equally many rows, those that the cache has room for): it sees
+    # every row of its last step
+    rng = np.random.default_rng(sum(new) + heads)
+    t, d, room = sum(new), 64, 150
+    q, kn, vn = normal(rng, t, heads, d), normal(rng, t, h, d), normal(rng, t, h, d)
+    kp, vp = normal(rng, h, p, d), normal(rng, h, p, d)
+    kc, vc = normal(rng, len(new), h, room, d), normal(rng, len(new), h, room, d)
+    lens, at = [n + before for n in new], 0
+    for i, n in enumerate(new):
+        last = min(lens[i], room) - 1  # the last row that is seen
+        for row, value in ((last, np.inf), (last // 64 * 64, np.nan), (max(last - 2, 0), -np.inf)):
+            rows, j = (vn, at + row - before) if row >= before else (vc[i].transpose(1, 0, 2), row)
+            rows[j, 0, 3 + row % 7] = value
+        at += n
+    with np.errstate(invalid="ignore"):
+        ref, size, _, _ = so.prefix_attention(q, kp, vp, kc, vc, lens, new, 0.125, kn, vn)
+        out = prefix.attention(dev(q), dev(kp), dev(vp), dev(kc), dev(vc), torch.tensor(lens, dtype=torch.int32, device=DEV), 0.125,
+                               starts=starts_of(new), k_new=dev(kn), v_new=dev(vn)).float().cpu().numpy()
+    assert not np.isfinite(ref).all()
+    assert np.array_equal(np.isfinite(out), np.isfinite(ref))
+    assert np.array_equal(out == np.inf, ref == np.inf) and np.array_equal(out == -np.inf, ref == -np.inf)
+    fine = np.isfinite(ref)
+    assert (np.abs(out[fine] - ref[fine]) <= TOL * size[fine] + 1e-6).all()
