@@ -35,9 +35,9 @@ struct EvictArgs {
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
 
-// Order of weights as unsigned numbers; a NaN is the lowest.
+// Order of weights as unsigned numbers; a NaN is the lowest, and both zeros are the same (-0 + 0 is 0).
 __device__ __forceinline__ uint32_t order_of(float w) {
-    const uint32_t u = bit_cast<uint32_t>(w);
+    const uint32_t u = bit_cast<uint32_t>(w + 0.f);
     return w != w ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 

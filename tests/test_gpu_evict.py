@@ -309,3 +309,24 @@ def test_weights_under_keys_that_are_no_numbers(evict):
     k[:, 1, :70] = np.nan
     got = evict.attention_weights(dev(q), dev(k), 0.125).cpu().numpy()
     assert np.isfinite(got[0, 0]).all() and np.isnan(got[0, 1]).all()
+
+
+def test_zeros_of_both_signs_are_equal(evict):
+    # among equals the lowest row goes, and the lower one stays
+    rng = np.random.default_rng(6)
+    b, h, room, d = 3, 2, 90, 64
+    seen = np.full(b, 300, np.int32)
+    kc, vc, weight, position = state(rng, b, h, room, d, seen, 2, 5)
+    weight[:] = np.where(rng.random(weight.shape) < 0.5, 0.0, -0.0)
+    q, kn, vn = normal(rng, b, h, d), normal(rng, b, h, d), normal(rng, b, h, d)
+    want = so.evict_step(q, kn, vn, kc, vc, weight, position, seen, 0.125, 2, 5)
+    cache = [dev(x) for x in (kc, vc, weight, position)]
+    _, slot = evict.attention(dev(q), dev(kn), dev(vn), *cache, dev(seen), 0.125, 2, 5)
+    assert np.array_equal(slot.cpu().numpy(), want[2]) and np.array_equal(cache[3].cpu().numpy(), want[6])
+    for s in (200, 33000):  # either way that rows are kept
+        k, w = dev(normal(rng, b, h, s, d)), np.where(rng.random((b, h, s)) < 0.5, 0.0, -0.0).astype(np.float32)
+        w[:, :, 7::50], w[:, :, 9::50] = 1.0, -1.0
+        rows = evict.keep(k, k.clone(), dev(w), *cache, 3, 4).cpu().numpy()
+        for i in range(b):
+            for j in range(h):
+                assert rows[i, j].tolist() == so.keep_rows(w[i, j], s, room, 3, 4), (s, i, j)
