@@ -599,8 +599,9 @@ int sq_evict_keep(const void* k, const void* v, const void* weight, const void* 
                   const long* strides, void* stream);
 
 /* Rules on logits x [M][V] (fp16 where elem_bytes is 2, fp32 where it is 4; rows strides[0] elements apart) into y (rows
- * strides[1] apart; may be x), and the best token of each row (int64 [M]; the lowest among equals, NaN never wins, 0 where there
- * is none).  In this order, each step rounded once in fp32:
+ * strides[1] apart; may be x), and the best token of each row of the result (int64 [M]; the lowest among equals; NaN never wins, 0
+ * where all are; where nothing is above -inf the lowest token that is -inf, which may be a masked one).  In this order, each step
+ * rounded once in fp32:
  *   x > 0 ? x / repetition[m] : x * repetition[m]   tokens that stand in the row's text
  *   x - frequency[m] * c, then x - presence[m]       tokens that stand c > 0 times in the generated part of it
  *   x + bias[m][j]                                   tokens that bias_ids[m][j] names (the last j among several)

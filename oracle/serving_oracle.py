@@ -129,6 +129,9 @@ def logit_rules(x, ids=None, lengths=None, generated=None, repetition=None, pres
 
 
 def best_token(y):
-    """The lowest of the largest, NaN never; 0 where none is above -inf."""
-    z = np.where(np.isnan(y), -np.inf, y.astype(np.float64))
-    return z.argmax(-1)
+    """The lowest of the largest (-inf among them), NaN never; 0 where all are."""
+    best = []
+    for row in y.astype(np.float64):
+        tokens = np.flatnonzero(~np.isnan(row))
+        best.append(tokens[row[tokens].argmax()] if len(tokens) else 0)
+    return np.array(best, dtype=np.int64)

@@ -30,7 +30,8 @@ struct LogitArgs {
     int slices;
 };
 
-__device__ __forceinline__ void better(float v, int i, float& best, int& arg) {  // (a NaN is never better)
+// (From -inf and no token on: -inf is better than none, a NaN never is.)
+__device__ __forceinline__ void better(float v, int i, float& best, int& arg) {
     if (v > best || (v == best && i < arg)) best = v, arg = i;
 }
 __device__ __forceinline__ void wave_best(float& best, int& arg) {

@@ -25,8 +25,9 @@ def apply_rules(logits, ids=None, lengths=None, generated_from=None, repetition=
         x + bias                                                 tokens that bias_ids names (the last entry of several counts)
         -inf                                                     tokens whose bit is 0
 
-    Ids outside the vocabulary are none.  The best token is that of the returned logits: the lowest among equals, NaN never
-    wins, 0 where none is above -inf.  out (which may be logits, or apart from them) and token receive the results where they
+    Ids outside the vocabulary are none.  The best token is that of the returned logits: the lowest among equals; NaN never
+    wins, and where all are NaN the token is 0.  Where none is above -inf it is the lowest that is -inf, which may be one that
+    the mask forbids: the row has no token that may be chosen.  out (which may be logits, or apart from them) and token receive the results where they
     are given.  All on the device and read by the kernels, so that a captured HIP graph follows them."""
     got = quant.logit_rules(logits, ids, lengths, generated_from, repetition, presence, frequency, bias_ids, bias, mask, out, token)
     if got is not None:

@@ -164,3 +164,20 @@ def test_refusals(logits):
             logits.apply_rules(*args, **kw)
     y, token = logits.apply_rules(x[:0])
     assert y.shape == (0, 100) and token.shape == (0,)
+
+
+@pytest.mark.parametrize("v,allowed", [(40, [3, 17]), (9000, [0, 5, 2100, 8999])])
+def test_rows_of_which_nothing_may_be_chosen(logits, v, allowed):
+    # all that the mask leaves is NaN: the lowest of the masked ones; with one number among them, that
+    x = np.full((3, v), 1.0, np.float32)
+    x[:2, allowed] = np.nan
+    x[1, allowed[1]] = -7.0
+    x[2] = np.nan
+    bits = np.zeros(((v + 31) // 32) * 32, np.uint64)
+    bits[allowed] = 1
+    mask = (bits.reshape(-1, 32) << np.arange(32, dtype=np.uint64)).sum(1).astype(np.uint32).view(np.int32)[None]
+    y, token = logits.apply_rules(dev(x), mask=dev(mask))
+    want = so.logit_rules(x, mask=mask, dtype=np.float32)
+    assert np.array_equal(y.cpu().numpy(), want, equal_nan=True)
+    lowest = next(i for i in range(v) if i not in allowed)
+    assert token.tolist() == so.best_token(want).tolist() == [lowest, allowed[1], lowest]

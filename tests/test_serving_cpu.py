@@ -162,3 +162,9 @@ def test_the_oracle_on_rules_by_hand():
     assert y.tolist() == [[2.0 / 2 - 0.5 * 2 - 0.25, -4.0, 4.0, -np.inf]]
     assert so.best_token(y).tolist() == [2]
     assert so.keep_rows(np.array([5.0, 1.0, np.nan, 3.0, 3.0, 0.0]), 6, 3, 0, 1) == [0, 3, 5]
+
+
+def test_the_oracle_on_rows_without_a_token():
+    inf, nan = np.inf, np.nan
+    y = np.array([[nan, -inf, -inf], [nan, nan, nan], [-inf, -inf, -inf], [nan, -inf, -3.0], [nan, 2.0, 2.0]])
+    assert so.best_token(y).tolist() == [1, 0, 0, 2, 1] and so.best_token(y[:0]).shape == (0,)
