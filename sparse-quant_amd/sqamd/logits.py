@@ -86,8 +86,12 @@ class Rules:
         self.repetition, self.presence, self.frequency, self.generated_from = repetition, presence, frequency, generated_from
         self.bias_ids, self.bias, self.mask = bias_ids, bias, mask
 
+    def penalises(self):
+        """Whether the texts count: one of the penalties is given."""
+        return any(x is not None for x in (self.repetition, self.presence, self.frequency))
+
     def apply(self, logits, ids=None, lengths=None, out=None, token=None):
-        if not any(x is not None for x in (self.repetition, self.presence, self.frequency)):
+        if not self.penalises():
             ids = lengths = None  # nobody asks for the texts
         return apply_rules(logits, ids, lengths, self.generated_from if ids is not None else None, self.repetition, self.presence,
                            self.frequency, self.bias_ids, self.bias, self.mask, out, token)

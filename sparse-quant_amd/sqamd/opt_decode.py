@@ -271,6 +271,9 @@ class OPTDecoder(nn.Module):
         as they leave them; the texts that penalties look at are the first step_t rows of history, which then hold the prompts
         and the tokens chosen so far, tok among them.  Returns the logits [B, vocab]."""
         b = tok.shape[0]
+        texts = history is not None and step_t is not None
+        if rules is not None and rules.penalises() and not texts:  # (the step itself could not be taken back)
+            raise ValueError("penalties are for the tokens of a text; pass history and step_t")
         if getattr(self, "_parts", None) is None:
             self._parts = capi.f16_gemv_parts(self.lm_head.shape[0], self.lm_head.device)
         x = capi.embed_rows(self.embed, self.pos, tok.view(-1), pos_t, 2).view(b, 1, self.hidden)
@@ -282,7 +285,6 @@ class OPTDecoder(nn.Module):
             capi.greedy_feedback(self._parts, b, tok.view(-1), pos=pos_t, history=history, step=step_t)
             return logits
         logits = capi.f16_gemv(x, self.lm_head)
-        texts = history is not None and step_t is not None
         _, best = rules.apply(logits, history.t() if texts else None, step_t.expand(b) if texts else None, out=logits)
         # the token itself as the only candidate: its feedback is the launch that a step without rules ends with
         one = torch.zeros((8, 1), dtype=torch.float32, device=x.device), torch.zeros((8, 1), dtype=torch.int32, device=x.device)

@@ -266,3 +266,15 @@ def test_end_to_end_over_a_cache_that_evicts_from_the_prompt_on(opt, monkeypatch
             for j in range(2):
                 kept = a.position[i, j].cpu().numpy()
                 assert all(len(set(kept[h])) == rows for h in range(kept.shape[0]))  # no token twice
+
+
+def test_rules_without_texts_are_refused_before_the_step(opt):
+    from sqamd import logits
+    model = small(opt)
+    cache = model.new_cache(2, 64, rows=20)
+    tok = model(ids_of(10, 2, 30), cache, 0).argmax(-1)
+    before = [x.clone() for x in (cache.k, cache.v, cache.weight, cache.position, tok)]
+    pos = torch.tensor([30], device=DEV)
+    with pytest.raises(ValueError):
+        model.greedy_step(tok, cache, pos, rules=logits.Rules(presence=torch.ones(2, device=DEV)))
+    assert int(pos) == 30 and all(torch.equal(a, c) for a, c in zip(before, (cache.k, cache.v, cache.weight, cache.position, tok)))
