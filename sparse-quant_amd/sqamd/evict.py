@@ -13,7 +13,7 @@ from the device, so that a captured HIP graph follows it.  Nothing here has a co
 import torch
 
 import quant
-from . import capi
+from . import capi, prefix
 from .prefix import _alike, _check_ints, _check_written, _readable, _rows_like
 
 
@@ -124,6 +124,35 @@ def keep(k, v, weight, k_cache, v_cache, cache_weight, cache_position, keep_firs
     return got
 
 
+_MOST_ROWS, _MOST_HEADS = 1 << 25, 1 << 22  # (token, query head) and (sequence, query head) pairs of a call of prefix.attention
+
+
+def _prompt_attention(q, k, v, sm_scale):
+    """Causal attention of prompts q fp16 [B, heads, T, D] over k, v [B, kv_heads, T, D] -> [B, T, heads, D]: that of a batch whose
+    own rows are all there is, in as many calls as its limits on tokens and heads ask for."""
+    b, heads, t, d = q.shape
+    h = k.shape[1]
+    if h < 1 or heads % h:
+        raise ValueError("%d query heads over %d key/value heads" % (heads, h))
+    share = heads // h
+    at_once = max(1, min(h, _MOST_ROWS // max(t * share, 1)))                                       # key/value heads
+    most = max(1, min(_MOST_ROWS // max(t * share * at_once, 1), _MOST_HEADS // (share * at_once)))  # sequences
+    none = torch.empty((h, 0, d), dtype=q.dtype, device=q.device)
+    lengths = torch.full((b,), t, dtype=torch.int32, device=q.device)
+    if b <= most and h <= at_once:
+        return prefix.attention(q.transpose(1, 2).reshape(b * t, heads, d), none, none, k, v, lengths, sm_scale).view(b, t, heads, d)
+    out = torch.empty((b, t, heads, d), dtype=q.dtype, device=q.device)
+    for i in range(0, b, most):
+        for j in range(0, h, at_once):
+            mine = slice(j * share, (j + at_once) * share)
+            rows = q[i:i + most, mine].transpose(1, 2)
+            n, _, g, _ = rows.shape
+            got = prefix.attention(rows.reshape(n * t, g, d), none[j:j + at_once], none[j:j + at_once], k[i:i + most, j:j + at_once],
+                                   v[i:i + most, j:j + at_once], lengths[i:i + most], sm_scale)
+            out[i:i + most, :, mine] = got.view(n, t, g, d)
+    return out
+
+
 def _extent(x):
     last = sum((n - 1) * st for n, st in zip(x.shape, x.stride())) if x.numel() else 0
     return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size() if x.numel() else x.data_ptr()
@@ -178,11 +207,10 @@ class EvictCache:
         if t == 1:
             q, k, v = (x[:, :, 0] for x in (q, k, v))
             return attention(q, k, v, *cache, self.seen[:b], sm_scale, self.keep_first, self.keep_last)[0].view(b, 1, h, d)
-        if k.shape[1] == h and capi.lut_attention_strided_ok(q, k, v):
+        if capi.lut_attention_strided_ok(q, k, v):
             out = capi.lut_attention_strided(q, k, v, None, sm_scale, True, rows_first=True)
         else:
-            out = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True, scale=sm_scale,
-                                                                   enable_gqa=k.shape[1] != h).transpose(1, 2)
+            out = _prompt_attention(q, k, v, sm_scale)
         weight = attention_weights(q, k, sm_scale, self.window)
         keep(k, v, weight, *cache, self.keep_first, self.keep_last)
         return out

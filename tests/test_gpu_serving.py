@@ -278,3 +278,75 @@ def test_rules_without_texts_are_refused_before_the_step(opt):
     with pytest.raises(ValueError):
         model.greedy_step(tok, cache, pos, rules=logits.Rules(presence=torch.ones(2, device=DEV)))
     assert int(pos) == 30 and all(torch.equal(a, c) for a, c in zip(before, (cache.k, cache.v, cache.weight, cache.position, tok)))
+
+
+@pytest.mark.parametrize("heads,h,d,n", [(8, 2, 64, 50), (6, 1, 128, 131), (4, 4, 64, 50), (8, 2, 64, 1), (8, 2, 64, 0)])
+def test_an_evicting_cache_with_shared_heads(opt, heads, h, d, n):
+    from sqamd import evict
+    rng = np.random.default_rng(heads + n)
+    b, room, first, last, scale = 2, 40, 2, 8, 0.11
+    cache = evict.EvictCache(1, b + 1, h, d, room, first, last, device=DEV)
+
+    def rows(t):
+        x = rng.normal(0, 1, (b, t, heads + 2 * h, d)).astype(np.float16)
+        y = torch.from_numpy(x).to(DEV).transpose(1, 2)
+        return [v.transpose(0, 2, 1, 3) for v in np.split(x, [heads, heads + h], 2)], (y[:, :heads], y[:, heads:heads + h], y[:, heads + h:])
+
+    (q, k, v), given = rows(n)
+    cache.set_position(b, 0, n)
+    a = cache.attention(0, *given, scale)
+    assert a.shape == (b, n, heads, d)
+    share = heads // h
+    if n:
+        a = a.transpose(1, 2).cpu().numpy()
+        for i in range(n):
+            p = so._softmax(np.einsum("bhd,bhnd->bhn", q[:, :, i].astype(np.float64), k[:, :, :i + 1].repeat(share, 1).astype(np.float64)) * scale)
+            wide = v[:, :, :i + 1].repeat(share, 1).astype(np.float64)
+            want, size = np.einsum("bhn,bhnd->bhd", p, wide), np.einsum("bhn,bhnd->bhd", p, np.abs(wide))
+            assert (np.abs(a[:, :, i] - want) <= TOL * size + 1e-6).all(), i
+        w = so.attention_weights(q, k, [n] * b, scale)
+        weight, pos = cache.weight[0].cpu().numpy(), cache.position[0].cpu().numpy()
+        for i in range(b):
+            for j in range(h):
+                kept = pos[i, j, :min(n, room)]
+                assert np.allclose(weight[i, j, :len(kept)], w[i, j, kept], rtol=4e-4, atol=0)
+                assert np.array_equal(cache.k[0, i, j, :len(kept)].cpu().numpy(), k[i, j, kept])
+    for step in range(3):
+        before = [x[0, :b].cpu().numpy() for x in (cache.k, cache.v, cache.weight, cache.position)]
+        (q, k, v), given = rows(1)
+        cache.set_position(b, n + step, 1)
+        a = cache.attention(0, *given, scale)[:, 0].cpu().numpy()
+        out, size, _, kr, vr, wr, pr = so.evict_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], *before, np.full(b, n + step + 1), scale, first, last)
+        assert (np.abs(a - out) <= TOL * size + 1e-6).all()
+        assert np.array_equal(cache.k[0, :b].cpu().numpy(), kr) and np.array_equal(cache.position[0, :b].cpu().numpy(), pr)
+        assert np.allclose(cache.weight[0, :b].cpu().numpy(), wr, rtol=4e-4, atol=0)
+    assert (cache.k[0, b:] == 0).all() and (cache.weight[0, b:] == 0).all()
+
+
+def test_a_prompt_of_too_many_rows_for_one_call(built_lib):
+    # 2^21 tokens of 32 heads are twice what a call takes: sequences and heads are dealt to several, and agree with one of the parts
+    from sqamd import evict, prefix
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    b, heads, h, t, d = 2100, 32, 16, 512, 64
+    q, k = (torch.randn((b, n, 1, d), device=DEV, generator=gen).half().expand(b, n, t, d) for n in (heads, h))
+    v = torch.randn((1, h, t, d), device=DEV, generator=gen).half().expand(b, h, t, d)
+    assert b * t * heads > 1 << 25
+    out = evict._prompt_attention(q, k, v, 0.125)
+    # all keys of a sequence are one, so the rows are the means of the values so far
+    want = v[0].double().cumsum(1) / torch.arange(1, t + 1, device=DEV)[:, None]
+    size = v[0].double().abs().cumsum(1) / torch.arange(1, t + 1, device=DEV)[:, None]
+    off = (out.view(b, t, h, 2, d) - want.transpose(0, 1)[None, :, :, None]).abs().amax((0, 3))
+    assert (off <= TOL * size.transpose(0, 1) + 1e-6).all()
+
+
+@pytest.mark.parametrize("rows", [1, 50 * 2 * 3, 50 * 8 * 2])
+def test_a_prompt_dealt_to_several_calls(built_lib, monkeypatch, rows):
+    # a head at a time, three heads, two sequences of three
+    from sqamd import evict
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((3, 50, 16, 64), device=DEV, generator=gen).half().transpose(1, 2)
+    q, k, v = x[:, :8], x[:, 8:12], x[:, 12:]
+    monkeypatch.setattr(evict, "_MOST_ROWS", rows)
+    a = evict._prompt_attention(q, k, v, 0.125).transpose(1, 2).cpu().numpy()
+    q, k, v = (y.cpu().numpy() for y in (q, k.repeat_interleave(2, 1), v.repeat_interleave(2, 1)))
+    check_causal(a, q, k, v, 0, rows)
