@@ -661,6 +661,12 @@ at::Tensor scratch(size_t bytes, const at::Tensor& like) {
 void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* pointer(const Opt& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 constexpr int64_t INTS = 1LL << 31;
+// Whether a call was taken.  A refusal launches nothing, and the Python modules look for its reason and may call again; a launch
+// that the runtime rejected is an error at once: another may have run in front of it.
+bool taken(int rc, const char* what) {
+    if (rc == SQ_ERR_LAUNCH) raise_if_error(rc, what);
+    return rc == SQ_OK;
+}
 
 Opt prefix_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& kc, const at::Tensor& vc,
                      const at::Tensor& lengths, double sm_scale, const Opt& starts, const Opt& into, const Opt& kn,
@@ -685,7 +691,7 @@ Opt prefix_attention(const at::Tensor& q, const at::Tensor& kp, const at::Tensor
     const int rc = sq_prefix_attention(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), kc.data_ptr(), vc.data_ptr(), lengths.data_ptr(),
                                        pointer(starts), pointer(kn), pointer(vn), out.data_ptr(), (int)T, (int)B, (int)Hq, (int)H,
                                        (int)D, (int)P, (int)L, strides, (float)sm_scale, pointer(ws), need, current_stream(q));
-    if (rc != SQ_OK) return c10::nullopt;
+    if (!taken(rc, "sq_prefix_attention")) return c10::nullopt;
     return out;
 }
 
@@ -712,7 +718,7 @@ c10::optional<std::pair<at::Tensor, at::Tensor>> evict_attention(
                                       position.data_ptr(), seen.data_ptr(), out.data_ptr(), slot.data_ptr(), (int)B, (int)Hq, (int)H,
                                       (int)D, (int)R, (int)first, (int)last, strides, (float)sm_scale, pointer(ws), need,
                                       current_stream(q));
-    if (rc != SQ_OK) return c10::nullopt;
+    if (!taken(rc, "sq_evict_attention")) return c10::nullopt;
     return std::make_pair(out, slot);
 }
 
@@ -730,7 +736,7 @@ Opt evict_weights(const at::Tensor& q, const at::Tensor& k, double sm_scale, int
     const long strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2)};
     const int rc = sq_attention_weights(q.data_ptr(), k.data_ptr(), pointer(lengths), w.data_ptr(), (int)B, (int)Hq, (int)H, (int)D,
                                         (int)S, (int)window, strides, (float)sm_scale, pointer(ws), need, current_stream(q));
-    if (rc != SQ_OK) return c10::nullopt;
+    if (!taken(rc, "sq_attention_weights")) return c10::nullopt;
     return w;
 }
 
@@ -752,7 +758,7 @@ Opt evict_keep(const at::Tensor& k, const at::Tensor& v, const at::Tensor& weigh
     const int rc = sq_evict_keep(k.data_ptr(), v.data_ptr(), weight.data_ptr(), pointer(lengths), kc.data_ptr(), vc.data_ptr(),
                                  cweight.data_ptr(), cposition.data_ptr(), rows.data_ptr(), (int)B, (int)H, (int)D, (int)S, (int)R,
                                  (int)first, (int)last, strides, current_stream(k));
-    if (rc != SQ_OK) return c10::nullopt;
+    if (!taken(rc, "sq_evict_keep")) return c10::nullopt;
     return rows;
 }
 
@@ -820,7 +826,7 @@ c10::optional<std::pair<at::Tensor, at::Tensor>> logit_rules(const at::Tensor& x
                                   pointer(repetition), pointer(presence), pointer(frequency), pointer(bias_ids), pointer(bias),
                                   pointer(mask), token.data_ptr(), (int)M, (int)V, (int)L, (int)nb, strides, pointer(ws), need,
                                   current_stream(x));
-    if (rc != SQ_OK) return c10::nullopt;
+    if (!taken(rc, "sq_logit_rules")) return c10::nullopt;
     return std::make_pair(out, token);
 }
 
@@ -985,6 +991,7 @@ PYBIND11_MODULE(quant, m) {
     m.def("kv4_attention", &kv4_attention);
     m.def("kv4_select", &kv4_select);
     m.def("kv4_copy_pages", &kv4_copy_pages);
+    m.def("taken", &taken);
     m.def("prefix_attention", &prefix_attention);
     m.def("evict_attention", &evict_attention);
     m.def("evict_weights", &evict_weights);

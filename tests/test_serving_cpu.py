@@ -168,3 +168,14 @@ def test_the_oracle_on_rows_without_a_token():
     inf, nan = np.inf, np.nan
     y = np.array([[nan, -inf, -inf], [nan, nan, nan], [-inf, -inf, -inf], [nan, -inf, -3.0], [nan, 2.0, 2.0]])
     assert so.best_token(y).tolist() == [1, 0, 0, 2, 1] and so.best_token(y[:0]).shape == (0,)
+
+
+def test_a_launch_that_failed_is_no_refusal(built_lib):
+    # a refusal is looked into and may be called again; what may have run in part is not
+    import torch  # noqa: F401
+    import quant
+    from sqamd import capi
+    assert quant.taken(capi.SQ_OK, "call")
+    assert not any(quant.taken(rc, "call") for rc in (capi.SQ_ERR_BAD_SHAPE, capi.SQ_ERR_MISALIGNED, capi.SQ_ERR_WORKSPACE))
+    with pytest.raises(RuntimeError, match="call"):
+        quant.taken(capi.SQ_ERR_LAUNCH, "call")
