@@ -247,6 +247,9 @@ class OPTDecoder(nn.Module):
                 and self.pos.dtype == self.embed.dtype:
             x = self.embed[ids].add_(self.pos[pos0 + 2:pos0 + t + 2])  # consecutive positions: a slice of the table
         else:
+            if pos_ids is None and isinstance(pos0, int) and t and pos0 + t + 2 > self.pos.shape[0]:
+                # (no cache need end there: one that evicts has no last row, and reading behind the table ends the process)
+                raise ValueError("positions %d .. %d of a model for %d" % (pos0, pos0 + t - 1, self.pos.shape[0] - 2))
             if pos_ids is None:
                 pos_ids = torch.arange(pos0, pos0 + t, device=ids.device) + 2
             x = self.embed[ids] + self.pos[pos_ids]

@@ -350,3 +350,16 @@ def test_a_prompt_dealt_to_several_calls(built_lib, monkeypatch, rows):
     a = evict._prompt_attention(q, k, v, 0.125).transpose(1, 2).cpu().numpy()
     q, k, v = (y.cpu().numpy() for y in (q, k.repeat_interleave(2, 1), v.repeat_interleave(2, 1)))
     check_causal(a, q, k, v, 0, rows)
+
+
+def test_positions_behind_the_models_last_are_refused(opt):
+    model = small(opt)
+    cache = model.new_cache(2, 64, rows=20)
+    last = model.pos.shape[0] - 2  # (512)
+    model(ids_of(11, 2, 30), cache, 0)
+    seen = cache.seen.clone()
+    for ids, pos in ((ids_of(12, 2, 1), last), (ids_of(12, 2, 1), 1 << 40), (ids_of(12, 2, last + 1), 0)):
+        with pytest.raises(ValueError):
+            model(ids, cache, pos)
+    assert torch.equal(cache.seen, seen)
+    model(ids_of(12, 2, 1), cache, last - 1)
