@@ -283,3 +283,38 @@ def test_infinities_and_nan_in_front_of_a_tile_of_one_token(prefix, heads, h, ne
     assert np.array_equal(out == np.inf, ref == np.inf) and np.array_equal(out == -np.inf, ref == -np.inf)
     fine = np.isfinite(ref)
     assert (np.abs(out[fine] - ref[fine]) <= TOL * size[fine] + 1e-6).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,heads,h,new,p,ragged,given", [
+    (9, 16, 8, 130, 0, False, True), (9, 16, 8, 130, 100, True, True), (9, 16, 8, 130, 257, False, False), (5, 40, 8, 70, 300, True, False),
+    (36, 8, 8, 130, 300, False, True), (36, 8, 8, 130, 300, True, True)])
+def test_prompts_in_tiles_of_128_rows(prefix, d, b, heads, h, new, p, ragged, given):
+    # more than 64 rows of a sequence and more than 64 such tiles of all heads; with 36 sequences more than 512, of which the last
+    # are cut into parts (576 of equally many tokens, fewer of ragged ones)
+    rng = np.random.default_rng(b + p + d)
+    tokens = [new] * b if not ragged else [new if i % 3 else int(rng.integers(1, 2 * new)) for i in range(b)]
+    lens = [n + int(rng.integers(0, 90)) for n in tokens]
+    run(prefix, rng, b, heads, h, d, p, lens, tokens, max(lens) + 5, ragged=ragged, given=given)
+
+
+def test_prompts_in_tiles_of_128_rows_with_large_scores(prefix):
+    rng = np.random.default_rng(11)
+    run(prefix, rng, 9, 16, 8, 64, 200, [150 + i for i in range(9)], [130] * 9, 170, q_scale=8.0)
+
+
+def test_infinities_and_nan_under_tiles_of_128_rows(prefix):
+    rng = np.random.default_rng(12)
+    b, heads, h, new, p, d = 9, 16, 8, 130, 70, 64
+    t = b * new
+    q, kn, vn = normal(rng, t, heads, d), normal(rng, t, h, d), normal(rng, t, h, d)
+    kp, vp = normal(rng, h, p, d), normal(rng, h, p, d)
+    kc, vc = np.full((2, b, h, 140, d), np.nan, np.float16)
+    vn[30, 0, 5], vn[new + 70, 1, 63], kn[33, 2, 0], vn[2 * new - 1, 0, 9] = np.inf, np.nan, np.nan, -np.inf
+    with np.errstate(invalid="ignore"):
+        ref, size, _, _ = so.prefix_attention(q, kp, vp, kc, vc, [new] * b, [new] * b, 0.125, kn, vn)
+        out = prefix.attention(dev(q), dev(kp), dev(vp), dev(kc), dev(vc), torch.full((b,), new, dtype=torch.int32, device=DEV), 0.125,
+                               k_new=dev(kn), v_new=dev(vn)).float().cpu().numpy()
+    assert np.array_equal(np.isfinite(out), np.isfinite(ref)) and np.array_equal(out == np.inf, ref == np.inf)
+    fine = np.isfinite(ref)
+    assert (np.abs(out[fine] - ref[fine]) <= TOL * size[fine] + 1e-6).all()
