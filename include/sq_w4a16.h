@@ -537,7 +537,7 @@ int sq_kv4_copy_pages(void* pool, const void* src, const void* dst, int n, int n
 /* Causal attention of a batch of sequences that share a long prefix, which is read once for all of them:
  *   out[t, h, :] = sum_j P[j] v_j, P = softmax_j(sm_scale q[t, h, :] . k_j) over the P rows of the prefix and the rows of t's
  * own sequence up to t's; query head h reads key/value head h / (Hq / H).  fp16, softmax and sums in fp32, the probabilities
- * rounded to fp16 where they meet the values.
+ * rounded to fp16 where they meet the values (steps of 2^-31 of the largest or finer: smaller ones may count as 0).
  *   q          element (t, h, d) at q[t * strides[0] + h * strides[1] + d]
  *   k_prefix, v_prefix  row j of head h at [h * strides[2] + j * strides[3]]; may be NULL where P is 0
  *   k_cache, v_cache    row j of (sequence b, head h) at [b * strides[4] + h * strides[5] + j * strides[6]], room for Lmax rows

@@ -35,11 +35,16 @@ struct Divisor {
     }
 };
 
-// How much of a state (maximum, sum) counts beside a maximum m of them all.  One without a maximum has seen nothing, sum 0, or
+// How much of a state (reference, sum) counts beside the highest reference m.  One without a reference has seen nothing, sum 0, or
 // scores that are no numbers, sum NaN: it counts as its sum.
 __device__ __forceinline__ float share_of(float2 s, float m) {
     return s.x == -INFINITY ? s.y : __builtin_amdgcn_exp2f(s.x - m);
 }
+
+// Probabilities meet the values in fp16, as 2^(score - reference): the reference lies 2^7 below the largest score when it is set and
+// moves when one exceeds it by more than 2^15, so that p stays inside fp16 and nothing needs rescaling until then, and what is
+// 2^-32 of the largest or more is not 0.  (With the largest at 1, a million rows of 2^-26 beside it, 1.5 % of the sum, were lost.)
+constexpr float REF_BELOW = 7.f, REF_MOVES = 15.f;
 
 template <int D>
 struct RowsAttn {
@@ -54,7 +59,7 @@ struct RowsAttn {
 
     half8_t qf[NK];
     float16_t acc[DT];
-    float ref, top, sum;  // reference maximum (0 while unset), the score above it at which it moves, this lane's share of the sum
+    float ref, top, sum;  // reference (0 while unset), the score above it at which it moves, this lane's share of the sum
 
     static __device__ __forceinline__ int swz(bool value, int row) { return value ? v_swz<D>(row) : k_swz<D>(row); }
 
@@ -149,8 +154,6 @@ struct RowsAttn {
             scored(blk, st);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (next < blk1) issue(next, false, kt0);  // (the keys are in registers)
-            // The reference maximum moves only when a score exceeds it by more than 2^8 (or when it is still unset): until
-            // then p stays inside fp16 and nothing needs rescaling.
             float mx = -INFINITY;
 #pragma unroll
             for (int v = 0; v < 16; v++) {
@@ -160,10 +163,10 @@ struct RowsAttn {
             if (__builtin_amdgcn_ballot_w64(mx > top) != 0) {
                 const float mq = fmaxf(mx, __shfl_xor(mx, 32));
                 const bool upd = mq > top;
-                const float delta = upd ? mq : 0.f;
+                const float delta = upd ? mq - REF_BELOW : 0.f;
                 const float alpha = (upd && top != -INFINITY) ? __builtin_amdgcn_exp2f(-delta) : 1.f;
                 ref += delta;
-                top = upd ? 8.f : top;
+                top = upd ? REF_MOVES : top;
                 sum *= alpha;
 #pragma unroll
                 for (int v = 0; v < 16; v++) st[v] -= delta;
@@ -206,7 +209,7 @@ struct RowsAttn {
         static_assert(NL == 8 || NL == 4);
     }
 
-    // The waves' states of a row joined: emit(row, column, four sums, maximum, sum) for the first `rows` rows.  stat: [4][32].
+    // The waves' states of a row joined: emit(row, column, four sums, reference, sum) for the first `rows` rows.  stat: [4][32].
     template <class Emit>
     __device__ __forceinline__ void join(uint8_t* lds, float2* stat, int rows, Emit emit) {
         const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lc = lane >> 5;

@@ -59,7 +59,7 @@ __device__ __forceinline__ void nothing_seen(const EvictStep& t, int bh) {
 }
 
 // What the query heads g0 .. g0 + heads - 1 give to the rows r0 .. r0 + EJ_ROWS - 1 is added to their weights; state holds the
-// heads' maximum (in units of log2) and the reciprocal of their sum.  The row of the slot begins anew, with the first heads.
+// heads' reference (in units of log2) and the reciprocal of their sum.  The row of the slot begins anew, with the first heads.
 constexpr int EJ_ROWS = 1024;
 __device__ __forceinline__ void add_weights(const EvictArgs& a, int bh, int r0, int n, int seen, int slot, const float2* state, int g0,
                                             int heads) {

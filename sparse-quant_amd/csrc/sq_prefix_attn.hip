@@ -32,7 +32,7 @@ constexpr int PA_STEP = 64;  // keys of a step
 // How a call is cut.  Packed: rows of all sequences against pieces of the prefix (a), a sequence's against pieces of its own rows
 // (b).  Otherwise tiles of a sequence's rows against the prefix and its own rows, as `Deal` has it.
 struct PrefixPlan {
-    float* po;  // partial outputs, then (maximum, sum) of each
+    float* po;  // partial outputs, then (reference, sum) of each
     float2* pml;
     int packed, qa, qb, rows_b;                                // tiles of 32 qa and 32 qb rows
     int tiles_a, parts_a, steps_a, tiles_b, parts_b, steps_b;  // steps of 64 keys of a part
@@ -371,8 +371,8 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
                         (((4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ v_swz<D>(key)) * 16) + 8 * (lane & 1);
     }
 
-    // Reference maximum of the row (0 while unset), the score above it at which it moves (any score while unset), and
-    // this lane's share of the row sum.
+    // Reference of the row (0 while unset), the score above it at which it moves (any score while unset), and this lane's share
+    // of the row sum.
     float ref = 0.f, top = -INFINITY, l_i = 0.f;
     float16_t acc[DT];
 #pragma unroll
@@ -430,8 +430,6 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
                     st[b][v] = key <= last ? st[b][v] : -INFINITY;
                 }
         }
-        // The reference maximum moves only when a score exceeds it by more than 2^8 (or when it is still unset): until
-        // then p = exp2(score) stays inside fp16 and nothing needs rescaling.
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < KS; b++)
@@ -440,10 +438,10 @@ __device__ __forceinline__ void many_rows(const PrefixArgs& a, const Work& w, ui
         if (__builtin_amdgcn_ballot_w64(mx > top) != 0) {
             const float mq = fmaxf(mx, __shfl_xor(mx, 32));
             const bool upd = mq > top;
-            const float delta = upd ? mq : 0.f;
+            const float delta = upd ? mq - REF_BELOW : 0.f;
             const float alpha = (upd && top != -INFINITY) ? __builtin_amdgcn_exp2f(-delta) : 1.f;
             ref += delta;
-            top = upd ? 8.f : top;
+            top = upd ? REF_MOVES : top;
             l_i *= alpha;
 #pragma unroll
             for (int b = 0; b < KS; b++)

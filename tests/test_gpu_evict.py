@@ -330,3 +330,17 @@ def test_zeros_of_both_signs_are_equal(evict):
         for i in range(b):
             for j in range(h):
                 assert rows[i, j].tolist() == so.keep_rows(w[i, j], s, room, 3, 4), (s, i, j)
+
+
+def test_what_many_rows_add_up_to_beside_one_large_score(evict):
+    # as in test_gpu_prefix.py: a million rows of 2^-26 of the largest probability, which is given to a value of 0
+    d, room = 64, 1 << 20
+    kc = torch.zeros((1, 1, room, d), dtype=torch.float16, device=DEV)
+    vc = torch.ones_like(kc)
+    kc[:, :, 7, 0], vc[:, :, 7] = 26.0, 0.0
+    weight, position = torch.zeros((1, 1, room), device=DEV), torch.arange(room, dtype=torch.int32, device=DEV).view(1, 1, room)
+    q, kn, vn = (torch.zeros((1, n, d), dtype=torch.float16, device=DEV) for n in (2, 1, 1))
+    q[:, :, 0], vn[:] = 1.0, 1.0
+    out, _ = evict.attention(q, kn, vn, kc, vc, weight, position, torch.tensor([room], dtype=torch.int32, device=DEV), np.log(2.0), 8, 8)
+    want = (room - 1) * 2.0 ** -26 / (1 + (room - 1) * 2.0 ** -26)
+    assert ((out.double() - want).abs() <= TOL * want).all(), (out.min().item(), out.max().item(), want)

@@ -318,3 +318,18 @@ def test_infinities_and_nan_under_tiles_of_128_rows(prefix):
     assert np.array_equal(np.isfinite(out), np.isfinite(ref)) and np.array_equal(out == np.inf, ref == np.inf)
     fine = np.isfinite(ref)
     assert (np.abs(out[fine] - ref[fine]) <= TOL * size[fine] + 1e-6).all()
+
+
+def test_what_many_rows_add_up_to_beside_one_large_score(prefix):
+    # one row of the largest score, and so many others of 2^-26 of its probability that they make a hundredth of the sum
+    d, h, p = 64, 1, 1 << 20
+    kp = torch.zeros((h, p, d), dtype=torch.float16, device=DEV)
+    vp = torch.ones((h, p, d), dtype=torch.float16, device=DEV)
+    kp[:, 7, 0], vp[:, 7] = 26.0, 0.0
+    kc = torch.zeros((1, h, 40, d), dtype=torch.float16, device=DEV)
+    for t, heads in ((1, 1), (33, 2), (40, 4)):
+        q = torch.zeros((t, heads, d), dtype=torch.float16, device=DEV)
+        q[:, :, 0] = 1.0
+        got = prefix.attention(q, kp, vp, kc, kc, torch.zeros(1, dtype=torch.int32, device=DEV), np.log(2.0)).double()
+        want = (p - 1) * 2.0 ** -26 / (1 + (p - 1) * 2.0 ** -26)
+        assert ((got - want).abs() <= TOL * want).all(), (t, heads, got.min().item(), got.max().item(), want)
