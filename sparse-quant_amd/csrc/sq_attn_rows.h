@@ -16,7 +16,8 @@ namespace sq {
 constexpr int RA_WAVES = 4;
 constexpr int RA_BLOCK = 32;  // keys
 
-// Division of 32-bit numbers by one that the host knows: a multiplication instead of twenty instructions.
+// Division of 32-bit numbers by one that the host knows: a multiplication instead of twenty instructions (Granlund and Montgomery,
+// Division by invariant integers using multiplication, 1994: the multiplier rounded up).
 struct Divisor {
     uint32_t mul, shift, value;
     __host__ static Divisor of(uint32_t d) {

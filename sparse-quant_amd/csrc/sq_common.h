@@ -337,7 +337,10 @@ __device__ __forceinline__ void load_to_lds_x1(const void* g, uint32_t lds_byte)
     asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(lds_byte) : "memory");
 }
 // The same with the address split into a wave-uniform base and a 32-bit byte offset per lane: a loop that
-// walks along K then advances one scalar instead of one 64-bit sum per lane and load.
+// walks along K then advances one scalar instead of one 64-bit sum per lane and load.  A memory instruction may read the base five
+// wait states after a vector instruction has written it, which nobody counts in front of inline assembly: a base out of
+// v_readfirstlane goes through uniform() (sq_attn_tile.h), and tests/test_wait_states_cpu.py looks through the built
+// kernels for any that comes too early, reloads of spilled registers among them.
 __device__ __forceinline__ void load_to_lds_x4(const void* base, uint32_t lane_byte, uint32_t lds_byte) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_byte), "s"(base), "{m0}"(lds_byte) : "memory");
 }

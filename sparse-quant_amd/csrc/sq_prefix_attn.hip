@@ -739,7 +739,8 @@ constexpr int PA_WGS_OWN = 1024;
 // the prefix (from L2).  Packed / not, us, 32 heads over 8: 64 x 1 token behind 512 rows 23.5 / 20.3, 1024 23.5 / 26.6, 8192
 // 44 / 125; 64 x 8 behind 1024 45 / 32, 2048 52 / 45, 4096 70 / 74; where the tiles do not fill the chip 16 x 1 behind 64 12.2 / 9.0,
 // 256 12.7 / 12.3, 1024 13.8 / 16.2; 16 x 8 16.9 / 11.8, 17.9 / 19.3, 19.2 / 23.6.  More than 32 rows of a sequence (64 x 16 tokens
-// behind 4096) 107 / 102.
+// behind 4096) 107 / 102.  The average number of rows decides, since only the device knows each sequence's: one prompt of 1024
+// tokens beside 63 single ones behind 4096 rows takes 231, the two apart 116 and 32.
 bool pack(int P, int B, long each, long tiles) {
     return B > 1 && each <= 32 && P > (tiles >= PA_SLOTS ? 512 + 64 * each : PA_STEP);
 }

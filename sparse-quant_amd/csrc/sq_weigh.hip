@@ -5,9 +5,11 @@
 // key/value head are packed, so that its keys are read once for all of its heads.
 //
 // What bounds it: vector instructions beside the products; an exponential of 8 cycles and two to three others of 4 per score and pass,
-// and a score's share of the products is 4 (D = 128).  8 prompts of 2048, 32 heads: 275 GFLOP in both passes, 350 us, 0.78 PFLOP/s;
-// the two products alone would take 236 at a large product's rate.  The second product cannot be avoided: the sums are known only
-// behind a row's last key, and the scores in memory would be 1 GB.  A window of 64 queries over 4 x 8191 rows takes 43 us for 26 MB:
+// and a score's share of the products is 4 (D = 128).  8 prompts of 2048, 32 heads: 275 GFLOP in both passes, 350 us, 0.78 PFLOP/s
+// (vector issue 0.81 of the time in both, matrix pipes 0.56 and 0.44); the two products alone would take 236 at a large product's
+// rate.  Where queries and keys are all that is given the second product cannot be avoided: the sums are known only behind a
+// row's last key, and the scores in memory would be 1 GB.  (A prompt's attention forms the same sums; it does not hand them on, so
+// that a cache that evicts pays for the first pass again.)  A window of 64 queries over 4 x 8191 rows takes 43 us for 26 MB:
 // two launches, of which the first goes through all keys with one tile of queries a workgroup.
 #include "sq_attn_rows.h"
 #include "sq_kernels.h"
